@@ -142,6 +142,20 @@ SIGNATURES = {
     "ops_attention_batch": (None, [_O, _I, Opnd, _L, Opnd, _L, Opnd, _L, Opnd, _L, _I,
                                    _I, _I, _I, _F, Mem]),
     "ops_rope": (None, [_O, Mem, _L, _I, _L, _I, _I, _I, Mem, _I]),
+    "ops_q8_pitch": (_I, [_I]),
+    "ops_quant_rows": (None, [_O, _L, _I, Mem, _L, _I, Mem, Mem]),
+    "ops_linear_qq": (None, [_O, _I, _I, _I, Mem, Mem, Mem, Mem, Mem, Mem, _L, Mem, _L, _I, _I, _F]),
+    "ops_linear_q8_work_bytes": (C.c_size_t, [_I, _I]),
+    "ops_linear_q8": (None, [_O, _I, _I, _I, Mem, _L, _I, Mem, Mem, Mem, Mem, _L, Mem, _L, _I, _I, _F, Mem]),
+    "ops_rope_freqs": (None, [_P, _I, _I, C.c_double, _I, C.c_double, C.c_double, C.c_double, C.c_double]),
+    "ops_rope_pos": (None, [_O, _L, _I, _I, _I, Mem, Mem, _F, _I, Opnd, Opnd, _I, Opnd, Opnd, _I]),
+    "ops_key_blocks": (_I, [_I, _I]),
+    "ops_block_index": (None, [_O, Opnd, _I, _I, _I, _I, Mem, _I, _I, Mem, Mem]),
+    "ops_block_select_work_bytes": (C.c_size_t, [_I, _I, _I, _I]),
+    "ops_block_select": (None, [_O, Opnd, _I, _I, _I, _I, Mem, Mem, _I, _I, Mem, Mem]),
+    "ops_attention_blocks_work_bytes": (C.c_size_t, [_I, _I, _I, _I, _I, _I, _I]),
+    "ops_attention_blocks": (None, [_O, Opnd, Opnd, Opnd, Opnd, _I, _I, _I, _I, _I, _I, _I, Mem, _F,
+                                    Mem, Mem]),
     "ops_resize": (None, [_O, Mem, _I, _I, _I, Mem, _I, _I, _I, _I, _F]),
     "ops_grid_sample": (None, [_O, Mem, _I, _I, _I, Mem, _I, _I, Mem]),
     "ops_unfold": (None, [_O, Mem, _I, _I, _I, C.POINTER(ConvGeom), Mem]),
@@ -249,6 +263,8 @@ SIGNATURES = {
 # Entry points that never raise through the fatal path (no error check).
 _NO_CHECK = {"ocl_graph_free", "icoreg_set_fatal_mode", "icoreg_last_error", "icoreg_clear_error",
              "ocl_errstr", "ops_mat", "ops_bmat", "ops_geom", "ops_conv_out",
+             "ops_q8_pitch", "ops_linear_q8_work_bytes", "ops_key_blocks",
+             "ops_block_select_work_bytes", "ops_attention_blocks_work_bytes",
              "ocl_wrap", "icoreg_prof_entry", "icoreg_prof_reset", "icoreg_prof_flush", "ops_report",
              "pth_find", "pth_numel", "pth_bytes", "pth_strip_prefix",
              "icoreg_pth_new", "icoreg_eloftr_new", "icoreg_struct_delete",

@@ -43,6 +43,18 @@ void need_floats(cl_mem b, long long off, long long n, const char *op,
 /* Same in bytes. */
 void need_bytes(cl_mem b, long long off, long long n, const char *op,
                 const char *operand);
+/* Fatal if buffer b does not start on a multiple of n bytes. */
+void need_aligned(cl_mem b, int n, const char *op, const char *operand);
+/* Fatal if [aoff, aoff + an) bytes of a and [boff, boff + bn) of b overlap in
+ * memory (also as views into one allocation). */
+void need_apart(cl_mem a, long long aoff, long long an, cl_mem b, long long boff, long long bn,
+                const char *op, const char *operands);
+/* Fatal if a row of one operand (rows of w floats, ld floats apart) shares a
+ * float with a row of the other; rows of one packed buffer may lie side by
+ * side. */
+void need_rows_apart(const float *p, long long ldp, long long wp, long long rp, const float *q,
+                     long long ldq, long long wq, long long rq, const char *op,
+                     const char *operands);
 /* Element counts handed to kernels as int (ops.c:79-84). */
 int count32(long long n, const char *what);
 

@@ -60,6 +60,43 @@ void need_floats(cl_mem b, long long off, long long n, const char *op,
     need_bytes(b, off * 4, n * 4, op, operand);
 }
 
+void need_aligned(cl_mem b, int n, const char *op, const char *operand)
+{
+    if (b && (uintptr_t)b->ptr % n)
+        icoreg_fatal("%s: %s does not start on a multiple of %d bytes", op, operand, n);
+}
+
+void need_apart(cl_mem a, long long aoff, long long an, cl_mem b, long long boff, long long bn,
+                const char *op, const char *operands)
+{
+    if (!a || !b || an <= 0 || bn <= 0)
+        return;
+    const uintptr_t x = (uintptr_t)a->ptr + aoff, y = (uintptr_t)b->ptr + boff;
+
+    if (x < y + bn && y < x + an)
+        icoreg_fatal("%s: %s must not overlap", op, operands);
+}
+
+void need_rows_apart(const float *p, long long ldp, long long wp, long long rp, const float *q,
+                     long long ldq, long long wq, long long rq, const char *op,
+                     const char *operands)
+{
+    if (rp <= 0 || rq <= 0)
+        return;
+    const uintptr_t a = (uintptr_t)p, b = (uintptr_t)q;
+    const uintptr_t an = 4 * ((rp - 1) * ldp + wp), bn = 4 * ((rq - 1) * ldq + wq);
+
+    if (a >= b + bn || b >= a + an)
+        return;
+    if (ldp == ldq && (a - b) % 4 == 0) {
+        const long long diff = (long long)(b - a) / 4, m = (diff % ldp + ldp) % ldp;
+
+        if (m >= wp && m + wq <= ldp)
+            return;
+    }
+    icoreg_fatal("%s: %s must not overlap", op, operands);
+}
+
 int count32(long long n, const char *what)
 {
     if (n < 0 || n > 0x7fffffffLL)

@@ -180,6 +180,115 @@ void ops_attention_batch(struct ops *o, int nb, struct opnd Q, long bq,
 void ops_rope(struct ops *o, cl_mem X, long off, int ld, long rows, int nh,
               int d, int npos, cl_mem cs, int interleaved);
 
+/* ---- Long token sequences and large tiles --------------------------------
+ * Extensions with no counterpart in the reference, for transformer layers on
+ * more tokens than the networks here were trained on: products in 8-bit
+ * integers, rotary positions computed from the tokens' coordinates, and
+ * attention over the blocks of keys that a cheap score selects. They
+ * allocate nothing and leave the ops work buffer alone: what they need for
+ * themselves is the caller's `work` buffer, of the size that the call's
+ * _work_bytes function gives (0 where the sizes are invalid), 16-byte
+ * aligned, its content of no meaning between calls. Calls that may overlap
+ * on the device (recorded graphs replayed side by side among them) need work
+ * buffers of their own. */
+
+/* 8-bit codes and scales of rows of C floats, row r at float xoff + r ldx of
+ * X: with a = max |x|, S[r] = a / 127 and code(x) = x (127 / a) in float32,
+ * rounded to the nearest integer, ties to even, so that x = code S within
+ * S / 2. A row with a < 2^-100 counts as zero (S = 0); a row with a value
+ * that is not finite gets S = NaN, codes 0. Row r of Q starts at byte r
+ * ops_q8_pitch(C) (C rounded up to 64), zeros behind the C codes. Q 16-byte
+ * aligned; X, Q and S apart. The same call makes the codes of a PyTorch
+ * [out, in] weight (rows = out, C = in). */
+int ops_q8_pitch(int C);
+void ops_quant_rows(struct ops *o, long rows, int C, cl_mem X, long xoff,
+                    int ldx, cl_mem Q, cl_mem S);
+
+/* Y = act(XS[i] WS[j] sum_k XQ[i][k] WQ[j][k] + b[j]) + R, token-major: XQ,
+ * XS rows tokens, WQ, WS out channels as ops_quant_rows makes them, in <=
+ * 2^17 of both, the sum exact in 32-bit integers. Row i of Y starts at float
+ * yoff + i ldy; b and R NULL for none, R with Y's row stride from roff, and
+ * it may be Y itself. */
+void ops_linear_qq(struct ops *o, int rows, int in, int out, cl_mem XQ,
+                   cl_mem XS, cl_mem WQ, cl_mem WS, cl_mem b, cl_mem R,
+                   long roff, cl_mem Y, long yoff, int ldy, int act,
+                   float slope);
+
+/* ops_quant_rows of the float tokens X, then ops_linear_qq. */
+size_t ops_linear_q8_work_bytes(int rows, int in);
+void ops_linear_q8(struct ops *o, int rows, int in, int out, cl_mem X,
+                   long xoff, int ldx, cl_mem WQ, cl_mem WS, cl_mem b,
+                   cl_mem R, long roff, cl_mem Y, long yoff, int ldy, int act,
+                   float slope, cl_mem work);
+
+/* Frequencies (radians a position) of the rot / 2 pairs for ops_rope_pos, on
+ * the host: pair p belongs to coordinate p % axes and is the k-th, k = p /
+ * axes, of its n = rot / axes channels; trained frequency w = base^(-2 k /
+ * n). For coordinates beyond the trained ones, factor > 1 stretches them:
+ * ROPE_LINEAR all alike (w / factor), ROPE_REBASE by the base (base
+ * factor^(n / (n - 2))), ROPE_PARTS only pairs that turn few times over the
+ * `trained` positions: w (g + (1 - g) / factor), g = (trained w / 2 pi -
+ * slow) / (fast - slow) held to 0 .. 1. rot a multiple of 2 axes. */
+#define ROPE_TRAINED 0
+#define ROPE_LINEAR 1
+#define ROPE_REBASE 2
+#define ROPE_PARTS 3
+void ops_rope_freqs(double *freq, int rot, int axes, double base, int kind,
+                    double factor, double trained, double slow, double fast);
+
+/* Rotary encoding by coordinates of two tensors (queries and keys; nh2 = 0
+ * for one) of rows x (nh heads of d): the first rot channels of each head are
+ * turned, pair p by the angle pos[row axes + p % axes] freq[p] (pos: int32,
+ * freq: rot / 2 doubles; the angle in 64 bits), and multiplied by mult; the
+ * others are copied. ROPE_INTERLEAVED: pairs (2 p, 2 p + 1), else (p, p + rot
+ * / 2). ROPE_INVERSE: by the negative angle, the gradient of the forward
+ * call. Xi to Yi, rows at the operands' offsets and ld (packed projections);
+ * Yi may be Xi (same offset and ld), any other overlap of an output is an
+ * error (rows side by side in one packed buffer do not overlap). rot 0 .. min(d, 2048), even; axes 1 .. 4. */
+#define ROPE_INTERLEAVED 1
+#define ROPE_INVERSE 2
+void ops_rope_pos(struct ops *o, long rows, int d, int rot, int axes,
+                  cl_mem pos, cl_mem freq, float mult, int flags,
+                  struct opnd X1, struct opnd Y1, int nh1, struct opnd X2,
+                  struct opnd Y2, int nh2);
+
+/* Attention over selected blocks of bs = 16, 32, 64 or 128 keys, the last one
+ * shorter: nh query heads on nhk key heads (nh a multiple; query head h on
+ * key head h / (nh / nhk)) of d <= 128 channels, head h at columns h d.
+ *
+ * ops_block_index: codes KC and scales KS of blocks b0 .. b0 + nb - 1, block
+ * b, key head h at row b nhk + h: the mean of the block's kept keys (kmask:
+ * Nk bytes, 0 = leave the key out, or NULL), rounded to float32 and coded as
+ * by ops_quant_rows; scale -1 where no key is kept. An index that is kept
+ * with a growing sequence has its last blocks made again. ops_key_blocks:
+ * the number of blocks of Nk keys. */
+int ops_key_blocks(int Nk, int bs);
+void ops_block_index(struct ops *o, struct opnd K, int Nk, int nhk, int d,
+                     int bs, cl_mem kmask, int b0, int nb, cl_mem KC,
+                     cl_mem KS);
+
+/* SEL[(query nh + head) top + i], int32: the blocks with the top (1 .. 64)
+ * largest scores KS (q . KC), q the query's 8-bit codes, best first, ties to
+ * the lower block, NaN above all numbers, -1 behind the last block that keeps
+ * a key. The sum of the codes' products is exact: the same selection from
+ * every kernel. */
+size_t ops_block_select_work_bytes(int Nq, int nh, int nblk, int top);
+void ops_block_select(struct ops *o, struct opnd Q, int Nq, int nh, int nhk,
+                      int d, cl_mem KC, cl_mem KS, int nblk, int top,
+                      cl_mem SEL, cl_mem work);
+
+/* O = softmax(scale Q K^T) V over the kept keys of each query and head's
+ * listed blocks (SEL as above; entries that are no block are skipped, a block
+ * listed twice counts once). No key left: zeros. A NaN among the kept scores
+ * makes the row NaN; what left-out keys and values hold does not matter. O
+ * may be Q (same offset and ld), any other overlap of O is an error. */
+size_t ops_attention_blocks_work_bytes(int Nq, int Nk, int nh, int nhk, int d,
+                                       int bs, int top);
+void ops_attention_blocks(struct ops *o, struct opnd Q, struct opnd K,
+                          struct opnd V, struct opnd O, int Nq, int Nk, int nh,
+                          int nhk, int d, int bs, int top, cl_mem SEL,
+                          float scale, cl_mem kmask, cl_mem work);
+
 /* Bilinear resampling of in (C, h, w) into channels coff.. of out
  * (*, H, W). align_corners 0: scale > 0 gives source step 1 / scale,
  * scale 0 the size ratio. ops.h:133-134. */
