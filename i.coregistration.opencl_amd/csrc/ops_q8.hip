@@ -11,9 +11,12 @@
 
 #include <hip/hip_runtime.h>
 
+#include <type_traits>
+
 #include "act.h"
 #include "common.h"
 #include "gemm_dev.h"
+#include "load4.h"
 #include "ops.h"
 #include "q8.h"
 
@@ -26,17 +29,19 @@ typedef int q8_i16 __attribute__((ext_vector_type(16)));
 
 /* ---- codes of rows --------------------------------------------------------- */
 
-/* One wave a row, four channels a lane and step: the largest magnitude, then
- * the codes. Rows of up to 256 NV channels stay in registers between the two;
- * longer ones (NV = 0) are read again. */
-template <int NV, bool VEC>
+/* W waves a row (1 or 4), four channels a lane and step: the largest
+ * magnitude, then the codes. Rows of up to 256 NV W channels stay in registers
+ * between the two; longer ones (NV = 0) are read again. */
+template <int NV, int W>
 __global__ void __launch_bounds__(256)
     quant_rows_kernel(const float *__restrict__ X, long long ldx, long rows, int C,
                       unsigned *__restrict__ Q, float *__restrict__ S)
 {
-    const int lane = threadIdx.x & 63;
-    const long row = (long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int steps = NV ? NV : (C + 255) / 256;
+    __shared__ unsigned tops[W > 1 ? W : 1];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int sub = wave % W;
+    const long row = (long)blockIdx.x * (4 / W) + wave / W;
+    const int steps = NV ? NV : (C + 256 * W - 1) / (256 * W);
     const long long words = q8_pitch(C) / 4;
     float v[NV ? NV : 1][4];
     unsigned mag = 0;
@@ -46,22 +51,7 @@ __global__ void __launch_bounds__(256)
     X += row * ldx;
     Q += row * words;
     auto load = [&](int k, float (&x)[4]) {
-        const int c = 256 * k + 4 * lane;
-
-        if (VEC) {
-            const float4 a = *(const float4 *)(X + min(c, C - 4));
-            const bool in = c < C;
-
-            x[0] = in ? a.x : 0.0f;
-            x[1] = in ? a.y : 0.0f;
-            x[2] = in ? a.z : 0.0f;
-            x[3] = in ? a.w : 0.0f;
-        }
-        else {
-#pragma unroll
-            for (int j = 0; j < 4; j++)
-                x[j] = c + j < C ? X[c + j] : 0.0f;
-        }
+        load4_row(X, 256 * (W * k + sub) + 4 * lane, C, x);
     };
 #pragma unroll NV ? NV : 1
     for (int k = 0; k < steps; k++) {
@@ -72,13 +62,22 @@ __global__ void __launch_bounds__(256)
         for (int j = 0; j < 4; j++)
             mag = max(mag, q8_mag(x[j]));
     }
-    const q8_scale q = q8_scale_of(wave_umax(mag));
+    mag = wave_umax(mag);
+    if constexpr (W > 1) {
+        if (lane == 0)
+            tops[sub] = mag;
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < W; e++)
+            mag = max(mag, tops[e]);
+    }
+    const q8_scale q = q8_scale_of(mag);
 
-    if (lane == 0)
+    if (lane == 0 && sub == 0)
         S[row] = q.s;
 #pragma unroll NV ? NV : 1
     for (int k = 0; k < steps; k++) {
-        const int w = 64 * k + lane;
+        const int w = 64 * (W * k + sub) + lane;
         float(&x)[4] = v[NV ? k : 0];
 
         if (!NV)
@@ -91,24 +90,26 @@ __global__ void __launch_bounds__(256)
 static void quant_rows(struct ops *o, long rows, int C, const float *X, long long ldx, void *Q,
                        float *S)
 {
-    const bool vec = ((uintptr_t)X & 15) == 0 && ldx % 4 == 0 && C % 4 == 0;
-    const dim3 grid((unsigned)((rows + 3) / 4)), block(256);
+    /* Long rows, a block each: 4096 channels, 16 rows 4.2 -> 2.7 us, 785 rows 6.5
+     * -> 3.7. */
+    const bool wide = C > 1024;
+    const dim3 grid((unsigned)(wide ? rows : (rows + 3) / 4)), block(256);
     const hipStream_t s = stream_of(o->ocl);
 
     prof_scope ps(o->ocl, "quant_rows");
-#define QUANT_LAUNCH(NV_, VEC_)                                                          \
-    hipLaunchKernelGGL((quant_rows_kernel<NV_, VEC_>), grid, block, 0, s, X, ldx, rows, C, \
+#define QUANT_LAUNCH(NV_, W_)                                                               \
+    hipLaunchKernelGGL((quant_rows_kernel<NV_, W_>), grid, block, 0, s, X, ldx, rows, C,    \
                        (unsigned *)Q, S)
-    if (!vec)
-        QUANT_LAUNCH(0, false);
-    else if (C <= 256)
-        QUANT_LAUNCH(1, true);
+    if (C <= 256)
+        QUANT_LAUNCH(1, 1);
     else if (C <= 1024)
-        QUANT_LAUNCH(4, true);
+        QUANT_LAUNCH(4, 1);
     else if (C <= 4096)
-        QUANT_LAUNCH(16, true);
+        QUANT_LAUNCH(4, 4);
+    else if (C <= 16384)
+        QUANT_LAUNCH(16, 4);
     else
-        QUANT_LAUNCH(0, true);
+        QUANT_LAUNCH(0, 4);
 #undef QUANT_LAUNCH
     launch_check("quant_rows");
 }
@@ -153,69 +154,115 @@ struct q8_args {
     float slope;
 };
 
-/* act(sa sb sum + bias) + r, the sum converted once. */
-__device__ __forceinline__ float q8_out(const q8_args &g, int sum, float sa, float sb, float b,
-                                        float r)
+/* v times the normal distribution's integral to v: max(v, 0) - |v| g(|v|), g(z)
+ * = erfc(z / sqrt 2) / 2 = exp(-z^2 / 2) f(1 / (1 + 0.4 z / sqrt 2)), f a
+ * polynomial of degree 6 fitted to exp(x^2) erfc(x) / 2 (its error times
+ * exp(-x^2) at most 2e-8): within 4 2^-24 |v|, 15 instructions and no branch, where
+ * erff takes both sides of one (64 outputs a lane are the layer's epilogue). */
+__device__ __forceinline__ float q8_gelu(float v)
 {
-#pragma clang fp contract(off)
-    const float v = icoreg_act((sa * sb) * (float)sum + b, g.act, g.slope);
+    const float t = __builtin_amdgcn_rcpf(fmaf(fabsf(v), 0.282842712f, 1.0f));
+    const float e = __builtin_amdgcn_exp2f(v * -0.72134752f * v);
+    float p = fmaf(t, -1.036704183e-01f, 3.702977300e-01f);
 
-    return g.R ? v + r : v;
+    p = fmaf(t, p, -2.139942795e-01f);
+    p = fmaf(t, p, 2.611404359e-01f);
+    p = fmaf(t, p, 6.693785638e-02f);
+    p = fmaf(t, p, 1.196817234e-01f);
+    p = fmaf(t, p, -3.930720559e-04f);
+    return fmaf(-fabsf(v), e * p, fmaxf(v, 0.0f));
 }
 
-/* Blocks of BM x BN outputs, WM x WN waves, 128 bytes of both panels a step
- * by LDS DMA, two steps in flight, one barrier a step; rows hold their eight
- * 16-byte chunks in the order chunk ^ (row / 2 % 8), which spreads the rows
- * that a matrix instruction reads over the banks. v_mfma_i32_32x32x32_i8: lane
- * half h takes bytes 16 h .. of 32 of row lane % 32 of either operand. Columns
- * past a row's pitch, rows past M and N are outside the panels' windows and
- * read as zeros. */
-template <int BM, int BN, int WM, int WN>
-__global__ void __launch_bounds__(64 * WM * WN) q8_gemm(const q8_args g)
+/* The tanh form: 0.5 v (1 + tanh w) = v / (1 + exp(-2 w)). */
+__device__ __forceinline__ float q8_gelu_tanh(float v)
 {
-    constexpr int NT = 64 * WM * WN, BK = 128;
+    const float w = 0.79788456080286536f * fmaf(0.044715f * v * v, v, v);
+
+    return v / (1.0f + __builtin_amdgcn_exp2f(w * -2.88539008f));
+}
+
+/* act(sa sb sum + bias), the sum converted once. ACT: the activation, ACT_LEAKY
+ * for ReLU too (slope 0). */
+template <int ACT>
+__device__ __forceinline__ float q8_out(int sum, float sa, float sb, float b, float slope)
+{
+    const float v = fmaf(sa * sb, (float)sum, b);
+
+    if (ACT == ACT_GELU)
+        return q8_gelu(v);
+    if (ACT == ACT_GELU_TANH)
+        return q8_gelu_tanh(v);
+    if (ACT == ACT_LEAKY)
+        return v >= 0.0f ? v : slope * v;
+    return v;
+}
+
+/* gfx9 s_waitcnt immediate: at most n vector memory operations outstanding,
+ * every LDS read done. */
+constexpr int q8_wait(int n) { return 0x0070 | (n & 15) | (n >> 4) << 14; }
+
+/* Blocks of BM tokens x BN channels, WM x WN waves. 64 bytes of both panels a
+ * step by LDS DMA, four buffers, three steps in flight, one barrier a step:
+ * what is waited for at the top of step k are the loads of step k alone, and
+ * the buffer that step k + 3 then loads into was last read in step k - 1.
+ * Steps past the last load zeros, so that the count of loads stays the same.
+ * Rows hold their four 16-byte chunks in the order chunk ^ (row / 4 % 4),
+ * which spreads the rows that a matrix instruction reads over the banks.
+ * v_mfma_i32_32x32x32_i8 with the channels as rows and the tokens as columns:
+ * lane half h takes bytes 16 h .. of 32 of row lane % 32 of either operand, and
+ * a lane's sums are four runs of four neighbouring channels of one token,
+ * stored 16 bytes at a time. Operands of the next 32 bytes are read while
+ * this one's products run. Rows past M and N are outside the panels' windows
+ * and read as zeros. */
+template <int BM, int BN, int WM, int WN, int BK, int KS, int ST, int ACT>
+__global__ void __launch_bounds__(64 * WM * WN * KS) q8_gemm(const q8_args g)
+{
+    constexpr int NT = 64 * WM * WN * KS, CH = BK / 16, KK = BK / 32 / KS;
     constexpr int TM = BM / WM / 32, TN = BN / WN / 32;
-    constexpr int ASZ = BM * BK, BSZ = BN * BK;
+    constexpr int ASZ = BM * BK, BSZ = BN * BK, SZ = ASZ + BSZ;
     constexpr int AL = ASZ / 16 / NT, BL = BSZ / 16 / NT;
     static_assert(AL >= 1 && BL >= 1 && ASZ % (16 * NT) == 0 && BSZ % (16 * NT) == 0, "tile shape");
-    __shared__ __align__(16) signed char lds[2 * (ASZ + BSZ)];
-    signed char *const A0 = lds, *const B0 = lds + ASZ, *const A1 = lds + ASZ + BSZ,
-                      *const B1 = lds + 2 * ASZ + BSZ;
+    __shared__ __align__(16) signed char s0[SZ], s1[SZ], s2[ST > 2 ? SZ : 16],
+        s3[ST > 3 ? SZ : 16];
 
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int wm = wave / WN, wn = wave % WN, h = lane >> 5, r32 = lane & 31;
-    const int tiles_n = (g.N + BN - 1) / BN;
-    const int tile = xcd_tile(blockIdx.x, gridDim.x);
-    const int m0 = (tile / tiles_n) * BM, n0 = (tile % tiles_n) * BN;
+    const int kg = wave / (WM * WN), wm = wave / WN % WM, wn = wave % WN;
+    const int h = lane >> 5, r32 = lane & 31;
+    /* Bands of 4 rows of tiles, so that the tiles in flight on an XCD share
+     * rows of both operands. */
+    const int tiles_n = (g.N + BN - 1) / BN, tiles_m = (g.M + BM - 1) / BM;
+    const int tile = xcd_tile(blockIdx.x, gridDim.x), band = tile / (4 * tiles_n);
+    const int in_band = tile - band * 4 * tiles_n, high = min(4, tiles_m - 4 * band);
+    const int m0 = (4 * band + in_band % high) * BM, n0 = in_band / high * BN;
     const int pitch = (int)g.pitch;
     const signed char *A = g.A + m0 * g.pitch, *B = g.B + n0 * g.pitch;
     const long long abytes = min(BM, g.M - m0) * g.pitch, bbytes = min(BN, g.N - n0) * g.pitch;
     int aoff[AL], boff[BL], ak[AL], bk[BL];
-    q8_i16 acc[TM][TN];
+    q8_i16 acc[TN][TM];
 
 #pragma unroll
-    for (int i = 0; i < TM; i++)
+    for (int i = 0; i < TN; i++)
 #pragma unroll
-        for (int j = 0; j < TN; j++)
+        for (int j = 0; j < TM; j++)
 #pragma unroll
             for (int r = 0; r < 16; r++)
                 acc[i][j][r] = 0;
 #pragma unroll
     for (int q = 0; q < AL; q++) {
-        const int sl = tid + NT * q, row = sl / 8;
+        const int sl = tid + NT * q, row = sl / CH;
 
-        ak[q] = 16 * ((sl % 8) ^ ((row >> 1) & 7));
+        ak[q] = 16 * ((sl % CH) ^ (row / (16 / CH) % CH));
         aoff[q] = row * pitch + ak[q];
     }
 #pragma unroll
     for (int q = 0; q < BL; q++) {
-        const int sl = tid + NT * q, row = sl / 8;
+        const int sl = tid + NT * q, row = sl / CH;
 
-        bk[q] = 16 * ((sl % 8) ^ ((row >> 1) & 7));
+        bk[q] = 16 * ((sl % CH) ^ (row / (16 / CH) % CH));
         boff[q] = row * pitch + bk[q];
     }
-    auto load = [&](int k0, signed char *__restrict__ As, signed char *__restrict__ Bs) {
+    auto load = [&](int k0, signed char *s) {
         const __amdgpu_buffer_rsrc_t ra = gemm_rsrc((const float *)A, abytes);
         const __amdgpu_buffer_rsrc_t rb = gemm_rsrc((const float *)B, bbytes);
 
@@ -224,7 +271,7 @@ __global__ void __launch_bounds__(64 * WM * WN) q8_gemm(const q8_args g)
             const unsigned off = k0 + ak[q] < pitch ? (unsigned)(aoff[q] + k0) : GEMM_OOB;
 
             __builtin_amdgcn_raw_ptr_buffer_load_lds(
-                ra, (__attribute__((address_space(3))) void *)(As + 16 * (NT * q + 64 * wave)), 16,
+                ra, (__attribute__((address_space(3))) void *)(s + 16 * (NT * q + 64 * wave)), 16,
                 (int)off, 0, 0, 0);
         }
 #pragma unroll
@@ -232,109 +279,444 @@ __global__ void __launch_bounds__(64 * WM * WN) q8_gemm(const q8_args g)
             const unsigned off = k0 + bk[q] < pitch ? (unsigned)(boff[q] + k0) : GEMM_OOB;
 
             __builtin_amdgcn_raw_ptr_buffer_load_lds(
-                rb, (__attribute__((address_space(3))) void *)(Bs + 16 * (NT * q + 64 * wave)), 16,
+                rb, (__attribute__((address_space(3))) void *)(s + ASZ + 16 * (NT * q + 64 * wave)), 16,
                 (int)off, 0, 0, 0);
         }
     };
-    auto compute = [&](const signed char *__restrict__ As, const signed char *__restrict__ Bs) {
+    auto read = [&](const signed char *s, int kk, q8_i4 (&a)[TM], q8_i4 (&b)[TN]) {
 #pragma unroll
-        for (int kk = 0; kk < BK / 32; kk++) {
-            q8_i4 a[TM], b[TN];
+        for (int j = 0; j < TM; j++) {
+            const int row = wm * (BM / WM) + j * 32 + r32;
 
-#pragma unroll
-            for (int i = 0; i < TM; i++) {
-                const int row = wm * (BM / WM) + i * 32 + r32;
-
-                a[i] = *(const q8_i4 *)(As + row * BK + 16 * ((2 * kk + h) ^ ((row >> 1) & 7)));
-            }
-#pragma unroll
-            for (int j = 0; j < TN; j++) {
-                const int row = wn * (BN / WN) + j * 32 + r32;
-
-                b[j] = *(const q8_i4 *)(Bs + row * BK + 16 * ((2 * kk + h) ^ ((row >> 1) & 7)));
-            }
-#pragma unroll
-            for (int i = 0; i < TM; i++)
-#pragma unroll
-                for (int j = 0; j < TN; j++)
-                    acc[i][j] =
-                        __builtin_amdgcn_mfma_i32_32x32x32_i8(a[i], b[j], acc[i][j], 0, 0, 0);
+            a[j] = *(const q8_i4 *)(s + row * BK + 16 * ((2 * (KK * kg + kk) + h) ^ (row / (16 / CH) % CH)));
         }
+#pragma unroll
+        for (int i = 0; i < TN; i++) {
+            const int row = wn * (BN / WN) + i * 32 + r32;
+
+            b[i] = *(const q8_i4 *)(s + ASZ + row * BK + 16 * ((2 * (KK * kg + kk) + h) ^ (row / (16 / CH) % CH)));
+        }
+    };
+    auto multiply = [&](const q8_i4 (&a)[TM], const q8_i4 (&b)[TN]) {
+#pragma unroll
+        for (int i = 0; i < TN; i++)
+#pragma unroll
+            for (int j = 0; j < TM; j++)
+                acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(b[i], a[j], acc[i][j], 0, 0, 0);
     };
     const int nk = (pitch + BK - 1) / BK;
-    auto step = [&](int kt, const signed char *__restrict__ Ac, const signed char *__restrict__ Bc,
-                    signed char *__restrict__ An, signed char *__restrict__ Bn) {
-        if (kt + 1 < nk)
-            load((kt + 1) * BK, An, Bn);
-        compute(Ac, Bc);
-        __builtin_amdgcn_s_waitcnt(GEMM_WAIT_VM0);
-        __syncthreads();
+    q8_i4 a[2][TM], b[2][TN];
+    /* One operand read, one product, and so on; the loads behind them. */
+    auto mix = [&]() {
+#pragma unroll
+        for (int e = 0; e < TM + TN; e++) {
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            if (e < TM * TN)
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        }
     };
+    auto meet = [&](auto n) {
+        __builtin_amdgcn_s_waitcnt(q8_wait(decltype(n)::value * (AL + BL)));
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+    auto step = [&](int kt, signed char *now, const signed char *next) {
+#pragma unroll
+        for (int kk = 0; kk < KK; kk++) {
+            if (kk + 1 < KK)
+                read(now, kk + 1, a[(kk + 1) & 1], b[(kk + 1) & 1]);
+            else {
+                meet(std::integral_constant<int, ST - 2>());
+                load((kt + ST) * BK, now);
+                read(next, 0, a[0], b[0]);
+            }
+            multiply(a[kk & 1], b[kk & 1]);
+            mix();
+        }
+    };
+    static_assert(KK % 2 == 0, "operands alternate");
 
-    load(0, A0, B0);
-    __builtin_amdgcn_s_waitcnt(GEMM_WAIT_VM0);
-    __syncthreads();
-    for (int kt = 0; kt < nk; kt += 2) {
-        step(kt, A0, B0, A1, B1);
+    load(0, s0);
+    load(BK, s1);
+    if (ST > 2)
+        load(2 * BK, s2);
+    if (ST > 3)
+        load(3 * BK, s3);
+    meet(std::integral_constant<int, ST - 1>());
+    read(s0, 0, a[0], b[0]);
+    for (int kt = 0; kt < nk; kt += ST) {
+        step(kt, s0, s1);
         if (kt + 1 < nk)
-            step(kt + 1, A1, B1, A0, B0);
+            step(kt + 1, s1, ST > 2 ? s2 : s0);
+        if (ST > 2 && kt + 2 < nk)
+            step(kt + 2, s2, ST > 3 ? s3 : s0);
+        if (ST > 3 && kt + 3 < nk)
+            step(kt + 3, s3, s0);
+    }
+    __builtin_amdgcn_s_waitcnt(q8_wait(0));
+    if constexpr (KS > 1) {
+        /* Two groups of waves have summed halves of every step: each takes
+         * the other's sums of half its channels and finishes those. */
+        static_assert(KS == 2 && TN % 2 == 0 && WM * WN * (TN / 2) * TM * 4096 <= SZ, "exchange");
+        const int w = (wm * WN + wn) * (TN / 2) * TM;
+        q8_i4 *out = (q8_i4 *)(kg ? s0 : s1) + w * 256 + lane;
+        const q8_i4 *in = (const q8_i4 *)(kg ? s1 : s0) + w * 256 + lane;
+
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < TN / 2; i++)
+#pragma unroll
+            for (int j = 0; j < TM; j++)
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    const q8_i16 &x = kg ? acc[i][j] : acc[i + TN / 2][j];
+
+                    out[((i * TM + j) * 4 + q) * 64] =
+                        q8_i4{x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]};
+                }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < TN / 2; i++)
+#pragma unroll
+            for (int j = 0; j < TM; j++) {
+                if (kg)
+                    acc[i][j] = acc[i + TN / 2][j];
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    const q8_i4 y = in[((i * TM + j) * 4 + q) * 64];
+
+#pragma unroll
+                    for (int r = 0; r < 4; r++)
+                        acc[i][j][4 * q + r] += y[r];
+                }
+            }
     }
 
-    /* Register r of a 32 x 32 tile: row (r / 4) * 8 + 4 h + r % 4, column
-     * lane % 32. Loads before stores: C may be R. */
+    /* Register r of a tile: channel (r / 4) * 8 + 4 h + r % 4, token lane % 32.
+     * Loads before stores: C may be R. */
 #pragma unroll
-    for (int j = 0; j < TN; j++) {
-        const int n = n0 + wn * (BN / WN) + j * 32 + r32;
-        const float sb = g.sb[min(n, g.N - 1)];
-        const float b = g.bias ? g.bias[min(n, g.N - 1)] : 0.0f;
+    for (int i = 0; i < TN / KS; i++) {
+        const int n = n0 + wn * (BN / WN) + (i + kg * (TN / 2)) * 32 + 4 * h;
+        float sb[16], b[16];
 
 #pragma unroll
-        for (int i = 0; i < TM; i++) {
-            const int ri = m0 + wm * (BM / WM) + i * 32 + 4 * h;
-            float sa[16], x[16];
+        for (int r = 0; r < 16; r++) {
+            const int at = min(n + (r >> 2) * 8 + (r & 3), g.N - 1);
+
+            sb[r] = g.sb[at];
+            b[r] = g.bias ? g.bias[at] : 0.0f;
+        }
+#pragma unroll
+        for (int j = 0; j < TM; j++) {
+            const int m = m0 + wm * (BM / WM) + j * 32 + r32;
+            const float sa = g.sa[min(m, g.M - 1)];
+            float *c = g.C + m * g.ldc + n;
+            const float *x = g.R + m * g.ldc + n;
+            float v[16];
 
 #pragma unroll
-            for (int r = 0; r < 16; r++) {
-                const int m = min(ri + (r >> 2) * 8 + (r & 3), g.M - 1);
-
-                sa[r] = g.sa[m];
-                x[r] = g.R && n < g.N ? g.R[m * g.ldc + n] : 0.0f;
-            }
+            for (int r = 0; r < 16; r++)
+                v[r] = q8_out<ACT>(acc[i][j][r], sa, sb[r], b[r], g.slope);
+            if (m >= g.M)
+                continue;
 #pragma unroll
-            for (int r = 0; r < 16; r++) {
-                const int m = ri + (r >> 2) * 8 + (r & 3);
+            for (int q = 0; q < 4; q++) {
+                const int left = g.N - n - 8 * q;
+                float *y = v + 4 * q;
 
-                if (m < g.M && n < g.N)
-                    g.C[m * g.ldc + n] = q8_out(g, acc[i][j][r], sa[r], sb, b, x[r]);
+                if (left >= 4) {
+                    float old[4] = {0, 0, 0, 0};
+
+                    if (g.R)
+                        load4(x + 8 * q, old);
+                    store4(c + 8 * q, y[0] + old[0], y[1] + old[1], y[2] + old[2], y[3] + old[3]);
+                }
+                else
+                    for (int r = 0; r < left; r++)
+                        c[8 * q + r] = g.R ? y[r] + x[8 * q + r] : y[r];
             }
         }
     }
 }
 
-template <int BM, int BN, int WM, int WN> static void q8_launch(const q8_args &g, hipStream_t s)
-{
-    const long long tiles = (long long)((g.M + BM - 1) / BM) * ((g.N + BN - 1) / BN);
+/* Few tokens: what counts is the weights' bytes and the latency. Blocks of 16
+ * channels x 16 TT tokens, 64 bytes of the sum (one matrix instruction) a wave
+ * and turn, the 8 waves' sums joined in LDS. Both operands come straight from
+ * memory: 4 lanes read 64 bytes of a row. FUSED: every block codes its tokens
+ * itself, into LDS (rows 16 bytes further apart, so that 16 of them spread
+ * over the banks), while its first weights are on their way. */
+#define Q8_SW 8              /* waves */
+#define Q8_FUSED_BYTES 40960 /* codes in LDS */
 
-    hipLaunchKernelGGL((q8_gemm<BM, BN, WM, WN>), dim3((unsigned)count32(tiles, "q8 tiles")),
-                       dim3(64 * WM * WN), 0, s, g);
+template <int TT, bool FUSED, int ACT>
+__global__ void __launch_bounds__(64 * Q8_SW)
+    q8_skinny(const q8_args g, const float *__restrict__ X, long long ldx, int in)
+{
+    constexpr int AHEAD = 4;
+    __shared__ __align__(16) signed char xs[FUSED ? Q8_FUSED_BYTES : 16];
+    __shared__ q8_i4 sums[Q8_SW][TT][64];
+    __shared__ unsigned tops[16 * TT][Q8_SW];
+    __shared__ float scales[16 * TT];
+    const int tid = threadIdx.x, lane = tid & 63, c16 = lane & 15, part = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int tiles_n = (g.N + 15) / 16, pitch = (int)g.pitch, nk = pitch / 64;
+    const int n0 = blockIdx.x % tiles_n * 16, m0 = blockIdx.x / tiles_n * 16 * TT;
+    const signed char *w = g.B + (long long)min(n0 + c16, g.N - 1) * pitch + 16 * part;
+    q8_i4 a[AHEAD], acc[TT];
+
+#pragma unroll
+    for (int t = 0; t < TT; t++)
+        acc[t] = q8_i4{0, 0, 0, 0};
+#pragma unroll
+    for (int e = 0; e < AHEAD; e++)
+        a[e] = *(const q8_i4 *)(w + 64 * min(wave + Q8_SW * e, nk - 1));
+    if constexpr (FUSED) {
+        /* 1, 2, 4 or 8 waves a token. */
+        const int tokens = min(16 * TT, g.M - m0);
+        const int each = tokens > 4 ? 1 : tokens > 2 ? 2 : tokens > 1 ? 4 : 8;
+        const int first = wave / each, sub = wave % each, step = 64 * each;
+
+        for (int m = first; m < tokens; m += Q8_SW / each) {
+            const float *x = X + (m0 + m) * ldx;
+            unsigned top = 0;
+
+            for (int c = sub * 64 + lane; 4 * c < in; c += step) {
+                float v[4];
+
+                load4_row(x, 4 * c, in, v);
+                top = max(max(max(q8_mag(v[0]), q8_mag(v[1])), max(q8_mag(v[2]), q8_mag(v[3]))),
+                          top);
+            }
+            top = wave_umax(top);
+            if (lane == 0)
+                tops[m][sub] = top;
+        }
+        __syncthreads();
+        for (int m = first; m < tokens; m += Q8_SW / each) {
+            const float *x = X + (m0 + m) * ldx;
+            unsigned *out = (unsigned *)(xs + m * (pitch + 16));
+            unsigned top = 0;
+
+            for (int e = 0; e < each; e++)
+                top = max(top, tops[m][e]);
+            const q8_scale q = q8_scale_of(top);
+
+            for (int c = sub * 64 + lane; c < pitch / 4; c += step) {
+                float v[4];
+
+                load4_row(x, 4 * c, in, v);
+                out[c] = q8_code4(v[0], v[1], v[2], v[3], q.r);
+            }
+            if (sub == 0 && lane == 0)
+                scales[m] = q.s;
+        }
+        __syncthreads();
+    }
+    for (int k = wave; k < nk; k += Q8_SW * AHEAD) {
+        q8_i4 now[AHEAD];
+
+#pragma unroll
+        for (int e = 0; e < AHEAD; e++) {
+            now[e] = a[e];
+            a[e] = *(const q8_i4 *)(w + 64 * min(k + Q8_SW * (AHEAD + e), nk - 1));
+        }
+#pragma unroll
+        for (int e = 0; e < AHEAD; e++) {
+            const int kk = k + Q8_SW * e;
+
+            if (kk < nk) {
+#pragma unroll
+                for (int t = 0; t < TT; t++) {
+                    const int m = min(16 * t + c16, g.M - 1 - m0);
+                    const signed char *x = FUSED ? xs + m * (pitch + 16)
+                                                 : g.A + (long long)(m0 + m) * pitch;
+                    const q8_i4 b = *(const q8_i4 *)(x + 64 * kk + 16 * part);
+
+                    acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(now[e], b, acc[t], 0, 0, 0);
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < TT; t++)
+        sums[wave][t][lane] = acc[t];
+    __syncthreads();
+    /* Sum r of lane l: channel 4 (l / 16) + r, token l % 16. Outputs in the
+     * order of memory, a run of 16 channels a token. */
+    for (int e = tid; e < 256 * TT; e += 64 * Q8_SW) {
+        const int n = n0 + e % 16, tok = e / 16, m = m0 + tok;
+        const int l = e % 16 / 4 * 16 + tok % 16;
+        int v = 0;
+
+#pragma unroll
+        for (int q = 0; q < Q8_SW; q++)
+            v += ((const int *)&sums[q][tok / 16][l])[e % 4];
+        if (n < g.N && m < g.M) {
+            const float sa = FUSED ? scales[tok] : g.sa[m];
+            const float y = q8_out<ACT>(v, sa, g.sb[n], g.bias ? g.bias[n] : 0.0f, g.slope);
+
+            g.C[m * g.ldc + n] = g.R ? y + g.R[m * g.ldc + n] : y;
+        }
+    }
 }
 
-static void q8_product(struct ops *o, const q8_args &g)
+template <int TT, bool FUSED>
+static void q8_skinny_launch(const q8_args &g, const float *X, long long ldx, int in, hipStream_t s)
+{
+    const long long tiles = (long long)((g.N + 15) / 16) * ((g.M + 16 * TT - 1) / (16 * TT));
+    const dim3 grid((unsigned)count32(tiles, "q8 tiles")), block(64 * Q8_SW);
+
+    switch (g.act) {
+    case ACT_GELU:
+        hipLaunchKernelGGL((q8_skinny<TT, FUSED, ACT_GELU>), grid, block, 0, s, g, X, ldx, in);
+        break;
+    case ACT_GELU_TANH:
+        hipLaunchKernelGGL((q8_skinny<TT, FUSED, ACT_GELU_TANH>), grid, block, 0, s, g, X, ldx, in);
+        break;
+    case ACT_LEAKY:
+        hipLaunchKernelGGL((q8_skinny<TT, FUSED, ACT_LEAKY>), grid, block, 0, s, g, X, ldx, in);
+        break;
+    default:
+        hipLaunchKernelGGL((q8_skinny<TT, FUSED, ACT_NONE>), grid, block, 0, s, g, X, ldx, in);
+    }
+}
+
+template <int BM, int BN, int WM, int WN, int BK, int KS, int ST> static void q8_launch(const q8_args &g, hipStream_t s)
+{
+    const long long tiles = (long long)((g.M + BM - 1) / BM) * ((g.N + BN - 1) / BN);
+    const dim3 grid((unsigned)count32(tiles, "q8 tiles")), block(64 * WM * WN * KS);
+    switch (g.act) {
+    case ACT_GELU:
+        hipLaunchKernelGGL((q8_gemm<BM, BN, WM, WN, BK, KS, ST, ACT_GELU>), grid, block, 0, s, g);
+        break;
+    case ACT_GELU_TANH:
+        hipLaunchKernelGGL((q8_gemm<BM, BN, WM, WN, BK, KS, ST, ACT_GELU_TANH>), grid, block, 0, s, g);
+        break;
+    case ACT_LEAKY:
+        hipLaunchKernelGGL((q8_gemm<BM, BN, WM, WN, BK, KS, ST, ACT_LEAKY>), grid, block, 0, s, g);
+        break;
+    default:
+        hipLaunchKernelGGL((q8_gemm<BM, BN, WM, WN, BK, KS, ST, ACT_NONE>), grid, block, 0, s, g);
+    }
+}
+
+/* The kernels, and what a launch takes on 256 CUs: us = fixed + c (tile +
+ * sum in / 1024), c the tiles of a CU (its rounds where a CU holds one), from
+ * times of 8 .. 12805 tokens on 256 .. 4096 channels of either side. Both
+ * sides of some borders, us: 400 x 256 x 256 skinny 3.4, 64 x 64 tiles 4.7;
+ * 64 x 1024 x 4096 7.9, 6.5; 785 x 1024 x 1024 64 x 64 7.1, 128 x 128 10.2;
+ * 3202 x 1024 x 1024 15.5, 12.5; 6400 x 1024 x 1024 128 x 128 21.1, 256 x 128
+ * 18.3; 3202 x 1024 x 4096 256 x 128 33.6, 256 x 256 27.8; 3202 x 4096 x 4096
+ * 72.8, 65.4. */
+enum { Q8_256, Q8_256_128, Q8_128, Q8_64, Q8_SKINNY2, Q8_SKINNY1, Q8_FORMS };
+
+static const struct q8_form {
+    int bm, bn;
+    float fixed, tile, sum;
+} q8_forms[Q8_FORMS] = {{256, 256, 2.0f, 12.0f, 12.3f}, {256, 128, 2.0f, 9.5f, 6.5f},
+                        {128, 128, 2.0f, 6.5f, 3.9f},   {64, 64, 4.4f, 1.4f, 1.9f},
+                        {32, 16, 2.2f, 1.7f, 1.25f},    {16, 16, 2.2f, 1.4f, 0.95f}};
+
+static float q8_cost(int form, int M, int N, int pitch, int cus)
+{
+    const q8_form &f = q8_forms[form];
+    const long long tiles = (long long)((M + f.bm - 1) / f.bm) * ((N + f.bn - 1) / f.bn);
+
+    return f.fixed + (float)((tiles + cus - 1) / cus) * (f.tile + f.sum * pitch / 1024.0f);
+}
+
+static int q8_best(int M, int N, int pitch, int cus, float &cost)
+{
+    int best = 0;
+
+    for (int i = 0; i < Q8_FORMS; i++) {
+        const float c = q8_cost(i, M, N, pitch, cus);
+
+        if (i == 0 || c < cost) {
+            best = i;
+            cost = c;
+        }
+    }
+    return best;
+}
+
+/* The kernel of M tokens, and how many of them it takes: a last round of few
+ * large tiles leaves most CUs waiting (12805 x 4096 x 4096: 816 tiles of 256 x
+ * 256, 48 of them alone in a fourth round, 244 us), so its tokens may go to
+ * another kernel (12288 tokens, then 517 in tiles of 128 x 128: 234 us). */
+static int q8_choose(int M, int N, int pitch, int cus, int &rows)
+{
+    float cost = 0.0f;
+    int best = q8_best(M, N, pitch, cus, cost);
+
+    rows = M;
+    for (int i = Q8_256; i <= Q8_256_128; i++) {
+        const long long tn = (N + q8_forms[i].bn - 1) / q8_forms[i].bn;
+        const long long rounds = ((M + q8_forms[i].bm - 1) / q8_forms[i].bm) * tn / cus;
+        const long long m = rounds * cus / tn * q8_forms[i].bm;
+        float rest = 0.0f;
+
+        if (m <= 0 || m >= M)
+            continue;
+        (void)q8_best(M - (int)m, N, pitch, cus, rest);
+        rest += q8_cost(i, (int)m, N, pitch, cus);
+        if (rest < cost) {
+            cost = rest;
+            best = i;
+            rows = (int)m;
+        }
+    }
+    return best;
+}
+
+static void q8_product(struct ops *o, q8_args g)
 {
     const hipStream_t s = stream_of(o->ocl);
-    const long long cus = o->ocl->cu_count;
-    auto tiles = [&](int bm, int bn) {
-        return (long long)((g.M + bm - 1) / bm) * ((g.N + bn - 1) / bn);
-    };
+    const int M = g.M;
 
     prof_scope ps(o->ocl, "gemm_q8");
-    if (tiles(256, 256) >= 2 * cus)
-        q8_launch<256, 256, 2, 4>(g, s);
-    else if (tiles(128, 128) >= cus / 2)
-        q8_launch<128, 128, 2, 2>(g, s);
-    else
-        q8_launch<64, 64, 2, 2>(g, s);
-    launch_check("gemm_q8");
+    for (int m = 0; m < M; m += g.M) {
+        const int form = q8_choose(M - m, g.N, (int)g.pitch, o->ocl->cu_count, g.M);
+
+        switch (form) {
+        case Q8_256:
+            q8_launch<256, 256, 2, 4, 128, 1, 2>(g, s);
+            break;
+        case Q8_256_128:
+            q8_launch<256, 128, 4, 2, 128, 1, 3>(g, s);
+            break;
+        case Q8_128:
+            q8_launch<128, 128, 2, 2, 128, 2, 3>(g, s);
+            break;
+        case Q8_64:
+            q8_launch<64, 64, 2, 2, 128, 1, 3>(g, s);
+            break;
+        case Q8_SKINNY2:
+            q8_skinny_launch<2, false>(g, nullptr, 0, 0, s);
+            break;
+        default:
+            q8_skinny_launch<1, false>(g, nullptr, 0, 0, s);
+        }
+        launch_check("gemm_q8");
+        g.A += g.M * g.pitch;
+        g.sa += g.M;
+        g.C += g.M * g.ldc;
+        if (g.R)
+            g.R += g.M * g.ldc;
+    }
+}
+
+extern "C" int icoreg_q8_choice(struct ops *o, int rows, int in, int out, int *first)
+{
+    int n = 0, form;
+
+    if (rows < 1 || in < 1 || in > Q8_MAX_IN || out < 1)
+        return -1;
+    form = q8_choose(rows, out, (int)q8_pitch(in), o->ocl->cu_count, n);
+    if (first)
+        *first = n;
+    return form;
 }
 
 /* The checks of both calls and the arguments of the product, its first
@@ -371,8 +753,8 @@ static q8_args q8_make(const char *op, int rows, int in, int out, cl_mem WQ, cl_
     g.R = R ? cfptr(R) + roff : nullptr;
     g.C = fptr(Y) + yoff;
     g.ldc = ldy;
-    g.act = act;
-    g.slope = slope;
+    g.act = act == ACT_RELU ? ACT_LEAKY : act;
+    g.slope = act == ACT_RELU ? 0.0f : slope;
     return g;
 }
 
@@ -427,6 +809,27 @@ extern "C" void ops_linear_q8(struct ops *o, int rows, int in, int out, cl_mem X
     need_apart(Y, yoff * 4, ybytes, X, xoff * 4, xbytes, op, "Y and X");
     g.A = (const signed char *)work->ptr;
     g.sa = (const float *)((const char *)work->ptr + codes);
+    {
+        /* One launch where coding its tokens costs a block little: against
+         * two, us a call, 1 x 1024 x 4096 4.9, 7.4; 32 x 256 x 256 4.9, 7.3;
+         * 16 x 1024 x 1024 7.2, 7.4; 400 x 256 x 512 (two blocks a CU) 8.6, 7.3;
+         * 16 x 2048 x 1024 9.9, 8.2; a few tokens 4 x 8192 x 1024 14.3, 24.7. */
+        int n = 0;
+        const int form = q8_choose(rows, out, (int)g.pitch, o->ocl->cu_count, n);
+        const int tokens = min(rows, form == Q8_SKINNY2 ? 32 : 16);
+        const long long blocks = (out + 15) / 16 * ((rows + tokens - 1LL) / tokens);
+
+        if (form >= Q8_SKINNY2 && tokens * (g.pitch + 16) <= Q8_FUSED_BYTES &&
+            (rows <= 4 || (tokens * in <= 16384 && blocks <= o->ocl->cu_count))) {
+            prof_scope ps(o->ocl, "linear_q8");
+            if (form == Q8_SKINNY2)
+                q8_skinny_launch<2, true>(g, cfptr(X) + xoff, ldx, in, stream_of(o->ocl));
+            else
+                q8_skinny_launch<1, true>(g, cfptr(X) + xoff, ldx, in, stream_of(o->ocl));
+            launch_check("linear_q8");
+            return;
+        }
+    }
     quant_rows(o, rows, in, cfptr(X) + xoff, ldx, work->ptr, (float *)g.sa);
     q8_product(o, g);
     ICOREG_API_END

@@ -95,6 +95,12 @@ int icoreg_conv_wino_choice(struct ops *o, int nb, int C, int H, int W, int K);
  * ones with the input channels in that many pieces. For tests. */
 int icoreg_gemm_choice(struct ops *o, int M, int N, int K, int b, int nb, int aligned);
 int icoreg_conv5_choice(struct ops *o, int nb, int C, int H, int W, int K, int pad);
+/* The kernel that ops_linear_qq takes for rows x in x out and, in *first (may
+ * be NULL), the rows it takes it for (the rest: what the same call says of
+ * them): 0 tiles of 256 x 256, 1 of 256 x 128, 2 of 128 x 128, 3 of 64 x 64
+ * tokens x channels, 4, 5 blocks of 32, 16 tokens x 16 channels; -1 for sizes
+ * that it refuses. For tests. */
+int icoreg_q8_choice(struct ops *o, int rows, int in, int out, int *first);
 /* How many times roma_match has re-run a GP solve through
  * roma_gp_solve_events after the in-kernel wait gave up. */
 int icoreg_roma_gp_retries(const struct roma_model *m);

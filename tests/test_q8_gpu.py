@@ -81,7 +81,9 @@ SHAPES = [
     (16, 320, 77, 0, 1, 2, 2), (17, 1000, 256, 1, 1, 0, 0), (64, 192, 64, 0, 1, 0, 0), (65, 128, 65, 0, 0, 1, 1),
     (127, 300, 129, 2, 1, 0, 0), (400, 256, 256, 0, 0, 0, 0), (333, 517, 1001, 4, 1, 1, 5),
     (1601, 1024, 1024, 0, 1, 2, 0), (785, 2048, 900, 1, 1, 0, 0), (3202, 1024, 2049, 0, 1, 0, 0),
-    (6000, 320, 6100, 0, 1, 0, 0)]
+    (6000, 320, 6100, 0, 1, 0, 0), (4000, 100, 4097, 0, 1, 1, 3), (6400, 192, 1024, 1, 1, 0, 0),
+    (3100, 260, 1028, 0, 0, 1, 4), (40, 700, 530, 1, 1, 2, 2), (9000, 64, 1000, 0, 1, 0, 0),
+    (60, 300, 4100, 1, 1, 0, 4), (200, 4096, 1500, 0, 0, 0, 0)]
 
 
 def operands(shape, seed=0):
@@ -111,6 +113,18 @@ def strided(dev, y, off, ld, fill=7.0):
     view = host[off:off + rows * ld].reshape(rows, ld)
     view[:, :n] = y
     return dev.upload(host)
+
+
+def test_every_kernel_is_among_the_shapes(dev, ic):
+    """The shapes below reach every kernel, and one is cut by tokens."""
+    got, cut = set(), 0
+    for rows, cin, cout, *_ in SHAPES:
+        while rows:
+            n = ic.C.c_int()
+            got.add(ic.lib().icoreg_q8_choice(dev.po, rows, cin, cout, ic.C.byref(n)))
+            cut += n.value < rows
+            rows -= n.value
+    assert got == set(range(6)) and cut
 
 
 @pytest.mark.parametrize("entry", ["q8", "qq"])
