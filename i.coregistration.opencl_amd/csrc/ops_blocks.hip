@@ -24,6 +24,7 @@
 #include <math.h>
 
 #include "common.h"
+#include "load4.h"
 #include "ops.h"
 #include "q8.h"
 #include "split.h"
@@ -301,82 +302,95 @@ __device__ __forceinline__ void sel_top(const int (&k)[N], const int (&i)[N], in
     __builtin_amdgcn_wave_barrier();
 }
 
-#define SEL_SLOTS 8 /* scores a lane holds at a time */
+/* What a selection reads, and where it writes. */
+struct sel_args {
+    const float *Q;
+    const signed char *KC;
+    const float *KS;
+    int *SEL;
+    long long ldq;
+    int Nq, nh, nhk, d, nblk, top;
+};
 
-/* A block of W waves selects for one query and head: every wave scores its
- * share of the key blocks, lane by lane, SEL_SLOTS x 64 at a time, and keeps
- * the best so far beside the next ones; wave 0 selects among the waves'. */
-template <int W, int DW> /* DW: words of a code row that are not padding */
-__global__ void __launch_bounds__(64 * W)
-    block_select_kernel(const float *__restrict__ Q, long long ldq, int Nq, int nh, int nhk, int d,
-                        const signed char *__restrict__ KC, const float *__restrict__ KS, int nblk,
-                        int top, int *__restrict__ SEL)
+/* A wave selects the best of the blocks b0 .. b1 - 1 for one query and head:
+ * every lane scores blocks of its own, 2 or 4 x 64 at a time, and the best so
+ * far are kept beside the next ones. Sorted results in the lanes, as
+ * sel_top leaves them. codes, list: 128 bytes and words of LDS of this wave.
+ * DW: words of a code row that are not padding. */
+template <int DW>
+__device__ __forceinline__ void sel_row(const sel_args &a, int query, int h, int b0, int b1,
+                                        unsigned char *codes, int *list, int &key, int &idx)
+{
+    constexpr int SLOTS = DW > 16 ? 2 : 4; /* a lane's codes are registers */
+    const int lane = threadIdx.x & 63, kvh = h / (a.nh / a.nhk), c = 2 * lane;
+    const float *q = a.Q + query * a.ldq + (long long)h * a.d;
+    const float x = c < a.d ? q[c] : 0.0f, y = c + 1 < a.d ? q[c + 1] : 0.0f;
+    const q8_scale s = q8_scale_of(wave_umax(max(q8_mag(x), q8_mag(y))));
+    const bool bad = s.s != s.s; /* not finite: NaN everywhere */
+    const long long pitch = q8_pitch(a.d);
+    unsigned qc[DW];
+
+    codes[c] = (unsigned char)q8_code(x, s.r);
+    codes[c + 1] = (unsigned char)q8_code(y, s.r);
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int j = 0; j < DW; j++)
+        qc[j] = __builtin_amdgcn_readfirstlane(((const unsigned *)codes)[j]);
+    key = SEL_NONE;
+    idx = -1;
+    for (; b0 < b1; b0 += 64 * SLOTS) {
+        int k[SLOTS + 1], i[SLOTS + 1];
+        uint4 w[SLOTS][DW / 4];
+        float ks[SLOTS];
+
+        k[0] = key;
+        i[0] = idx;
+#pragma unroll
+        for (int j = 0; j < SLOTS; j++) {
+            const long long at = (long long)min(b0 + 64 * j + lane, b1 - 1) * a.nhk + kvh;
+            const uint4 *p = (const uint4 *)(a.KC + at * pitch);
+
+            ks[j] = a.KS[at];
+#pragma unroll
+            for (int e = 0; e < DW / 4; e++)
+                w[j][e] = p[e];
+        }
+#pragma unroll
+        for (int j = 0; j < SLOTS; j++) {
+            const int b = b0 + 64 * j + lane;
+            int dot = 0;
+
+#pragma unroll
+            for (int e = 0; e < DW / 4; e++) {
+                dot = __builtin_amdgcn_sdot4((int)w[j][e].x, (int)qc[4 * e], dot, false);
+                dot = __builtin_amdgcn_sdot4((int)w[j][e].y, (int)qc[4 * e + 1], dot, false);
+                dot = __builtin_amdgcn_sdot4((int)w[j][e].z, (int)qc[4 * e + 2], dot, false);
+                dot = __builtin_amdgcn_sdot4((int)w[j][e].w, (int)qc[4 * e + 3], dot, false);
+            }
+            i[j + 1] = b;
+            k[j + 1] = b >= b1 || ks[j] < 0.0f ? SEL_NONE
+                                               : bad ? SEL_NAN : sel_key(ks[j] * (float)dot);
+        }
+        sel_top(k, i, a.top, list, key, idx);
+    }
+}
+
+/* A block of W waves for one query and head, each on its share of the key
+ * blocks; wave 0 selects among the waves' best. */
+template <int W, int DW>
+__global__ void __launch_bounds__(64 * W) block_select_kernel(const sel_args a)
 {
     __shared__ int lists[W][128];
     __shared__ __align__(16) unsigned char codes[W][128];
     __shared__ int best[W > 1 ? W * 128 : 1];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int row = blockIdx.x, h = row % nh, kvh = h / (nh / nhk);
-    const float *q = Q + (long long)(row / nh) * ldq + (long long)h * d;
-    const long long pitch = q8_pitch(d);
-    int *list = lists[wave];
-    unsigned qc[DW];
-    int key = SEL_NONE, idx = -1;
+    const int row = blockIdx.x, share = ((a.nblk + W - 1) / W + 63) / 64 * 64;
+    int key, idx;
 
-    {
-        const int c = 2 * lane;
-        const float a = c < d ? q[c] : 0.0f, b = c + 1 < d ? q[c + 1] : 0.0f;
-        const q8_scale s = q8_scale_of(wave_umax(max(q8_mag(a), q8_mag(b))));
-
-        codes[wave][c] = (unsigned char)q8_code(a, s.r);
-        codes[wave][c + 1] = (unsigned char)q8_code(b, s.r);
-        __builtin_amdgcn_wave_barrier();
-#pragma unroll
-        for (int j = 0; j < DW; j++)
-            qc[j] = __builtin_amdgcn_readfirstlane(((const unsigned *)codes[wave])[j]);
-        /* A query that is not finite scores NaN everywhere. */
-        if (s.s != s.s)
-            key = SEL_NAN;
-    }
-    const bool bad = key == SEL_NAN;
-    const int share = ((nblk + W - 1) / W + 63) / 64 * 64;
-    const int b1 = min(nblk, (wave + 1) * share);
-
-    key = SEL_NONE;
-    for (int b0 = wave * share; b0 < b1; b0 += 64 * SEL_SLOTS) {
-        int k[SEL_SLOTS + 1], i[SEL_SLOTS + 1];
-
-        k[0] = key;
-        i[0] = idx;
-#pragma unroll
-        for (int j = 0; j < SEL_SLOTS; j++) {
-            const int b = b0 + 64 * j + lane;
-
-            k[j + 1] = SEL_NONE;
-            i[j + 1] = b;
-            if (b < b1) {
-                const long long at = (long long)b * nhk + kvh;
-                const uint4 *p = (const uint4 *)(KC + at * pitch);
-                const float s = KS[at];
-                int dot = 0;
-
-#pragma unroll
-                for (int w = 0; w < DW / 4; w++) {
-                    const uint4 x = p[w];
-
-                    dot = __builtin_amdgcn_sdot4((int)x.x, (int)qc[4 * w], dot, false);
-                    dot = __builtin_amdgcn_sdot4((int)x.y, (int)qc[4 * w + 1], dot, false);
-                    dot = __builtin_amdgcn_sdot4((int)x.z, (int)qc[4 * w + 2], dot, false);
-                    dot = __builtin_amdgcn_sdot4((int)x.w, (int)qc[4 * w + 3], dot, false);
-                }
-                if (!(s < 0.0f))
-                    k[j + 1] = bad ? SEL_NAN : sel_key(s * (float)dot);
-            }
-        }
-        sel_top(k, i, top, list, key, idx);
-    }
-    if (W > 1) {
+    sel_row<DW>(a, row / a.nh, row % a.nh, wave * share, min(a.nblk, (wave + 1) * share),
+                codes[wave], lists[wave], key, idx);
+    if constexpr (W > 1) {
         best[wave * 64 + lane] = key;
         best[(W + wave) * 64 + lane] = idx;
         __syncthreads();
@@ -389,10 +403,247 @@ __global__ void __launch_bounds__(64 * W)
             k[w] = best[w * 64 + lane];
             i[w] = best[(W + w) * 64 + lane];
         }
-        sel_top(k, i, top, list, key, idx);
+        sel_top(k, i, a.top, lists[0], key, idx);
     }
-    if (lane < top)
-        SEL[(long long)row * top + lane] = key == SEL_NONE ? -1 : idx;
+    if (lane < a.top)
+        a.SEL[(long long)row * a.top + lane] = key == SEL_NONE ? -1 : idx;
+}
+
+/* Many queries on at most 16 T key blocks: a wave takes 16 rows (a query and
+ * head each, of one key head; row r of a key head is query r / g, query head r
+ * % g of its g). v_mfma_i32_16x16x64_i8 with the blocks' codes as rows and the
+ * queries' as columns leaves a row's scores in 4 lanes, 4 T in each, where they
+ * stay. The smallest of the maxima of 16 G / 4 groups, at least top of them, is
+ * reached by top scores; from there the range is halved until no more than CAP
+ * reach the threshold (8 instructions a row and step, where a wave a row
+ * takes 16 and more; mostly 2 or 3 steps). Those go to LDS and are ranked
+ * against each other, ties by their numbers. A query, scale or score that is
+ * not finite, or more equal scores than CAP, sends the wave's rows to sel_row
+ * one by one. */
+#define SEL_TW 4 /* waves */
+
+template <int T, int KCH, int CAP>
+__global__ void __launch_bounds__(64 * SEL_TW, T > 16 ? 2 : T > 4 ? 3 : 4)
+    block_select_tile(const sel_args a)
+{
+    constexpr int OWN = CAP / 4, G = CAP > 24 ? 8 : 4; /* groups of a lane */
+    typedef int i4 __attribute__((ext_vector_type(4)));
+    typedef unsigned long long u64;
+    __shared__ __align__(16) float scale[16 * T], none[16 * T];
+    __shared__ u64 cand[SEL_TW][16][CAP + 1];
+    __shared__ int lists[SEL_TW][128];
+    __shared__ __align__(16) unsigned char codes[SEL_TW][128];
+    const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, part = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int kvh = blockIdx.y, g = a.nh / a.nhk, rows = a.Nq * g;
+    const int r0 = (blockIdx.x * SEL_TW + wave) * 16, r = min(r0 + col, rows - 1);
+    const int query = r / g, h = kvh * g + r % g;
+    const long long pitch = 64 * KCH, row = (long long)query * a.nh + h;
+    i4 q[KCH];
+    bool odd = false;
+
+    /* Scores s (cq . c) + 0, minus infinity for what is no block. */
+    for (int b = tid; b < 16 * T; b += 64 * SEL_TW) {
+        const float k = b < a.nblk ? a.KS[(long long)b * a.nhk + kvh] : -1.0f;
+
+        scale[b] = fmaxf(k, 0.0f);
+        none[b] = k < 0.0f ? -INFINITY : 0.0f;
+        odd = odd || !(k < 1e32f);
+    }
+    odd = __syncthreads_or(odd);
+    if (r0 >= rows)
+        return;
+    /* The query's codes: channels 64 c + 16 part .. + 15 in this lane. */
+    {
+        const float *p = a.Q + query * a.ldq + (long long)h * a.d;
+        float x[KCH][4][4];
+        unsigned top = 0;
+
+#pragma unroll
+        for (int c = 0; c < KCH; c++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                load4_row(p, 64 * c + 16 * part + 4 * e, a.d, x[c][e]);
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    top = max(top, q8_mag(x[c][e][j]));
+            }
+        top = max(top, (unsigned)__shfl_xor((int)top, 16, 64));
+        top = max(top, (unsigned)__shfl_xor((int)top, 32, 64));
+        const q8_scale s = q8_scale_of(top);
+
+        odd = odd || s.s != s.s;
+#pragma unroll
+        for (int c = 0; c < KCH; c++)
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                q[c][e] = (int)q8_code4(x[c][e][0], x[c][e][1], x[c][e][2], x[c][e][3], s.r);
+    }
+    /* Register 4 t + e: block 16 t + 4 part + e. */
+    float s[4 * T], most[G];
+
+#pragma unroll
+    for (int e = 0; e < G; e++)
+        most[e] = -INFINITY;
+#pragma unroll
+    for (int t0 = 0; t0 < T; t0 += 4) {
+        i4 w[4][KCH];
+
+        /* Four tiles' codes on their way at once, and no more: the scores
+         * fill the registers. */
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int t = 0; t < 4; t++)
+#pragma unroll
+            for (int c = 0; c < KCH; c++) {
+                const int b = min(16 * (t0 + t) + col, a.nblk - 1);
+
+                w[t][c] = *(const i4 *)(a.KC + ((long long)b * a.nhk + kvh) * pitch + 64 * c +
+                                        16 * part);
+            }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            const int at = 16 * (t0 + t) + 4 * part;
+            const float4 k = *(const float4 *)(scale + at), n = *(const float4 *)(none + at);
+            const float kk[4] = {k.x, k.y, k.z, k.w}, nn[4] = {n.x, n.y, n.z, n.w};
+            i4 dot = {0, 0, 0, 0};
+
+#pragma unroll
+            for (int c = 0; c < KCH; c++)
+                dot = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[t][c], q[c], dot, 0, 0, 0);
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int i = 4 * (t0 + t) + e;
+
+                s[i] = fmaf((float)dot[e], kk[e], nn[e]);
+                most[i % G] = fmaxf(most[i % G], s[i]);
+            }
+        }
+    }
+    auto over4 = [](float v, auto f) {
+        v = f(v, __shfl_xor(v, 16, 64));
+        return f(v, __shfl_xor(v, 32, 64));
+    };
+    auto larger = [](float x, float y) { return fmaxf(x, y); };
+    auto smaller = [](float x, float y) { return fminf(x, y); };
+    auto count = [&](float v) {
+        int n = 0;
+
+#pragma unroll
+        for (int e = 0; e < 4 * T; e++)
+            n += s[e] >= v;
+        n += __shfl_xor(n, 16, 64);
+        return n + __shfl_xor(n, 32, 64);
+    };
+    float hi, lo;
+
+    /* 4, 8, 16 or 32 groups a row. */
+#pragma unroll
+    for (int n = G / 2; n >= 1; n /= 2)
+        if (a.top <= 4 * n) {
+#pragma unroll
+            for (int e = 0; e < n; e++)
+                most[e] = fmaxf(most[e], most[e + n]);
+#pragma unroll
+            for (int e = n; e < G; e++)
+                most[e] = most[e % n];
+        }
+    hi = most[0];
+    lo = most[0];
+#pragma unroll
+    for (int e = 1; e < G; e++) {
+        hi = fmaxf(hi, most[e]);
+        lo = fminf(lo, most[e]);
+    }
+    hi = over4(hi, larger);
+    lo = over4(lo, smaller);
+    if (__any(lo == -INFINITY)) {
+        /* Groups of no block: the smallest score there is. */
+        float v = INFINITY;
+
+#pragma unroll
+        for (int e = 0; e < 4 * T; e++)
+            v = fminf(v, s[e] == -INFINITY ? INFINITY : s[e]);
+        v = over4(v, smaller);
+        lo = lo == -INFINITY ? v : lo;
+    }
+    int n = count(lo);
+    bool done = n <= CAP;
+
+    for (int step = 0; step < 48 && !__any(odd) && !__all(done); step++) {
+        /* Values of very different size: by bits. */
+        const float mid = step == 0   ? 0.75f * lo + 0.25f * hi
+                          : step < 12 ? 0.5f * lo + 0.5f * hi
+                                      : sel_value((int)(((long long)sel_key(lo) + sel_key(hi)) >> 1));
+        const int m = count(mid);
+
+        if (!done) {
+            if (m >= a.top) {
+                lo = mid;
+                done = m <= CAP;
+            }
+            else
+                hi = mid;
+        }
+    }
+    if (__any(odd || !done)) {
+        for (int e = 0; e < min(16, rows - r0); e++) {
+            const int rr = r0 + e;
+            int key, idx;
+
+            sel_row<16 * KCH>(a, rr / g, kvh * g + rr % g, 0, a.nblk, codes[wave], lists[wave], key,
+                              idx);
+            if (lane < a.top)
+                a.SEL[((long long)(rr / g) * a.nh + kvh * g + rr % g) * a.top + lane] =
+                    key == SEL_NONE ? -1 : idx;
+        }
+        return;
+    }
+    /* The candidates into LDS, lane by lane of the row, as whole numbers that
+     * order like the scores and, where those are equal, against their own. */
+    n = 0;
+#pragma unroll
+    for (int e = 0; e < 4 * T; e++)
+        n += s[e] >= lo;
+    const int n16 = __shfl_xor(n, 16, 64), pair = n + n16, other = __shfl_xor(pair, 32, 64);
+    const int total = pair + other;
+    u64 *c = cand[wave][col];
+    u64 *at = c + (part & 1 ? n16 : 0) + (part & 2 ? other : 0);
+
+#pragma unroll
+    for (int e = 0; e < 4 * T; e++)
+        if (s[e] >= lo) {
+            *at++ = (u64)((unsigned)sel_key(s[e]) ^ 0x80000000u) << 32 |
+                    (unsigned)~(16 * (e / 4) + 4 * part + e % 4);
+        }
+    __builtin_amdgcn_wave_barrier();
+    /* Candidate 4 o + part of the row is this lane's. */
+    u64 mine[OWN];
+    int rank[OWN];
+
+#pragma unroll
+    for (int o = 0; o < OWN; o++) {
+        mine[o] = 4 * o + part < total ? c[4 * o + part] : ~0ull;
+        rank[o] = 0;
+    }
+    for (int j = 0; __any(j < total); j++) {
+        const u64 x = j < total ? c[j] : 0;
+
+#pragma unroll
+        for (int o = 0; o < OWN; o++)
+            rank[o] += x > mine[o];
+    }
+    if (r0 + col >= rows)
+        return;
+    int *out = a.SEL + row * a.top;
+
+#pragma unroll
+    for (int o = 0; o < OWN; o++)
+        if (4 * o + part < total && rank[o] < a.top)
+            out[rank[o]] = ~(int)(unsigned)mine[o];
+    for (int e = total + part; e < a.top; e += 4)
+        out[e] = -1;
 }
 
 extern "C" size_t ops_block_select_work_bytes(int Nq, int nh, int nblk, int top)
@@ -425,27 +676,54 @@ extern "C" void ops_block_select(struct ops *o, struct opnd Q, int Nq, int nh, i
     need_aligned(KC, 16, op, "KC");
     need_floats(KS, 0, (long long)nblk * nhk, op, "KS");
     need_bytes(SEL, 0, rows * top * 4, op, "SEL");
-    const int grid = count32(rows, "selection rows");
+    const int grid = count32(rows, "selection rows"), g = nh / nhk;
+    const hipStream_t s = stream_of(o->ocl);
+    sel_args a = {cfptr(Q.buf) + Q.off, (const signed char *)(KC ? KC->ptr : nullptr), cfptr(KS),
+                  (int *)SEL->ptr, Q.ld, Nq, nh, nhk, d, nblk, top};
 
     prof_scope ps(o->ocl, "block_select");
-#define SELECT_LAUNCH(W_, D_)                                                                   \
-    hipLaunchKernelGGL((block_select_kernel<W_, D_>), dim3(grid), dim3(64 * W_), 0,             \
-                       stream_of(o->ocl), cfptr(Q.buf) + Q.off, (long long)Q.ld, Nq, nh, nhk, d, \
-                       (const signed char *)(KC ? KC->ptr : nullptr), cfptr(KS), nblk, top,     \
-                       (int *)SEL->ptr)
-#define SELECT_WIDTH(W_)        \
-    do {                        \
-        if (d <= 32)            \
+#define SELECT_LAUNCH(W_, D_) \
+    hipLaunchKernelGGL((block_select_kernel<W_, D_>), dim3(grid), dim3(64 * W_), 0, s, a)
+#define SELECT_WIDTH(W_)           \
+    do {                           \
+        if (d <= 32)               \
             SELECT_LAUNCH(W_, 8);  \
-        else if (d <= 64)       \
+        else if (d <= 64)          \
             SELECT_LAUNCH(W_, 16); \
-        else                    \
+        else                       \
             SELECT_LAUNCH(W_, 32); \
     } while (0)
-    if (nblk > 128 && rows < 4 * o->ocl->cu_count)
-        SELECT_WIDTH(8);
+#define TILE_LAUNCH(T_, K_, C_)                                                              \
+    hipLaunchKernelGGL((block_select_tile<T_, K_, C_>),                                      \
+                       dim3((unsigned)(((long long)Nq * g + 16 * SEL_TW - 1) / (16 * SEL_TW)), nhk), \
+                       dim3(64 * SEL_TW), 0, s, a)
+#define TILE_WIDTH(T_)             \
+    do {                           \
+        if (top <= 16 && d <= 64)  \
+            TILE_LAUNCH(T_, 1, 24); \
+        else if (top <= 16)        \
+            TILE_LAUNCH(T_, 2, 24); \
+        else if (d <= 64)          \
+            TILE_LAUNCH(T_, 1, 40); \
+        else                       \
+            TILE_LAUNCH(T_, 2, 40); \
+    } while (0)
+    if (nblk >= 1 && nblk <= 512 && top <= 32 && rows >= 16LL * o->ocl->cu_count && nhk <= 65535) {
+        if (nblk <= 64)
+            TILE_WIDTH(4);
+        else if (nblk <= 128)
+            TILE_WIDTH(8);
+        else if (nblk <= 256)
+            TILE_WIDTH(16);
+        else
+            TILE_WIDTH(32);
+    }
+    else if (nblk > 256 && rows < 4 * o->ocl->cu_count)
+        SELECT_WIDTH(16);
     else
         SELECT_WIDTH(1);
+#undef TILE_WIDTH
+#undef TILE_LAUNCH
 #undef SELECT_WIDTH
 #undef SELECT_LAUNCH
     launch_check("block_select");
@@ -461,7 +739,7 @@ struct blk_args {
     const unsigned char *kmask;
     long long ldq, ldk, ldv, ldo;
     int q0, Nq; /* the queries of this pass: q0 .. q0 + Nq - 1 */
-    int Nk, nh, nhk, d, bs, sub, nblk, top, vec;
+    int Nk, nh, nhk, d, bs, sub, nblk, top;
     float scale;
     /* Work: units' outputs (DP floats each) and (maximum, sum), rows of this
      * pass x top x sub; bits[head][block][tile of 64 rows]. */
@@ -490,19 +768,14 @@ __device__ __forceinline__ void blk_unit_f32(const blk_args &a, int qi, int h, i
         const float *kp = K + kk * a.ldk;
         float s = 0.0f;
 
-        if (a.vec) {
-            for (int c = 4 * part4; c < d; c += 16) {
-                const float4 x = *(const float4 *)(kp + c), y = *(const float4 *)(q + c);
+        for (int c = 4 * part4; c < d; c += 16) {
+            float x[4], y[4];
 
-                s = fmaf(x.x, y.x, s);
-                s = fmaf(x.y, y.y, s);
-                s = fmaf(x.z, y.z, s);
-                s = fmaf(x.w, y.w, s);
-            }
-        }
-        else {
-            for (int c = part4; c < d; c += 4)
-                s = fmaf(kp[c], q[c], s);
+            load4_row(kp, c, d, x);
+            load4_row(q, c, d, y);
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                s = fmaf(x[e], y[e], s);
         }
         s += dpp_f(s, 0xB1);
         s += dpp_f(s, 0x4E);
@@ -531,31 +804,90 @@ __device__ __forceinline__ void blk_unit_f32(const blk_args &a, int qi, int h, i
     __builtin_amdgcn_wave_barrier();
 }
 
-/* Few queries: a wave a unit. */
+/* Few queries: a block of threads a unit, everything that it reads on its way
+ * at once. Scores: 4 lanes a key, DP / 16 times 4 channels each. Output: DP / 4
+ * lanes a key, KV keys each, joined in LDS. */
 template <int DP> __global__ void __launch_bounds__(256) blk_direct_kernel(const blk_args a)
 {
-    __shared__ float sc[4][64];
-    const int lane = threadIdx.x & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const long long units = (long long)a.Nq * a.nh * a.top * a.sub;
-    const long long u = (long long)blockIdx.x * 4 + wave;
-
-    if (u >= units)
-        return;
+    constexpr int NK = DP / 16, LV = DP / 4, GV = 256 / LV, KV = 64 / GV;
+    __shared__ float sc[64];
+    __shared__ float out[GV][DP];
+    const int tid = threadIdx.x, lane = tid & 63, d = a.d;
+    const long long u = blockIdx.x;
     const int sub = (int)(u % a.sub), slot = (int)(u / a.sub % a.top);
-    const int row = (int)(u / a.sub / a.top), h = row % a.nh;
+    const int row = (int)(u / a.sub / a.top), h = row % a.nh, kvh = h / (a.nh / a.nhk);
     const int *sel = a.SEL + ((long long)a.q0 * a.nh + row) * a.top;
     const int b = sel[slot];
     const bool twice = __any(lane < slot && sel[min(lane, a.top - 1)] == b);
-    const int ss = a.bs / a.sub, k0 = b * a.bs + sub * ss;
+    const int ss = a.bs / a.sub;
+    const bool is = b >= 0 && b < a.nblk && !twice && b * a.bs + sub * ss < a.Nk;
 
-    if (b < 0 || b >= a.nblk || twice || k0 >= a.Nk) {
-        if (lane == 0)
+    if (!is) {
+        if (tid == 0)
             a.ml[u] = make_float2(-INFINITY, 0.0f);
         return;
     }
-    blk_unit_f32(a, a.q0 + row / a.nh, h, k0, min(a.Nk, k0 + ss), a.part + u * DP, a.ml + u,
-                 sc[wave]);
+    const int k0 = b * a.bs + sub * ss, n = min(a.Nk - k0, ss);
+    const float *q = a.Q + (a.q0 + row / a.nh) * a.ldq + (long long)h * d;
+    const float *K = a.K + k0 * a.ldk + (long long)kvh * d;
+    const float *V = a.V + k0 * a.ldv + (long long)kvh * d;
+    const int key = tid >> 2, part = tid & 3, cv = 4 * (tid % LV), gv = tid / LV;
+    const bool in = key < n && (!a.kmask || a.kmask[k0 + key]);
+    float x[NK][4], y[NK][4], v[KV][4];
+    bool keep[KV];
+
+#pragma unroll
+    for (int i = 0; i < NK; i++) {
+        load4_row(K + min(key, n - 1) * a.ldk, 16 * i + 4 * part, d, x[i]);
+        load4_row(q, 16 * i + 4 * part, d, y[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < KV; i++) {
+        const int k = gv + GV * i;
+
+        load4_row(V + min(k, n - 1) * a.ldv, cv, d, v[i]);
+        keep[i] = k < n && (!a.kmask || a.kmask[k0 + k]);
+    }
+    float s = 0.0f;
+
+#pragma unroll
+    for (int i = 0; i < NK; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            s = fmaf(x[i][j], y[i][j], s);
+    s += dpp_f(s, 0xB1);
+    s += dpp_f(s, 0x4E);
+    if (part == 0)
+        sc[key] = in ? s * (a.scale * BLK_LOG2E) : -INFINITY;
+    __syncthreads();
+    /* Every wave for itself: lane k holds key k. */
+    const float t = sc[lane];
+    const bool nan = __any(t != t);
+    const float m = wave_max_full(t);
+    const float p = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(t - m);
+    const float l = nan ? __builtin_nanf("") : wave_sum_full(p);
+    float o[4] = {0, 0, 0, 0};
+
+#pragma unroll
+    for (int i = 0; i < KV; i++) {
+        const float w = __shfl(p, gv + GV * i, 64);
+
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            o[j] = keep[i] ? fmaf(w, v[i][j], o[j]) : o[j];
+    }
+    *(float4 *)&out[gv][cv] = make_float4(o[0], o[1], o[2], o[3]);
+    __syncthreads();
+    if (tid < DP) {
+        float r = 0.0f;
+
+#pragma unroll
+        for (int i = 0; i < GV; i++)
+            r += out[i][tid];
+        a.part[u * DP + tid] = nan ? __builtin_nanf("") : r;
+    }
+    if (tid == 0)
+        a.ml[u] = make_float2(nan ? 0.0f : m, l);
 }
 
 /* Many queries, first step: bit r of bits[kvh][b][t] says that row 64 t + r
@@ -606,20 +938,21 @@ __global__ void __launch_bounds__(64 * BLK_TW) blk_bits_kernel(const blk_args a)
 /* Second step: a block of threads holds a unit's keys and values in LDS, both
  * split in three bf16 parts (split.h), and computes them for the rows that
  * list it, 32 a wave and turn. */
-#define BLK_PIECE 2048 /* rows whose bits are read at a time */
+#define BLK_PIECE 1024 /* rows whose bits are read at a time */
+#define BLK_CHUNKS 32  /* pieces of rows a block of threads takes at most */
+#define BLK_VMAX 0x1p70f /* 64 probabilities times values stay finite below */
 
 template <int ND, int NB>
-__global__ void __launch_bounds__(256, ND == 4 ? 1 : 2) blk_unit_kernel(const blk_args a)
+__global__ void __launch_bounds__(256, ND == 4 ? 1 : 3) blk_unit_kernel(const blk_args a)
 {
     constexpr int DP = 32 * ND, CH = DP / 8, SB = 32 * NB, KC = SB / 8;
     constexpr int RW = 16 / CH < 1 ? 1 : 16 / CH;  /* K rows in 256 bytes */
     constexpr int RV = 16 / KC < 1 ? 1 : 16 / KC;  /* V rows */
     constexpr int PK = SB * CH;                    /* 16-byte chunks of a part */
     __shared__ split_u4 ks[3 * PK], vs[3 * PK];
-    __shared__ int list[BLK_PIECE + 128];
+    __shared__ unsigned short list[BLK_PIECE + 128];
     __shared__ int wsum[4];
     __shared__ float sc[4][64];
-    __shared__ unsigned long long keep_s;
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, col = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = a.nh / a.nhk, d = a.d;
@@ -631,21 +964,15 @@ __global__ void __launch_bounds__(256, ND == 4 ? 1 : 2) blk_unit_kernel(const bl
     const int nchunk = (words * 32 + BLK_PIECE - 1) / BLK_PIECE;
     const int c0 = (int)((long long)nchunk * piece / a.pieces);
     const int c1 = (int)((long long)nchunk * (piece + 1) / a.pieces);
+    const int base = c0 * BLK_PIECE; /* rows in the list count from here */
 
     if (c0 >= c1)
         return;
     /* The last block's second unit may lie past the keys. */
     const bool nothing = n <= 0;
-
-    if (tid < 64) {
-        const bool in = tid < n && (!a.kmask || a.kmask[k0 + min(tid, n - 1)]);
-        const unsigned long long k = __ballot(in);
-
-        if (tid == 0)
-            keep_s = k;
-    }
-    __syncthreads();
-    const unsigned long long keep = keep_s;
+    const unsigned long long keep =
+        __ballot(lane < n && (!a.kmask || a.kmask[k0 + min(lane, n - 1)]));
+    bool wild = false; /* values that the split's sums cannot hold */
 
     /* Keys and values that are left out are zero here: what they hold meets
      * probabilities of zero. */
@@ -657,12 +984,14 @@ __global__ void __launch_bounds__(256, ND == 4 ? 1 : 2) blk_unit_kernel(const bl
             const int key = e / CH, dd = e % CH * 8;
             const bool in = keep >> key & 1;
             const float *p = K + (long long)min(key, n - 1) * a.ldk;
-            float x[8];
+            float x[8], y[2][4];
             split_u4 h, m, l;
 
+            load4_row(p, dd, d, y[0]);
+            load4_row(p, dd + 4, d, y[1]);
 #pragma unroll
             for (int j = 0; j < 8; j++)
-                x[j] = in && dd + j < d ? p[min(dd + j, d - 1)] : 0.0f;
+                x[j] = in ? y[j / 4][j % 4] : 0.0f;
             split8(x, 1.0f, h, m, l);
             const int at = key * CH + ((e % CH) ^ (key / RW % CH));
 
@@ -681,9 +1010,15 @@ __global__ void __launch_bounds__(256, ND == 4 ? 1 : 2) blk_unit_kernel(const bl
 #pragma unroll
             for (int j = 0; j < 8; j++) {
                 const int key = (c >> 1) * 16 + (j >> 2) * 8 + (c & 1) * 4 + (j & 3);
-                const bool in = keep >> key & 1;
 
-                x[j] = in && dd < d ? V[(long long)min(key, n - 1) * a.ldv + min(dd, d - 1)] : 0.0f;
+                x[j] = V[(long long)min(key, n - 1) * a.ldv + min(dd, d - 1)];
+            }
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const int key = (c >> 1) * 16 + (j >> 2) * 8 + (c & 1) * 4 + (j & 3);
+
+                x[j] = (keep >> key & 1) && dd < d ? x[j] : 0.0f;
+                wild = wild || !(fabsf(x[j]) < BLK_VMAX);
             }
             split8(x, SPLIT_UP, h, m, l);
             const int at = dd * KC + (c ^ (dd / RV % KC));
@@ -693,42 +1028,55 @@ __global__ void __launch_bounds__(256, ND == 4 ? 1 : 2) blk_unit_kernel(const bl
             vs[2 * PK + at] = l;
         }
     }
+    wild = __syncthreads_or(wild);
 
-    auto tile = [&](const int *rows, int count) {
-        const bool live = col < count;
-        const int r = rows[live ? col : 0], qi = r / g, h = kvh * g + r % g;
-        const long long row = (long long)qi * a.nh + h;
-        const float *qp = a.Q + (a.q0 + qi) * a.ldq + (long long)h * d;
+    auto row_of = [&](int r) { return (long long)(r / g) * a.nh + kvh * g + r % g; };
+    /* The place of b in a row's list, each lane half looking through its
+     * part; the row lists b. */
+    auto slot_of = [&](long long row) {
         const int *sel = a.SEL + ((long long)a.q0 * a.nh + row) * a.top;
+        const int from = half * ((a.top + 1) / 2), to = half ? a.top : (a.top + 1) / 2;
+        int slot = BLK_MAX_TOP;
+
+        for (int s = from; s < to; s += 4) {
+            int v[4];
+
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                v[j] = sel[min(s + j, a.top - 1)];
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                slot = v[j] == b ? min(slot, min(s + j, a.top - 1)) : slot;
+        }
+        return min(slot, __shfl_xor(slot, 32, 64));
+    };
+    auto tile = [&](const unsigned short *rows, int count) {
+        const bool live = col < count;
+        const int r = base + rows[live ? col : 0], qi = r / g, h = kvh * g + r % g;
+        const long long row = row_of(r);
+        const float *qp = a.Q + (a.q0 + qi) * a.ldq + (long long)h * d;
         const float up = a.scale * BLK_LOG2E * BLK_QUP;
         split_u4 q[2 * ND][3];
-        split_f16x s[NB], o[ND], low[ND];
+        split_f16x s[NB];
         constexpr int pa[6] = {0, 2, 1, 0, 1, 0}, pb[6] = {2, 0, 1, 1, 0, 0};
-        int slot = 0;
 
-        while (slot < a.top - 1 && sel[slot] != b)
-            slot++;
+        {
+            float x[2 * ND][2][4];
+
 #pragma unroll
-        for (int st = 0; st < 2 * ND; st++) {
-            const int dd = st * 16 + half * 8;
-            float x[8];
-
-            if (a.vec) {
-                const float4 u = *(const float4 *)(qp + min(dd, d - 4));
-                const float4 v = *(const float4 *)(qp + min(dd + 4, d - 4));
-
-                x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w;
-                x[4] = v.x, x[5] = v.y, x[6] = v.z, x[7] = v.w;
+            for (int st = 0; st < 2 * ND; st++) {
+                load4_row(qp, st * 16 + half * 8, d, x[st][0]);
+                load4_row(qp, st * 16 + half * 8 + 4, d, x[st][1]);
             }
-            else {
+#pragma unroll
+            for (int st = 0; st < 2 * ND; st++) {
+                float y[8];
+
 #pragma unroll
                 for (int j = 0; j < 8; j++)
-                    x[j] = qp[min(dd + j, d - 1)];
+                    y[j] = x[st][j / 4][j % 4];
+                split8(y, up, q[st][0], q[st][1], q[st][2]);
             }
-#pragma unroll
-            for (int j = 0; j < 8; j++)
-                x[j] = dd + j < d ? x[j] * up : 0.0f;
-            split8(x, 1.0f, q[st][0], q[st][1], q[st][2]);
         }
         auto key = [&](int p, int t, int st) {
             const int kk = 32 * t + col;
@@ -758,26 +1106,37 @@ __global__ void __launch_bounds__(256, ND == 4 ? 1 : 2) blk_unit_kernel(const bl
         }
         float mx = -INFINITY, l = 0.0f, p[NB][16];
 
+        if (keep != (SB == 64 ? ~0ull : 0xffffffffull)) {
+#pragma unroll
+            for (int t = 0; t < NB; t++) {
+                const unsigned k = (unsigned)(keep >> (32 * t)) >> (4 * half);
+
+#pragma unroll
+                for (int e = 0; e < 16; e++)
+                    s[t][e] = k >> ((e >> 2) * 8 + (e & 3)) & 1 ? s[t][e] : -INFINITY;
+            }
+        }
 #pragma unroll
         for (int t = 0; t < NB; t++)
 #pragma unroll
-            for (int e = 0; e < 16; e++) {
-                const int kk = 32 * t + (e >> 2) * 8 + half * 4 + (e & 3);
-
-                p[t][e] = keep >> kk & 1 ? s[t][e] * (1.0f / BLK_QUP) : -INFINITY;
-                mx = fmaxf(mx, p[t][e]);
-            }
-        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+            for (int e = 0; e < 16; e++)
+                mx = fmaxf(mx, s[t][e]);
+        mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * (1.0f / BLK_QUP);
         const float ref = mx == -INFINITY ? 0.0f : mx;
 
 #pragma unroll
         for (int t = 0; t < NB; t++)
 #pragma unroll
             for (int e = 0; e < 16; e++) {
-                p[t][e] = __builtin_amdgcn_exp2f(p[t][e] - ref);
+                p[t][e] = __builtin_amdgcn_exp2f(fmaf(s[t][e], 1.0f / BLK_QUP, -ref));
                 l += p[t][e];
             }
         l += __shfl_xor(l, 32, 64);
+
+        const int slot = slot_of(row);
+        const long long at = (row * a.top + slot) * a.sub + sub;
+        split_f16x o[ND], low[ND];
+
 #pragma unroll
         for (int tt = 0; tt < ND; tt++)
 #pragma unroll
@@ -810,43 +1169,37 @@ __global__ void __launch_bounds__(256, ND == 4 ? 1 : 2) blk_unit_kernel(const bl
                 }
             }
         }
-        float z = l * 0.0f;
-
-#pragma unroll
-        for (int tt = 0; tt < ND; tt++)
-#pragma unroll
-            for (int e = 0; e < 16; e++) {
-                o[tt][e] += low[tt][e];
-                z = fmaf(o[tt][e], 0.0f, z);
-            }
-        const long long at = (row * a.top + slot) * a.sub + sub;
-        /* Infinities, NaN and values that have no split: again in float32. So
-         * are scores below the range of the split. */
-        const bool again = z != 0.0f || (l == 0.0f && keep);
+        /* Scores that are not finite or below the range of the split (no
+         * probability at all for keys that are kept), and wild values: again in
+         * float32. */
+        const bool again = wild || !(l < INFINITY) || (l == 0.0f && keep);
         const unsigned long long redo = __ballot(again && live);
 
-        if (live && !(redo >> col & 1) && !(redo >> (col + 32) & 1)) {
+        if (live && !again) {
             float *out = a.part + at * DP;
 
 #pragma unroll
             for (int tt = 0; tt < ND; tt++)
 #pragma unroll
-                for (int e = 0; e < 4; e++)
+                for (int e = 0; e < 4; e++) {
+                    float x[4];
+
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        x[j] = (o[tt][4 * e + j] + low[tt][4 * e + j]) * SPLIT_DOWN;
                     *(float4 *)(out + tt * 32 + e * 8 + half * 4) =
-                        make_float4(o[tt][4 * e] * SPLIT_DOWN, o[tt][4 * e + 1] * SPLIT_DOWN,
-                                    o[tt][4 * e + 2] * SPLIT_DOWN, o[tt][4 * e + 3] * SPLIT_DOWN);
+                        make_float4(x[0], x[1], x[2], x[3]);
+                }
             if (half == 0)
                 a.ml[at] = make_float2(mx, l);
         }
         if (redo)
             for (int e = 0; e < count; e++)
-                if ((redo >> e | redo >> (e + 32)) & 1) {
-                    const int rr = rows[e], qq = rr / g;
-                    const long long to =
-                        (long long)(unsigned)__builtin_amdgcn_readlane((int)(at & 0xffffffff), e) |
-                        (long long)__builtin_amdgcn_readlane((int)(at >> 32), e) << 32;
+                if (redo >> e & 1) {
+                    const int rr = base + rows[e], sl = __builtin_amdgcn_readlane(slot, e);
+                    const long long to = (row_of(rr) * a.top + sl) * a.sub + sub;
 
-                    blk_unit_f32(a, a.q0 + qq, kvh * g + rr % g, k0, k0 + n, a.part + to * DP,
+                    blk_unit_f32(a, a.q0 + rr / g, kvh * g + rr % g, k0, k0 + n, a.part + to * DP,
                                  a.ml + to, sc[wave]);
                 }
     };
@@ -854,9 +1207,9 @@ __global__ void __launch_bounds__(256, ND == 4 ? 1 : 2) blk_unit_kernel(const bl
     int have = 0;
 
     for (int c = c0; c < c1; c++) {
-        /* 8 rows a thread: their bits, the place of the first of them. */
-        const int r0 = c * BLK_PIECE + 8 * tid, w = r0 >> 5;
-        unsigned m = w < words ? bits[w] >> (r0 & 31) & 0xffu : 0u;
+        /* 4 rows a thread: their bits, the place of the first of them. */
+        const int r0 = c * BLK_PIECE + 4 * tid, w = r0 >> 5;
+        unsigned m = w < words ? bits[w] >> (r0 & 31) & 0xfu : 0u;
         int p = __popc(m), before = 0;
 
 #pragma unroll
@@ -874,7 +1227,7 @@ __global__ void __launch_bounds__(256, ND == 4 ? 1 : 2) blk_unit_kernel(const bl
         int at = have + before + p - __popc(m);
 
         while (m) {
-            list[at++] = r0 + __ffs(m) - 1;
+            list[at++] = (unsigned short)(r0 - base + __ffs(m) - 1);
             m &= m - 1;
         }
         have += added;
@@ -883,69 +1236,91 @@ __global__ void __launch_bounds__(256, ND == 4 ? 1 : 2) blk_unit_kernel(const bl
         const int todo = c + 1 == c1 ? have : have / 128 * 128;
 
         for (int e = wave * 32; e < todo; e += 128) {
-            if (nothing) {
-                if (lane < min(32, todo - e)) {
-                    const int r = list[e + lane], h = kvh * g + r % g;
-                    const long long row = (long long)(r / g) * a.nh + h;
-                    const int *sel = a.SEL + ((long long)a.q0 * a.nh + row) * a.top;
-                    int slot = 0;
+            const int count = min(32, todo - e);
 
-                    while (slot < a.top - 1 && sel[slot] != b)
-                        slot++;
+            if (nothing) {
+                const long long row = row_of(base + list[e + (col < count ? col : 0)]);
+                const int slot = slot_of(row);
+
+                if (lane < count)
                     a.ml[(row * a.top + slot) * a.sub + sub] = make_float2(-INFINITY, 0.0f);
-                }
             }
             else
-                tile(list + e, min(32, todo - e));
+                tile(list + e, count);
         }
         __syncthreads();
-        const int rest = have - todo, keepv = tid < rest ? list[todo + tid] : 0;
+        const int rest = have - todo, kept = tid < rest ? list[todo + tid] : 0;
 
         __syncthreads();
         if (tid < rest)
-            list[tid] = keepv;
+            list[tid] = (unsigned short)kept;
         have = rest;
     }
 }
 
-/* Units of a row merged: softmax over all of them from their maxima and
- * sums, in the order of the list. Four channels a thread. */
+/* Units of a row merged: softmax over all of them from their maxima and sums.
+ * A wave a row: lane u has unit u's weight (and unit 64 + u's), then DP / 4
+ * lanes a unit add the outputs, 256 / DP units at a time. */
 template <int DP> __global__ void __launch_bounds__(256) blk_merge_kernel(const blk_args a)
 {
-    const int units = a.top * a.sub;
-    const long long e = (long long)blockIdx.x * 256 + threadIdx.x;
-    const long long row = e / (DP / 4);
-    const int c = (int)(e % (DP / 4)) * 4, d = a.d;
+    constexpr int LV = DP / 4, GV = 64 / LV;
+    const int units = a.top * a.sub, lane = threadIdx.x & 63, c = 4 * (lane % LV), gv = lane / LV;
+    const long long row =
+        (long long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
-    if (row >= (long long)a.Nq * a.nh || c >= d)
+    if (row >= (long long)a.Nq * a.nh)
         return;
+    const float2 none = make_float2(-INFINITY, 0.0f);
     const float2 *ml = a.ml + row * units;
     const float *part = a.part + row * units * DP + c;
-    float m = -INFINITY, l = 0.0f, o[4] = {0, 0, 0, 0};
+    const float2 x = lane < units ? ml[lane] : none;
+    const float2 y = 64 + lane < units ? ml[64 + lane] : none;
+    const float m = wave_max_full(fmaxf(x.y != 0.0f ? x.x : -INFINITY, y.y != 0.0f ? y.x : -INFINITY));
+    const float wx = x.y != 0.0f ? __builtin_amdgcn_exp2f(x.x - m) : 0.0f;
+    const float wy = y.y != 0.0f ? __builtin_amdgcn_exp2f(y.x - m) : 0.0f;
+    const float l = wave_sum_full(x.y * wx + y.y * wy);
+    float o[4] = {0, 0, 0, 0};
 
-    for (int u = 0; u < units; u++)
-        if (ml[u].y != 0.0f)
-            m = fmaxf(m, ml[u].x);
-    for (int u = 0; u < units; u++) {
-        const float2 x = ml[u];
-
-        if (x.y == 0.0f)
-            continue;
-        const float w = __builtin_amdgcn_exp2f(x.x - m);
-        const float4 p = *(const float4 *)(part + (long long)u * DP);
-
-        l = fmaf(x.y, w, l);
-        o[0] = fmaf(p.x, w, o[0]);
-        o[1] = fmaf(p.y, w, o[1]);
-        o[2] = fmaf(p.z, w, o[2]);
-        o[3] = fmaf(p.w, w, o[3]);
-    }
-    float *out = a.O + (a.q0 + row / a.nh) * a.ldo + (row % a.nh) * d + c;
+    /* Four loads on their way at once; units with no key hold nothing. */
+    for (int u0 = gv; u0 < units + gv; u0 += 4 * GV) {
+        float4 p[4];
+        float w[4];
 
 #pragma unroll
-    for (int j = 0; j < 4; j++)
-        if (c + j < d)
-            out[j] = l == 0.0f ? 0.0f : o[j] / l;
+        for (int i = 0; i < 4; i++) {
+            const int u = u0 + i * GV, at = min(u, units - 1);
+            const float wu = __shfl(u < 64 ? wx : wy, u & 63, 64);
+            const float s = __shfl(u < 64 ? x.y : y.y, u & 63, 64);
+
+            p[i] = *(const float4 *)(part + (long long)at * DP);
+            w[i] = u < units && s != 0.0f ? wu : -1.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (!(w[i] < 0.0f)) {
+                o[0] = fmaf(p[i].x, w[i], o[0]);
+                o[1] = fmaf(p[i].y, w[i], o[1]);
+                o[2] = fmaf(p[i].z, w[i], o[2]);
+                o[3] = fmaf(p[i].w, w[i], o[3]);
+            }
+    }
+#pragma unroll
+    for (int s = LV; s < 64; s *= 2)
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            o[j] += __shfl_xor(o[j], s, 64);
+    if (gv == 0) {
+        float *out = a.O + (a.q0 + row / a.nh) * a.ldo + (row % a.nh) * a.d;
+
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            o[j] = l == 0.0f ? 0.0f : o[j] / l;
+        if (c + 4 <= a.d)
+            store4(out + c, o[0], o[1], o[2], o[3]);
+        else
+            for (int j = 0; c + j < a.d; j++)
+                out[c + j] = o[j];
+    }
 }
 
 /* The passes of a call: queries a pass, and what one needs of the work
@@ -967,9 +1342,10 @@ static blk_plan blk_plan_of(int Nq, int Nk, int nh, int nhk, int d, int bs, int 
     p.sub = blk_sub(bs);
     p.dp = d <= 32 ? 32 : d <= 64 ? 64 : 128;
     const long long row = (long long)top * p.sub * (p.dp + 2) * 4; /* bytes a row */
-    const long long most = max(1LL, BLK_PART_BYTES / (row * nh));
+    const long long most = max(512LL, BLK_PART_BYTES / (row * nh));
+    const long long passes = (Nq + most - 1) / most;
 
-    p.pass = (int)min((long long)Nq, max(most, 512LL));
+    p.pass = (int)((Nq + passes - 1) / passes);
     p.direct = p.nblk == 0 || (long long)p.pass * g * top < 16LL * max(p.nblk, 1) ||
                (long long)Nq * nh * top <= 4096;
     p.tiles = ((p.pass * g + 63) / 64 + BLK_TW - 1) / BLK_TW * BLK_TW;
@@ -1041,7 +1417,6 @@ extern "C" void ops_attention_blocks(struct ops *o, struct opnd Q, struct opnd K
     count32((long long)p.pass * nh * top * p.sub, "units of a pass");
 
     blk_args a = {};
-    auto al = [](const float *q, int ld) { return ((uintptr_t)q & 15) == 0 && ld % 4 == 0; };
 
     a.Q = cfptr(Q.buf) + Q.off;
     a.K = Nk ? cfptr(K.buf) + K.off : nullptr;
@@ -1061,7 +1436,6 @@ extern "C" void ops_attention_blocks(struct ops *o, struct opnd Q, struct opnd K
     a.sub = p.sub;
     a.nblk = p.nblk;
     a.top = top;
-    a.vec = d % 4 == 0 && al(a.Q, Q.ld) && (!Nk || (al(a.K, K.ld) && al(a.V, V.ld)));
     a.scale = scale;
     a.part = fptr(work);
     a.ml = (float2 *)((char *)work->ptr + p.part);
@@ -1077,7 +1451,7 @@ extern "C" void ops_attention_blocks(struct ops *o, struct opnd Q, struct opnd K
 
         a.tiles = ((a.Nq * g + 63) / 64 + BLK_TW - 1) / BLK_TW * BLK_TW;
         if (p.direct) {
-            const dim3 grid((unsigned)count32((units + 3) / 4, "units"));
+            const dim3 grid((unsigned)count32(units, "units"));
 
             if (p.dp == 32)
                 hipLaunchKernelGGL(blk_direct_kernel<32>, grid, dim3(256), 0, s, a);
@@ -1094,8 +1468,9 @@ extern "C" void ops_attention_blocks(struct ops *o, struct opnd Q, struct opnd K
             const long long each = max(1LL, (long long)a.Nq * g * top / p.nblk / 256);
             const int chunks = (a.tiles * 64 + BLK_PIECE - 1) / BLK_PIECE;
 
-            a.pieces = (int)max(1LL, min(min(each, (long long)chunks),
-                                         (4LL * o->ocl->cu_count + lists - 1) / lists));
+            a.pieces = (int)max((chunks + BLK_CHUNKS - 1LL) / BLK_CHUNKS,
+                                min(min(each, (long long)chunks),
+                                    (4LL * o->ocl->cu_count + lists - 1) / lists));
             hipLaunchKernelGGL(blk_bits_kernel, dim3(a.tiles / BLK_TW, nhk), dim3(64 * BLK_TW), 0, s,
                                a);
             launch_check("attention_blocks bits");
@@ -1117,7 +1492,7 @@ extern "C" void ops_attention_blocks(struct ops *o, struct opnd Q, struct opnd K
 #undef UNIT_LAUNCH
             launch_check("attention_blocks units");
         }
-        const dim3 grid((unsigned)count32((rows * (p.dp / 4) + 255) / 256, "merge"));
+        const dim3 grid((unsigned)count32((rows + 3) / 4, "merge"));
 
         if (p.dp == 32)
             hipLaunchKernelGGL(blk_merge_kernel<32>, grid, dim3(256), 0, s, a);

@@ -308,7 +308,11 @@ def test_scores_far_from_zero(nq, d, dev, ic):
 @pytest.mark.parametrize("eq,ek,ev", [(-116, 116, 0), (90, -90, 0), (0, 0, -116), (0, 0, 60)])
 def test_powers_of_two(eq, ek, ev, nq, dev, ic):
     """Scaling queries against keys, or values, by powers of two changes no
-    bit but the exponents."""
+    bit but the exponents. Values of 2^-116 times small probabilities are
+    subnormal: each of at most 2 x 64 products and as many sums of them may
+    lose 2^-150, together 2^-142, of outputs of at least 2^-116: less than U /
+    4. That moves the roundings that follow, of a unit's sum, of the merge's and
+    of the quotient, by one place (2 U) each at most."""
     print(f"[blocks] 2^{eq} 2^{ek} 2^{ev} {nq}", flush=True)
     rng = np.random.default_rng(nq)
     h, d, nk = 2, 64, 128
@@ -321,7 +325,10 @@ def test_powers_of_two(eq, ek, ev, nq, dev, ic):
         dev.write(c.SEL, sel)
         c.attend()
         outs.append(c.out())
-    assert np.array_equal(outs[1], np.ldexp(outs[0], ev))
+    if ev > -100:
+        assert np.array_equal(outs[1], np.ldexp(outs[0], ev))
+    else:
+        assert np.all(np.abs(np.ldexp(outs[1].astype(np.float64), -ev) - outs[0]) <= 6 * U * np.abs(outs[0]))
 
 
 @pytest.mark.parametrize("nq", [3, 700])
