@@ -10,6 +10,7 @@
 #include <hip/hip_runtime.h>
 
 typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));
+typedef int int4u __attribute__((ext_vector_type(4), aligned(4)));
 
 static __device__ __forceinline__ void load4(const float *p, float (&x)[4])
 {

@@ -971,7 +971,7 @@ template <int CTRL> __device__ __forceinline__ int quad_i(int v)
 #define BLK_CHUNKS 32  /* pieces of rows a block of threads takes at most */
 #define BLK_VMAX 0x1p90f /* 64 scaled values stay finite below */
 
-template <int ND, int NB>
+template <int ND, int NB, bool FULL>
 __global__ void __launch_bounds__(256, ND == 4 ? 1 : ND * NB == 4 ? 3 : 4) blk_unit_kernel(const blk_args a)
 {
     constexpr int DP = 32 * ND, CH = DP / 8, SB = 32 * NB, KC = SB / 8;
@@ -984,7 +984,7 @@ __global__ void __launch_bounds__(256, ND == 4 ? 1 : ND * NB == 4 ? 3 : 4) blk_u
     __shared__ float sc[4][64];
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, col = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int g = a.nh / a.nhk, d = a.d;
+    const int g = a.nh / a.nhk, d = FULL ? DP : a.d;
     const int unit = blockIdx.x / a.pieces, piece = blockIdx.x % a.pieces;
     const int sub = unit % a.sub, b = unit / a.sub % a.nblk, kvh = unit / a.sub / a.nblk;
     const int ss = a.bs / a.sub, k0 = b * a.bs + sub * ss, n = min(a.Nk - k0, ss);
@@ -1028,8 +1028,14 @@ __global__ void __launch_bounds__(256, ND == 4 ? 1 : ND * NB == 4 ? 3 : 4) blk_u
             const float *p = K + (long long)key * a.ldk;
             float u[4], v[4];
 
-            load4_row(p, dd, d, u);
-            load4_row(p, dd + 4, d, v);
+            if (FULL) {
+                load4(p + dd, u);
+                load4(p + dd + 4, v);
+            }
+            else {
+                load4_row(p, dd, d, u);
+                load4_row(p, dd + 4, d, v);
+            }
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 x[i][j] = u[j];
@@ -1097,9 +1103,16 @@ __global__ void __launch_bounds__(256, ND == 4 ? 1 : ND * NB == 4 ? 3 : 4) blk_u
         for (int s = from; s < to; s += 4) {
             int v[4];
 
+            if (a.top % 8 == 0) {
+                const int4u x = *(const int4u *)(sel + s);
+
+                v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
+            }
+            else {
 #pragma unroll
-            for (int j = 0; j < 4; j++)
-                v[j] = sel[min(s + j, a.top - 1)];
+                for (int j = 0; j < 4; j++)
+                    v[j] = sel[min(s + j, a.top - 1)];
+            }
 #pragma unroll
             for (int j = 0; j < 4; j++)
                 slot = v[j] == b ? min(slot, min(s + j, a.top - 1)) : slot;
@@ -1119,7 +1132,7 @@ __global__ void __launch_bounds__(256, ND == 4 ? 1 : ND * NB == 4 ? 3 : 4) blk_u
             const float *p = a.Q + (a.q0 + qi) * a.ldq + (long long)h * d;
             float x[2 * ND][2][4];
 
-            if (d == DP) {
+            if constexpr (FULL) {
 #pragma unroll
                 for (int st = 0; st < 2 * ND; st++) {
                     load4(p + st * 16 + half * 8, x[st][0]);
@@ -1174,8 +1187,11 @@ __global__ void __launch_bounds__(256, ND == 4 ? 1 : ND * NB == 4 ? 3 : 4) blk_u
         if (keep != (SB == 64 ? ~0ull : 0xffffffffull)) {
 #pragma unroll
             for (int t = 0; t < NB; t++) {
-                const unsigned k = (unsigned)(keep >> (32 * t)) >> (4 * half);
+                unsigned k = (unsigned)(keep >> (32 * t)) >> (4 * half);
 
+                /* Tested here: as 16 conditions kept over all tiles they
+                 * fill the scalar registers. */
+                asm volatile("" : "+v"(k));
 #pragma unroll
                 for (int e = 0; e < 16; e++)
                     s[t][e] = k >> ((e >> 2) * 8 + (e & 3)) & 1 ? s[t][e] : -INFINITY;
@@ -1253,6 +1269,7 @@ __global__ void __launch_bounds__(256, ND == 4 ? 1 : ND * NB == 4 ? 3 : 4) blk_u
          * and a store writes whole 128-byte lines (8 rows) instead of 32 bytes
          * of 32 rows. */
         const int to = live && !again ? (int)at : -1;
+        const bool whole = __all(to >= 0);
 
         if (half == 0 && to >= 0)
             a.ml[to] = make_float2(mx, l);
@@ -1284,12 +1301,13 @@ __global__ void __launch_bounds__(256, ND == 4 ? 1 : ND * NB == 4 ? 3 : 4) blk_u
             }
             const int there[4] = {quad_i<0x00>(to), quad_i<0x55>(to), quad_i<0xAA>(to),
                                   quad_i<0xFF>(to)};
+            const unsigned run = tt * 32 + (lane & 3) * 8 + half * 4;
 
 #pragma unroll
             for (int e = 0; e < 4; e++)
-                if (there[e] >= 0)
-                    *(float4 *)(a.part + (long long)there[e] * DP + tt * 32 + (lane & 3) * 8 +
-                                half * 4) = make_float4(x[e][0], x[e][1], x[e][2], x[e][3]);
+                if (whole || there[e] >= 0)
+                    *(float4 *)((char *)a.part + 4u * ((unsigned)there[e] * DP + run)) =
+                        make_float4(x[e][0], x[e][1], x[e][2], x[e][3]);
         }
         if (redo)
             for (int e = 0; e < count; e++)
@@ -1515,7 +1533,7 @@ static blk_plan blk_plan_of(int Nq, int Nk, int nh, int nhk, int d, int bs, int 
     p.sub = blk_sub(bs);
     p.dp = d <= 32 ? 32 : d <= 64 ? 64 : 128;
     const long long row = (long long)top * p.sub * (p.dp + 2) * 4; /* bytes a row */
-    const long long most = max(512LL, BLK_PART_BYTES / (row * nh));
+    const long long most = max(1LL, BLK_PART_BYTES / (row * nh));
     const long long passes = (Nq + most - 1) / most;
 
     p.pass = (int)((Nq + passes - 1) / passes);
@@ -1649,19 +1667,27 @@ extern "C" void ops_attention_blocks(struct ops *o, struct opnd Q, struct opnd K
             launch_check("attention_blocks bits");
             const dim3 grid((unsigned)count32((long long)lists * a.pieces, "lists"));
 
-#define UNIT_LAUNCH(ND_)                                                                  \
-    do {                                                                                  \
-        if (bs / p.sub <= 32)                                                             \
-            hipLaunchKernelGGL((blk_unit_kernel<ND_, 1>), grid, dim3(256), 0, s, a);      \
-        else                                                                              \
-            hipLaunchKernelGGL((blk_unit_kernel<ND_, 2>), grid, dim3(256), 0, s, a);      \
+#define UNIT_LAUNCH(ND_, NB_)                                                                 \
+    do {                                                                                      \
+        if (d == 32 * ND_)                                                                    \
+            hipLaunchKernelGGL((blk_unit_kernel<ND_, NB_, true>), grid, dim3(256), 0, s, a);  \
+        else                                                                                  \
+            hipLaunchKernelGGL((blk_unit_kernel<ND_, NB_, false>), grid, dim3(256), 0, s, a); \
+    } while (0)
+#define UNIT_KEYS(ND_)          \
+    do {                        \
+        if (bs / p.sub <= 32)   \
+            UNIT_LAUNCH(ND_, 1); \
+        else                    \
+            UNIT_LAUNCH(ND_, 2); \
     } while (0)
             if (p.dp == 32)
-                UNIT_LAUNCH(1);
+                UNIT_KEYS(1);
             else if (p.dp == 64)
-                UNIT_LAUNCH(2);
+                UNIT_KEYS(2);
             else
-                UNIT_LAUNCH(4);
+                UNIT_KEYS(4);
+#undef UNIT_KEYS
 #undef UNIT_LAUNCH
             launch_check("attention_blocks units");
         }
