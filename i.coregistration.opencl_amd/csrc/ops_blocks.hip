@@ -24,6 +24,7 @@
 #include <math.h>
 
 #include "common.h"
+#include "gemm_dev.h"
 #include "load4.h"
 #include "ops.h"
 #include "q8.h"
@@ -145,6 +146,11 @@ extern "C" void ops_block_index(struct ops *o, struct opnd K, int Nk, int nhk, i
         need_bytes(KC, 0, cells * q8_pitch(d), op, "KC");
         need_aligned(KC, 16, op, "KC");
         need_floats(KS, 0, cells, op, "KS");
+        const long long kbytes = ((Nk - 1) * (long long)K.ld + (long long)nhk * d) * 4;
+
+        need_apart(KC, 0, cells * q8_pitch(d), K.buf, K.off * 4, kbytes, op, "KC and K");
+        need_apart(KS, 0, cells * 4, K.buf, K.off * 4, kbytes, op, "KS and K");
+        need_apart(KC, 0, cells * q8_pitch(d), KS, 0, cells * 4, op, "KC and KS");
     }
     const int grid = count32((long long)nb * nhk, "block index");
 
@@ -322,7 +328,7 @@ struct sel_args {
  * 64 SLOTS at a time, the best so far kept beside the next ones. The PL = 4 or 8
  * lanes of a code row read 16 bytes each, neighbours of one line (a row a lane
  * fetches every line PL times: 2047 blocks of 128 channels, 16 rows 25 us, so
- * MEASURED), and add their sums; lane l keeps the score of block l of 64. Sorted
+ * 20), and add their sums; lane l keeps the score of block l of 64. Sorted
  * results in the lanes, as sel_top leaves them. codes, list: 128 bytes and
  * words of LDS of this wave. */
 template <int PL>
@@ -662,6 +668,25 @@ __global__ void __launch_bounds__(64 * SEL_TW, T > 16 ? 2 : T > 8 ? 3 : 4)
         out[e] = -1;
 }
 
+/* The kernel of a selection. us, a wave a row and tiles of 16 rows: 4096 rows of
+ * 256 blocks 11.3, 17.2; 8192 17.7, 16.4; 65536 197, 37; of 51 blocks, 4096 rows
+ * 10.2, 9.2. One wave and 16 a row: 16 rows of 2047 blocks 65, 14; 1024 rows 71,
+ * 41; 4096 rows 119, 144; of 256 blocks, 16 rows 11.4, 11.2. */
+enum { SEL_WAVE, SEL_WAVES, SEL_TILE };
+
+static int sel_choose(long long rows, int nhk, int nblk, int top, int cus)
+{
+    if (nblk >= 1 && nblk <= 512 && top <= 32 && nhk <= 65535 &&
+        rows >= (nblk <= 128 ? 16LL : 32LL) * cus)
+        return SEL_TILE;
+    return nblk > rows + 256 ? SEL_WAVES : SEL_WAVE;
+}
+
+extern "C" int icoreg_select_choice(struct ops *o, int Nq, int nh, int nhk, int nblk, int top)
+{
+    return sel_choose((long long)Nq * nh, nhk, nblk, top, o->ocl->cu_count);
+}
+
 extern "C" size_t ops_block_select_work_bytes(int Nq, int nh, int nblk, int top)
 {
     (void)Nq, (void)nh, (void)nblk, (void)top;
@@ -692,6 +717,10 @@ extern "C" void ops_block_select(struct ops *o, struct opnd Q, int Nq, int nh, i
     need_aligned(KC, 16, op, "KC");
     need_floats(KS, 0, (long long)nblk * nhk, op, "KS");
     need_bytes(SEL, 0, rows * top * 4, op, "SEL");
+    need_apart(SEL, 0, rows * top * 4, Q.buf, Q.off * 4,
+               ((Nq - 1) * (long long)Q.ld + (long long)nh * d) * 4, op, "SEL and Q");
+    need_apart(SEL, 0, rows * top * 4, KC, 0, (long long)nblk * nhk * q8_pitch(d), op, "SEL and KC");
+    need_apart(SEL, 0, rows * top * 4, KS, 0, (long long)nblk * nhk * 4, op, "SEL and KS");
     const int grid = count32(rows, "selection rows"), g = nh / nhk;
     const hipStream_t s = stream_of(o->ocl);
     sel_args a = {cfptr(Q.buf) + Q.off, (const signed char *)(KC ? KC->ptr : nullptr), cfptr(KS),
@@ -722,7 +751,9 @@ extern "C" void ops_block_select(struct ops *o, struct opnd Q, int Nq, int nh, i
         else                       \
             TILE_LAUNCH(T_, 2, 40); \
     } while (0)
-    if (nblk >= 1 && nblk <= 512 && top <= 32 && rows >= 16LL * o->ocl->cu_count && nhk <= 65535) {
+    const int form = sel_choose(rows, nhk, nblk, top, o->ocl->cu_count);
+
+    if (form == SEL_TILE) {
         if (nblk <= 64)
             TILE_WIDTH(4);
         else if (nblk <= 128)
@@ -732,7 +763,7 @@ extern "C" void ops_block_select(struct ops *o, struct opnd Q, int Nq, int nh, i
         else
             TILE_WIDTH(32);
     }
-    else if (nblk > 256 && rows < 4 * o->ocl->cu_count)
+    else if (form == SEL_WAVES)
         SELECT_WIDTH(16);
     else
         SELECT_WIDTH(1);
@@ -985,7 +1016,10 @@ __global__ void __launch_bounds__(256, ND == 4 ? 1 : ND * NB == 4 ? 3 : 4) blk_u
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, col = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = a.nh / a.nhk, d = FULL ? DP : a.d;
-    const int unit = blockIdx.x / a.pieces, piece = blockIdx.x % a.pieces;
+    /* An XCD takes a band of them: few key heads, whose queries stay in its
+     * L2. */
+    const int job = xcd_tile(blockIdx.x, gridDim.x);
+    const int unit = job / a.pieces, piece = job % a.pieces;
     const int sub = unit % a.sub, b = unit / a.sub % a.nblk, kvh = unit / a.sub / a.nblk;
     const int ss = a.bs / a.sub, k0 = b * a.bs + sub * ss, n = min(a.Nk - k0, ss);
     const unsigned *bits = (const unsigned *)(a.bits + ((long long)kvh * a.nblk + b) * a.tiles);
@@ -1521,8 +1555,9 @@ struct blk_plan {
     long long part, ml, bits; /* bytes */
 };
 
-extern "C" int icoreg_blk_each, icoreg_blk_mul, icoreg_blk_part; int icoreg_blk_each = 256; int icoreg_blk_mul = 8, icoreg_blk_part = 512;
-#define BLK_PART_BYTES ((long long)icoreg_blk_part << 20)
+/* Units of a pass: 8192 x 8 rows of 16 units of 64 channels 294 us in two
+ * passes of 256 MiB, 270 in one; 350 in three. */
+#define BLK_PART_BYTES (512LL << 20)
 
 static blk_plan blk_plan_of(int Nq, int Nk, int nh, int nhk, int d, int bs, int top)
 {
@@ -1533,12 +1568,20 @@ static blk_plan blk_plan_of(int Nq, int Nk, int nh, int nhk, int d, int bs, int 
     p.sub = blk_sub(bs);
     p.dp = d <= 32 ? 32 : d <= 64 ? 64 : 128;
     const long long row = (long long)top * p.sub * (p.dp + 2) * 4; /* bytes a row */
-    const long long most = max(1LL, BLK_PART_BYTES / (row * nh));
+    /* A query's units and bits. */
+    const long long most = max(1LL, BLK_PART_BYTES / (row * nh + (long long)nh * p.nblk / 8 + 1));
     const long long passes = (Nq + most - 1) / most;
 
     p.pass = (int)((Nq + passes - 1) / passes);
-    p.direct = p.nblk == 0 || (long long)p.pass * g * top < 16LL * max(p.nblk, 1) ||
-               (long long)Nq * nh * top <= 4096;
+    /* Units one by one or by lists, us: 8 heads of 64 on 256 blocks of 64 keys,
+     * 16 listed, 16 queries 16, 29; 64 queries 35, 27; 1024 queries 431, 58. 8 heads
+     * of 128, 8 of 64 blocks, 64 queries 41, 41; of 32, 8 of 100 blocks, 64 queries
+     * 18, 31, 256 queries 42, 28. Lists of a few rows stage a block's keys for
+     * nothing. */
+    const long long units = (long long)p.pass * nh * top * p.sub;
+
+    p.direct = p.nblk == 0 || nhk > 65535 || units * (p.dp + 32) <= 600000 ||
+               (long long)p.pass * g * top < 4LL * p.nblk;
     p.tiles = ((p.pass * g + 63) / 64 + BLK_TW - 1) / BLK_TW * BLK_TW;
     p.part = (long long)p.pass * nh * top * p.sub * p.dp * 4;
     p.ml = (long long)p.pass * nh * top * p.sub * 8;
@@ -1560,6 +1603,13 @@ extern "C" size_t ops_attention_blocks_work_bytes(int Nq, int Nk, int nh, int nh
     const blk_plan p = blk_plan_of(Nq, Nk, nh, nhk, d, bs, top);
 
     return (size_t)(p.part + p.ml + p.bits);
+}
+
+extern "C" int icoreg_blocks_choice(int Nq, int Nk, int nh, int nhk, int d, int bs, int top)
+{
+    if (!blk_sizes_ok(Nq, Nk, nh, nhk, d, bs, top) || Nq == 0)
+        return -1;
+    return !blk_plan_of(Nq, Nk, nh, nhk, d, bs, top).direct;
 }
 
 extern "C" void ops_attention_blocks(struct ops *o, struct opnd Q, struct opnd K, struct opnd V,
@@ -1604,6 +1654,9 @@ extern "C" void ops_attention_blocks(struct ops *o, struct opnd Q, struct opnd K
                         "O and V");
     }
     need_apart(O.buf, O.off * 4, obytes, work, 0, wbytes, op, "O and work");
+    need_apart(SEL, 0, (long long)Nq * nh * top * 4, O.buf, O.off * 4, obytes, op, "SEL and O");
+    if (kmask)
+        need_apart(kmask, 0, Nk, O.buf, O.off * 4, obytes, op, "kmask and O");
     need_apart(SEL, 0, (long long)Nq * nh * top * 4, work, 0, wbytes, op, "SEL and work");
     count32((long long)p.pass * nh * top * p.sub, "units of a pass");
 
@@ -1654,14 +1707,15 @@ extern "C" void ops_attention_blocks(struct ops *o, struct opnd Q, struct opnd K
         }
         else {
             const int lists = count32((long long)nhk * p.nblk * p.sub, "units of keys");
-            /* Splits of a list: enough blocks of threads, each of which has
-             * some 256 rows to compute. */
-            const long long each = max(1LL, (long long)a.Nq * g * top / p.nblk / icoreg_blk_each);
+            /* Splits of a list: 8 blocks of threads a CU, if each of them has
+             * some 256 rows to compute (4 a CU 274, 8 251, 8 of 128 rows 255 us
+             * for 8192 x 8 rows of 256 blocks). */
+            const long long each = max(1LL, (long long)a.Nq * g * top / p.nblk / 256);
             const int chunks = (a.tiles * 64 + BLK_PIECE - 1) / BLK_PIECE;
 
             a.pieces = (int)max((chunks + BLK_CHUNKS - 1LL) / BLK_CHUNKS,
                                 min(min(each, (long long)chunks),
-                                    (icoreg_blk_mul * o->ocl->cu_count + lists - 1LL) / lists));
+                                    (8LL * o->ocl->cu_count + lists - 1LL) / lists));
             hipLaunchKernelGGL(blk_bits_kernel, dim3(a.tiles / BLK_TW, nhk), dim3(64 * BLK_TW), 0, s,
                                a);
             launch_check("attention_blocks bits");

@@ -23,6 +23,8 @@
 using namespace icoreg;
 
 #define Q8_MAX_IN (1 << 17)
+#define Q8_MAX_C (1 << 30)        /* channels are counted in int, past the last too */
+#define Q8_ROWS (1L << 23)        /* rows of a launch: 2^32 threads are too many */
 
 typedef int q8_i4 __attribute__((ext_vector_type(4)));
 typedef int q8_i16 __attribute__((ext_vector_type(16)));
@@ -93,30 +95,34 @@ static void quant_rows(struct ops *o, long rows, int C, const float *X, long lon
     /* Long rows, a block each: 4096 channels, 16 rows 4.2 -> 2.7 us, 785 rows 6.5
      * -> 3.7. */
     const bool wide = C > 1024;
-    const dim3 grid((unsigned)(wide ? rows : (rows + 3) / 4)), block(256);
     const hipStream_t s = stream_of(o->ocl);
 
     prof_scope ps(o->ocl, "quant_rows");
-#define QUANT_LAUNCH(NV_, W_)                                                               \
-    hipLaunchKernelGGL((quant_rows_kernel<NV_, W_>), grid, block, 0, s, X, ldx, rows, C,    \
-                       (unsigned *)Q, S)
-    if (C <= 256)
-        QUANT_LAUNCH(1, 1);
-    else if (C <= 1024)
-        QUANT_LAUNCH(4, 1);
-    else if (C <= 4096)
-        QUANT_LAUNCH(4, 4);
-    else if (C <= 16384)
-        QUANT_LAUNCH(16, 4);
-    else
-        QUANT_LAUNCH(0, 4);
+    for (long r = 0; r < rows; r += Q8_ROWS) {
+        const long n = rows - r < Q8_ROWS ? rows - r : Q8_ROWS;
+        const dim3 grid((unsigned)(wide ? n : (n + 3) / 4)), block(256);
+
+#define QUANT_LAUNCH(NV_, W_)                                                                 \
+    hipLaunchKernelGGL((quant_rows_kernel<NV_, W_>), grid, block, 0, s, X + r * ldx, ldx, n, C, \
+                       (unsigned *)((char *)Q + r * q8_pitch(C)), S + r)
+        if (C <= 256)
+            QUANT_LAUNCH(1, 1);
+        else if (C <= 1024)
+            QUANT_LAUNCH(4, 1);
+        else if (C <= 4096)
+            QUANT_LAUNCH(4, 4);
+        else if (C <= 16384)
+            QUANT_LAUNCH(16, 4);
+        else
+            QUANT_LAUNCH(0, 4);
 #undef QUANT_LAUNCH
-    launch_check("quant_rows");
+        launch_check("quant_rows");
+    }
 }
 
 extern "C" int ops_q8_pitch(int C)
 {
-    return C < 1 || C > 0x7fffffff - Q8_PITCH ? 0 : (int)q8_pitch(C);
+    return C < 1 || C > Q8_MAX_C ? 0 : (int)q8_pitch(C);
 }
 
 extern "C" void ops_quant_rows(struct ops *o, long rows, int C, cl_mem X, long xoff, int ldx,
@@ -125,7 +131,7 @@ extern "C" void ops_quant_rows(struct ops *o, long rows, int C, cl_mem X, long x
     ICOREG_API_BEGIN
     const char *op = "ops_quant_rows";
 
-    if (rows < 0 || rows > 0x7fffffffL || C < 1 || C > 0x7fffffff - Q8_PITCH || ldx < C || xoff < 0)
+    if (rows < 0 || rows > 0x7fffffffL || C < 1 || C > Q8_MAX_C || ldx < C || xoff < 0)
         icoreg_fatal("%s: invalid sizes rows=%ld C=%d ldx=%d", op, rows, C, ldx);
     if (rows == 0)
         return;
@@ -743,7 +749,8 @@ static q8_args q8_make(const char *op, int rows, int in, int out, cl_mem WQ, cl_
         need_floats(R, roff, span, op, "R");
     need_apart(Y, yoff * 4, span * 4, WQ, 0, out * q8_pitch(in), op, "Y and WQ");
     if (R && cfptr(R) + roff != cfptr(Y) + yoff)
-        need_apart(Y, yoff * 4, span * 4, R, roff * 4, span * 4, op, "Y and R (unless the same)");
+        need_rows_apart(cfptr(Y) + yoff, ldy, out, rows, cfptr(R) + roff, ldy, out, rows, op,
+                        "Y and R (unless the same)");
     g.M = rows;
     g.N = out;
     g.pitch = q8_pitch(in);
@@ -806,7 +813,7 @@ extern "C" void ops_linear_q8(struct ops *o, int rows, int in, int out, cl_mem X
     need_aligned(work, 16, op, "work");
     need_apart(X, xoff * 4, xbytes, work, 0, codes + rows * 4LL, op, "X and work");
     need_apart(Y, yoff * 4, ybytes, work, 0, codes + rows * 4LL, op, "Y and work");
-    need_apart(Y, yoff * 4, ybytes, X, xoff * 4, xbytes, op, "Y and X");
+    need_rows_apart(cfptr(Y) + yoff, ldy, out, rows, cfptr(X) + xoff, ldx, in, rows, op, "Y and X");
     g.A = (const signed char *)work->ptr;
     g.sa = (const float *)((const char *)work->ptr + codes);
     {

@@ -204,6 +204,16 @@ extern "C" void ops_rope_pos(struct ops *o, long rows, int d, int rot, int axes,
     }
     a.s[0] = rope_make(op, rows, d, nh1, X1, Y1, "X1 or Y1");
     a.s[1] = rope_make(op, rows, d, nh2, X2, Y2, "X2 or Y2");
+    for (const rope_side &p : a.s) {
+        const long long span = (rows - 1) * p.ldy + (long long)p.nh * d;
+
+        if (!p.nh || !rot)
+            continue;
+        need_rows_apart(p.y, span, span, 1, (const float *)pos->ptr, rows * (long long)axes,
+                        rows * (long long)axes, 1, op, "an output and pos");
+        need_rows_apart(p.y, span, span, 1, (const float *)freq->ptr, rot, rot, 1, op,
+                        "an output and freq");
+    }
     for (int i = 0; i < 2; i++)
         for (int j = 0; j < 2; j++) {
             const rope_side &p = a.s[i], &q = a.s[j];

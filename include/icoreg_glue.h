@@ -101,6 +101,11 @@ int icoreg_conv5_choice(struct ops *o, int nb, int C, int H, int W, int K, int p
  * tokens x channels, 4, 5 blocks of 32, 16 tokens x 16 channels; -1 for sizes
  * that it refuses. For tests. */
 int icoreg_q8_choice(struct ops *o, int rows, int in, int out, int *first);
+/* What the library runs for ops_block_select: 0 a wave a row, 1 sixteen waves a
+ * row, 2 tiles of 16 rows; and for ops_attention_blocks: 0 the units one by one,
+ * 1 lists of the rows of each (-1: sizes that it refuses). For tests. */
+int icoreg_select_choice(struct ops *o, int Nq, int nh, int nhk, int nblk, int top);
+int icoreg_blocks_choice(int Nq, int Nk, int nh, int nhk, int d, int bs, int top);
 /* How many times roma_match has re-run a GP solve through
  * roma_gp_solve_events after the in-kernel wait gave up. */
 int icoreg_roma_gp_retries(const struct roma_model *m);

@@ -118,7 +118,25 @@ SHAPES = [
     # Many queries for few blocks: lists of rows.
     (700, 300, 4, 4, 64, 64, 3, 0, 0, 0), (650, 333, 4, 2, 32, 32, 4, 1, 0, 0), (600, 100, 4, 1, 128, 64, 2, 1, 0, 4),
     (900, 270, 2, 2, 33, 16, 7, 0, 1, 1), (800, 500, 4, 2, 40, 128, 2, 1, 0, 0), (513, 257, 8, 8, 65, 64, 4, 0, 0, 0),
-    (2100, 129, 4, 4, 16, 16, 9, 1, 0, 0), (520, 1024, 8, 1, 64, 32, 16, 0, 0, 0), (560, 210, 8, 4, 128, 128, 1, 0, 0, 0)]
+    (2100, 129, 4, 4, 16, 16, 9, 1, 0, 0), (520, 1024, 8, 1, 64, 32, 16, 0, 0, 0), (560, 210, 8, 4, 128, 128, 1, 0, 0, 0),
+    (1200, 150, 4, 2, 32, 64, 3, 1, 0, 0), (1300, 200, 4, 4, 20, 64, 3, 0, 1, 2), (700, 120, 4, 4, 128, 32, 3, 1, 0, 0),
+    (700, 120, 4, 2, 90, 32, 3, 0, 2, 0)]
+MANY = [(1, 20000), (300, 3000), (3000, 40), (4100, 300), (2100, 128), (4100, 500), (130, 2000)]
+
+
+def test_every_kernel_is_among_the_shapes(dev, ic):
+    """The shapes below and those of the selection's own tests reach every
+    selection, the units one by one and by lists, of every width."""
+    lib, how, sel = ic.lib(), set(), set()
+    for nq, nk, h, kv, d, bs, top, *_ in SHAPES:
+        lists = lib.icoreg_blocks_choice(nq, nk, h, kv, d, bs, top)
+        how.add((lists, min(128, 32 << max(0, (d - 1) // 32)), lists and min(bs, 64) > 32, lists and d in (32, 64, 128)))
+        sel.add(lib.icoreg_select_choice(dev.po, nq, h, kv, -(-nk // bs), top))
+    assert {(0, d, 0, 0) for d in (32, 64, 128)} <= how
+    assert {(1, d, k, f) for d in (32, 64, 128) for k in (False, True) for f in (False, True)} <= how
+    for rows, n in MANY:
+        sel.add(lib.icoreg_select_choice(dev.po, rows, 2, 1, n, 16))
+    assert sel == {0, 1, 2}
 
 
 @pytest.mark.parametrize("shape", SHAPES, ids=[str(s) for s in SHAPES])
@@ -154,19 +172,27 @@ def test_refreshed_index(dev, ic):
     assert (ks[rest] == 99).all() and (kc[rest] == 99).all()
 
 
-@pytest.mark.parametrize("n,top", [(5, 5), (64, 8), (65, 64), (513, 16), (1100, 64), (1600, 3), (9000, 20)])
-def test_selection_of_ties(n, top, dev, ic):
+# Few queries, and enough for tiles of rows.
+TIES = [(5, 5), (64, 8), (65, 32), (65, 64), (200, 16), (256, 17), (500, 9), (513, 16), (1100, 64), (1600, 3), (9000, 20)]
+
+
+@pytest.mark.parametrize("n,top,nq", [t + (9,) for t in TIES] + [t + (2100,) for t in TIES if t[0] <= 513])
+def test_selection_of_ties(n, top, nq, dev, ic):
     """Scores that repeat, zeros of both signs, scales of zero, blocks without
     keys and NaN scales: lower blocks first."""
-    print(f"[blocks] ties {n} {top}", flush=True)
+    print(f"[blocks] ties {n} {top} {nq}", flush=True)
     rng = np.random.default_rng(n)
-    kv, d, h, nq = 2, 16, 4, 9
+    kv, d, h = 2, 16, 4
     kc = rng.integers(-2, 3, (n, kv, d)).astype(np.int8)
     ks = rng.choice([0.5, 0.5, 1.0, 0.0, -1.0], (n, kv)).astype(np.float32)
     if n > 500:
         ks[rng.integers(0, n, 3), 0] = np.nan
     q = rng.integers(-1, 2, (nq, h, d)).astype(np.float32)
     q[:, :, 0] = 2
+    if nq > 9:
+        # Scores that differ, too, and rows that go their own way among them.
+        q[:1500] = rng.standard_normal((1500, h, d))
+        q[700:703, 1] = np.inf
     q[1] = 0
     q[2, 1, 3], q[3, 2, 0], q[4] = np.nan, -np.inf, 1e-38
     full = np.zeros((n, kv, 64), np.int8)
@@ -179,7 +205,7 @@ def test_selection_of_ties(n, top, dev, ic):
     assert np.array_equal(got, ref.select(q, kc, ks, top))
 
 
-@pytest.mark.parametrize("rows,n", [(1, 20000), (300, 3000), (3000, 40)])
+@pytest.mark.parametrize("rows,n", MANY)
 def test_selection_of_many(rows, n, dev, ic):
     print(f"[blocks] many {rows} {n}", flush=True)
     rng = np.random.default_rng(rows)
@@ -196,7 +222,7 @@ def test_selection_of_many(rows, n, dev, ic):
 
 # Few queries, and enough for lists.
 @pytest.mark.parametrize("nq", [3, 900])
-@pytest.mark.parametrize("bs,d", [(64, 64), (32, 128), (128, 32), (16, 100)])
+@pytest.mark.parametrize("bs,d", [(64, 64), (32, 128), (128, 32), (16, 100), (32, 64)])
 def test_lists_that_a_caller_makes(nq, bs, d, dev, ic):
     """Entries that are no block are skipped, blocks listed twice count once,
     rows that list nothing or only left-out keys are zero."""
@@ -232,7 +258,7 @@ def test_no_keys(nq, dev, ic):
     assert not c.out().any()
 
 
-@pytest.mark.parametrize("nq", [4, 600])
+@pytest.mark.parametrize("nq", [4, 800])
 @pytest.mark.parametrize("d", [32, 64, 128])
 def test_values_that_are_not_finite(nq, d, dev, ic):
     """In left-out keys and values they do not matter; kept ones give what
@@ -282,7 +308,7 @@ def test_values_that_are_not_finite(nq, d, dev, ic):
     assert np.allclose(got[~up, 4], want[~up], rtol=0, atol=1e-5)
 
 
-@pytest.mark.parametrize("nq", [3, 600])
+@pytest.mark.parametrize("nq", [3, 2400])
 @pytest.mark.parametrize("d", [32, 64, 128])
 def test_scores_far_from_zero(nq, d, dev, ic):
     """Every score near -2^120 or 2^100: each query takes its best key's
@@ -304,7 +330,7 @@ def test_scores_far_from_zero(nq, d, dev, ic):
             assert np.allclose(got[:, i], v[best[i], i], rtol=8 * U, atol=0)
 
 
-@pytest.mark.parametrize("nq", [2, 640])
+@pytest.mark.parametrize("nq", [2, 640, 3000])
 @pytest.mark.parametrize("eq,ek,ev", [(-116, 116, 0), (90, -90, 0), (0, 0, -116), (0, 0, 60)])
 def test_powers_of_two(eq, ek, ev, nq, dev, ic):
     """Scaling queries against keys, or values, by powers of two changes no
@@ -325,13 +351,13 @@ def test_powers_of_two(eq, ek, ev, nq, dev, ic):
         dev.write(c.SEL, sel)
         c.attend()
         outs.append(c.out())
-    if ev > -100:
+    if ev > -100 or nq == 3000:  # lists: values are scaled
         assert np.array_equal(outs[1], np.ldexp(outs[0], ev))
     else:
         assert np.all(np.abs(np.ldexp(outs[1].astype(np.float64), -ev) - outs[0]) <= 6 * U * np.abs(outs[0]))
 
 
-@pytest.mark.parametrize("nq", [3, 700])
+@pytest.mark.parametrize("nq", [3, 1500])
 def test_output_in_place_and_packed(nq, dev, ic):
     """The output over the queries, in the middle of packed rows."""
     print(f"[blocks] in place {nq}", flush=True)
@@ -351,7 +377,7 @@ def test_output_in_place_and_packed(nq, dev, ic):
     assert np.array_equal(got[:, 0], k) and np.array_equal(got[:, 2], v)
 
 
-@pytest.mark.parametrize("nq", [1, 600])
+@pytest.mark.parametrize("nq", [1, 2500])
 def test_long_cache_offsets(nq, dev, ic):
     """Keys and values whose rows lie past 2^31 floats."""
     print(f"[blocks] long offsets {nq}", flush=True)
@@ -431,9 +457,9 @@ def test_results_do_not_depend_on_the_other_queries(dev, ic):
     nothing with it but the keys (both of many queries)."""
     print("[blocks] other queries", flush=True)
     h, kv, d, nk, bs, top = 4, 2, 64, 300, 64, 2
-    q, k, v, _ = draw(1400, nk, h, kv, d)
+    q, k, v, _ = draw(3000, nk, h, kv, d)
     outs = []
-    for lo, hi in ((0, 1400), (600, 1400), (0, 701)):
+    for lo, hi in ((0, 3000), (1400, 3000), (0, 1501)):
         c = Case(dev, ic, q[lo:hi], k, v, bs, top, 0.125)
         c.index()
         c.select()

@@ -53,7 +53,8 @@ def test_work_stays_bounded(ic):
 def test_quant_rows(ic, env):
     a, o, v = env
     x, q, s = v(0, 4000), v(8192, 2560), v(16384, 40)
-    for sizes in ((-1, 100, 100), (10, 0, 100), (10, 100, 99), (1 << 31, 1, 1)):
+    for sizes in ((-1, 100, 100), (10, 0, 100), (10, 100, 99), (1 << 31, 1, 1),
+                  (1, (1 << 30) + 1, 1 << 31 - 1)):
         with refused(ic, "ops_quant_rows: invalid sizes"):
             a.ops_quant_rows(o, sizes[0], sizes[1], x, 0, sizes[2], q, s)
     with refused(ic, "ops_quant_rows: X accessed"):
@@ -151,6 +152,10 @@ def test_rope(ic, env):
     with refused(ic, "an output and an input"):
         # Keys over the queries' inputs.
         rope(n2=1, x2=op(z, 0, 16), y2=op(x, 48, 64))
+    for bad, match in ((dict(y1=op(pos, 0, 64), rows=1, n1=1, d=8, rot=8, x1=op(x, 0, 64)), "an output and pos"),
+                       (dict(y1=op(freq, 0, 64), rows=1, n1=1, d=8, rot=8, x1=op(x, 0, 64)), "an output and freq")):
+        with refused(ic, match):
+            rope(**bad)
     with refused(ic, "Y1 and Y2"):
         rope(n2=1, x2=op(z, 0, 16), y2=op(y, 63, 64))
     rope(rows=0)
@@ -193,6 +198,7 @@ def test_blocks(ic, env):
     a, o, v = env
     M = 1 << 22
     q, k, val, out, kc, ks, sel, mask, work = (v(i * M, M) for i in range(9))
+    kb, vb, qb, ob = k, val, q, out
     op = lambda b, off, ld: ic.Opnd(b, off, ld, 0, 0)  # noqa: E731
     nq, nk, h, kv, d, bs, top = 20, 100, 4, 2, 32, 16, 3
 
@@ -206,7 +212,8 @@ def test_blocks(ic, env):
                        (dict(k=op(k, -1, 64)), "invalid sizes"), (dict(k=op(k, M // 4 - 6399, 64)), "K accessed"),
                        (dict(mask=v(0, 99)), "kmask accessed"), (dict(kc=v(0, 14 * 64 - 1)), "KC accessed"),
                        (dict(ks=v(0, 14 * 4 - 1)), "KS accessed"), (dict(kc=v(8, M)), "KC does not start"),
-                       (dict(nk=2 ** 31 - 1, nb=0), "invalid sizes")):
+                       (dict(nk=2 ** 31 - 1, nb=0), "invalid sizes"), (dict(kc=kb), "KC and K"),
+                       (dict(ks=kb), "KS and K"), (dict(ks=kc), "KC and KS")):
         with refused(ic, "ops_block_index: .*" + match):
             index(**bad)
     index(nb=0)
@@ -219,7 +226,8 @@ def test_blocks(ic, env):
                        (dict(n=-1), "invalid sizes"), (dict(q=op(q, 0, 127)), "invalid sizes"),
                        (dict(q=op(q, M // 4 - 2559, 128)), "Q accessed"), (dict(kc=v(0, 14 * 64 - 1)), "KC accessed"),
                        (dict(ks=None), "KS is NULL"), (dict(sel=v(0, 959)), "SEL accessed"),
-                       (dict(kc=v(8, M)), "KC does not start")):
+                       (dict(kc=v(8, M)), "KC does not start"), (dict(sel=qb), "SEL and Q"),
+                       (dict(sel=kc), "SEL and KC"), (dict(sel=ks), "SEL and KS")):
         with refused(ic, "ops_block_select: .*" + match):
             select(**bad)
     select(nq=0)
@@ -228,7 +236,6 @@ def test_blocks(ic, env):
                d=d, bs=bs, top=top, sel=sel, mask=mask, work=work):
         a.ops_attention_blocks(o, q, k, val, out, nq, nk, h, kv, d, bs, top, sel, 0.2, mask, work)
 
-    kb, vb, qb, ob = (v(i * M, M) for i in (1, 2, 0, 3))
     for bad, match in ((dict(d=129), "invalid sizes"), (dict(bs=8), "invalid sizes"), (dict(top=65), "invalid sizes"),
                        (dict(kv=3), "invalid sizes"), (dict(nk=-1), "invalid sizes"), (dict(nq=-1), "invalid sizes"),
                        (dict(q=op(qb, 0, 127)), "short row"), (dict(val=op(vb, 0, 63)), "short row"),
@@ -240,7 +247,7 @@ def test_blocks(ic, env):
                        (dict(work=None), "work is NULL"), (dict(work=v(8 * M + 4, M)), "work does not start"),
                        (dict(out=op(qb, 4, 128)), "O and Q"), (dict(out=op(kb, 0, 128)), "O and K"),
                        (dict(out=op(vb, 0, 128)), "O and V"), (dict(work=ob), "O and work"),
-                       (dict(work=sel), "SEL and work")):
+                       (dict(work=sel), "SEL and work"), (dict(sel=ob), "SEL and O"), (dict(mask=ob), "kmask and O")):
         with refused(ic, "ops_attention_blocks: .*" + match):
             attend(**bad)
     attend(nq=0)
