@@ -462,15 +462,22 @@ __global__ void __launch_bounds__(64 * Q8_SW)
     constexpr int AHEAD = 4;
     __shared__ __align__(16) signed char xs[FUSED ? Q8_FUSED_BYTES : 16];
     __shared__ q8_i4 sums[Q8_SW][TT][64];
-    __shared__ unsigned tops[16 * TT][Q8_SW];
+    __shared__ unsigned tops[16 * TT];
     __shared__ float scales[16 * TT];
     const int tid = threadIdx.x, lane = tid & 63, c16 = lane & 15, part = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int tiles_n = (g.N + 15) / 16, pitch = (int)g.pitch, nk = pitch / 64;
     const int n0 = blockIdx.x % tiles_n * 16, m0 = blockIdx.x / tiles_n * 16 * TT;
     const signed char *w = g.B + (long long)min(n0 + c16, g.N - 1) * pitch + 16 * part;
+    /* This thread's output: a run of 16 channels a token, in memory's order.
+     * What it needs is read at the start too. */
+    const int n = n0 + tid % 16, tok = tid / 16, m = m0 + tok;
+    const bool mine = tok < 16 * TT && n < g.N && m < g.M;
+    const float sb = mine ? g.sb[n] : 0.0f, bias = mine && g.bias ? g.bias[n] : 0.0f;
+    const float res = mine && g.R ? g.R[m * g.ldc + n] : 0.0f;
     q8_i4 a[AHEAD], acc[TT];
 
+    static_assert(16 * TT * 16 <= 64 * Q8_SW, "an output a thread");
 #pragma unroll
     for (int t = 0; t < TT; t++)
         acc[t] = q8_i4{0, 0, 0, 0};
@@ -478,45 +485,65 @@ __global__ void __launch_bounds__(64 * Q8_SW)
     for (int e = 0; e < AHEAD; e++)
         a[e] = *(const q8_i4 *)(w + 64 * min(wave + Q8_SW * e, nk - 1));
     if constexpr (FUSED) {
-        /* 1, 2, 4 or 8 waves a token. */
-        const int tokens = min(16 * TT, g.M - m0);
-        const int each = tokens > 4 ? 1 : tokens > 2 ? 2 : tokens > 1 ? 4 : 8;
-        const int first = wave / each, sub = wave % each, step = 64 * each;
+        /* Pieces of 256 channels of a token, dealt to the waves; the first
+         * HOLD of a wave's stay in registers from the maximum to the codes. */
+        constexpr int HOLD = 8;
+        const int tokens = min(16 * TT, g.M - m0), pieces = (pitch + 255) / 256;
+        const int all = tokens * pieces;
+        float v[HOLD][4];
+        auto fetch = [&](int e, float (&x)[4]) {
+            const int t = e / pieces, c = 256 * (e - t * pieces) + 4 * lane;
 
-        for (int m = first; m < tokens; m += Q8_SW / each) {
-            const float *x = X + (m0 + m) * ldx;
-            unsigned top = 0;
+            load4_row(X + (m0 + t) * ldx, c, in, x);
+            return t;
+        };
 
-            for (int c = sub * 64 + lane; 4 * c < in; c += step) {
-                float v[4];
+#pragma unroll
+        for (int e = 0; e < HOLD; e++)
+            if (wave + Q8_SW * e < all)
+                fetch(wave + Q8_SW * e, v[e]);
+        if (tid < 16 * TT)
+            tops[tid] = 0;
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < HOLD; e++)
+            if (wave + Q8_SW * e < all) {
+                const unsigned top = wave_umax(max(max(q8_mag(v[e][0]), q8_mag(v[e][1])),
+                                                   max(q8_mag(v[e][2]), q8_mag(v[e][3]))));
 
-                load4_row(x, 4 * c, in, v);
-                top = max(max(max(q8_mag(v[0]), q8_mag(v[1])), max(q8_mag(v[2]), q8_mag(v[3]))),
-                          top);
+                if (lane == 0)
+                    atomicMax(&tops[(wave + Q8_SW * e) / pieces], top);
             }
-            top = wave_umax(top);
+        for (int e = wave + Q8_SW * HOLD; e < all; e += Q8_SW) {
+            float x[4];
+            const int t = fetch(e, x);
+            const unsigned top =
+                wave_umax(max(max(q8_mag(x[0]), q8_mag(x[1])), max(q8_mag(x[2]), q8_mag(x[3]))));
+
             if (lane == 0)
-                tops[m][sub] = top;
+                atomicMax(&tops[t], top);
         }
         __syncthreads();
-        for (int m = first; m < tokens; m += Q8_SW / each) {
-            const float *x = X + (m0 + m) * ldx;
-            unsigned *out = (unsigned *)(xs + m * (pitch + 16));
-            unsigned top = 0;
+        auto code = [&](int e, const float (&x)[4]) {
+            const int t = e / pieces, c = 64 * (e - t * pieces) + lane;
+            const q8_scale q = q8_scale_of(tops[t]);
 
-            for (int e = 0; e < each; e++)
-                top = max(top, tops[m][e]);
-            const q8_scale q = q8_scale_of(top);
+            if (4 * c < pitch)
+                ((unsigned *)(xs + t * (pitch + 16)))[c] = q8_code4(x[0], x[1], x[2], x[3], q.r);
+        };
 
-            for (int c = sub * 64 + lane; c < pitch / 4; c += step) {
-                float v[4];
+#pragma unroll
+        for (int e = 0; e < HOLD; e++)
+            if (wave + Q8_SW * e < all)
+                code(wave + Q8_SW * e, v[e]);
+        for (int e = wave + Q8_SW * HOLD; e < all; e += Q8_SW) {
+            float x[4];
 
-                load4_row(x, 4 * c, in, v);
-                out[c] = q8_code4(v[0], v[1], v[2], v[3], q.r);
-            }
-            if (sub == 0 && lane == 0)
-                scales[m] = q.s;
+            fetch(e, x);
+            code(e, x);
         }
+        if (tid < tokens)
+            scales[tid] = q8_scale_of(tops[tid]).s;
         __syncthreads();
     }
     for (int k = wave; k < nk; k += Q8_SW * AHEAD) {
@@ -548,22 +575,17 @@ __global__ void __launch_bounds__(64 * Q8_SW)
     for (int t = 0; t < TT; t++)
         sums[wave][t][lane] = acc[t];
     __syncthreads();
-    /* Sum r of lane l: channel 4 (l / 16) + r, token l % 16. Outputs in the
-     * order of memory, a run of 16 channels a token. */
-    for (int e = tid; e < 256 * TT; e += 64 * Q8_SW) {
-        const int n = n0 + e % 16, tok = e / 16, m = m0 + tok;
-        const int l = e % 16 / 4 * 16 + tok % 16;
+    /* Sum r of lane l: channel 4 (l / 16) + r, token l % 16. */
+    if (mine) {
+        const int l = tid % 16 / 4 * 16 + tok % 16;
         int v = 0;
 
 #pragma unroll
         for (int q = 0; q < Q8_SW; q++)
-            v += ((const int *)&sums[q][tok / 16][l])[e % 4];
-        if (n < g.N && m < g.M) {
-            const float sa = FUSED ? scales[tok] : g.sa[m];
-            const float y = q8_out<ACT>(v, sa, g.sb[n], g.bias ? g.bias[n] : 0.0f, g.slope);
+            v += ((const int *)&sums[q][tok / 16][l])[tid % 4];
+        const float y = q8_out<ACT>(v, FUSED ? scales[tok] : g.sa[m], sb, bias, g.slope);
 
-            g.C[m * g.ldc + n] = g.R ? y + g.R[m * g.ldc + n] : y;
-        }
+        g.C[m * g.ldc + n] = g.R ? y + res : y;
     }
 }
 
