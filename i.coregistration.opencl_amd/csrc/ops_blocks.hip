@@ -23,6 +23,8 @@
 
 #include <math.h>
 
+#include <type_traits>
+
 #include "common.h"
 #include "gemm_dev.h"
 #include "load4.h"
@@ -205,9 +207,9 @@ template <class F> __device__ __forceinline__ int wave_fold(int v, F f)
 /* The top `top` of a wave's candidates, slot j of lane l before slot j of
  * lane l + 1 before slot j + 1, equal keys in that order: returned sorted,
  * candidate i in lane i of (key, idx), SEL_NONE behind the last. A threshold
- * that between top and 64 of them reach is found, and those are ranked; it
- * starts at the smallest of at least top maxima of groups of lanes and
- * mostly stays there. list: 2 x 64 words of LDS of this wave. */
+ * that between top and top + 8 of them reach is found (or 64, where equal ones
+ * allow no other), and those are ranked; it starts at the smallest of at least
+ * top maxima of groups of lanes, a few halvings away. list: 2 x 64 words of LDS of this wave. */
 template <int N>
 __device__ __forceinline__ void sel_top(const int (&k)[N], const int (&i)[N], int top, int *list,
                                         int &key, int &idx)
@@ -248,7 +250,9 @@ __device__ __forceinline__ void sel_top(const int (&k)[N], const int (&i)[N], in
     }
     int nlo = count(lo), nhi = 0;
 
-    for (int step = 0; nlo > 64 && (unsigned)hi - (unsigned)lo > 1; step++) {
+    const int most_wanted = min(64, top + 8);
+
+    for (int step = 0; nlo > most_wanted && (unsigned)hi - (unsigned)lo > 1; step++) {
         int mid = (int)((unsigned)lo + ((unsigned)hi - (unsigned)lo) / 2);
 
         if (step < 16) {
@@ -298,10 +302,14 @@ __device__ __forceinline__ void sel_top(const int (&k)[N], const int (&i)[N], in
     const int mine = list[lane], who = list[64 + lane];
     int rank = 0;
 
-    for (int j = 0; j < at; j++) {
-        const int other = __builtin_amdgcn_readlane(mine, j);
+    /* Four at a time; behind the last there is SEL_NONE. */
+    for (int j0 = 0; j0 < at; j0 += 4) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const int other = __builtin_amdgcn_readlane(mine, j0 + e);
 
-        rank += other + (j < lane) > mine;
+            rank += other + (j0 + e < lane) > mine;
+        }
     }
     __builtin_amdgcn_wave_barrier();
     if (lane < at) {
@@ -416,16 +424,24 @@ __global__ void __launch_bounds__(64 * W) block_select_kernel(const sel_args a)
         __syncthreads();
         if (wave)
             return;
-        int k[W], i[W];
+        auto join = [&](auto n) {
+            constexpr int N = decltype(n)::value;
+            int k[N], i[N];
 
 #pragma unroll
-        for (int w = 0; w < W; w++) {
-            const int at = 64 * w + lane;
+            for (int w = 0; w < N; w++) {
+                const int at = 64 * w + lane;
 
-            k[w] = at < W * a.top ? best[at] : SEL_NONE;
-            i[w] = at < W * a.top ? best[W * 64 + at] : -1;
-        }
-        sel_top(k, i, a.top, lists[0], key, idx);
+                k[w] = at < W * a.top ? best[at] : SEL_NONE;
+                i[w] = at < W * a.top ? best[W * 64 + at] : -1;
+            }
+            sel_top(k, i, a.top, lists[0], key, idx);
+        };
+
+        if (a.top <= 16)
+            join(std::integral_constant<int, W / 4>());
+        else
+            join(std::integral_constant<int, W>());
     }
     if (lane < a.top)
         a.SEL[(long long)row * a.top + lane] = key == SEL_NONE ? -1 : idx;
