@@ -58,6 +58,9 @@ void need_rows_apart(const float *p, long long ldp, long long wp, long long rp, 
 /* Element counts handed to kernels as int (ops.c:79-84). */
 int count32(long long n, const char *what);
 
+/* Blocks of a launch: fewer than 2^31, their threads fewer than 2^32. */
+unsigned grid_of(long long blocks, int threads, const char *what);
+
 inline float *fptr(cl_mem b) { return b ? (float *)b->ptr : nullptr; }
 inline const float *cfptr(cl_mem b) { return b ? (const float *)b->ptr : nullptr; }
 

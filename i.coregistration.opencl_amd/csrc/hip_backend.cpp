@@ -104,6 +104,13 @@ int count32(long long n, const char *what)
     return (int)n;
 }
 
+unsigned grid_of(long long blocks, int threads, const char *what)
+{
+    if (blocks * threads > 0xffffffffLL)
+        icoreg_fatal("HIP: %s: %lld blocks of %d threads exceed a launch", what, blocks, threads);
+    return (unsigned)count32(blocks, what);
+}
+
 void launch_check(const char *what)
 {
     hipError_t e = hipGetLastError();

@@ -153,8 +153,10 @@ extern "C" void ops_block_index(struct ops *o, struct opnd K, int Nk, int nhk, i
         need_apart(KC, 0, cells * q8_pitch(d), K.buf, K.off * 4, kbytes, op, "KC and K");
         need_apart(KS, 0, cells * 4, K.buf, K.off * 4, kbytes, op, "KS and K");
         need_apart(KC, 0, cells * q8_pitch(d), KS, 0, cells * 4, op, "KC and KS");
+        need_apart(KC, 0, cells * q8_pitch(d), kmask, 0, Nk, op, "KC and kmask");
+        need_apart(KS, 0, cells * 4, kmask, 0, Nk, op, "KS and kmask");
     }
-    const int grid = count32((long long)nb * nhk, "block index");
+    const unsigned grid = grid_of((long long)nb * nhk, 256, "block index");
 
     prof_scope ps(o->ocl, "block_index");
 #define INDEX_LAUNCH(L_)                                                                       \
@@ -720,8 +722,8 @@ extern "C" void ops_block_select(struct ops *o, struct opnd Q, int Nq, int nh, i
         icoreg_fatal("%s: head dimension %d is not 1 .. %d", op, d, OPS_MAX_HEAD_DIM);
     if (top < 1 || top > BLK_MAX_TOP)
         icoreg_fatal("%s: %d blocks a query are not 1 .. %d", op, top, BLK_MAX_TOP);
-    if (Nq < 0 || nh < 1 || nhk < 1 || nh % nhk || nblk < 0 || Q.off < 0 ||
-        Q.ld < (long long)nh * d)
+    if (Nq < 0 || nh < 1 || nhk < 1 || nh % nhk || nblk < 0 || nblk > BLK_MAX_KEYS / 16 + 1 ||
+        Q.off < 0 || Q.ld < (long long)nh * d)
         icoreg_fatal("%s: invalid sizes Nq=%d nh=%d nhk=%d d=%d ld=%d blocks=%d", op, Nq, nh, nhk,
                      d, Q.ld, nblk);
     if (Nq == 0)
@@ -737,10 +739,16 @@ extern "C" void ops_block_select(struct ops *o, struct opnd Q, int Nq, int nh, i
                ((Nq - 1) * (long long)Q.ld + (long long)nh * d) * 4, op, "SEL and Q");
     need_apart(SEL, 0, rows * top * 4, KC, 0, (long long)nblk * nhk * q8_pitch(d), op, "SEL and KC");
     need_apart(SEL, 0, rows * top * 4, KS, 0, (long long)nblk * nhk * 4, op, "SEL and KS");
-    const int grid = count32(rows, "selection rows"), g = nh / nhk;
+    const int form = sel_choose(rows, nhk, nblk, top, o->ocl->cu_count), g = nh / nhk;
+    const unsigned grid =
+        form == SEL_TILE ? 0 : grid_of(rows, form == SEL_WAVES ? 1024 : 64, "selection rows");
+    const unsigned tiles = grid_of(((long long)Nq * g + 16 * SEL_TW - 1) / (16 * SEL_TW), 64 * SEL_TW,
+                                   "selection tiles");
+
+    count32(rows + 64, "selection rows"); /* counted past the last */
     const hipStream_t s = stream_of(o->ocl);
-    sel_args a = {cfptr(Q.buf) + Q.off, (const signed char *)(KC ? KC->ptr : nullptr), cfptr(KS),
-                  (int *)SEL->ptr, Q.ld, Nq, nh, nhk, d, nblk, top};
+    const sel_args a = {cfptr(Q.buf) + Q.off, (const signed char *)(KC ? KC->ptr : nullptr), cfptr(KS),
+                        (int *)SEL->ptr, Q.ld, Nq, nh, nhk, d, nblk, top};
 
     prof_scope ps(o->ocl, "block_select");
 #define SELECT_LAUNCH(W_, P_) \
@@ -752,10 +760,8 @@ extern "C" void ops_block_select(struct ops *o, struct opnd Q, int Nq, int nh, i
         else                      \
             SELECT_LAUNCH(W_, 8); \
     } while (0)
-#define TILE_LAUNCH(T_, K_, C_)                                                              \
-    hipLaunchKernelGGL((block_select_tile<T_, K_, C_>),                                      \
-                       dim3((unsigned)(((long long)Nq * g + 16 * SEL_TW - 1) / (16 * SEL_TW)), nhk), \
-                       dim3(64 * SEL_TW), 0, s, a)
+#define TILE_LAUNCH(T_, K_, C_) \
+    hipLaunchKernelGGL((block_select_tile<T_, K_, C_>), dim3(tiles, nhk), dim3(64 * SEL_TW), 0, s, a)
 #define TILE_WIDTH(T_)             \
     do {                           \
         if (top <= 16 && d <= 64)  \
@@ -767,8 +773,6 @@ extern "C" void ops_block_select(struct ops *o, struct opnd Q, int Nq, int nh, i
         else                       \
             TILE_LAUNCH(T_, 2, 40); \
     } while (0)
-    const int form = sel_choose(rows, nhk, nblk, top, o->ocl->cu_count);
-
     if (form == SEL_TILE) {
         if (nblk <= 64)
             TILE_WIDTH(4);
@@ -1596,8 +1600,9 @@ static blk_plan blk_plan_of(int Nq, int Nk, int nh, int nhk, int d, int bs, int 
      * nothing. */
     const long long units = (long long)p.pass * nh * top * p.sub;
 
-    p.direct = p.nblk == 0 || nhk > 65535 || units * (p.dp + 32) <= 600000 ||
-               (long long)p.pass * g * top < 4LL * p.nblk;
+    /* Lists place their outputs by 32 bits (a query of very many heads passes them). */
+    p.direct = p.nblk == 0 || nhk > 65535 || units * p.dp * 4 > 1LL << 32 ||
+               units * (p.dp + 32) <= 600000 || (long long)p.pass * g * top < 4LL * p.nblk;
     p.tiles = ((p.pass * g + 63) / 64 + BLK_TW - 1) / BLK_TW * BLK_TW;
     p.part = (long long)p.pass * nh * top * p.sub * p.dp * 4;
     p.ml = (long long)p.pass * nh * top * p.sub * 8;
@@ -1670,6 +1675,15 @@ extern "C" void ops_attention_blocks(struct ops *o, struct opnd Q, struct opnd K
                         "O and V");
     }
     need_apart(O.buf, O.off * 4, obytes, work, 0, wbytes, op, "O and work");
+    need_apart(Q.buf, Q.off * 4, ((Nq - 1) * (long long)Q.ld + qw) * 4, work, 0, wbytes, op,
+               "Q and work");
+    if (Nk) {
+        need_apart(K.buf, K.off * 4, ((Nk - 1) * (long long)K.ld + kw) * 4, work, 0, wbytes, op,
+                   "K and work");
+        need_apart(V.buf, V.off * 4, ((Nk - 1) * (long long)V.ld + kw) * 4, work, 0, wbytes, op,
+                   "V and work");
+    }
+    need_apart(kmask, 0, Nk, work, 0, wbytes, op, "kmask and work");
     need_apart(SEL, 0, (long long)Nq * nh * top * 4, O.buf, O.off * 4, obytes, op, "SEL and O");
     if (kmask)
         need_apart(kmask, 0, Nk, O.buf, O.off * 4, obytes, op, "kmask and O");
@@ -1711,7 +1725,7 @@ extern "C" void ops_attention_blocks(struct ops *o, struct opnd Q, struct opnd K
 
         a.tiles = ((a.Nq * g + 63) / 64 + BLK_TW - 1) / BLK_TW * BLK_TW;
         if (p.direct) {
-            const dim3 grid((unsigned)count32(units, "units"));
+            const dim3 grid(grid_of(units, 256, "units"));
 
             if (p.dp == 32)
                 hipLaunchKernelGGL(blk_direct_kernel<32>, grid, dim3(256), 0, s, a);
@@ -1735,7 +1749,7 @@ extern "C" void ops_attention_blocks(struct ops *o, struct opnd Q, struct opnd K
             hipLaunchKernelGGL(blk_bits_kernel, dim3(a.tiles / BLK_TW, nhk), dim3(64 * BLK_TW), 0, s,
                                a);
             launch_check("attention_blocks bits");
-            const dim3 grid((unsigned)count32((long long)lists * a.pieces, "lists"));
+            const dim3 grid(grid_of((long long)lists * a.pieces, 256, "lists"));
 
 #define UNIT_LAUNCH(ND_, NB_)                                                                 \
     do {                                                                                      \
@@ -1764,7 +1778,7 @@ extern "C" void ops_attention_blocks(struct ops *o, struct opnd Q, struct opnd K
         /* Both, us: 51200 rows of 8 units of 32 channels 21.1, 10.8; 25616 of 8 of
          * 64 12.6, 10.5; 65536 of 16 of 64 43.4, 52.0. */
         const bool few = top * p.sub <= 8;
-        const dim3 grid((unsigned)count32(few ? (rows + 15) / 16 : (rows + 3) / 4, "merge"));
+        const dim3 grid(grid_of(few ? (rows + 15) / 16 : (rows + 3) / 4, 256, "merge"));
 
 #define MERGE_LAUNCH(DP_)                                                           \
     do {                                                                            \

@@ -25,6 +25,7 @@ using namespace icoreg;
 #define Q8_MAX_IN (1 << 17)
 #define Q8_MAX_C (1 << 30)        /* channels are counted in int, past the last too */
 #define Q8_ROWS (1L << 23)        /* rows of a launch: 2^32 threads are too many */
+#define Q8_MAX_SIDE 0x7ffffe00    /* tokens and channels of a product, counted past the last too */
 
 typedef int q8_i4 __attribute__((ext_vector_type(4)));
 typedef int q8_i16 __attribute__((ext_vector_type(16)));
@@ -593,7 +594,7 @@ template <int TT, bool FUSED>
 static void q8_skinny_launch(const q8_args &g, const float *X, long long ldx, int in, hipStream_t s)
 {
     const long long tiles = (long long)((g.N + 15) / 16) * ((g.M + 16 * TT - 1) / (16 * TT));
-    const dim3 grid((unsigned)count32(tiles, "q8 tiles")), block(64 * Q8_SW);
+    const dim3 grid(grid_of(tiles, 64 * Q8_SW, "q8 tiles")), block(64 * Q8_SW);
 
     switch (g.act) {
     case ACT_GELU:
@@ -610,10 +611,12 @@ static void q8_skinny_launch(const q8_args &g, const float *X, long long ldx, in
     }
 }
 
-template <int BM, int BN, int WM, int WN, int BK, int KS, int ST> static void q8_launch(const q8_args &g, hipStream_t s)
+template <int BM, int BN, int WM, int WN, int BK, int KS, int ST>
+static void q8_launch(const q8_args &g, hipStream_t s)
 {
     const long long tiles = (long long)((g.M + BM - 1) / BM) * ((g.N + BN - 1) / BN);
-    const dim3 grid((unsigned)count32(tiles, "q8 tiles")), block(64 * WM * WN * KS);
+    const dim3 grid(grid_of(tiles, 64 * WM * WN * KS, "q8 tiles")), block(64 * WM * WN * KS);
+
     switch (g.act) {
     case ACT_GELU:
         hipLaunchKernelGGL((q8_gemm<BM, BN, WM, WN, BK, KS, ST, ACT_GELU>), grid, block, 0, s, g);
@@ -739,7 +742,7 @@ extern "C" int icoreg_q8_choice(struct ops *o, int rows, int in, int out, int *f
 {
     int n = 0, form;
 
-    if (rows < 1 || in < 1 || in > Q8_MAX_IN || out < 1)
+    if (rows < 1 || rows > Q8_MAX_SIDE || in < 1 || in > Q8_MAX_IN || out < 1 || out > Q8_MAX_SIDE)
         return -1;
     form = q8_choose(rows, out, (int)q8_pitch(in), o->ocl->cu_count, n);
     if (first)
@@ -755,7 +758,8 @@ static q8_args q8_make(const char *op, int rows, int in, int out, cl_mem WQ, cl_
     q8_args g = {};
     const long long span = (long long)(rows - 1) * ldy + out;
 
-    if (rows < 0 || in < 1 || in > Q8_MAX_IN || out < 0 || ldy < out || yoff < 0 || roff < 0)
+    if (rows < 0 || rows > Q8_MAX_SIDE || in < 1 || in > Q8_MAX_IN || out < 0 || out > Q8_MAX_SIDE ||
+        ldy < out || yoff < 0 || roff < 0)
         icoreg_fatal("%s: invalid sizes rows=%d in=%d out=%d ldy=%d", op, rows, in, out, ldy);
     if (act < ACT_NONE || act > ACT_GELU_TANH)
         icoreg_fatal("%s: invalid activation %d", op, act);
@@ -770,6 +774,8 @@ static q8_args q8_make(const char *op, int rows, int in, int out, cl_mem WQ, cl_
     if (R)
         need_floats(R, roff, span, op, "R");
     need_apart(Y, yoff * 4, span * 4, WQ, 0, out * q8_pitch(in), op, "Y and WQ");
+    need_apart(Y, yoff * 4, span * 4, WS, 0, out * 4LL, op, "Y and WS");
+    need_apart(Y, yoff * 4, span * 4, b, 0, out * 4LL, op, "Y and bias");
     if (R && cfptr(R) + roff != cfptr(Y) + yoff)
         need_rows_apart(cfptr(Y) + yoff, ldy, out, rows, cfptr(R) + roff, ldy, out, rows, op,
                         "Y and R (unless the same)");
@@ -802,6 +808,8 @@ extern "C" void ops_linear_qq(struct ops *o, int rows, int in, int out, cl_mem X
     need_floats(XS, 0, rows, op, "XS");
     need_apart(Y, yoff * 4, ((rows - 1) * (long long)ldy + out) * 4, XQ, 0, rows * q8_pitch(in), op,
                "Y and XQ");
+    need_apart(Y, yoff * 4, ((rows - 1) * (long long)ldy + out) * 4, XS, 0, rows * 4LL, op,
+               "Y and XS");
     g.A = (const signed char *)XQ->ptr;
     g.sa = cfptr(XS);
     q8_product(o, g);
@@ -811,7 +819,7 @@ extern "C" void ops_linear_qq(struct ops *o, int rows, int in, int out, cl_mem X
 /* Work of ops_linear_q8: the tokens' codes, then their scales. */
 extern "C" size_t ops_linear_q8_work_bytes(int rows, int in)
 {
-    if (rows < 1 || in < 1 || in > Q8_MAX_IN)
+    if (rows < 1 || rows > Q8_MAX_SIDE || in < 1 || in > Q8_MAX_IN)
         return 0;
     return (size_t)rows * q8_pitch(in) + (size_t)rows * 4;
 }
@@ -824,7 +832,7 @@ extern "C" void ops_linear_q8(struct ops *o, int rows, int in, int out, cl_mem X
     const char *op = "ops_linear_q8";
     q8_args g = q8_make(op, rows, in, out, WQ, WS, b, R, roff, Y, yoff, ldy, act, slope);
     const long long codes = rows * q8_pitch(in), ybytes = ((rows - 1) * (long long)ldy + out) * 4;
-    const long long xbytes = ((rows - 1) * (long long)ldx + in) * 4;
+    const long long xbytes = ((rows - 1) * (long long)ldx + in) * 4, wbytes = codes + rows * 4LL;
 
     if (ldx < in || xoff < 0)
         icoreg_fatal("%s: invalid sizes in=%d ldx=%d", op, in, ldx);
@@ -833,8 +841,12 @@ extern "C" void ops_linear_q8(struct ops *o, int rows, int in, int out, cl_mem X
     need_bytes(X, xoff * 4, xbytes, op, "X");
     need_bytes(work, 0, (long long)ops_linear_q8_work_bytes(rows, in), op, "work");
     need_aligned(work, 16, op, "work");
-    need_apart(X, xoff * 4, xbytes, work, 0, codes + rows * 4LL, op, "X and work");
-    need_apart(Y, yoff * 4, ybytes, work, 0, codes + rows * 4LL, op, "Y and work");
+    need_apart(X, xoff * 4, xbytes, work, 0, wbytes, op, "X and work");
+    need_apart(Y, yoff * 4, ybytes, work, 0, wbytes, op, "Y and work");
+    need_apart(WQ, 0, out * q8_pitch(in), work, 0, wbytes, op, "WQ and work");
+    need_apart(WS, 0, out * 4LL, work, 0, wbytes, op, "WS and work");
+    need_apart(b, 0, out * 4LL, work, 0, wbytes, op, "bias and work");
+    need_apart(R, roff * 4, ybytes, work, 0, wbytes, op, "R and work");
     need_rows_apart(cfptr(Y) + yoff, ldy, out, rows, cfptr(X) + xoff, ldx, in, rows, op, "Y and X");
     g.A = (const signed char *)work->ptr;
     g.sa = (const float *)((const char *)work->ptr + codes);

@@ -195,7 +195,7 @@ extern "C" void ops_rope_pos(struct ops *o, long rows, int d, int rot, int axes,
         axes > 4 || nh1 < 0 || nh2 < 0 || flags & ~(ROPE_INTERLEAVED | ROPE_INVERSE))
         icoreg_fatal("%s: invalid sizes rows=%ld d=%d rot=%d axes=%d nh=%d, %d flags=%d", op, rows,
                      d, rot, axes, nh1, nh2, flags);
-    if (rows == 0 || nh1 + nh2 == 0)
+    if (rows == 0 || (nh1 == 0 && nh2 == 0))
         return;
     if (rot) {
         need_bytes(pos, 0, (long long)rows * axes * 4, op, "pos");
@@ -240,13 +240,13 @@ extern "C" void ops_rope_pos(struct ops *o, long rows, int d, int rot, int axes,
         a.units = in_place ? rot / (2 * v) : (d + 2 * v - 1) / (2 * v);
         if (a.units == 0)
             return;
-        const long long per_row = (long long)(nh1 + nh2) * a.units;
+        const long long per_row = ((long long)nh1 + nh2) * a.units;
         long long n = (2048 + per_row - 1) / per_row;
 
         if (rot)
             n = min(n, 2LL * ROPE_PAIRS / rot);
         n = min(n, (long long)rows);
-        count32(n * per_row, "rope units");
+        count32(n * per_row + 256, "rope units"); /* counted past the end */
         a.pos = pos ? (const int *)pos->ptr : nullptr;
         a.freq = freq ? (const double *)freq->ptr : nullptr;
         a.rows = rows;
@@ -256,7 +256,7 @@ extern "C" void ops_rope_pos(struct ops *o, long rows, int d, int rot, int axes,
         a.block_rows = (int)n;
         a.mult = mult;
         a.sign = flags & ROPE_INVERSE ? -1.0f : 1.0f;
-        const dim3 grid((unsigned)count32((rows + n - 1) / n, "rope blocks")), block(256);
+        const dim3 grid(grid_of((rows + n - 1) / n, 256, "rope blocks")), block(256);
         const hipStream_t s = stream_of(o->ocl);
 
         prof_scope ps(o->ocl, "rope_pos");

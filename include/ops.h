@@ -208,7 +208,7 @@ void ops_quant_rows(struct ops *o, long rows, int C, cl_mem X, long xoff,
  * XS rows tokens, WQ, WS out channels as ops_quant_rows makes them, in <=
  * 2^17 of both, the sum exact in 32-bit integers. Row i of Y starts at float
  * yoff + i ldy; b and R NULL for none, R with Y's row stride from roff, and
- * it may be Y itself. */
+ * it may be Y itself, any other overlap of Y is an error. */
 void ops_linear_qq(struct ops *o, int rows, int in, int out, cl_mem XQ,
                    cl_mem XS, cl_mem WQ, cl_mem WS, cl_mem b, cl_mem R,
                    long roff, cl_mem Y, long yoff, int ldy, int act,
@@ -244,7 +244,8 @@ void ops_rope_freqs(double *freq, int rot, int axes, double base, int kind,
  * / 2). ROPE_INVERSE: by the negative angle, the gradient of the forward
  * call. Xi to Yi, rows at the operands' offsets and ld (packed projections);
  * Yi may be Xi (same offset and ld), any other overlap of an output is an
- * error (rows side by side in one packed buffer do not overlap). rot 0 .. min(d, 2048), even; axes 1 .. 4. */
+ * error (rows side by side in one packed buffer do not overlap). rot 0 ..
+ * min(d, 2048), even; axes 1 .. 4. */
 #define ROPE_INTERLEAVED 1
 #define ROPE_INVERSE 2
 void ops_rope_pos(struct ops *o, long rows, int d, int rot, int axes,
@@ -271,7 +272,7 @@ void ops_block_index(struct ops *o, struct opnd K, int Nk, int nhk, int d,
  * largest scores KS (q . KC), q the query's 8-bit codes, best first, ties to
  * the lower block, NaN above all numbers, -1 behind the last block that keeps
  * a key. The sum of the codes' products is exact: the same selection from
- * every kernel. */
+ * every kernel. No kernel needs work here: the size is 0, work may be NULL. */
 size_t ops_block_select_work_bytes(int Nq, int nh, int nblk, int top);
 void ops_block_select(struct ops *o, struct opnd Q, int Nq, int nh, int nhk,
                       int d, cl_mem KC, cl_mem KS, int nblk, int top,

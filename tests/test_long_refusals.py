@@ -90,6 +90,11 @@ def test_linear(ic, env):
                 dict(yoff=-1), dict(roff=-1), dict(ldx=99), dict(xoff=-1)):
         with refused(ic, "ops_linear_q8: invalid sizes"):
             q8(**bad)
+    # Tokens and channels are counted past the last.
+    for bad in (dict(rows=2 ** 31 - 1), dict(cout=2 ** 31 - 1, ldy=2 ** 31 - 1)):
+        with refused(ic, "ops_linear_q8: invalid sizes"):
+            q8(**bad)
+    assert a.ops_linear_q8_work_bytes(2 ** 31 - 1, 64) == 0
     with refused(ic, "invalid activation 5"):
         q8(act=5)
     for bad, name in ((dict(xoff=M // 4 - 799), "X"), (dict(wq=v(M, 3839)), "WQ"), (dict(ws=v(2 * M, 119)), "WS"),
@@ -102,7 +107,10 @@ def test_linear(ic, env):
     with refused(ic, "work does not start"):
         q8(work=v(6 * M + 8, M))
     for bad, names in ((dict(y=x), "Y and X"), (dict(y=wq, wq=wq), "Y and WQ"), (dict(work=y), "Y and work"),
-                       (dict(work=x), "X and work"), (dict(r=y, roff=1), "Y and R")):
+                       (dict(work=x), "X and work"), (dict(r=y, roff=1), "Y and R"),
+                       (dict(y=v(2 * M, M)), "Y and WS"), (dict(y=v(3 * M, M)), "Y and bias"),
+                       (dict(work=v(M, M)), "WQ and work"), (dict(work=v(2 * M, M)), "WS and work"),
+                       (dict(work=v(3 * M, M)), "bias and work"), (dict(r=work), "R and work")):
         with refused(ic, names):
             q8(**bad)
     q8(rows=0)
@@ -113,7 +121,8 @@ def test_linear(ic, env):
         a.ops_linear_qq(o, rows, cin, cout, xq, xs, wq, ws, b, None, 0, y, 0, cout, 0, 0.0)
 
     for bad, match in ((dict(xq=v(7 * M, 1023)), "XQ accessed"), (dict(xs=v(8 * M, 31)), "XS accessed"),
-                       (dict(xq=v(7 * M + 1, 2048)), "XQ does not start"), (dict(y=v(7 * M + 1000, M)), "Y and XQ")):
+                       (dict(xq=v(7 * M + 1, 2048)), "XQ does not start"), (dict(y=v(7 * M + 1000, M)), "Y and XQ"),
+                       (dict(y=v(8 * M + 16, M)), "Y and XS")):
         with refused(ic, "ops_linear_qq: " + match):
             qq(**bad)
 
@@ -213,7 +222,8 @@ def test_blocks(ic, env):
                        (dict(mask=v(0, 99)), "kmask accessed"), (dict(kc=v(0, 14 * 64 - 1)), "KC accessed"),
                        (dict(ks=v(0, 14 * 4 - 1)), "KS accessed"), (dict(kc=v(8, M)), "KC does not start"),
                        (dict(nk=2 ** 31 - 1, nb=0), "invalid sizes"), (dict(kc=kb), "KC and K"),
-                       (dict(ks=kb), "KS and K"), (dict(ks=kc), "KC and KS")):
+                       (dict(ks=kb), "KS and K"), (dict(ks=kc), "KC and KS"), (dict(mask=kc), "KC and kmask"),
+                       (dict(mask=ks), "KS and kmask")):
         with refused(ic, "ops_block_index: .*" + match):
             index(**bad)
     index(nb=0)
@@ -223,7 +233,8 @@ def test_blocks(ic, env):
 
     for bad, match in ((dict(d=129), "head dimension"), (dict(top=0), "0 blocks"), (dict(top=65), "65 blocks"),
                        (dict(kv=3), "invalid sizes"), (dict(h=0), "invalid sizes"), (dict(nq=-1), "invalid sizes"),
-                       (dict(n=-1), "invalid sizes"), (dict(q=op(q, 0, 127)), "invalid sizes"),
+                       (dict(n=-1), "invalid sizes"), (dict(n=2 ** 27 + 1), "invalid sizes"),
+                       (dict(q=op(q, 0, 127)), "invalid sizes"),
                        (dict(q=op(q, M // 4 - 2559, 128)), "Q accessed"), (dict(kc=v(0, 14 * 64 - 1)), "KC accessed"),
                        (dict(ks=None), "KS is NULL"), (dict(sel=v(0, 959)), "SEL accessed"),
                        (dict(kc=v(8, M)), "KC does not start"), (dict(sel=qb), "SEL and Q"),
@@ -247,7 +258,31 @@ def test_blocks(ic, env):
                        (dict(work=None), "work is NULL"), (dict(work=v(8 * M + 4, M)), "work does not start"),
                        (dict(out=op(qb, 4, 128)), "O and Q"), (dict(out=op(kb, 0, 128)), "O and K"),
                        (dict(out=op(vb, 0, 128)), "O and V"), (dict(work=ob), "O and work"),
-                       (dict(work=sel), "SEL and work"), (dict(sel=ob), "SEL and O"), (dict(mask=ob), "kmask and O")):
+                       (dict(work=sel), "SEL and work"), (dict(sel=ob), "SEL and O"), (dict(mask=ob), "kmask and O"),
+                       (dict(work=qb), "Q and work"), (dict(work=kb), "K and work"), (dict(work=vb), "V and work"),
+                       (dict(work=mask), "kmask and work")):
         with refused(ic, "ops_attention_blocks: .*" + match):
             attend(**bad)
     attend(nq=0)
+
+
+def test_launches(ic, env):
+    """More blocks of threads than a launch takes are refused by name, and
+    units too many for the 32-bit places of the lists go one by one."""
+    a, o, _ = env
+    huge = [ic.lib().ocl_wrap(C.c_void_p((i + 1) << 44), 1 << 43) for i in range(4)]
+    op = lambda b, ld: ic.Opnd(b, 0, ld, 0, 0)  # noqa: E731
+    with refused(ic, "selection rows: 67108864 blocks of 64 threads exceed a launch"):
+        a.ops_block_select(o, op(huge[0], 1), 1 << 26, 1, 1, 1, huge[1], huge[2], 600, 1, huge[3], None)
+    with refused(ic, "block index: 16777216 blocks of 256 threads exceed a launch"):
+        a.ops_block_index(o, op(huge[0], 16), 1 << 24, 16, 1, 16, None, 0, 1 << 20, huge[1], huge[2])
+    # A row in several units of 2048 channels.
+    with refused(ic, "rope blocks: 16777216 blocks of 256 threads exceed a launch"):
+        a.ops_rope_pos(o, 1 << 24, 2048, 2048, 1, huge[2], huge[3], 1.0, 0, op(huge[0], 2048), op(huge[0], 2048), 1,
+                       op(None, 0), op(None, 0), 0)
+    for m in huge:
+        ic.lib().ocl_release(C.byref(m))
+    choose = ic.lib().icoreg_blocks_choice
+    assert choose(1, 2048, 65536, 1, 128, 64, 64) == 1
+    assert choose(1, 2048, 131072, 1, 128, 64, 64) == 1
+    assert choose(1, 2048, 131073, 1, 128, 64, 64) == 0
