@@ -1018,8 +1018,8 @@ template <int CTRL> __device__ __forceinline__ int quad_i(int v)
 /* Second step: a block of threads holds a unit's keys and values in LDS, both
  * split in three bf16 parts (split.h), and computes them for the rows that
  * list it, 32 a wave and turn. */
-#define BLK_PIECE 1024 /* rows whose bits are read at a time */
-#define BLK_CHUNKS 32  /* pieces of rows a block of threads takes at most */
+#define BLK_RING 128   /* rows of a wave's list at most */
+#define BLK_TILES 1024 /* tiles of 64 rows a block of threads takes at most */
 #define BLK_VMAX 0x1p90f /* 64 scaled values stay finite below */
 
 template <int ND, int NB, bool FULL>
@@ -1030,8 +1030,7 @@ __global__ void __launch_bounds__(256, ND == 4 ? 1 : ND * NB == 4 ? 3 : 4) blk_u
     constexpr int RV = 16 / KC < 1 ? 1 : 16 / KC;  /* V rows */
     constexpr int PK = SB * CH;                    /* 16-byte chunks of a part */
     __shared__ split_u4 ks[3 * PK], vs[3 * PK];
-    __shared__ unsigned short list[BLK_PIECE + 128];
-    __shared__ int wsum[4];
+    __shared__ unsigned short list[4][BLK_RING];
     __shared__ float sc[4][64];
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, col = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -1042,12 +1041,10 @@ __global__ void __launch_bounds__(256, ND == 4 ? 1 : ND * NB == 4 ? 3 : 4) blk_u
     const int unit = job / a.pieces, piece = job % a.pieces;
     const int sub = unit % a.sub, b = unit / a.sub % a.nblk, kvh = unit / a.sub / a.nblk;
     const int ss = a.bs / a.sub, k0 = b * a.bs + sub * ss, n = min(a.Nk - k0, ss);
-    const unsigned *bits = (const unsigned *)(a.bits + ((long long)kvh * a.nblk + b) * a.tiles);
-    const int words = 2 * a.tiles; /* of 32 rows */
-    const int nchunk = (words * 32 + BLK_PIECE - 1) / BLK_PIECE;
-    const int c0 = (int)((long long)nchunk * piece / a.pieces);
-    const int c1 = (int)((long long)nchunk * (piece + 1) / a.pieces);
-    const int base = c0 * BLK_PIECE; /* rows in the list count from here */
+    const unsigned long long *bits = a.bits + ((long long)kvh * a.nblk + b) * a.tiles;
+    const int c0 = (int)((long long)a.tiles * piece / a.pieces);
+    const int c1 = (int)((long long)a.tiles * (piece + 1) / a.pieces);
+    const int base = c0 * 64; /* rows in the list count from here */
 
     if (c0 >= c1)
         return;
@@ -1056,13 +1053,6 @@ __global__ void __launch_bounds__(256, ND == 4 ? 1 : ND * NB == 4 ? 3 : 4) blk_u
     const unsigned long long keep =
         __ballot(lane < n && (!a.kmask || a.kmask[k0 + min(lane, n - 1)]));
     bool wild = false; /* values that the split's sums cannot hold */
-    /* 4 rows a thread and piece: their bits, read a piece ahead. */
-    auto bits_of = [&](int c) {
-        const int r0 = c * BLK_PIECE + 4 * tid, w = r0 >> 5;
-
-        return c < c1 && w < words ? bits[w] >> (r0 & 31) & 0xfu : 0u;
-    };
-    unsigned next = bits_of(c0);
 
     /* Keys and values that are left out are zero here: what they hold meets
      * probabilities of zero. */
@@ -1173,9 +1163,9 @@ __global__ void __launch_bounds__(256, ND == 4 ? 1 : ND * NB == 4 ? 3 : 4) blk_u
         }
         return min(slot, __shfl_xor(slot, 32, 64));
     };
-    auto tile = [&](const unsigned short *rows, int count) {
+    auto tile = [&](const unsigned short *rows, int first, int count) {
         const bool live = col < count;
-        const int r = base + rows[live ? col : 0], qi = g == 1 ? r : r / g, h = kvh * g + r - qi * g;
+        const int r = base + rows[first + (live ? col : 0) & BLK_RING - 1], qi = g == 1 ? r : r / g, h = kvh * g + r - qi * g;
         const long long row = (long long)qi * a.nh + h;
         const float up = a.scale * BLK_LOG2E * BLK_QUP;
         split_u4 q[2 * ND][3];
@@ -1326,7 +1316,7 @@ __global__ void __launch_bounds__(256, ND == 4 ? 1 : ND * NB == 4 ? 3 : 4) blk_u
         const bool whole = __all(to >= 0);
 
         if (half == 0 && to >= 0)
-            a.ml[to] = make_float2(mx, l);
+            a.ml[to] = make_float2(mx, -l);
 #pragma unroll
         for (int tt = 0; tt < ND; tt++) {
             float x[4][4];
@@ -1335,7 +1325,7 @@ __global__ void __launch_bounds__(256, ND == 4 ? 1 : ND * NB == 4 ? 3 : 4) blk_u
             for (int e = 0; e < 4; e++)
 #pragma unroll
                 for (int j = 0; j < 4; j++)
-                    x[e][j] = o[tt][4 * e + j] * (1.0f / SPLIT_UP);
+                    x[e][j] = o[tt][4 * e + j];
 #pragma unroll
             for (int j = 0; j < 4; j++) {
 #pragma unroll
@@ -1366,7 +1356,7 @@ __global__ void __launch_bounds__(256, ND == 4 ? 1 : ND * NB == 4 ? 3 : 4) blk_u
         if (redo)
             for (int e = 0; e < count; e++)
                 if (redo >> e & 1) {
-                    const int rr = base + rows[e], sl = __builtin_amdgcn_readlane(slot, e);
+                    const int rr = base + rows[first + e & BLK_RING - 1], sl = __builtin_amdgcn_readlane(slot, e);
                     const long long to = (row_of(rr) * a.top + sl) * a.sub + sub;
 
                     blk_unit_f32(a, a.q0 + rr / g, kvh * g + rr % g, k0, k0 + n, a.part + to * DP,
@@ -1374,59 +1364,60 @@ __global__ void __launch_bounds__(256, ND == 4 ? 1 : ND * NB == 4 ? 3 : 4) blk_u
                 }
     };
 
-    int have = 0;
+    auto turn = [&](const unsigned short *rows, int first, int count) {
+        __builtin_amdgcn_wave_barrier();
+        if (nothing) {
+            const long long row = row_of(base + rows[first + (col < count ? col : 0) & BLK_RING - 1]);
+            const int slot = slot_of(row);
 
-    for (int c = c0; c < c1; c++) {
-        const int r0 = c * BLK_PIECE + 4 * tid;
-        unsigned m = next;
-        int p = __popc(m), before = 0;
-
-        next = bits_of(c + 1);
-
-#pragma unroll
-        for (int s = 1; s < 64; s <<= 1) {
-            const int v = __shfl_up(p, s, 64);
-
-            p += lane >= s ? v : 0;
+            if (lane < count)
+                a.ml[(row * a.top + slot) * a.sub + sub] = make_float2(-INFINITY, 0.0f);
         }
-        if (lane == 63)
-            wsum[wave] = p;
-        __syncthreads();
-        for (int i = 0; i < wave; i++)
-            before += wsum[i];
-        const int added = wsum[0] + wsum[1] + wsum[2] + wsum[3];
-        int at = have + before + p - __popc(m);
+        else
+            tile(rows, first, count);
+        __builtin_amdgcn_wave_barrier();
+    };
+    unsigned short *mine = list[wave];
+    int first = 0, have = 0;
 
-        while (m) {
-            list[at++] = (unsigned short)(r0 - base + __ffs(m) - 1);
-            m &= m - 1;
+    /* Tiles of 64 rows, every fourth one this wave's, the bits of 64 of them
+     * read at once. */
+    for (int t0 = c0 + wave; t0 < c1; t0 += 4 * 64) {
+        const int mt = t0 + 4 * lane;
+        const unsigned long long word = mt < c1 ? bits[mt] : 0;
+        const int n64 = min(64, (c1 - t0 + 3) / 4);
+
+        for (int i = 0; i < n64; i++) {
+            const unsigned low = __builtin_amdgcn_readlane((int)word, i);
+            const unsigned high = __builtin_amdgcn_readlane((int)(word >> 32), i);
+            const int before = __builtin_amdgcn_mbcnt_hi(high, __builtin_amdgcn_mbcnt_lo(low, 0));
+
+            if ((half ? high : low) >> col & 1)
+                mine[first + have + before & BLK_RING - 1] =
+                    (unsigned short)((t0 + 4 * i) * 64 + lane - base);
+            have += __popc(low) + __popc(high);
+            for (; have >= 32; have -= 32, first += 32)
+                turn(mine, first, 32);
         }
-        have += added;
-        __syncthreads();
-        /* Whole turns of 4 waves, the rest with the next rows. */
-        const int todo = c + 1 == c1 ? have : have / 128 * 128;
-
-        for (int e = wave * 32; e < todo; e += 128) {
-            const int count = min(32, todo - e);
-
-            if (nothing) {
-                const long long row = row_of(base + list[e + (col < count ? col : 0)]);
-                const int slot = slot_of(row);
-
-                if (lane < count)
-                    a.ml[(row * a.top + slot) * a.sub + sub] = make_float2(-INFINITY, 0.0f);
-            }
-            else
-                tile(list + e, count);
-        }
-        __syncthreads();
-        const int rest = have - todo, kept = tid < rest ? list[todo + tid] : 0;
-
-        __syncthreads();
-        if (tid < rest)
-            list[tid] = (unsigned short)kept;
-        have = rest;
     }
+    /* What is left of the four waves, fewer than 32 rows each, together. */
+    __shared__ unsigned short rest[BLK_RING];
+    __shared__ int left[4];
+
+    if (lane == 0)
+        left[wave] = have;
+    __syncthreads();
+    int at = 0;
+
+    for (int i = 0; i < wave; i++)
+        at += left[i];
+    if (lane < have)
+        rest[at + lane] = mine[first + lane & BLK_RING - 1];
+    const int all = left[0] + left[1] + left[2] + left[3];
+
+    __syncthreads();
+    if (32 * wave < all)
+        turn(rest, 32 * wave, min(32, all - 32 * wave));
 }
 
 /* Units of a row merged: softmax over all of them from their maxima and sums.
@@ -1449,7 +1440,8 @@ template <int DP> __global__ void __launch_bounds__(256) blk_merge_kernel(const 
     const float m = wave_max_full(fmaxf(x.y != 0.0f ? x.x : -INFINITY, y.y != 0.0f ? y.x : -INFINITY));
     const float wx = x.y != 0.0f ? __builtin_amdgcn_exp2f(x.x - m) : 0.0f;
     const float wy = y.y != 0.0f ? __builtin_amdgcn_exp2f(y.x - m) : 0.0f;
-    const float l = wave_sum_full(x.y * wx + y.y * wy);
+    const float l = wave_sum_full(fabsf(x.y) * wx + fabsf(y.y) * wy);
+    const float vx = x.y < 0.0f ? wx * (1.0f / SPLIT_UP) : x.y != 0.0f ? wx : -1.0f, vy = y.y < 0.0f ? wy * (1.0f / SPLIT_UP) : y.y != 0.0f ? wy : -1.0f;
     float o[4] = {0, 0, 0, 0};
 
     /* Four loads on their way at once; units with no key hold nothing. */
@@ -1460,11 +1452,10 @@ template <int DP> __global__ void __launch_bounds__(256) blk_merge_kernel(const 
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const int u = u0 + i * GV, at = min(u, units - 1);
-            const float wu = __shfl(u < 64 ? wx : wy, u & 63, 64);
-            const float s = __shfl(u < 64 ? x.y : y.y, u & 63, 64);
+            const float wu = __shfl(u < 64 ? vx : vy, u & 63, 64);
 
             p[i] = *(const float4 *)(part + (long long)at * DP);
-            w[i] = u < units && s != 0.0f ? wu : -1.0f;
+            w[i] = u < units ? wu : -1.0f;
         }
 #pragma unroll
         for (int i = 0; i < 4; i++)
@@ -1514,7 +1505,8 @@ template <int DP> __global__ void __launch_bounds__(256) blk_merge16_kernel(cons
     m = fmaxf(m, dpp_f(m, 0x141));
     m = fmaxf(m, dpp_f(m, 0x140));
     const float w = x.y != 0.0f ? __builtin_amdgcn_exp2f(x.x - m) : -1.0f;
-    float l = x.y != 0.0f ? x.y * w : 0.0f;
+    float l = x.y != 0.0f ? fabsf(x.y) * w : 0.0f;
+    const float wv = x.y < 0.0f ? w * (1.0f / SPLIT_UP) : w;
 
     l += dpp_f(l, 0xB1);
     l += dpp_f(l, 0x4E);
@@ -1527,7 +1519,7 @@ template <int DP> __global__ void __launch_bounds__(256) blk_merge16_kernel(cons
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const int u = u0 + i * GV + gv, at = min(u, units - 1);
-            const float v = __shfl(w, (lane & 48) | at, 64);
+            const float v = __shfl(wv, (lane & 48) | at, 64);
 
             wu[i] = u < units ? v : -1.0f;
 #pragma unroll
@@ -1741,10 +1733,9 @@ extern "C" void ops_attention_blocks(struct ops *o, struct opnd Q, struct opnd K
              * some 256 rows to compute (4 a CU 274, 8 251, 8 of 128 rows 255 us
              * for 8192 x 8 rows of 256 blocks). */
             const long long each = max(1LL, (long long)a.Nq * g * top / p.nblk / 256);
-            const int chunks = (a.tiles * 64 + BLK_PIECE - 1) / BLK_PIECE;
 
-            a.pieces = (int)max((chunks + BLK_CHUNKS - 1LL) / BLK_CHUNKS,
-                                min(min(each, (long long)chunks),
+            a.pieces = (int)max((a.tiles + BLK_TILES - 1LL) / BLK_TILES,
+                                min(min(each, (long long)a.tiles),
                                     (8LL * o->ocl->cu_count + lists - 1LL) / lists));
             hipLaunchKernelGGL(blk_bits_kernel, dim3(a.tiles / BLK_TW, nhk), dim3(64 * BLK_TW), 0, s,
                                a);
