@@ -1022,16 +1022,27 @@ template <int CTRL> __device__ __forceinline__ int quad_i(int v)
 #define BLK_TILES 1024 /* tiles of 64 rows a block of threads takes at most */
 #define BLK_VMAX 0x1p90f /* 64 scaled values stay finite below */
 
+/* Waves of a block of threads, and of a SIMD. LDS holds two blocks of threads of
+ * 64 keys of 64 channels in 48 KB and some, one of 128 channels in 96: of 8 waves
+ * each where there is so little room. 4 and 8 waves, us: 4096 x 8 rows of 16
+ * units of 64 keys of 128 channels 190, 151; 8 of 100 channels 124, 96; of 2 x
+ * 64 keys of 48 channels 85, 71. Smaller units: 32 keys of 64 channels 33, 37; of
+ * 128 68, 75; 64 keys of 32 channels 49, 53. */
+constexpr int blk_waves(int nd, int nb) { return nd * nb >= 4 && nb == 2 ? 8 : 4; }
+constexpr int blk_simd(int nd, int nb) { return nd < 4 ? 4 : nb == 1 ? 3 : 2; }
+
 template <int ND, int NB, bool FULL>
-__global__ void __launch_bounds__(256, ND == 4 ? 1 : ND * NB == 4 ? 3 : 4) blk_unit_kernel(const blk_args a)
+__global__ void __launch_bounds__(64 * blk_waves(ND, NB), blk_simd(ND, NB))
+    blk_unit_kernel(const blk_args a)
 {
+    constexpr int W = blk_waves(ND, NB), NT = 64 * W;
     constexpr int DP = 32 * ND, CH = DP / 8, SB = 32 * NB, KC = SB / 8;
     constexpr int RW = 16 / CH < 1 ? 1 : 16 / CH;  /* K rows in 256 bytes */
     constexpr int RV = 16 / KC < 1 ? 1 : 16 / KC;  /* V rows */
     constexpr int PK = SB * CH;                    /* 16-byte chunks of a part */
     __shared__ split_u4 ks[3 * PK], vs[3 * PK];
-    __shared__ unsigned short list[4][BLK_RING];
-    __shared__ float sc[4][64];
+    __shared__ unsigned short list[W][BLK_RING];
+    __shared__ float sc[W][64];
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, col = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = a.nh / a.nhk, d = FULL ? DP : a.d;
@@ -1057,7 +1068,7 @@ __global__ void __launch_bounds__(256, ND == 4 ? 1 : ND * NB == 4 ? 3 : 4) blk_u
     /* Keys and values that are left out are zero here: what they hold meets
      * probabilities of zero. */
     if (!nothing) {
-        constexpr int NL = (PK + 255) / 256;
+        constexpr int NL = (PK + NT - 1) / NT;
         const float *K = a.K + k0 * a.ldk + (long long)kvh * d;
         const float *V = a.V + k0 * a.ldv + (long long)kvh * d;
         float x[NL][8], y[NL][8];
@@ -1068,7 +1079,7 @@ __global__ void __launch_bounds__(256, ND == 4 ? 1 : ND * NB == 4 ? 3 : 4) blk_u
          * 8 (c / 2 % 2) + j of the scores' tile c / 4 holds in lane half c % 2. */
 #pragma unroll
         for (int i = 0; i < NL; i++) {
-            const int e = min(tid + 256 * i, PK - 1), key = min(e / CH, n - 1), dd = e % CH * 8;
+            const int e = min(tid + NT * i, PK - 1), key = min(e / CH, n - 1), dd = e % CH * 8;
             const float *p = K + (long long)key * a.ldk;
             float u[4], v[4];
 
@@ -1088,7 +1099,7 @@ __global__ void __launch_bounds__(256, ND == 4 ? 1 : ND * NB == 4 ? 3 : 4) blk_u
         }
 #pragma unroll
         for (int i = 0; i < NL; i++) {
-            const int e = min(tid + 256 * i, PK - 1), dd = min(e % DP, d - 1), c = e / DP;
+            const int e = min(tid + NT * i, PK - 1), dd = min(e % DP, d - 1), c = e / DP;
 
 #pragma unroll
             for (int j = 0; j < 8; j++) {
@@ -1099,7 +1110,7 @@ __global__ void __launch_bounds__(256, ND == 4 ? 1 : ND * NB == 4 ? 3 : 4) blk_u
         }
 #pragma unroll
         for (int i = 0; i < NL; i++) {
-            const int e = tid + 256 * i;
+            const int e = tid + NT * i;
 
             if (e < PK) {
                 const int key = e / CH, at = key * CH + ((e % CH) ^ (key / RW % CH));
@@ -1116,7 +1127,7 @@ __global__ void __launch_bounds__(256, ND == 4 ? 1 : ND * NB == 4 ? 3 : 4) blk_u
         }
 #pragma unroll
         for (int i = 0; i < NL; i++) {
-            const int e = tid + 256 * i;
+            const int e = tid + NT * i;
 
             if (e < PK) {
                 const int dd = e % DP, c = e / DP, at = dd * KC + (c ^ (dd / RV % KC));
@@ -1380,12 +1391,12 @@ __global__ void __launch_bounds__(256, ND == 4 ? 1 : ND * NB == 4 ? 3 : 4) blk_u
     unsigned short *mine = list[wave];
     int first = 0, have = 0;
 
-    /* Tiles of 64 rows, every fourth one this wave's, the bits of 64 of them
+    /* Tiles of 64 rows, every W-th one this wave's, the bits of 64 of them
      * read at once. */
-    for (int t0 = c0 + wave; t0 < c1; t0 += 4 * 64) {
-        const int mt = t0 + 4 * lane;
+    for (int t0 = c0 + wave; t0 < c1; t0 += W * 64) {
+        const int mt = t0 + W * lane;
         const unsigned long long word = mt < c1 ? bits[mt] : 0;
-        const int n64 = min(64, (c1 - t0 + 3) / 4);
+        const int n64 = min(64, (c1 - t0 + W - 1) / W);
 
         for (int i = 0; i < n64; i++) {
             const unsigned low = __builtin_amdgcn_readlane((int)word, i);
@@ -1394,30 +1405,32 @@ __global__ void __launch_bounds__(256, ND == 4 ? 1 : ND * NB == 4 ? 3 : 4) blk_u
 
             if ((half ? high : low) >> col & 1)
                 mine[first + have + before & BLK_RING - 1] =
-                    (unsigned short)((t0 + 4 * i) * 64 + lane - base);
+                    (unsigned short)((t0 + W * i) * 64 + lane - base);
             have += __popc(low) + __popc(high);
             for (; have >= 32; have -= 32, first += 32)
                 turn(mine, first, 32);
         }
     }
-    /* What is left of the four waves, fewer than 32 rows each, together. */
-    __shared__ unsigned short rest[BLK_RING];
-    __shared__ int left[4];
+    /* What is left of the waves, fewer than 32 rows each, together. */
+    __shared__ unsigned short rest[32 * W];
+    __shared__ int left[W];
 
     if (lane == 0)
         left[wave] = have;
     __syncthreads();
-    int at = 0;
+    int at = 0, all = 0;
 
-    for (int i = 0; i < wave; i++)
-        at += left[i];
+#pragma unroll
+    for (int i = 0; i < W; i++) {
+        at += i < wave ? left[i] : 0;
+        all += left[i];
+    }
     if (lane < have)
         rest[at + lane] = mine[first + lane & BLK_RING - 1];
-    const int all = left[0] + left[1] + left[2] + left[3];
 
     __syncthreads();
     if (32 * wave < all)
-        turn(rest, 32 * wave, min(32, all - 32 * wave));
+        turn(rest + 32 * wave, 0, min(32, all - 32 * wave));
 }
 
 /* Units of a row merged: softmax over all of them from their maxima and sums.
@@ -1729,29 +1742,35 @@ extern "C" void ops_attention_blocks(struct ops *o, struct opnd Q, struct opnd K
         }
         else {
             const int lists = count32((long long)nhk * p.nblk * p.sub, "units of keys");
-            /* Splits of a list: 8 blocks of threads a CU, if each of them has
-             * some 256 rows to compute (4 a CU 274, 8 251, 8 of 128 rows 255 us
-             * for 8192 x 8 rows of 256 blocks). */
-            const long long each = max(1LL, (long long)a.Nq * g * top / p.nblk / 256);
+            /* Splits of a list: twice the blocks of threads that a CU holds, if
+             * each wave has some 64 rows to compute. Units of 64 keys, us: of 64
+             * channels (2 held), 2, 4, 8 a CU 184, 170, 181; of 128 (1 held) 151,
+             * 169, 215. 32, 64 rows a wave: 400 x 100 blocks of 32 channels 51.7,
+             * 48.7; 128 blocks of 128 channels the same. */
+            const int nd = p.dp / 32, nb = bs / p.sub <= 32 ? 1 : 2;
+            const int held = 4 * blk_simd(nd, nb) / blk_waves(nd, nb);
+            const long long each = max(1LL, (long long)a.Nq * g * top / p.nblk / (64 * blk_waves(nd, nb)));
 
             a.pieces = (int)max((a.tiles + BLK_TILES - 1LL) / BLK_TILES,
                                 min(min(each, (long long)a.tiles),
-                                    (8LL * o->ocl->cu_count + lists - 1LL) / lists));
+                                    (2LL * held * o->ocl->cu_count + lists - 1LL) / lists));
             hipLaunchKernelGGL(blk_bits_kernel, dim3(a.tiles / BLK_TW, nhk), dim3(64 * BLK_TW), 0, s,
                                a);
             launch_check("attention_blocks bits");
-            const dim3 grid(grid_of((long long)lists * a.pieces, 256, "lists"));
+            const dim3 grid(grid_of((long long)lists * a.pieces, 64 * blk_waves(nd, nb), "lists"));
 
 #define UNIT_LAUNCH(ND_, NB_)                                                                 \
     do {                                                                                      \
+        const dim3 block(64 * blk_waves(ND_, NB_));                                           \
+                                                                                              \
         if (d == 32 * ND_)                                                                    \
-            hipLaunchKernelGGL((blk_unit_kernel<ND_, NB_, true>), grid, dim3(256), 0, s, a);  \
+            hipLaunchKernelGGL((blk_unit_kernel<ND_, NB_, true>), grid, block, 0, s, a);      \
         else                                                                                  \
-            hipLaunchKernelGGL((blk_unit_kernel<ND_, NB_, false>), grid, dim3(256), 0, s, a); \
+            hipLaunchKernelGGL((blk_unit_kernel<ND_, NB_, false>), grid, block, 0, s, a);     \
     } while (0)
 #define UNIT_KEYS(ND_)          \
     do {                        \
-        if (bs / p.sub <= 32)   \
+        if (nb == 1)            \
             UNIT_LAUNCH(ND_, 1); \
         else                    \
             UNIT_LAUNCH(ND_, 2); \
