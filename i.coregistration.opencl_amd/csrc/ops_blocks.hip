@@ -48,7 +48,10 @@ static bool blk_size_ok(int bs) { return bs == 16 || bs == 32 || bs == 64 || bs 
 /* ---- the index of the blocks -------------------------------------------------- */
 
 /* A block of threads makes the code of one key block and head: L lanes of
- * four channels a key, 256 / L keys at a time, sums in 64 bits. */
+ * four channels a key, 256 / L keys at a time, sums in 64 bits (float32 sums
+ * would depend on the order, and with them the codes next to a border). 16380
+ * keys of 2 heads of 64, 8.4 MB: 7.3 us; one block 5.5: loads, two barriers and
+ * the rounding behind each other. */
 template <int L>
 __global__ void __launch_bounds__(256)
     block_index_kernel(const float *__restrict__ K, long long ldk, int Nk, int nhk, int d, int bs,
@@ -133,8 +136,8 @@ extern "C" void ops_block_index(struct ops *o, struct opnd K, int Nk, int nhk, i
         icoreg_fatal("%s: block size %d is not 16, 32, 64 or 128", op, bs);
     if (d < 1 || d > OPS_MAX_HEAD_DIM)
         icoreg_fatal("%s: head dimension %d is not 1 .. %d", op, d, OPS_MAX_HEAD_DIM);
-    if (Nk < 0 || Nk > BLK_MAX_KEYS || nhk < 1 || b0 < 0 || nb < 0 || (long long)b0 + nb > nblk || K.off < 0 ||
-        K.ld < (long long)nhk * d)
+    if (Nk < 0 || Nk > BLK_MAX_KEYS || nhk < 1 || b0 < 0 || nb < 0 ||
+        (long long)b0 + nb > nblk || K.off < 0 || K.ld < (long long)nhk * d)
         icoreg_fatal("%s: invalid sizes Nk=%d nhk=%d d=%d ld=%d, blocks %d + %d of %d", op, Nk, nhk,
                      d, K.ld, b0, nb, nblk);
     if (nb == 0)
@@ -337,10 +340,11 @@ struct sel_args {
 /* A wave selects the best of the blocks b0 .. b1 - 1 for one query and head,
  * 64 SLOTS at a time, the best so far kept beside the next ones. The PL = 4 or 8
  * lanes of a code row read 16 bytes each, neighbours of one line (a row a lane
- * fetches every line PL times: 2047 blocks of 128 channels, 16 rows 25 us, so
- * 20), and add their sums; lane l keeps the score of block l of 64. Sorted
- * results in the lanes, as sel_top leaves them. codes, list: 128 bytes and
- * words of LDS of this wave. */
+ * fetches every line PL times: a step from 25 to 20 us for 16 rows of 2047
+ * blocks of 128 channels, 10.4 now: the codes' way from memory, then about
+ * fifteen counts of the threshold and the ranks, twice), and add their sums;
+ * lane l keeps the score of block l of 64. Sorted results in the lanes, as
+ * sel_top leaves them. codes, list: 128 bytes and words of LDS of this wave. */
 template <int PL>
 __device__ __forceinline__ void sel_row(const sel_args &a, int query, int h, int b0, int b1,
                                         unsigned char *codes, int *list, int &key, int &idx)
@@ -459,7 +463,8 @@ __global__ void __launch_bounds__(64 * W) block_select_kernel(const sel_args a)
  * takes 16 and more; mostly 2 or 3 steps). Those go to LDS and are ranked
  * against each other, ties by their numbers. A query, scale or score that is
  * not finite, or more equal scores than CAP, sends the wave's rows to sel_row
- * one by one. */
+ * one by one. 65536 rows of 256 blocks 40 us (a wave a row 197), vector
+ * instructions in 41 % of it, mostly the counts; the products 2 %. */
 #define SEL_TW 4 /* waves */
 
 template <int T, int KCH, int CAP>
@@ -871,7 +876,8 @@ __device__ __forceinline__ void blk_unit_f32(const blk_args &a, int qi, int h, i
 
 /* Few queries: a block of threads a unit, everything that it reads on its way
  * at once. Scores: 4 lanes a key, DP / 16 times 4 channels each. Output: DP / 4
- * lanes a key, KV keys each, joined in LDS. */
+ * lanes a key, KV keys each, joined in LDS. 256 units of 64 keys of 128 channels,
+ * 16.8 MB: 4.7 us, 3.6 TB/s. */
 template <int DP> __global__ void __launch_bounds__(256) blk_direct_kernel(const blk_args a)
 {
     constexpr int NK = DP / 16, LV = DP / 4, GV = 256 / LV, KV = 64 / GV;
@@ -957,8 +963,10 @@ template <int DP> __global__ void __launch_bounds__(256) blk_direct_kernel(const
 
 /* Many queries, first step: bit r of bits[kvh][b][t] says that row 64 t + r
  * (of the kv head's rows: query-major, its query heads within) lists block
- * b. A wave a tile, eight tiles a block of threads; entries that are no block
- * or a repeated one get an empty unit. */
+ * b. A wave a tile, eight tiles a block of threads, so that a block's words
+ * leave in runs of 64 bytes; entries that are no block or a repeated one get an
+ * empty unit. Or of bits in LDS has no order that matters. 65536 rows of 16:
+ * 8.6 us. */
 #define BLK_TW 8
 #define BLK_RANGE 1024 /* key blocks at a time */
 
@@ -1016,8 +1024,20 @@ template <int CTRL> __device__ __forceinline__ int quad_i(int v)
 }
 
 /* Second step: a block of threads holds a unit's keys and values in LDS, both
- * split in three bf16 parts (split.h), and computes them for the rows that
- * list it, 32 a wave and turn. */
+ * split in three bf16 parts (split.h: float32 products without loss), and
+ * computes them for the rows that list it, 32 a wave and turn. A key block is
+ * read once for all of them, where a row on its own would read its 16 blocks
+ * of keys and values again, 512 KB. Each wave collects its own rows and meets the
+ * others at the start and at the end only (with barriers in between 184 us, without
+ * 180, by 8 waves 172). Outputs leave times SPLIT_UP, marked by a negative sum, which the merge
+ * takes into its weights.
+ *
+ * 65536 rows of 16 units of 64 keys of 64 channels: 172 us, 600 TFLOP/s of bf16
+ * products. The matrix cores are busy 28 % of it, vector instructions (splits
+ * of queries and probabilities, exponentials, the exchange before the stores)
+ * 44 %, and half of the waves' time goes to waits: loads of queries and lists at the
+ * start of a turn, one product's sum into the next. No stores: 168 of 184 us
+ * then; no look at the lists: 165; one query for all: 176. */
 #define BLK_RING 128   /* rows of a wave's list at most */
 #define BLK_TILES 1024 /* tiles of 64 rows a block of threads takes at most */
 #define BLK_VMAX 0x1p90f /* 64 scaled values stay finite below */
@@ -1176,7 +1196,8 @@ __global__ void __launch_bounds__(64 * blk_waves(ND, NB), blk_simd(ND, NB))
     };
     auto tile = [&](const unsigned short *rows, int first, int count) {
         const bool live = col < count;
-        const int r = base + rows[first + (live ? col : 0) & BLK_RING - 1], qi = g == 1 ? r : r / g, h = kvh * g + r - qi * g;
+        const int r = base + rows[first + (live ? col : 0) & BLK_RING - 1];
+        const int qi = g == 1 ? r : r / g, h = kvh * g + r - qi * g;
         const long long row = (long long)qi * a.nh + h;
         const float up = a.scale * BLK_LOG2E * BLK_QUP;
         split_u4 q[2 * ND][3];
@@ -1370,8 +1391,8 @@ __global__ void __launch_bounds__(64 * blk_waves(ND, NB), blk_simd(ND, NB))
                     const int rr = base + rows[first + e & BLK_RING - 1], sl = __builtin_amdgcn_readlane(slot, e);
                     const long long to = (row_of(rr) * a.top + sl) * a.sub + sub;
 
-                    blk_unit_f32(a, a.q0 + rr / g, kvh * g + rr % g, k0, k0 + n, a.part + to * DP,
-                                 a.ml + to, sc[wave]);
+                    blk_unit_f32(a, a.q0 + rr / g, kvh * g + rr % g, k0, k0 + n,
+                                 a.part + to * DP, a.ml + to, sc[wave]);
                 }
     };
 
@@ -1435,7 +1456,9 @@ __global__ void __launch_bounds__(64 * blk_waves(ND, NB), blk_simd(ND, NB))
 
 /* Units of a row merged: softmax over all of them from their maxima and sums.
  * A wave a row: lane u has unit u's weight (and unit 64 + u's), then DP / 4
- * lanes a unit add the outputs, 256 / DP units at a time. */
+ * lanes a unit add the outputs, 256 / DP units at a time. A negative sum: the
+ * outputs are SPLIT_UP times as large. Bound by memory: 65536 rows of 16 units
+ * of 64 channels, 285 MB, 43 us, half of it from the last cache. */
 template <int DP> __global__ void __launch_bounds__(256) blk_merge_kernel(const blk_args a)
 {
     constexpr int LV = DP / 4, GV = 64 / LV;
@@ -1454,7 +1477,10 @@ template <int DP> __global__ void __launch_bounds__(256) blk_merge_kernel(const 
     const float wx = x.y != 0.0f ? __builtin_amdgcn_exp2f(x.x - m) : 0.0f;
     const float wy = y.y != 0.0f ? __builtin_amdgcn_exp2f(y.x - m) : 0.0f;
     const float l = wave_sum_full(fabsf(x.y) * wx + fabsf(y.y) * wy);
-    const float vx = x.y < 0.0f ? wx * (1.0f / SPLIT_UP) : x.y != 0.0f ? wx : -1.0f, vy = y.y < 0.0f ? wy * (1.0f / SPLIT_UP) : y.y != 0.0f ? wy : -1.0f;
+    auto weight = [](float w, float sum) {
+        return sum < 0.0f ? w * (1.0f / SPLIT_UP) : sum != 0.0f ? w : -1.0f;
+    };
+    const float vx = weight(wx, x.y), vy = weight(wy, y.y);
     float o[4] = {0, 0, 0, 0};
 
     /* Four loads on their way at once; units with no key hold nothing. */

@@ -96,7 +96,11 @@ template <int V> __device__ __forceinline__ void rope_store(float *p, const rope
 
 /* A unit is 2 V channels of a head: V pairs among the first rot channels (2 V
  * neighbours interleaved, V of either half otherwise), or 2 V channels to
- * copy. With V = 1 the last unit of an odd head is one channel. */
+ * copy. With V = 1 the last unit of an odd head is one channel. Bound by
+ * memory: 65533 rows of 20 heads of 128, 64 of them turned, 671 MB in and out
+ * each, 268 us, 5.0 TB/s (a large copy 4.8); 6400 rows of 16 heads of 32, 26 MB,
+ * 7.4 us. A table read instead of the cosines would add its bytes and hold
+ * only the positions that it was made for. */
 template <int V, bool INTER>
 __global__ void __launch_bounds__(256) rope_pos_kernel(const rope_args a)
 {

@@ -245,6 +245,29 @@ def test_lists_that_a_caller_makes(nq, bs, d, dev, ic):
     check(c, q, k, v, mask, sel, got)
 
 
+@pytest.mark.parametrize("nq,nk,h,kv,d,bs,top", [
+    (70001, 32003, 2, 1, 16, 16, 1), (70001, 32003, 2, 1, 33, 64, 1), (2503, 700, 2, 2, 64, 64, 3),
+    (2503, 700, 4, 2, 128, 64, 3), (2503, 700, 2, 1, 128, 32, 3), (1301, 700, 8, 2, 50, 128, 3)])
+def test_crowded_lists(nq, nk, h, kv, d, bs, top, dev, ic):
+    """Every row lists the first block and stretches of rows the same others:
+    lists of all rows (more than 2^16 of a key head), of whole tiles of 64 rows
+    and of next to none."""
+    print(f"[blocks] crowded {nq} {nk} {h} {kv} {d} {bs} {top}", flush=True)
+    assert ic.lib().icoreg_blocks_choice(nq, nk, h, kv, d, bs, top) == 1
+    q, k, v, _ = draw(nq, nk, h, kv, d)
+    rng = np.random.default_rng(nq)
+    c = Case(dev, ic, q, k, v, bs, top, d ** -0.5)
+    sel = rng.integers(0, c.n, (nq // 97 + 1, h, top)).astype(np.int32).repeat(97, 0)[:nq]
+    sel[:, :, 0] = np.where(np.arange(nq) % 11 < 10, 0, c.n - 1)[:, None]
+    dev.write(c.SEL, np.concatenate([sel.ravel(), np.full(4, 99, np.int32)]))
+    c.attend()
+    got = c.out()
+    some = np.unique(np.concatenate([rng.integers(0, nq, 1200), np.arange(0, 70), np.arange(nq - 70, nq)]))
+    check(c, q[some], k, v, None, sel[some], got[some])
+    c.attend()
+    assert np.array_equal(c.out(), got)
+
+
 @pytest.mark.parametrize("nq", [2, 700])
 def test_no_keys(nq, dev, ic):
     print(f"[blocks] no keys {nq}", flush=True)
