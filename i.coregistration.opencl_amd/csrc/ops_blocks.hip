@@ -1458,7 +1458,7 @@ __global__ void __launch_bounds__(64 * blk_waves(ND, NB), blk_simd(ND, NB))
  * A wave a row: lane u has unit u's weight (and unit 64 + u's), then DP / 4
  * lanes a unit add the outputs, 256 / DP units at a time. A negative sum: the
  * outputs are SPLIT_UP times as large. Bound by memory: 65536 rows of 16 units
- * of 64 channels, 285 MB, 43 us, half of it from the last cache. */
+ * of 64 channels, 285 MB, 43 us, 6.6 TB/s. */
 template <int DP> __global__ void __launch_bounds__(256) blk_merge_kernel(const blk_args a)
 {
     constexpr int LV = DP / 4, GV = 64 / LV;
