@@ -50,7 +50,7 @@ static bool blk_size_ok(int bs) { return bs == 16 || bs == 32 || bs == 64 || bs 
 /* A block of threads makes the code of one key block and head: L lanes of
  * four channels a key, 256 / L keys at a time, sums in 64 bits (float32 sums
  * would depend on the order, and with them the codes next to a border). 16380
- * keys of 2 heads of 64, 8.4 MB: 7.3 us; one block 5.5: loads, two barriers and
+ * keys of 2 heads of 64, 8.4 MB: 7.3 us; one block 5.4: loads, two barriers and
  * the rounding behind each other. */
 template <int L>
 __global__ void __launch_bounds__(256)
@@ -59,6 +59,7 @@ __global__ void __launch_bounds__(256)
                        signed char *__restrict__ KC, float *__restrict__ KS)
 {
     constexpr int G = 256 / L; /* keys at a time */
+    constexpr int U = L / 4;   /* times that: 64 keys on their way at once */
     __shared__ double part[G][4 * L];
     __shared__ int kept[G];
     __shared__ unsigned top;
@@ -71,20 +72,19 @@ __global__ void __launch_bounds__(256)
 
     if (tid == 0)
         top = 0;
-    /* Four keys on their way at once. */
-    for (int k = k0 + g; k < k1; k += 4 * G) {
-        float x[4][4];
-        bool in[4];
+    for (int k = k0 + g; k < k1; k += U * G) {
+        float x[U][4];
+        bool in[U];
 
 #pragma unroll
-        for (int u = 0; u < 4; u++) {
+        for (int u = 0; u < U; u++) {
             const int kk = min(k + u * G, k1 - 1);
 
             load4_row(K + kk * ldk + (long long)h * d, c, d, x[u]);
             in[u] = k + u * G < k1 && (!kmask || kmask[kk]);
         }
 #pragma unroll
-        for (int u = 0; u < 4; u++) {
+        for (int u = 0; u < U; u++) {
             n += in[u];
 #pragma unroll
             for (int j = 0; j < 4; j++)
