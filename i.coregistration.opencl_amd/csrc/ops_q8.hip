@@ -228,8 +228,8 @@ constexpr int q8_wait(int n) { return 0x0070 | (n & 15) | (n >> 4) << 14; }
  * this one's products run. Rows past M and N are outside the panels' windows
  * and read as zeros.
  *
- * 12288 x 4096 x 4096 on blocks of 256 x 256: 224 us, 1840 TOP/s, the matrix
- * cores busy 55 % of it (a library's plain int8 product, nothing scaled and 32
+ * 12288 x 4096 x 4096 on blocks of 256 x 256: 206 us, 2000 TOP/s (224 on
+ * another card), the matrix cores busy 54 % of it (a library's plain int8 product, nothing scaled and 32
  * bits out: 1860 at 4096 cubed, 2370 at 8192); what is left is the three rounds'
  * epilogues, 201 MB of outputs written while no product runs. 3202 x 1024 x
  * 4096 with GELU 31.6 us: one round, 8 steps and 52 MB to write. Two buffers of
