@@ -1625,15 +1625,16 @@ static blk_plan blk_plan_of(int Nq, int Nk, int nh, int nhk, int d, int bs, int 
 
     p.pass = (int)((Nq + passes - 1) / passes);
     /* Units one by one or by lists, us: 8 heads of 64 on 256 blocks of 64 keys,
-     * 16 listed, 16 queries 16, 29; 64 queries 35, 27; 1024 queries 431, 58. 8 heads
-     * of 128, 8 of 64 blocks, 64 queries 41, 41; of 32, 8 of 100 blocks, 64 queries
-     * 18, 31, 256 queries 42, 28. Lists of a few rows stage a block's keys for
-     * nothing. */
+     * 16 listed, 32 queries 22, 22; 48 queries 28, 22; 1024 queries 435, 49. 8 heads
+     * of 128, 8 of 64 blocks, 32 queries 24, 31; 64 queries 40, 32; of 32, 8 of 100
+     * blocks, 64 queries 15, 19; 128 queries 24, 19. Lists of a few rows stage a
+     * block's keys for nothing: 2 key heads of 128, 16 of 2047 blocks, 4 rows a list
+     * 152, 192; 8 rows 299, 199. */
     const long long units = (long long)p.pass * nh * top * p.sub;
 
     /* Lists place their outputs by 32 bits (a query of very many heads passes them). */
     p.direct = p.nblk == 0 || nhk > 65535 || units * p.dp * 4 > 1LL << 32 ||
-               units * (p.dp + 32) <= 600000 || (long long)p.pass * g * top < 4LL * p.nblk;
+               units * (p.dp + 32) <= 400000 || (long long)p.pass * g * top < 5LL * p.nblk;
     p.tiles = ((p.pass * g + 63) / 64 + BLK_TW - 1) / BLK_TW * BLK_TW;
     p.part = (long long)p.pass * nh * top * p.sub * p.dp * 4;
     p.ml = (long long)p.pass * nh * top * p.sub * 8;
