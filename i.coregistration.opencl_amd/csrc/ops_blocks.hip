@@ -692,15 +692,16 @@ __global__ void __launch_bounds__(64 * SEL_TW, T > 16 ? 2 : T > 8 ? 3 : 4)
 }
 
 /* The kernel of a selection. us, a wave a row and tiles of 16 rows: 4096 rows of
- * 256 blocks 11.3, 17.2; 8192 17.7, 16.4; 65536 197, 37; of 51 blocks, 4096 rows
- * 10.2, 9.2. One wave and 16 a row: 16 rows of 2047 blocks 65, 14; 1024 rows 71,
- * 41; 4096 rows 119, 144; of 256 blocks, 16 rows 11.4, 11.2. */
+ * 256 blocks 9.7, 17.4; 8192 15.5, 17.0; 16384 26, 16.8; 8192 rows of 500 24.9,
+ * 25.4; of 51 blocks, 4096 rows 8.5, 9.4; 8192 14.5, 9.4. One wave and 16 a row: 16
+ * rows of 2047 blocks 42, 10.6; 1024 rows 48, 36; 2048 rows 59, 60; of 256 blocks,
+ * 16 rows 5.2, 7.3. */
 enum { SEL_WAVE, SEL_WAVES, SEL_TILE };
 
 static int sel_choose(long long rows, int nhk, int nblk, int top, int cus)
 {
     if (nblk >= 1 && nblk <= 512 && top <= 32 && nhk <= 65535 &&
-        rows >= (nblk <= 128 ? 16LL : 32LL) * cus)
+        rows >= (nblk <= 128 ? 20LL : 36LL) * cus)
         return SEL_TILE;
     return nblk > rows + 256 ? SEL_WAVES : SEL_WAVE;
 }

@@ -176,7 +176,8 @@ def test_refreshed_index(dev, ic):
 TIES = [(5, 5), (64, 8), (65, 32), (65, 64), (200, 16), (256, 17), (500, 9), (513, 16), (1100, 64), (1600, 3), (9000, 20)]
 
 
-@pytest.mark.parametrize("n,top,nq", [t + (9,) for t in TIES] + [t + (2100,) for t in TIES if t[0] <= 513])
+@pytest.mark.parametrize("n,top,nq", [t + (9,) for t in TIES] + [t + (2100,) for t in TIES if t[0] <= 513] +
+                         [t + (2400,) for t in TIES if 128 < t[0] <= 512])
 def test_selection_of_ties(n, top, nq, dev, ic):
     """Scores that repeat, zeros of both signs, scales of zero, blocks without
     keys and NaN scales: lower blocks first."""
@@ -217,6 +218,32 @@ def test_selection_of_many(rows, n, dev, ic):
     SEL = dev.upload(np.full(rows * 2 * top, 99, np.int32))
     work = dev.alloc(dev.api.ops_block_select_work_bytes(rows, 2, n, top))
     dev.api.ops_block_select(dev.po, ic.mat(Q, 0, 2 * d), rows, 2, 1, d, KC.mem, KS.mem, n, top, SEL.mem, work.mem)
+    assert np.array_equal(dev.read(SEL, dtype=np.int32).reshape(rows, 2, top), ref.select(q, kc, ks, top))
+
+
+@pytest.mark.parametrize("top", [7, 16, 31])
+@pytest.mark.parametrize("d", [60, 128])
+@pytest.mark.parametrize("n", [50, 128, 255, 512])
+def test_selection_by_tiles(n, d, top, dev, ic):
+    """Rows for the matrix instructions at every width of them: scores that
+    differ, that repeat, blocks without keys, a query that is not finite."""
+    print(f"[blocks] tiles {n} {d} {top}", flush=True)
+    rows = 2700 if n <= 128 else 4700
+    assert ic.lib().icoreg_select_choice(dev.po, rows, 2, 1, n, top) == 2
+    rng = np.random.default_rng(n + d + top)
+    full = np.zeros((n, 1, 64 if d <= 64 else 128), np.int8)
+    full[..., :d] = rng.integers(-127, 128, (n, 1, d))
+    kc = full[..., :d]
+    kc[n // 3:n // 2] = kc[n // 3]
+    ks = rng.random((n, 1)).astype(np.float32)
+    ks[n // 3:n // 2] = 2.0
+    ks[rng.integers(0, n, 5)] = -1.0
+    q = rng.standard_normal((rows, 2, d)).astype(np.float32)
+    q[:64] = rng.integers(-1, 2, (64, 2, d))
+    q[1000, 1, 3] = np.inf
+    Q, KC, KS = dev.upload(q), dev.upload(full), dev.upload(ks)
+    SEL = dev.upload(np.full(rows * 2 * top, 99, np.int32))
+    dev.api.ops_block_select(dev.po, ic.mat(Q, 0, 2 * d), rows, 2, 1, d, KC.mem, KS.mem, n, top, SEL.mem, None)
     assert np.array_equal(dev.read(SEL, dtype=np.int32).reshape(rows, 2, top), ref.select(q, kc, ks, top))
 
 
