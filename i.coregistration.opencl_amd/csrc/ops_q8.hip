@@ -191,8 +191,8 @@ __device__ __forceinline__ float q8_gelu_tanh(float v)
     return v / (1.0f + __builtin_amdgcn_exp2f(w * -2.88539008f));
 }
 
-/* act(sa sb sum + bias), the sum converted once. ACT: the activation, ACT_LEAKY
- * for ReLU too (slope 0). */
+/* act(sa sb sum + bias), the sum converted once. ReLU is not the leaky one with
+ * slope 0, which makes NaN of minus infinity; a NaN stays one in both. */
 template <int ACT>
 __device__ __forceinline__ float q8_out(int sum, float sa, float sb, float b, float slope)
 {
@@ -202,6 +202,8 @@ __device__ __forceinline__ float q8_out(int sum, float sa, float sb, float b, fl
         return q8_gelu(v);
     if (ACT == ACT_GELU_TANH)
         return q8_gelu_tanh(v);
+    if (ACT == ACT_RELU)
+        return v < 0.0f ? 0.0f : v;
     if (ACT == ACT_LEAKY)
         return v >= 0.0f ? v : slope * v;
     return v;
@@ -620,6 +622,9 @@ static void q8_skinny_launch(const q8_args &g, const float *X, long long ldx, in
     case ACT_GELU_TANH:
         hipLaunchKernelGGL((q8_skinny<TT, FUSED, ACT_GELU_TANH>), grid, block, 0, s, g, X, ldx, in);
         break;
+    case ACT_RELU:
+        hipLaunchKernelGGL((q8_skinny<TT, FUSED, ACT_RELU>), grid, block, 0, s, g, X, ldx, in);
+        break;
     case ACT_LEAKY:
         hipLaunchKernelGGL((q8_skinny<TT, FUSED, ACT_LEAKY>), grid, block, 0, s, g, X, ldx, in);
         break;
@@ -640,6 +645,9 @@ static void q8_launch(const q8_args &g, hipStream_t s)
         break;
     case ACT_GELU_TANH:
         hipLaunchKernelGGL((q8_gemm<BM, BN, WM, WN, BK, KS, ST, ACT_GELU_TANH>), grid, block, 0, s, g);
+        break;
+    case ACT_RELU:
+        hipLaunchKernelGGL((q8_gemm<BM, BN, WM, WN, BK, KS, ST, ACT_RELU>), grid, block, 0, s, g);
         break;
     case ACT_LEAKY:
         hipLaunchKernelGGL((q8_gemm<BM, BN, WM, WN, BK, KS, ST, ACT_LEAKY>), grid, block, 0, s, g);
@@ -805,8 +813,8 @@ static q8_args q8_make(const char *op, int rows, int in, int out, cl_mem WQ, cl_
     g.R = R ? cfptr(R) + roff : nullptr;
     g.C = fptr(Y) + yoff;
     g.ldc = ldy;
-    g.act = act == ACT_RELU ? ACT_LEAKY : act;
-    g.slope = act == ACT_RELU ? 0.0f : slope;
+    g.act = act;
+    g.slope = slope;
     return g;
 }
 

@@ -232,3 +232,62 @@ def test_recorded_and_replayed(rows, dev, ic):
             assert np.all(np.abs(eager.reshape(rows, cout) - want) <= bound)
     finally:
         ic.lib().ocl_graph_free(graph)
+
+
+# Tokens, channels in and out: blocks of 16 and of 32 tokens that code their
+# tokens themselves and that do not, then each tile of the product.
+INFINITE = [(1, 96, 80), (20, 1000, 130), (400, 256, 256), (200, 300, 700), (785, 128, 1000), (1800, 64, 2100),
+            (2100, 64, 2100), (2000, 96, 4100)]
+
+
+def test_every_kernel_is_among_the_infinite_sums(dev, ic):
+    assert {ic.lib().icoreg_q8_choice(dev.po, *s, None) for s in INFINITE} == set(range(6))
+
+
+@pytest.mark.parametrize("entry", ["q8", "qq"])
+@pytest.mark.parametrize("act", [0, 2, 3, 4])
+@pytest.mark.parametrize("shape", INFINITE, ids=[str(s) for s in INFINITE])
+def test_infinite_sums(shape, act, entry, dev, ic):
+    """Finite tokens and weights, biases of either infinity and a token and two
+    channels whose products pass float32's range: the activations' own
+    values there, as the definition has them (ReLU of minus infinity is 0). A
+    token that is not finite stays NaN through each of them. Every other output
+    is within its bound."""
+    print(f"[q8] infinite sums {entry} {shape} {act}", flush=True)
+    rows, cin, cout = shape
+    x, w, b, _ = operands((rows, cin, cout, act, 1, 0, 0), 2)
+    x[0] *= 2.0 ** 100
+    w[2] *= 2.0 ** 60
+    w[3] = -w[2]
+    b[[0, 17]], b[[1, cout - 1]] = np.inf, -np.inf
+    if rows > 1:
+        x[-1, 5] = np.nan
+    X, W, B, Y = dev.upload(x), dev.upload(w), dev.upload(b), dev.zeros(rows * cout)
+    WQ, WS = dev.alloc(cout * ref.pitch(cin)), dev.alloc(cout * 4)
+    dev.api.ops_quant_rows(dev.po, cout, cin, W.mem, 0, cin, WQ.mem, WS.mem)
+    if entry == "q8":
+        work = dev.alloc(dev.api.ops_linear_q8_work_bytes(rows, cin))
+        dev.api.ops_linear_q8(dev.po, rows, cin, cout, X.mem, 0, cin, WQ.mem, WS.mem, B.mem, None, 0, Y.mem, 0, cout,
+                              act, 0.25, work.mem)
+    else:
+        XQ, XS = dev.alloc(rows * ref.pitch(cin)), dev.alloc(rows * 4)
+        dev.api.ops_quant_rows(dev.po, rows, cin, X.mem, 0, cin, XQ.mem, XS.mem)
+        dev.api.ops_linear_qq(dev.po, rows, cin, cout, XQ.mem, XS.mem, WQ.mem, WS.mem, B.mem, None, 0, Y.mem, 0, cout,
+                              act, 0.25)
+    got = dev.read(Y, rows * cout).reshape(rows, cout)
+    some = np.unique(np.r_[0:min(rows, 16), rows - 1, np.random.default_rng(rows).integers(0, rows, 24)])
+    (xc, xs), (wc, ws) = ref.quant(x[some]), ref.quant(w)
+    with np.errstate(all="ignore"):
+        v = (xc.astype(np.float64) @ wc.astype(np.float64).T) * xs[:, None].astype(np.float64) * ws.astype(np.float64)
+        t = v + b
+        # What float32 cannot hold is infinite before the activation.
+        t = np.where(np.abs(t) < 2.0 ** 128, t, np.sign(t) * np.inf)
+        want = ref.act(t, act, 0.25)
+        grow, own = (1.13, 8) if act in (1, 4) else (1, 1)
+        bound = U * (grow * (3 * np.abs(v) + np.abs(t)) + own * np.abs(t) + 2 * np.abs(want)) + 1e-37
+    # Token 0 passes the range in channels 2 and 3, one each way.
+    assert {t[0, 2], t[0, 3]} == {np.inf, -np.inf}
+    odd = ~np.isfinite(t)
+    assert rows == 1 or np.isnan(want[-1]).all()
+    assert np.array_equal(got[some][odd], want[odd].astype(np.float32), equal_nan=True)
+    assert np.all(np.abs(got[some][~odd] - want[~odd]) <= bound[~odd])
