@@ -1455,10 +1455,32 @@ __global__ void __launch_bounds__(64 * blk_waves(ND, NB), blk_simd(ND, NB))
         turn(rest + 32 * wave, 0, min(32, all - 32 * wave));
 }
 
+/* A unit's weight as the merge's lanes hand it round: negative (-0 too) where
+ * the outputs are scaled, BLK_NO_UNIT where there are none. */
+#define BLK_NO_UNIT 2.0f /* weights are at most 1, or NaN */
+
+__device__ __forceinline__ float blk_weight(float w, float sum)
+{
+    return sum < 0.0f ? -w : sum != 0.0f ? w : BLK_NO_UNIT;
+}
+
+__device__ __forceinline__ void blk_add(const float4 &p, float w, float (&o)[4])
+{
+    const float down = __builtin_signbitf(w) ? 1.0f / SPLIT_UP : 1.0f;
+
+    w = fabsf(w);
+    o[0] = fmaf(p.x * down, w, o[0]);
+    o[1] = fmaf(p.y * down, w, o[1]);
+    o[2] = fmaf(p.z * down, w, o[2]);
+    o[3] = fmaf(p.w * down, w, o[3]);
+}
+
 /* Units of a row merged: softmax over all of them from their maxima and sums.
  * A wave a row: lane u has unit u's weight (and unit 64 + u's), then DP / 4
  * lanes a unit add the outputs, 256 / DP units at a time. A negative sum: the
- * outputs are SPLIT_UP times as large. Bound by memory: 65536 rows of 16 units
+ * outputs are SPLIT_UP times as large, and the weight goes round with a minus;
+ * the outputs are unscaled, not the weight, whose last bits would be lost from
+ * 2^-102 on (2^-122: all of them, with values large enough to count). Bound by memory: 65536 rows of 16 units
  * of 64 channels, 285 MB, 43 us, 6.6 TB/s. */
 template <int DP> __global__ void __launch_bounds__(256) blk_merge_kernel(const blk_args a)
 {
@@ -1478,10 +1500,7 @@ template <int DP> __global__ void __launch_bounds__(256) blk_merge_kernel(const 
     const float wx = x.y != 0.0f ? __builtin_amdgcn_exp2f(x.x - m) : 0.0f;
     const float wy = y.y != 0.0f ? __builtin_amdgcn_exp2f(y.x - m) : 0.0f;
     const float l = wave_sum_full(fabsf(x.y) * wx + fabsf(y.y) * wy);
-    auto weight = [](float w, float sum) {
-        return sum < 0.0f ? w * (1.0f / SPLIT_UP) : sum != 0.0f ? w : -1.0f;
-    };
-    const float vx = weight(wx, x.y), vy = weight(wy, y.y);
+    const float vx = blk_weight(wx, x.y), vy = blk_weight(wy, y.y);
     float o[4] = {0, 0, 0, 0};
 
     /* Four loads on their way at once; units with no key hold nothing. */
@@ -1495,16 +1514,12 @@ template <int DP> __global__ void __launch_bounds__(256) blk_merge_kernel(const 
             const float wu = __shfl(u < 64 ? vx : vy, u & 63, 64);
 
             p[i] = *(const float4 *)(part + (long long)at * DP);
-            w[i] = u < units ? wu : -1.0f;
+            w[i] = u < units ? wu : BLK_NO_UNIT;
         }
 #pragma unroll
         for (int i = 0; i < 4; i++)
-            if (!(w[i] < 0.0f)) {
-                o[0] = fmaf(p[i].x, w[i], o[0]);
-                o[1] = fmaf(p[i].y, w[i], o[1]);
-                o[2] = fmaf(p[i].z, w[i], o[2]);
-                o[3] = fmaf(p[i].w, w[i], o[3]);
-            }
+            if (w[i] != BLK_NO_UNIT)
+                blk_add(p[i], w[i], o);
     }
 #pragma unroll
     for (int s = LV; s < 64; s *= 2)
@@ -1544,9 +1559,9 @@ template <int DP> __global__ void __launch_bounds__(256) blk_merge16_kernel(cons
     m = fmaxf(m, dpp_f(m, 0x4E));
     m = fmaxf(m, dpp_f(m, 0x141));
     m = fmaxf(m, dpp_f(m, 0x140));
-    const float w = x.y != 0.0f ? __builtin_amdgcn_exp2f(x.x - m) : -1.0f;
-    float l = x.y != 0.0f ? fabsf(x.y) * w : 0.0f;
-    const float wv = x.y < 0.0f ? w * (1.0f / SPLIT_UP) : w;
+    const float w = x.y != 0.0f ? __builtin_amdgcn_exp2f(x.x - m) : 0.0f;
+    float l = fabsf(x.y) * w;
+    const float wv = blk_weight(w, x.y);
 
     l += dpp_f(l, 0xB1);
     l += dpp_f(l, 0x4E);
@@ -1561,21 +1576,17 @@ template <int DP> __global__ void __launch_bounds__(256) blk_merge16_kernel(cons
             const int u = u0 + i * GV + gv, at = min(u, units - 1);
             const float v = __shfl(wv, (lane & 48) | at, 64);
 
-            wu[i] = u < units ? v : -1.0f;
+            wu[i] = u < units ? v : BLK_NO_UNIT;
 #pragma unroll
             for (int r = 0; r < RUNS; r++)
                 p[i][r] = *(const float4 *)(part + (long long)at * DP + 64 * r);
         }
 #pragma unroll
         for (int i = 0; i < 4; i++)
-            if (!(wu[i] < 0.0f)) {
+            if (wu[i] != BLK_NO_UNIT) {
 #pragma unroll
-                for (int r = 0; r < RUNS; r++) {
-                    o[r][0] = fmaf(p[i][r].x, wu[i], o[r][0]);
-                    o[r][1] = fmaf(p[i][r].y, wu[i], o[r][1]);
-                    o[r][2] = fmaf(p[i][r].z, wu[i], o[r][2]);
-                    o[r][3] = fmaf(p[i][r].w, wu[i], o[r][3]);
-                }
+                for (int r = 0; r < RUNS; r++)
+                    blk_add(p[i][r], wu[i], o[r]);
             }
     }
     if (GV == 2)

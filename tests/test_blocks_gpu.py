@@ -517,3 +517,51 @@ def test_results_do_not_depend_on_the_other_queries(dev, ic):
         outs.append((lo, c.out()))
     for lo, o in outs[1:]:
         assert np.array_equal(o, outs[0][1][lo:lo + len(o)])
+
+
+@pytest.mark.parametrize("top", [2, 9])
+@pytest.mark.parametrize("apart", [True], ids=["two units"])
+@pytest.mark.parametrize("ev", [70, 88])
+@pytest.mark.parametrize("nq,bs,d", [(5, 32, 64), (5, 64, 128), (5, 128, 20), (2600, 32, 64), (2600, 64, 32),
+                                     (2600, 64, 100), (2600, 32, 128), (2600, 128, 64)])
+def test_small_weights_of_large_values(nq, bs, d, ev, apart, top, dev, ic):
+    """A key of weight 1 beside keys of weights 2^-121 .. 2^-124 whose values
+    are 2^139 times as large: the output is the latter's, and keeps float32's
+    accuracy, in one unit of keys and in two, for few queries and for many.
+
+    One product of a score is not zero, and has few bits. So a score's error is
+    the scaling's: the constant log2 e, its product with scale, that with the
+    query, and two roundings of the sum of its parts, 5 U of the score, which a
+    weight has relatively beside 4 U for its exponential; the sums, the merge,
+    the division and the parts as in long_ref.attend."""
+    print(f"[blocks] small weights {nq} {bs} {d} 2^{ev} {apart} {top}", flush=True)
+    h, nk = 2, 2 * bs
+    rng = np.random.default_rng(nq + d + ev)
+    assert ic.lib().icoreg_blocks_choice(nq, nk, h, h, d, bs, top) == (nq > 5)
+    q, k, v = (rng.uniform(1, 2, (n, h, d)) for n in (nq, nk, nk))
+    k[:], v[:] = 0, 0
+    q[..., 0] = np.where(np.arange(nq) % 2, 255 / 256, 127 / 128)[:, None]
+    small = np.arange(bs + 3, bs + 9) if apart else np.arange(3, 9)
+    k[..., 0] = -2000.0
+    k[0, :, 0] = 0
+    k[small, :, 0] = -rng.integers(122, 125, (6, h))
+    v[0] = np.ldexp(rng.uniform(-2, 2, (h, d)), ev - 139)
+    v[small] = np.ldexp(rng.uniform(1, 2, (6, h, d)), ev)
+    scale = float(np.float32(np.log(2)))
+    q, k, v = (x.astype(np.float32) for x in (q, k, v))
+    c = Case(dev, ic, q, k, v, bs, top, scale)
+    sel = np.full((nq, h, top), -1, np.int32)
+    sel[..., -2:] = [1, 0]
+    dev.write(c.SEL, sel)
+    c.attend()
+    got = c.out().astype(np.float64)
+    s = scale * np.einsum("qh,kh->qhk", q[..., 0].astype(np.float64), k[..., 0].astype(np.float64))
+    p = np.exp(s - s.max(-1, keepdims=True))
+    p /= p.sum(-1, keepdims=True)
+    want = np.stack([p[:, i] @ v[:, i].astype(np.float64) for i in range(h)], 1)
+    size = np.abs(s[..., np.r_[0, small]]).max()
+    rel = 2 * (5 * size + 4) + 64 + 4 + 48
+    # Values of one sign where they count: sum p |v| is the output.
+    worst = np.max(np.abs(got - want) / (U * rel * want))
+    print(f"[blocks] worst {worst:.3f} of the bound", flush=True)
+    assert (want > 0).all() and worst <= 1
