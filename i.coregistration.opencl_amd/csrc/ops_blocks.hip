@@ -1030,8 +1030,9 @@ template <int CTRL> __device__ __forceinline__ int quad_i(int v)
  * read once for all of them, where a row on its own would read its 16 blocks
  * of keys and values again, 512 KB. Each wave collects its own rows and meets the
  * others at the start and at the end only (with barriers in between 184 us, without
- * 180, by 8 waves 172). Outputs leave times SPLIT_UP, marked by a negative sum, which the merge
- * takes into its weights.
+ * 180, by 8 waves 172). Outputs leave as the products give them, values and
+ * probabilities scaled by SPLIT_UP each, marked by a negative sum; the merge
+ * unscales them.
  *
  * 65536 rows of 16 units of 64 keys of 64 channels: 172 us, 600 TFLOP/s of bf16
  * products. The matrix cores are busy 28 % of it, vector instructions (splits
@@ -1041,7 +1042,7 @@ template <int CTRL> __device__ __forceinline__ int quad_i(int v)
  * then; no look at the lists: 165; one query for all: 176. */
 #define BLK_RING 128   /* rows of a wave's list at most */
 #define BLK_TILES 1024 /* tiles of 64 rows a block of threads takes at most */
-#define BLK_VMAX 0x1p90f /* 64 scaled values stay finite below */
+#define BLK_VMAX 0x1p73f /* 64 values times 2^48 stay finite below */
 
 /* Waves of a block of threads, and of a SIMD. LDS holds two blocks of threads of
  * 64 keys of 64 channels in 48 KB and some, one of 128 channels in 96: of 8 waves
@@ -1296,8 +1297,9 @@ __global__ void __launch_bounds__(64 * blk_waves(ND, NB), blk_simd(ND, NB))
         split_f16x o[ND];
         split_u4 high[2 * NB];
 
-        /* Again the small products first. Probabilities are not scaled: the
-         * largest is 1, and what those under 2^-110 lose is nothing to it. */
+        /* Again the small products first. Probabilities are scaled as values
+         * are: those under 2^-110 would lose bits (2^-124: all but ten), which
+         * counts beside values 2^100 times the largest probability's. */
 #pragma unroll
         for (int tt = 0; tt < ND; tt++)
 #pragma unroll
@@ -1317,7 +1319,7 @@ __global__ void __launch_bounds__(64 * blk_waves(ND, NB), blk_simd(ND, NB))
 #pragma unroll
             for (int j = 0; j < 8; j++)
                 x[j] = p[u / 2][8 * (u % 2) + j];
-            split8(x, 1.0f, pp[0], pp[1], pp[2]);
+            split8(x, SPLIT_UP, pp[0], pp[1], pp[2]);
             high[u] = pp[0];
 #pragma unroll
             for (int tt = 0; tt < ND; tt++) {
@@ -1466,7 +1468,7 @@ __device__ __forceinline__ float blk_weight(float w, float sum)
 
 __device__ __forceinline__ void blk_add(const float4 &p, float w, float (&o)[4])
 {
-    const float down = __builtin_signbitf(w) ? 1.0f / SPLIT_UP : 1.0f;
+    const float down = __builtin_signbitf(w) ? SPLIT_DOWN : 1.0f;
 
     w = fabsf(w);
     o[0] = fmaf(p.x * down, w, o[0]);
@@ -1478,9 +1480,9 @@ __device__ __forceinline__ void blk_add(const float4 &p, float w, float (&o)[4])
 /* Units of a row merged: softmax over all of them from their maxima and sums.
  * A wave a row: lane u has unit u's weight (and unit 64 + u's), then DP / 4
  * lanes a unit add the outputs, 256 / DP units at a time. A negative sum: the
- * outputs are SPLIT_UP times as large, and the weight goes round with a minus;
+ * outputs are scaled, and the weight goes round with a minus;
  * the outputs are unscaled, not the weight, whose last bits would be lost from
- * 2^-102 on (2^-122: all of them, with values large enough to count). Bound by memory: 65536 rows of 16 units
+ * 2^-78 on, with values large enough to count. Bound by memory: 65536 rows of 16 units
  * of 64 channels, 285 MB, 43 us, 6.6 TB/s. */
 template <int DP> __global__ void __launch_bounds__(256) blk_merge_kernel(const blk_args a)
 {

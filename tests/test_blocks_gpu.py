@@ -520,7 +520,7 @@ def test_results_do_not_depend_on_the_other_queries(dev, ic):
 
 
 @pytest.mark.parametrize("top", [2, 9])
-@pytest.mark.parametrize("apart", [True], ids=["two units"])
+@pytest.mark.parametrize("apart", [False, True], ids=["one unit", "two units"])
 @pytest.mark.parametrize("ev", [70, 88])
 @pytest.mark.parametrize("nq,bs,d", [(5, 32, 64), (5, 64, 128), (5, 128, 20), (2600, 32, 64), (2600, 64, 32),
                                      (2600, 64, 100), (2600, 32, 128), (2600, 128, 64)])
