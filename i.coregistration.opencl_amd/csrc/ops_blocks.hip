@@ -23,6 +23,7 @@
 
 #include <math.h>
 
+#include <algorithm>
 #include <type_traits>
 
 #include "common.h"
@@ -1616,9 +1617,21 @@ template <int DP> __global__ void __launch_bounds__(256) blk_merge16_kernel(cons
  * buffer. */
 struct blk_plan {
     bool direct;
-    int pass, tiles, dp, sub, nblk;
+    int pass, passes, tiles, dp, sub, nblk;
     long long part, ml, bits; /* bytes */
 };
+
+/* Units that lists pay for, see below. */
+#define BLK_LIST_UNITS 400000 /* units times (channels + 32), more than that */
+#define BLK_LIST_ROWS 5       /* rows that list a block, on average */
+
+static int blk_width(int d) { return d <= 32 ? 32 : d <= 64 ? 64 : 128; }
+
+/* Bytes of a query's units: outputs, maxima and sums. */
+static long long blk_query_bytes(int nh, int d, int bs, int top)
+{
+    return (long long)nh * top * blk_sub(bs) * (blk_width(d) + 2) * 4;
+}
 
 /* Units of a pass: 8192 x 8 rows of 16 units of 64 channels 294 us in two
  * passes of 256 MiB, 270 in one; 350 in three. */
@@ -1631,13 +1644,13 @@ static blk_plan blk_plan_of(int Nq, int Nk, int nh, int nhk, int d, int bs, int 
 
     p.nblk = ops_key_blocks(Nk, bs);
     p.sub = blk_sub(bs);
-    p.dp = d <= 32 ? 32 : d <= 64 ? 64 : 128;
-    const long long row = (long long)top * p.sub * (p.dp + 2) * 4; /* bytes a row */
+    p.dp = blk_width(d);
     /* A query's units and bits. */
-    const long long most = max(1LL, BLK_PART_BYTES / (row * nh + (long long)nh * p.nblk / 8 + 1));
-    const long long passes = (Nq + most - 1) / most;
+    const long long most = max(1LL, BLK_PART_BYTES / (blk_query_bytes(nh, d, bs, top) +
+                                                      (long long)nh * p.nblk / 8 + 1));
 
-    p.pass = (int)((Nq + passes - 1) / passes);
+    p.passes = (int)((Nq + most - 1) / most);
+    p.pass = (Nq - 1) / p.passes + 1;
     /* Units one by one or by lists, us: 8 heads of 64 on 256 blocks of 64 keys,
      * 16 listed, 32 queries 22, 22; 48 queries 28, 22; 1024 queries 435, 49. 8 heads
      * of 128, 8 of 64 blocks, 32 queries 24, 31; 64 queries 40, 32; of 32, 8 of 100
@@ -1648,12 +1661,35 @@ static blk_plan blk_plan_of(int Nq, int Nk, int nh, int nhk, int d, int bs, int 
 
     /* Lists place their outputs by 32 bits (a query of very many heads passes them). */
     p.direct = p.nblk == 0 || nhk > 65535 || units * p.dp * 4 > 1LL << 32 ||
-               units * (p.dp + 32) <= 400000 || (long long)p.pass * g * top < 5LL * p.nblk;
+               units * (p.dp + 32) <= BLK_LIST_UNITS ||
+               (long long)p.pass * g * top < (long long)BLK_LIST_ROWS * p.nblk;
     p.tiles = ((p.pass * g + 63) / 64 + BLK_TW - 1) / BLK_TW * BLK_TW;
     p.part = (long long)p.pass * nh * top * p.sub * p.dp * 4;
     p.ml = (long long)p.pass * nh * top * p.sub * 8;
     p.bits = p.direct ? 0 : (long long)nhk * p.nblk * p.tiles * 8;
     return p;
+}
+
+/* Bytes that cover this call and every one of fewer queries, keys or listed
+ * blocks, whatever their passes and kernels: the sizes of blk_plan's parts fall
+ * where a pass more or another kernel begins. Units of all queries and their
+ * bits, or, where passes end that, what blk_plan_of holds a pass to: q queries
+ * of u bytes have bits of at most q nh / 8 + 64 nhk bytes a key block (whole runs
+ * of tiles), and q (u + nh nblk / 8) <= BLK_PART_BYTES or q = 1. Lists need so many
+ * units, and are taken on at most so many blocks. */
+static size_t blk_work_bytes(int Nq, int Nk, int nh, int nhk, int d, int bs, int top)
+{
+    typedef __int128 wide; /* products of any sizes */
+    const int g = nh / nhk;
+    const wide u = blk_query_bytes(nh, d, bs, top), rows = (wide)Nq * g;
+    const bool lists = nhk <= 65535 &&
+                       (wide)Nq * nh * top * blk_sub(bs) * (blk_width(d) + 32) > BLK_LIST_UNITS;
+    const wide nblk = lists ? std::min<wide>(ops_key_blocks(Nk, bs), rows * top / BLK_LIST_ROWS) : 0;
+    const wide tiles = ((rows + 63) / 64 + BLK_TW - 1) / BLK_TW * BLK_TW;
+    const wide all = Nq * u + nhk * nblk * tiles * 8;
+    const wide held = std::max<wide>(BLK_PART_BYTES, u + nh * nblk / 8) + 64 * nhk * nblk;
+
+    return (size_t)std::min(all, held);
 }
 
 static bool blk_sizes_ok(int Nq, int Nk, int nh, int nhk, int d, int bs, int top)
@@ -1667,9 +1703,19 @@ extern "C" size_t ops_attention_blocks_work_bytes(int Nq, int Nk, int nh, int nh
 {
     if (!blk_sizes_ok(Nq, Nk, nh, nhk, d, bs, top) || Nq == 0)
         return 0;
+    return blk_work_bytes(Nq, Nk, nh, nhk, d, bs, top);
+}
+
+extern "C" int icoreg_blocks_passes(int Nq, int Nk, int nh, int nhk, int d, int bs, int top,
+                                    size_t *work)
+{
+    if (!blk_sizes_ok(Nq, Nk, nh, nhk, d, bs, top) || Nq == 0)
+        return -1;
     const blk_plan p = blk_plan_of(Nq, Nk, nh, nhk, d, bs, top);
 
-    return (size_t)(p.part + p.ml + p.bits);
+    if (work)
+        *work = (size_t)(p.part + p.ml + p.bits);
+    return p.passes;
 }
 
 extern "C" int icoreg_blocks_choice(int Nq, int Nk, int nh, int nhk, int d, int bs, int top)

@@ -106,6 +106,10 @@ int icoreg_q8_choice(struct ops *o, int rows, int in, int out, int *first);
  * 1 lists of the rows of each (-1: sizes that it refuses). For tests. */
 int icoreg_select_choice(struct ops *o, int Nq, int nh, int nhk, int nblk, int top);
 int icoreg_blocks_choice(int Nq, int Nk, int nh, int nhk, int d, int bs, int top);
+/* How many passes over the queries ops_attention_blocks takes and, in *work (may
+ * be NULL), the bytes of work that they use; -1 for sizes that it refuses. For
+ * tests. */
+int icoreg_blocks_passes(int Nq, int Nk, int nh, int nhk, int d, int bs, int top, size_t *work);
 /* How many times roma_match has re-run a GP solve through
  * roma_gp_solve_events after the in-kernel wait gave up. */
 int icoreg_roma_gp_retries(const struct roma_model *m);

@@ -188,9 +188,11 @@ void ops_rope(struct ops *o, cl_mem X, long off, int ld, long rows, int nh,
  * allocate nothing and leave the ops work buffer alone: what they need for
  * themselves is the caller's `work` buffer, of the size that the call's
  * _work_bytes function gives (0 where the sizes are invalid), 16-byte
- * aligned, its content of no meaning between calls. Calls that may overlap
- * on the device (recorded graphs replayed side by side among them) need work
- * buffers of their own. */
+ * aligned, its content of no meaning between calls. The size never falls as
+ * tokens, keys, channels in or listed blocks grow: a buffer for the longest
+ * call serves the shorter ones. Calls that may overlap on the device
+ * (recorded graphs replayed side by side among them) need work buffers of
+ * their own. */
 
 /* 8-bit codes and scales of rows of C floats, row r at float xoff + r ldx of
  * X: with a = max |x|, S[r] = a / 127 and code(x) = x (127 / a) in float32,

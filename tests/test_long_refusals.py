@@ -286,3 +286,33 @@ def test_launches(ic, env):
     assert choose(1, 2048, 65536, 1, 128, 64, 64) == 1
     assert choose(1, 2048, 131072, 1, 128, 64, 64) == 1
     assert choose(1, 2048, 131073, 1, 128, 64, 64) == 0
+
+
+# Heads, key heads, channels, block, top.
+WORK = [(8, 2, 64, 64, 16), (16, 16, 128, 64, 16), (4, 1, 32, 16, 1), (1, 1, 16, 128, 64), (12, 4, 100, 32, 7),
+        (16, 4, 128, 64, 16), (65540, 65540, 8, 16, 2)]
+
+
+@pytest.mark.parametrize("h,kv,d,bs,top", WORK)
+def test_work_covers_every_shorter_call(h, kv, d, bs, top, ic):
+    """The work of a call is enough for every call of fewer queries or keys:
+    across the border where one pass becomes two, and where units go by
+    lists, one by one otherwise."""
+    work = ic.api().ops_attention_blocks_work_bytes
+    rng = np.random.default_rng(h + d)
+    one = [work(n, 100, h, kv, d, bs, top) for n in (1, 2)]
+    border = (512 << 20) // max(1, one[1] - one[0])
+    queries = sorted({1, 2, 3, 64, *(max(1, m * border + e) for m in (1, 2, 3) for e in (-2, -1, 0, 1, 2)),
+                      *(int(x) for x in np.exp(rng.uniform(0, np.log(3 * border + 64), 40)))})
+    keys = sorted({0, 1, 16380, 52416, 52480, *(int(x) for x in np.exp(rng.uniform(0, np.log(4e6), 60)))})
+    size = np.array([[work(n, k, h, kv, d, bs, top) for k in keys] for n in queries])
+    used, passes, n = np.zeros_like(size), set(), C.c_size_t()
+    for i, nq in enumerate(queries):
+        for j, nk in enumerate(keys):
+            passes.add(ic.lib().icoreg_blocks_passes(nq, nk, h, kv, d, bs, top, C.byref(n)))
+            used[i, j] = n.value
+    assert (used <= size).all() and {1, 2, 3} <= passes
+    assert (np.diff(size, axis=0) >= 0).all() and (np.diff(size, axis=1) >= 0).all()
+    # By the number of blocks listed, too.
+    for n, k in ((1, 5000), (700, 5000), (border, 5000), (3 * border, 5000)):
+        assert (np.diff([work(n, k, h, kv, d, bs, t) for t in range(1, 65)]) >= 0).all()
