@@ -258,6 +258,7 @@ SIGNATURES = {
     "icoreg_gemm_choice": (_I, [_O, _I, _I, _I, _I, _I, _I]),
     "icoreg_select_choice": (_I, [_O, _I, _I, _I, _I, _I]),
     "icoreg_blocks_choice": (_I, [_I, _I, _I, _I, _I, _I, _I]),
+    "icoreg_blocks_budget": (None, [_L]),
     "icoreg_blocks_passes": (_I, [_I, _I, _I, _I, _I, _I, _I, C.POINTER(C.c_size_t)]),
     "icoreg_q8_choice": (_I, [_O, _I, _I, _I, C.POINTER(C.c_int)]),
     "icoreg_conv5_choice": (_I, [_O, _I, _I, _I, _I, _I, _I]),
@@ -280,7 +281,8 @@ _NO_CHECK = {"ocl_graph_free", "icoreg_set_fatal_mode", "icoreg_last_error", "ic
              "icoreg_roma_last", "disk_topn_work_bytes", "adalam_nearest_work_bytes",
              "icoreg_gp_test_wait", "icoreg_roma_gp_retries", "icoreg_conv_wino_form",
              "icoreg_conv_wino_choice", "icoreg_gemm_choice", "icoreg_conv5_choice",
-             "icoreg_q8_choice", "icoreg_select_choice", "icoreg_blocks_choice", "icoreg_blocks_passes"}
+             "icoreg_q8_choice", "icoreg_select_choice", "icoreg_blocks_choice", "icoreg_blocks_passes",
+             "icoreg_blocks_budget"}
 
 _lib = None
 

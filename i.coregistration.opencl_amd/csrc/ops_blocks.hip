@@ -1637,6 +1637,13 @@ static long long blk_query_bytes(int nh, int d, int bs, int top)
  * passes of 256 MiB, 270 in one; 350 in three. */
 #define BLK_PART_BYTES (512LL << 20)
 
+static long long g_blk_budget = BLK_PART_BYTES;
+
+extern "C" void icoreg_blocks_budget(long bytes)
+{
+    g_blk_budget = bytes > 0 ? bytes : BLK_PART_BYTES;
+}
+
 static blk_plan blk_plan_of(int Nq, int Nk, int nh, int nhk, int d, int bs, int top)
 {
     blk_plan p;
@@ -1646,8 +1653,8 @@ static blk_plan blk_plan_of(int Nq, int Nk, int nh, int nhk, int d, int bs, int 
     p.sub = blk_sub(bs);
     p.dp = blk_width(d);
     /* A query's units and bits. */
-    const long long most = max(1LL, BLK_PART_BYTES / (blk_query_bytes(nh, d, bs, top) +
-                                                      (long long)nh * p.nblk / 8 + 1));
+    const long long most = max(1LL, g_blk_budget / (blk_query_bytes(nh, d, bs, top) +
+                                                    (long long)nh * p.nblk / 8 + 1));
 
     p.passes = (int)((Nq + most - 1) / most);
     p.pass = (Nq - 1) / p.passes + 1;
@@ -1675,7 +1682,7 @@ static blk_plan blk_plan_of(int Nq, int Nk, int nh, int nhk, int d, int bs, int 
  * where a pass more or another kernel begins. Units of all queries and their
  * bits, or, where passes end that, what blk_plan_of holds a pass to: q queries
  * of u bytes have bits of at most q nh / 8 + 64 nhk bytes a key block (whole runs
- * of tiles), and q (u + nh nblk / 8) <= BLK_PART_BYTES or q = 1. Lists need so many
+ * of tiles), and q (u + nh nblk / 8) is within the budget or q = 1. Lists need so many
  * units, and are taken on at most so many blocks. */
 static size_t blk_work_bytes(int Nq, int Nk, int nh, int nhk, int d, int bs, int top)
 {
@@ -1687,7 +1694,7 @@ static size_t blk_work_bytes(int Nq, int Nk, int nh, int nhk, int d, int bs, int
     const wide nblk = lists ? std::min<wide>(ops_key_blocks(Nk, bs), rows * top / BLK_LIST_ROWS) : 0;
     const wide tiles = ((rows + 63) / 64 + BLK_TW - 1) / BLK_TW * BLK_TW;
     const wide all = Nq * u + nhk * nblk * tiles * 8;
-    const wide held = std::max<wide>(BLK_PART_BYTES, u + nh * nblk / 8) + 64 * nhk * nblk;
+    const wide held = std::max<wide>(g_blk_budget, u + nh * nblk / 8) + 64 * nhk * nblk;
 
     return (size_t)std::min(all, held);
 }

@@ -110,6 +110,10 @@ int icoreg_blocks_choice(int Nq, int Nk, int nh, int nhk, int d, int bs, int top
  * be NULL), the bytes of work that they use; -1 for sizes that it refuses. For
  * tests. */
 int icoreg_blocks_passes(int Nq, int Nk, int nh, int nhk, int d, int bs, int top, size_t *work);
+/* The bytes of work that a pass of ops_attention_blocks is held to, for the
+ * whole process (0: the library's own choice), also by its _work_bytes. For
+ * tests. */
+void icoreg_blocks_budget(long bytes);
 /* How many times roma_match has re-run a GP solve through
  * roma_gp_solve_events after the in-kernel wait gave up. */
 int icoreg_roma_gp_retries(const struct roma_model *m);

@@ -565,3 +565,73 @@ def test_small_weights_of_large_values(nq, bs, d, ev, apart, top, dev, ic):
     worst = np.max(np.abs(got - want) / (U * rel * want))
     print(f"[blocks] worst {worst:.3f} of the bound", flush=True)
     assert (want > 0).all() and worst <= 1
+
+
+# Queries a pass at most, passes, lists; then Nq, Nk, heads, kv heads, d,
+# block, top, mask, offset, pad. The last pass is shorter in all but the last.
+PASSES = [
+    (700, 2, 1, (1025, 300, 4, 4, 64, 64, 3, 1, 0, 0)), (700, 3, 1, (2000, 500, 6, 2, 33, 32, 4, 0, 2, 3)),
+    (110, 3, 1, (299, 2000, 2, 1, 128, 128, 64, 1, 0, 0)), (600, 4, 1, (2399, 90, 3, 1, 32, 16, 6, 1, 1, 0)),
+    (3, 3, 0, (7, 1000, 4, 2, 64, 16, 9, 1, 0, 4)), (9, 2, 0, (17, 3000, 6, 2, 100, 128, 11, 0, 1, 0)),
+    (1, 5, 0, (5, 400, 2, 2, 32, 32, 2, 0, 0, 0))]
+
+
+@pytest.mark.parametrize("place", ["apart", "over the queries"])
+@pytest.mark.parametrize("most,passes,lists,shape", PASSES, ids=[str(p[3]) for p in PASSES])
+def test_passes(most, passes, lists, shape, place, dev, ic):
+    """Calls whose work is held to a few queries' are cut in passes: what one
+    pass computes, bit for bit, and the definition; nothing behind the
+    work that they say they use."""
+    print(f"[blocks] passes {passes} {shape} {place}", flush=True)
+    nq, nk, h, kv, d, bs, top, masked, off, pad = shape
+    q, k, v, mask = draw(nq, nk, h, kv, d, masked)
+    if masked:
+        # A unit whose values go by float32.
+        mask[nk // 2], v[nk // 2, 0] = 1, v[nk // 2, 0] * 2.0 ** 80
+    scale, lib, used = float(np.float32(1.2 / d ** 0.5)), ic.lib(), ic.C.c_size_t()
+    sizes, outs, sel = (nq, nk, h, kv, d, bs, top), [], None
+    dp = 32 if d <= 32 else 64 if d <= 64 else 128
+    query = h * top * max(1, bs // 64) * (dp + 2) * 4 + h * (-(-nk // bs)) // 8 + 1
+    try:
+        for budget, n in ((0, 1), (most * query, passes)):
+            lib.icoreg_blocks_budget(budget)
+            assert lib.icoreg_blocks_passes(*sizes, ic.C.byref(used)) == n
+            assert lib.icoreg_blocks_choice(*sizes) == lists
+            c = Case(dev, ic, q, k, v, bs, top, scale, mask, off, pad)
+            if sel is None:
+                c.index()
+                c.select()
+                sel = c.sel()
+                # A row of nothing in every pass.
+                sel[::97] = -1
+            dev.write(c.SEL, sel)
+            O = c.Q if place != "apart" else None
+            c.attend(O)
+            outs.append(c.out(O))
+            assert used.value <= dev.api.ops_attention_blocks_work_bytes(*sizes)
+            assert np.isnan(dev.read(c.work)[used.value // 4:]).all()
+    finally:
+        lib.icoreg_blocks_budget(0)
+    assert np.array_equal(outs[0], outs[1])
+    border = np.arange(-(-nq // passes), nq, -(-nq // passes))
+    some = np.unique(np.clip(np.r_[0, nq - 1, 97, border - 1, border, border + 1,
+                                   np.random.default_rng(nq).integers(0, nq, 60)], 0, nq - 1))
+    check(c, q[some], k, v, mask, sel[some], outs[1][some])
+    assert not outs[1][::97].any()
+
+
+@pytest.mark.parametrize("place", ["apart", "over the queries"])
+def test_passes_of_a_long_batch(place, dev, ic):
+    """So many queries that the library cuts them by itself."""
+    print(f"[blocks] long batch {place}", flush=True)
+    nq, nk, h, kv, d, bs, top = sizes = (15901, 2000, 8, 2, 64, 64, 16)
+    assert ic.lib().icoreg_blocks_passes(*sizes, None) == 2 and ic.lib().icoreg_blocks_choice(*sizes) == 1
+    q, k, v, _ = draw(nq, nk, h, kv, d)
+    c = Case(dev, ic, q, k, v, bs, top, 0.125)
+    c.index()
+    c.select()
+    sel = c.sel()
+    O = c.Q if place != "apart" else None
+    c.attend(O)
+    some = np.r_[0:3, 7948:7953, 15898:15901, np.random.default_rng(1).integers(0, nq, 40)]
+    check(c, q[some], k, v, None, sel[some], c.out(O)[some])
