@@ -246,8 +246,8 @@ __global__ void __launch_bounds__(64 * WM * WN * KS) q8_gemm(const q8_args g)
     constexpr int ASZ = BM * BK, BSZ = BN * BK, SZ = ASZ + BSZ;
     constexpr int AL = ASZ / 16 / NT, BL = BSZ / 16 / NT;
     static_assert(AL >= 1 && BL >= 1 && ASZ % (16 * NT) == 0 && BSZ % (16 * NT) == 0, "tile shape");
-    __shared__ __align__(16) signed char s0[SZ], s1[SZ], s2[ST > 2 ? SZ : 16],
-        s3[ST > 3 ? SZ : 16];
+    static_assert(ST == 2 || ST == 3, "buffers");
+    __shared__ __align__(16) signed char s0[SZ], s1[SZ], s2[ST > 2 ? SZ : 16];
 
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -365,8 +365,6 @@ __global__ void __launch_bounds__(64 * WM * WN * KS) q8_gemm(const q8_args g)
     load(BK, s1);
     if (ST > 2)
         load(2 * BK, s2);
-    if (ST > 3)
-        load(3 * BK, s3);
     meet(std::integral_constant<int, ST - 1>());
     read(s0, 0, a[0], b[0]);
     for (int kt = 0; kt < nk; kt += ST) {
@@ -374,9 +372,7 @@ __global__ void __launch_bounds__(64 * WM * WN * KS) q8_gemm(const q8_args g)
         if (kt + 1 < nk)
             step(kt + 1, s1, ST > 2 ? s2 : s0);
         if (ST > 2 && kt + 2 < nk)
-            step(kt + 2, s2, ST > 3 ? s3 : s0);
-        if (ST > 3 && kt + 3 < nk)
-            step(kt + 3, s3, s0);
+            step(kt + 2, s2, s0);
     }
     __builtin_amdgcn_s_waitcnt(q8_wait(0));
     if constexpr (KS > 1) {

@@ -85,15 +85,4 @@ static __device__ __forceinline__ unsigned wave_umax(unsigned v)
                    (unsigned)__builtin_amdgcn_readlane((int)v, 48)));
 }
 
-static __device__ __forceinline__ int wave_isum(int v)
-{
-    const int ctl[4] = {0xB1, 0x4E, 0x141, 0x140};
-
-#pragma unroll
-    for (int k = 0; k < 4; k++)
-        v += dpp_i(v, ctl[k]);
-    return (__builtin_amdgcn_readlane(v, 0) + __builtin_amdgcn_readlane(v, 16)) +
-           (__builtin_amdgcn_readlane(v, 32) + __builtin_amdgcn_readlane(v, 48));
-}
-
 #endif /* ICOREG_Q8_H */
