@@ -15,7 +15,9 @@ sparse  the index of the key blocks, each query's selection, the attention
 
 `run` computes a case with elementary torch operations, or, with `own`, by
 the library's entry points. Tensors live in torch memory; the library gets
-views of it.
+views of it and queues its work on a stream of its own, which torch's streams
+and events know nothing of: what `run` returns then is valid, and a state may
+be written by torch or dropped, only after torch.cuda.synchronize().
 """
 
 import importlib.util
