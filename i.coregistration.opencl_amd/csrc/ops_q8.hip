@@ -167,7 +167,7 @@ struct q8_args {
 /* v times the normal distribution's integral to v: max(v, 0) - |v| g(|v|), g(z)
  * = erfc(z / sqrt 2) / 2 = exp(-z^2 / 2) f(1 / (1 + 0.4 z / sqrt 2)), f a
  * polynomial of degree 6 fitted to exp(x^2) erfc(x) / 2 (its error times
- * exp(-x^2) at most 2e-8): within 4 2^-24 |v|, 17 instructions and no branch, where
+ * exp(-x^2) at most 2e-8): within 4 2^-24 |v|, 16 instructions and no branch, where
  * erff takes both sides of one (64 outputs a lane are the layer's epilogue). */
 __device__ __forceinline__ float q8_gelu(float v)
 {
@@ -180,8 +180,9 @@ __device__ __forceinline__ float q8_gelu(float v)
     p = fmaf(t, p, 6.693785638e-02f);
     p = fmaf(t, p, 1.196817234e-01f);
     p = fmaf(t, p, -3.930720559e-04f);
-    /* Infinity as it is: the difference's second term is infinity times 0. */
-    return v == INFINITY ? v : fmaf(-fabsf(v), e * p, fmaxf(v, 0.0f));
+    /* Infinity stays what it is, where the second term would be infinity times
+     * 0 (3202 x 1024 x 4096 34.3 us without the minimum, 34.6, 34.8 with a select). */
+    return fmaf(-fabsf(fminf(v, 0x1p64f)), e * p, fmaxf(v, 0.0f));
 }
 
 /* The tanh form: 0.5 v (1 + tanh w) = v / (1 + exp(-2 w)). */

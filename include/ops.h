@@ -206,9 +206,11 @@ int ops_q8_pitch(int C);
 void ops_quant_rows(struct ops *o, long rows, int C, cl_mem X, long xoff,
                     int ldx, cl_mem Q, cl_mem S);
 
-/* Y = act(XS[i] WS[j] sum_k XQ[i][k] WQ[j][k] + b[j]) + R, token-major: XQ,
+/* Y = act((XS[i] WS[j]) sum_k XQ[i][k] WQ[j][k] + b[j]) + R, token-major: XQ,
  * XS rows tokens, WQ, WS out channels as ops_quant_rows makes them, in <=
- * 2^17 of both, the sum exact in 32-bit integers. Row i of Y starts at float
+ * 2^17 of both, the sum exact in 32-bit integers, the product of the two
+ * scales rounded to float32 first (its range ends at 2^128, and bits are lost
+ * under 2^-126). Row i of Y starts at float
  * yoff + i ldy; b and R NULL for none, R with Y's row stride from roff, and
  * it may be Y itself, any other overlap of Y is an error. */
 void ops_linear_qq(struct ops *o, int rows, int in, int out, cl_mem XQ,
@@ -283,7 +285,8 @@ void ops_block_select(struct ops *o, struct opnd Q, int Nq, int nh, int nhk,
 /* O = softmax(scale Q K^T) V over the kept keys of each query and head's
  * listed blocks (SEL as above; entries that are no block are skipped, a block
  * listed twice counts once). No key left: zeros. A NaN among the kept scores
- * makes the row NaN; what left-out keys and values hold does not matter. O
+ * makes the row NaN; what left-out keys and values hold does not matter; a
+ * key's weight under 2^-126 of the row's largest may count as zero. O
  * may be Q (same offset and ld), any other overlap of O is an error. */
 size_t ops_attention_blocks_work_bytes(int Nq, int Nk, int nh, int nhk, int d,
                                        int bs, int top);
