@@ -1035,10 +1035,10 @@ template <int CTRL> __device__ __forceinline__ int quad_i(int v)
  * probabilities scaled by SPLIT_UP each, marked by a negative sum; the merge
  * unscales them.
  *
- * 65536 rows of 16 units of 64 keys of 64 channels: 172 us, 600 TFLOP/s of bf16
+ * 65536 rows of 16 units of 64 keys of 64 channels: 167 us, 617 TFLOP/s of bf16
  * products. The matrix cores are busy 28 % of it, vector instructions (splits
  * of queries and probabilities, exponentials, the exchange before the stores)
- * 44 %, and half of the waves' time goes to waits: loads of queries and lists at the
+ * 45 %, and half of the waves' time goes to waits: loads of queries and lists at the
  * start of a turn, one product's sum into the next. No stores: 168 of 184 us
  * then; no look at the lists: 165; one query for all: 176. */
 #define BLK_RING 128   /* rows of a wave's list at most */
@@ -1483,8 +1483,8 @@ __device__ __forceinline__ void blk_add(const float4 &p, float w, float (&o)[4])
  * lanes a unit add the outputs, 256 / DP units at a time. A negative sum: the
  * outputs are scaled, and the weight goes round with a minus;
  * the outputs are unscaled, not the weight, whose last bits would be lost from
- * 2^-78 on, with values large enough to count. Bound by memory: 65536 rows of 16 units
- * of 64 channels, 285 MB, 43 us, 6.6 TB/s. */
+ * 2^-78 on, with values large enough to count. Bound by memory: 65536 rows of
+ * 16 units of 64 channels, 285 MB, 46 us, 6.2 TB/s. */
 template <int DP> __global__ void __launch_bounds__(256) blk_merge_kernel(const blk_args a)
 {
     constexpr int LV = DP / 4, GV = 64 / LV;
