@@ -286,7 +286,8 @@ void ops_block_select(struct ops *o, struct opnd Q, int Nq, int nh, int nhk,
  * listed blocks (SEL as above; entries that are no block are skipped, a block
  * listed twice counts once). No key left: zeros. A NaN among the kept scores
  * makes the row NaN; what left-out keys and values hold does not matter; a
- * key's weight under 2^-126 of the row's largest may count as zero. O
+ * key's weight under 2^-126 of the row's largest may count as zero, and sums of
+ * values from 2^115 on may pass float32's range before they are divided. O
  * may be Q (same offset and ld), any other overlap of O is an error. */
 size_t ops_attention_blocks_work_bytes(int Nq, int Nk, int nh, int nhk, int d,
                                        int bs, int top);

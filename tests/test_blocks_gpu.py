@@ -635,3 +635,22 @@ def test_passes_of_a_long_batch(place, dev, ic):
     c.attend(O)
     some = np.r_[0:3, 7948:7953, 15898:15901, np.random.default_rng(1).integers(0, nq, 40)]
     check(c, q[some], k, v, None, sel[some], c.out(O)[some])
+
+
+@pytest.mark.parametrize("nq", [2, 130])
+@pytest.mark.parametrize("d", [24, 64, 100])
+def test_longest_lists(nq, d, dev, ic):
+    """64 blocks of 128 keys a row, 128 units to merge: one by one and by lists."""
+    print(f"[blocks] longest lists {nq} {d}", flush=True)
+    nk, h, kv, bs, top = 9000, 2, 1, 128, 64
+    assert ic.lib().icoreg_blocks_choice(nq, nk, h, kv, d, bs, top) == (nq > 2)
+    q, k, v, mask = draw(nq, nk, h, kv, d, 1)
+    c = Case(dev, ic, q, k, v, bs, top, float(np.float32(1.2 / d ** 0.5)), mask)
+    c.index()
+    c.select()
+    sel = c.sel()
+    kc, ks = c.codes()
+    assert np.array_equal(sel, ref.select(q, kc, ks, top)) and (sel >= 0).all()
+    c.attend()
+    some = np.unique(np.r_[0, 1, nq - 1, np.random.default_rng(d).integers(0, nq, 12)])
+    check(c, q[some], k, v, mask, sel[some], c.out()[some])
