@@ -38,7 +38,7 @@ import torch
 ROOT = Path(__file__).resolve().parent.parent
 own = False
 
-EPS = 1e-6
+EPS = float(np.float32(1e-6))
 # The smallest row maximum that keeps its codes; rows below it count as zero.
 TINY = 2.0 ** -100
 # Queries of a piece of the plain form's window.
