@@ -74,6 +74,17 @@ class Opnd(C.Structure):
     ]
 
 
+class Cache(C.Structure):
+    """struct ops_cache."""
+    _fields_ = [("kc", Mem), ("vc", Mem), ("ks", Mem), ("vs", Mem), ("pages", C.c_int32), ("page", C.c_int32),
+                ("nhk", C.c_int32), ("d", C.c_int32)]
+
+
+class Seqs(C.Structure):
+    """struct ops_seqs."""
+    _fields_ = [("start", Mem), ("len", Mem), ("table", Mem), ("n", C.c_int32), ("ldt", C.c_int32)]
+
+
 class ConvGeom(C.Structure):
     _fields_ = [(n, C.c_int) for n in ("kh", "kw", "sy", "sx", "py", "px", "dy", "dx", "groups")]
 
@@ -81,6 +92,8 @@ class ConvGeom(C.Structure):
 _I, _L, _F, _P, _S = C.c_int, C.c_long, C.c_float, C.c_void_p, C.c_char_p
 _B = C.POINTER(OclBackend)
 _O = C.POINTER(Ops)
+_CA = C.POINTER(Cache)
+_SE = C.POINTER(Seqs)
 
 # name -> (restype, argtypes)
 SIGNATURES = {
@@ -156,6 +169,15 @@ SIGNATURES = {
     "ops_attention_blocks_work_bytes": (C.c_size_t, [_I, _I, _I, _I, _I, _I, _I]),
     "ops_attention_blocks": (None, [_O, Opnd, Opnd, Opnd, Opnd, _I, _I, _I, _I, _I, _I, _I, Mem, _F,
                                     Mem, Mem]),
+    "ops_rms_norm": (None, [_O, _L, _I, Opnd, Opnd, Mem, _F, Opnd, Opnd, Mem, Mem]),
+    "ops_cache_pitch": (_I, [_I]),
+    "ops_cache_write": (None, [_O, _CA, _SE, _I, Opnd, Opnd]),
+    "ops_cache_read": (None, [_O, _CA, _SE, _I, Opnd, Opnd]),
+    "ops_attention_window_work_bytes": (C.c_size_t, [_I, _I, _I]),
+    "ops_attention_window": (None, [_O, Opnd, Opnd, Opnd, Opnd, _I, _I, _I, _I, _I, _I, _I, _I, _I, _F,
+                                    Mem, Mem]),
+    "ops_attention_cache_work_bytes": (C.c_size_t, [_I, _I, _I]),
+    "ops_attention_cache": (None, [_O, _CA, _SE, _I, Opnd, Opnd, _I, _I, _I, _F, Mem]),
     "ops_resize": (None, [_O, Mem, _I, _I, _I, Mem, _I, _I, _I, _I, _F]),
     "ops_grid_sample": (None, [_O, Mem, _I, _I, _I, Mem, _I, _I, Mem]),
     "ops_unfold": (None, [_O, Mem, _I, _I, _I, C.POINTER(ConvGeom), Mem]),
@@ -234,6 +256,8 @@ SIGNATURES = {
     # binding glue (include/icoreg_glue.h)
     "icoreg_sizeof_backend": (C.c_size_t, []),
     "icoreg_sizeof_ops": (C.c_size_t, []),
+    "icoreg_sizeof_cache": (C.c_size_t, []),
+    "icoreg_sizeof_seqs": (C.c_size_t, []),
     "icoreg_pth_new": (_P, []),
     "icoreg_eloftr_new": (_P, []),
     "icoreg_struct_delete": (None, [_P]),
@@ -269,11 +293,12 @@ SIGNATURES = {
 _NO_CHECK = {"ocl_graph_free", "icoreg_set_fatal_mode", "icoreg_last_error", "icoreg_clear_error",
              "ocl_errstr", "ops_mat", "ops_bmat", "ops_geom", "ops_conv_out",
              "ops_q8_pitch", "ops_linear_q8_work_bytes", "ops_key_blocks",
-             "ops_block_select_work_bytes", "ops_attention_blocks_work_bytes",
+             "ops_block_select_work_bytes", "ops_attention_blocks_work_bytes", "ops_cache_pitch",
+             "ops_attention_window_work_bytes", "ops_attention_cache_work_bytes",
              "ocl_wrap", "icoreg_prof_entry", "icoreg_prof_reset", "icoreg_prof_flush", "ops_report",
              "pth_find", "pth_numel", "pth_bytes", "pth_strip_prefix",
              "icoreg_pth_new", "icoreg_eloftr_new", "icoreg_struct_delete",
-             "icoreg_sizeof_backend", "icoreg_sizeof_ops",
+             "icoreg_sizeof_backend", "icoreg_sizeof_ops", "icoreg_sizeof_cache", "icoreg_sizeof_seqs",
              "icoreg_eloftr_result", "icoreg_eloftr_coarse_stats",
              "icoreg_eloftr_set_pos_scale", "icoreg_eloftr_buffer", "roma_gp_work_bytes",
              "icoreg_roma_new", "icoreg_roma_result", "icoreg_roma_buffer",

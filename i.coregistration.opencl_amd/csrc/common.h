@@ -79,6 +79,14 @@ inline hipStream_t stream_of(struct ocl_backend *ocl)
     return (hipStream_t)ocl->stream;
 }
 
+/* The backend's device for the launches of a scope, where the caller's
+ * current one is another; the caller's again behind it. */
+struct device_scope {
+    explicit device_scope(const struct ocl_backend *ocl);
+    ~device_scope();
+    int before; /* -1: nothing to put back */
+};
+
 /* Channels per thread of the bilinear sampling kernels (warp sampling,
  * grid_sample): 8, or 4 when that leaves fewer idle slots in the last
  * group of C channels. */

@@ -111,6 +111,23 @@ unsigned grid_of(long long blocks, int threads, const char *what)
     return (unsigned)count32(blocks, what);
 }
 
+device_scope::device_scope(const struct ocl_backend *ocl) : before(-1)
+{
+    int now = 0;
+
+    hip_check(hipGetDevice(&now), "hipGetDevice");
+    if (now != ocl->device) {
+        hip_check(hipSetDevice(ocl->device), "hipSetDevice");
+        before = now;
+    }
+}
+
+device_scope::~device_scope()
+{
+    if (before >= 0)
+        (void)hipSetDevice(before);
+}
+
 void launch_check(const char *what)
 {
     hipError_t e = hipGetLastError();

@@ -18,10 +18,12 @@
 extern "C" {
 #endif
 
-/* sizeof(struct ocl_backend) and sizeof(struct ops), so that a binding
- * that mirrors their layouts can check them. */
+/* sizeof(struct ocl_backend), (struct ops), (struct ops_cache) and (struct
+ * ops_seqs), so that a binding that mirrors their layouts can check them. */
 size_t icoreg_sizeof_backend(void);
 size_t icoreg_sizeof_ops(void);
+size_t icoreg_sizeof_cache(void);
+size_t icoreg_sizeof_seqs(void);
 
 /* Zeroed structs on the heap, freed with free() after *_free / pth_close. */
 struct pth_file *icoreg_pth_new(void);

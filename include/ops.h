@@ -183,8 +183,10 @@ void ops_rope(struct ops *o, cl_mem X, long off, int ld, long rows, int nh,
 /* ---- Long token sequences and large tiles --------------------------------
  * Extensions with no counterpart in the reference, for transformer layers on
  * more tokens than the networks here were trained on: products in 8-bit
- * integers, rotary positions computed from the tokens' coordinates, and
- * attention over the blocks of keys that a cheap score selects. They
+ * integers, rotary positions computed from the tokens' coordinates,
+ * attention over the blocks of keys that a cheap score selects, norms that
+ * leave 8-bit codes, keys and values kept in 8 bits, and attention within a
+ * window. They
  * allocate nothing and leave the ops work buffer alone: what they need for
  * themselves is the caller's `work` buffer, of the size that the call's
  * _work_bytes function gives (0 where the sizes are invalid), 16-byte
@@ -295,6 +297,82 @@ void ops_attention_blocks(struct ops *o, struct opnd Q, struct opnd K,
                           struct opnd V, struct opnd O, int Nq, int Nk, int nh,
                           int nhk, int d, int bs, int top, cl_mem SEL,
                           float scale, cl_mem kmask, cl_mem work);
+
+/* H = X + R and Y = H g / sqrt(mean(H^2) + eps), token-major, rows at the
+ * operands' offsets and ld: the mean of a row's squares in 64 bits, the
+ * root's reciprocal i rounded to float32, Y = (H i) g with both products
+ * rounded, so that the codes are the same from every kernel. R.buf NULL: H is
+ * X; g (C floats) NULL: ones; eps > 0. Outputs, any of them NULL but not all:
+ * H, Y, and Y's 8-bit codes Q with their scales S as ops_quant_rows makes them
+ * (both or none), which ops_linear_qq takes. H and Y may each be X or R (same
+ * offset and ld), any other overlap of an output is an error. */
+void ops_rms_norm(struct ops *o, long rows, int C, struct opnd X,
+                  struct opnd R, cl_mem g, float eps, struct opnd H,
+                  struct opnd Y, cl_mem Q, cl_mem S);
+
+/* Keys and values kept in 8 bits, in pages of `page` = 16, 32, 64 or 128
+ * tokens: page p, key head h, place t at row (p nhk + h) page + t of the codes
+ * kc and vc (ops_cache_pitch(d) bytes a row: d rounded up to 16, zeros behind
+ * the d <= 128 codes; 16-byte aligned) and of the scales ks and vs (floats).
+ * Codes and scale of a token and head are those of ops_quant_rows. */
+struct ops_cache {
+    cl_mem kc, vc, ks, vs;
+    cl_int pages, page, nhk, d;
+};
+
+/* The sequences of a call, all in device memory and not looked at by the
+ * host. Rows start[b] .. start[b + 1] - 1 (int32, n + 1 of them, not falling)
+ * of the token-major operands are the last ones of sequence b, of which len[b]
+ * (int32) tokens are kept once the call's are: row start[b] + i is its
+ * position len[b] - (start[b + 1] - start[b]) + i. Position i is place i % page
+ * of page table[b ldt + i / page] (int32). A position that is negative or
+ * behind the table, or whose entry is no page (-1: given back), is not kept.
+ * Rows behind start[n] belong to no sequence. */
+struct ops_seqs {
+    cl_mem start, len, table;
+    cl_int n, ldt;
+};
+
+/* ops_cache_write: the rows' keys K and values V (nhk heads of d, head h at
+ * columns h d) to their places; rows without one are left out, places that no
+ * row has stay as they are. Two rows of a call must not have one place: which
+ * of them it keeps, and whether codes and scale are of the same, is not said.
+ * ops_cache_read: code times scale of the rows' positions to K and V (either
+ * may have no buffer), zeros where nothing is kept; rows of no sequence stay
+ * as they are. rows: those of the operands; start is held to 0 .. rows. */
+int ops_cache_pitch(int d);
+void ops_cache_write(struct ops *o, const struct ops_cache *c,
+                     const struct ops_seqs *s, int rows, struct opnd K,
+                     struct opnd V);
+void ops_cache_read(struct ops *o, const struct ops_cache *c,
+                    const struct ops_seqs *s, int rows, struct opnd K,
+                    struct opnd V);
+
+/* O = softmax(scale Q K^T) V within a window: query i, at position q0 + i,
+ * sees the keys j <= q0 + i + right of those with j >= q0 + i - left or j <
+ * sinks (left, right < 0: no limit; right = 0: no later key; sinks >= 0: the
+ * first keys stay visible), and of those the kept ones (kmask: Nk bytes, 0 =
+ * leave the key out, or NULL). nh query heads on nhk key heads of d <= 128 as
+ * for ops_attention_blocks. No key left: zeros. A NaN among the seen scores
+ * makes the row NaN; what unseen keys and values hold does not matter; a key's
+ * weight under 2^-126 of the row's largest may count as zero, and sums of
+ * values from 2^115 on may pass float32's range before they are divided. O may
+ * be Q (same offset and ld), any other overlap of O is an error. */
+size_t ops_attention_window_work_bytes(int Nq, int nh, int d);
+void ops_attention_window(struct ops *o, struct opnd Q, struct opnd K,
+                          struct opnd V, struct opnd O, int Nq, int Nk, int nh,
+                          int nhk, int d, int q0, int left, int right,
+                          int sinks, float scale, cl_mem kmask, cl_mem work);
+
+/* The same over a cache, right = 0: each row's query (nh heads of the
+ * cache's d, nh a multiple of its nhk) over the kept positions of its own
+ * sequence. Rows of no sequence stay as they are in O. A row's own key is
+ * seen like any other, so the call follows the rows' ops_cache_write. */
+size_t ops_attention_cache_work_bytes(int rows, int nh, int d);
+void ops_attention_cache(struct ops *o, const struct ops_cache *c,
+                         const struct ops_seqs *s, int rows, struct opnd Q,
+                         struct opnd O, int nh, int left, int sinks,
+                         float scale, cl_mem work);
 
 /* Bilinear resampling of in (C, h, w) into channels coff.. of out
  * (*, H, W). align_corners 0: scale > 0 gives source step 1 / scale,
