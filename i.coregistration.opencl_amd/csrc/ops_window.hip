@@ -18,6 +18,7 @@
 #include <algorithm>
 
 #include "common.h"
+#include "gemm_dev.h"
 #include "load4.h"
 #include "ops.h"
 #include "reduce.h"
@@ -204,6 +205,22 @@ static __device__ __forceinline__ void win_row_f32(const win_args &a, const win_
         m = 0.0f; /* NaN, whatever the other parts are */
 }
 
+/* What win_row_f32 leaves, to its place: the output, or a part of it. */
+static __device__ __forceinline__ void win_put(const win_args &a, long long row, int h, int split, int parts,
+                                               const float (&o)[2], float m, float l)
+{
+    const int lane = threadIdx.x & 63, dp = a.d <= 32 ? 32 : a.d <= 64 ? 64 : 128;
+    const long long u = (row * a.nh + h) * a.splits + split;
+    float *to = parts == 1 ? a.O + row * a.ldo + (long long)h * a.d : a.part + u * dp;
+
+#pragma unroll
+    for (int e = 0; e < 2; e++)
+        if (lane + 64 * e < a.d)
+            to[lane + 64 * e] = parts > 1 ? o[e] : l == 0.0f ? 0.0f : o[e] / l;
+    if (lane == 0 && a.splits > 1)
+        a.ml[u] = parts == 1 ? make_float2(0.0f, WIN_WRITTEN) : make_float2(m, l);
+}
+
 /* Parts that t tiles of keys are split into, of at most `splits`: at least 4
  * tiles each. */
 static __device__ __forceinline__ int win_parts(int tiles, int splits)
@@ -242,25 +259,493 @@ template <bool CACHE> __global__ void __launch_bounds__(256) win_row_kernel(cons
 
     win_row_f32<CACHE>(a, r, row, h, t, (int)((long long)t.n * split / parts),
                        (int)((long long)t.n * (split + 1) / parts), ps[wave], o, m, l);
-    if (parts == 1) {
-        float *out = a.O + row * a.ldo + (long long)h * a.d;
+    win_put(a, row, h, split, parts, o, m, l);
+}
 
-#pragma unroll
-        for (int e = 0; e < 2; e++)
-            if (lane + 64 * e < a.d)
-                out[lane + 64 * e] = l == 0.0f ? 0.0f : o[e] / l;
-        if (a.splits > 1 && lane == 0)
-            a.ml[u] = make_float2(0.0f, WIN_WRITTEN);
+/* ---- a tile of rows over a cache ------------------------------------------------ */
+
+typedef _Float16 win_h2 __attribute__((ext_vector_type(2)));
+typedef _Float16 win_h8 __attribute__((ext_vector_type(8)));
+typedef float win_f2 __attribute__((ext_vector_type(2)));
+typedef float win_f16x __attribute__((ext_vector_type(16)));
+typedef unsigned win_u4 __attribute__((ext_vector_type(4)));
+
+#define WIN_ROWS 128    /* rows (queries times the heads of a key head) of a tile */
+#define WIN_KT 64       /* keys of a tile */
+#define WIN_TAU 4.0f    /* the running maximum is raised when a score passes it by this (base 2) */
+#define WIN_VEXP 10     /* exponent of a tile's largest value scale: weights up to 2^TAU stay below 2^16 */
+#define WIN_VMIN 0.25f  /* smaller ones than this lose bits */
+
+/* Codes of 8 bits in f16, exactly: a byte u = code + 128 behind 0x64 is the
+ * f16 value 1024 + u. */
+static __device__ __forceinline__ unsigned win_codes(unsigned bytes)
+{
+    const win_h2 x = __builtin_bit_cast(win_h2, bytes), off = {(_Float16)-1152.0f, (_Float16)-1152.0f};
+
+    return __builtin_bit_cast(unsigned, x + off);
+}
+
+/* Two floats as the sum of two f16 values each, 11 bits and 11 more. */
+static __device__ __forceinline__ void win_split(float a, float b, unsigned &hi, unsigned &lo)
+{
+    const win_f2 v = {a, b};
+    const win_h2 h = __builtin_convertvector(v, win_h2);
+    const win_f2 r = {__builtin_fmaf((float)h[0], -1.0f, a), __builtin_fmaf((float)h[1], -1.0f, b)};
+
+    hi = __builtin_bit_cast(unsigned, h);
+    lo = __builtin_bit_cast(unsigned, __builtin_convertvector(r, win_h2));
+}
+
+/* What a block of threads computes: rows r0 .. r0 + n - 1 (query-major, the g
+ * heads of key head kvh within) of a sequence of nk keys whose first row of
+ * the operands is `first`, at position p0. n = 0: none. */
+struct win_job {
+    int b, kvh, r0, n, first, p0, nk;
+};
+
+template <bool CACHE>
+static __device__ __forceinline__ win_job win_job_of(const win_args &a, int tile, int kvh)
+{
+    const int g = a.nh / a.nhk;
+    win_job j = {0, kvh, 0, 0, 0, 0, 0};
+
+    if (!CACHE) {
+        j.r0 = tile * WIN_ROWS;
+        j.n = (int)min((long long)a.rows * g - j.r0, (long long)WIN_ROWS);
+        j.p0 = a.q0;
+        j.nk = a.Nk;
+        return j;
+    }
+    /* Sequence b has the tiles from start[b] g / WIN_ROWS + b on, one more than
+     * it can need; the last that starts at or before this one, 64 sequences
+     * at a time. */
+    auto from = [&](int b) { return (long long)seq_start(a.c, b) * g / WIN_ROWS + b; };
+    const int lane = threadIdx.x & 63;
+    int count = 0;
+
+    for (int b0 = 0; b0 < a.c.n; b0 += 64) {
+        const int n = __popcll(__ballot(b0 + lane < a.c.n && from(min(b0 + lane, a.c.n - 1)) <= tile));
+
+        count += n;
+        if (n < 64)
+            break;
+    }
+    j.b = max(count - 1, 0);
+    j.first = seq_start(a.c, j.b);
+    const int rows = max(seq_start(a.c, j.b + 1) - j.first, 0);
+
+    j.r0 = (int)max(tile - from(j.b), 0LL) * WIN_ROWS;
+    j.n = (int)min((long long)rows * g - j.r0, (long long)WIN_ROWS);
+    j.p0 = max(a.c.len[j.b], 0) - rows;
+    j.nk = seq_len(a.c, j.b);
+    return j;
+}
+
+/* A tile's place among a key head's: from both ends in turn, so that a stretch
+ * of them has short rows and long ones alike where later rows see more. */
+static __device__ __forceinline__ int win_order(int i, int n) { return i & 1 ? i >> 1 : n - 1 - (i >> 1); }
+
+template <int ND>
+__global__ void __launch_bounds__(256, ND == 4 ? 2 : 3) win_cache_kernel(const win_args a)
+{
+    constexpr int DP = 32 * ND, CH = DP / 8;
+    constexpr int RW = 16 / CH < 1 ? 1 : 16 / CH;  /* K rows in 256 bytes */
+    constexpr int KU = 4 * DP, NK = (KU + 255) / 256; /* 16-byte units of codes of a tile of K */
+    constexpr int VU = 2 * DP, NV = (VU + 255) / 256; /* units of 8 keys x 4 channels of V */
+    constexpr int KSZ = WIN_KT * CH, VSZ = DP * 8;    /* 16-byte chunks in LDS */
+    struct tile_lds {
+        win_u4 k[KSZ], v[VSZ];
+        float ks[WIN_KT], vs[WIN_KT];
+        unsigned long long keep;
+        float vf;
+        int wild;
+    };
+    __shared__ tile_lds lds[2];
+    __shared__ float ps[4][64];
+    const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, col = lane & 31;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int g = a.nh / a.nhk, d = a.d, pitch = a.c.pitch;
+    const int tiles = (int)((long long)a.rows * g / WIN_ROWS) + a.c.n;
+    const int unit = xcd_tile(blockIdx.x, gridDim.x), split = unit % a.splits;
+    const win_job jb = win_job_of<true>(a, win_order(unit / a.splits % tiles, tiles), unit / a.splits / tiles);
+
+    if (jb.n <= 0)
+        return;
+    const int last = jb.r0 + jb.n - 1;
+    const win_tiles span = win_span<WIN_KT>(a, jb.p0 + jb.r0 / g, jb.p0 + last / g, jb.nk);
+    const int parts = win_parts(span.n, a.splits);
+    /* This lane's row; lanes without one take the last. */
+    const int wr = jb.r0 + 32 * wave, r = min(wr + col, last), qi = r / g, h = jb.kvh * g + r - qi * g;
+    const bool mine = wr + col <= last;
+    const long long row = jb.first + qi, out = (row * a.nh + h) * a.splits + split;
+
+    if (split >= parts) {
+        if (mine && half == 0)
+            a.ml[out] = make_float2(-INFINITY, 0.0f);
         return;
     }
-    const int dp = a.d <= 32 ? 32 : a.d <= 64 ? 64 : 128;
+    const int t0 = (int)((long long)span.n * split / parts), t1 = (int)((long long)span.n * (split + 1) / parts);
+    const int p = jb.p0 + qi, hi = win_hi(a, p, jb.nk), lo = win_lo(a, p);
+    /* Those of the wave's first and last row, and whether it has any. */
+    const bool live = wr <= last;
+    const int pa = jb.p0 + min(wr, last) / g, pb = jb.p0 + min(wr + 31, last) / g;
+    const int hi0 = win_hi(a, pa, jb.nk), hi1 = win_hi(a, pb, jb.nk), lo0 = win_lo(a, pa), lo1 = win_lo(a, pb);
+    win_u4 qh[2 * ND], ql[2 * ND];
+    win_f16x o[ND];
+    float m = -INFINITY, l = 0.0f, qf;
+    bool wild = false;
+
+    /* The query times scale and log2 e, times a power of two that brings its
+     * largest magnitude to 2^14 .. 2^15; qf takes it back. */
+    {
+        const float *q = a.Q + row * a.ldq + (long long)h * d;
+        float x[2 * ND][8];
+        unsigned mag = 0;
 
 #pragma unroll
-    for (int e = 0; e < 2; e++)
-        if (lane + 64 * e < a.d)
-            a.part[u * dp + lane + 64 * e] = o[e];
-    if (lane == 0)
-        a.ml[u] = make_float2(m, l);
+        for (int st = 0; st < 2 * ND; st++) {
+            float u[4], v[4];
+
+            load4_row(q, st * 16 + half * 8, d, u);
+            load4_row(q, st * 16 + half * 8 + 4, d, v);
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                x[st][j] = (j < 4 ? u[j & 3] : v[j & 3]) * (a.scale * WIN_LOG2E);
+                mag = max(mag, q8_mag(x[st][j]));
+            }
+        }
+        mag = max(mag, (unsigned)__shfl_xor((int)mag, 32, 64));
+        const int e = min(max((int)(mag >> 23), 15), 254);
+        const float up = __builtin_bit_cast(float, (unsigned)(268 - e) << 23);
+
+        qf = __builtin_bit_cast(float, (unsigned)(e - 14) << 23);
+#pragma unroll
+        for (int st = 0; st < 2 * ND; st++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                unsigned u, v;
+
+                win_split(x[st][2 * j] * up, x[st][2 * j + 1] * up, u, v);
+                qh[st][j] = u;
+                ql[st][j] = v;
+            }
+    }
+#pragma unroll
+    for (int tt = 0; tt < ND; tt++)
+#pragma unroll
+        for (int e = 0; e < 16; e++)
+            o[tt][e] = 0.0f;
+
+    /* Units of this thread: K unit e is key e / (DP / 16), bytes 16 (e % (DP /
+     * 16)) ..; V unit e channels 4 (e % (DP / 4)) .., slots 8 c .. 8 c + 7, c = e / (DP
+     * / 4), slot 8 c + j being the key that register 8 (c / 2 % 2) + j of the
+     * scores' tile c / 4 holds in lane half c % 2: 16 c / 2 + 8 (j / 4) + 4 (c %
+     * 2) + j % 4. Pages hold at least 16 keys, so a unit lies in one. */
+    int kp[NK], vp[NV], sp;
+    bool kept = false;
+    uint4 kr[NK];
+    unsigned vr[NV][8];
+    float sr;
+
+    auto pages = [&](int t) {
+        const int k0 = span.tile(t) * WIN_KT;
+
+#pragma unroll
+        for (int i = 0; i < NK; i++) {
+            const int key = k0 + (tid + 256 * i) / (DP / 16);
+
+            kp[i] = key < jb.nk && tid + 256 * i < KU ? seq_page(a.c, jb.b, key) : -1;
+        }
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            const int key = k0 + (tid + 256 * i) / (DP / 4) / 2 * 16;
+
+            vp[i] = key < jb.nk && tid + 256 * i < VU ? seq_page(a.c, jb.b, key) : -1;
+        }
+        sp = -1;
+        if (wave < 2 && k0 + lane < jb.nk)
+            sp = seq_page(a.c, jb.b, k0 + lane);
+    };
+    /* Tile t into registers, its pages looked up before. Places of a page
+     * behind the last key hold old codes, which are bytes like others. */
+    auto fetch = [&](int t) {
+        const int k0 = span.tile(t) * WIN_KT;
+
+#pragma unroll
+        for (int i = 0; i < NK; i++) {
+            const int e = tid + 256 * i, key = k0 + e / (DP / 16), at = e % (DP / 16) * 16;
+
+            kr[i] = make_uint4(0, 0, 0, 0);
+            if (kp[i] >= 0 && at < pitch)
+                kr[i] = *(const uint4 *)(a.c.kc + cache_row(a.c, kp[i], jb.kvh, key) * pitch + at);
+        }
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            const int e = tid + 256 * i, c = e / (DP / 4), at = e % (DP / 4) * 4;
+            const signed char *v = a.c.vc + cache_row(a.c, max(vp[i], 0), jb.kvh, k0 + (c >> 1) * 16 + (c & 1) * 4) * pitch + at;
+
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                vr[i][j] = vp[i] >= 0 && at < pitch ? *(const unsigned *)(v + ((j >> 2) * 8 + (j & 3)) * pitch) : 0u;
+        }
+        sr = 0.0f;
+        kept = sp >= 0;
+        if (kept)
+            sr = (wave ? a.c.vs : a.c.ks)[cache_row(a.c, sp, jb.kvh, k0 + lane)];
+    };
+    auto stash = [&](tile_lds &s) {
+#pragma unroll
+        for (int i = 0; i < NK; i++) {
+            const int e = tid + 256 * i, key = e / (DP / 16), ch = e % (DP / 16) * 2;
+
+            if (KU % 256 == 0 || e < KU) {
+                const unsigned w[4] = {kr[i].x ^ 0x80808080u, kr[i].y ^ 0x80808080u, kr[i].z ^ 0x80808080u,
+                                       kr[i].w ^ 0x80808080u};
+                unsigned x[8];
+
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    x[2 * j] = win_codes(__builtin_amdgcn_perm(0x64646464u, w[j], 0x04010400u));
+                    x[2 * j + 1] = win_codes(__builtin_amdgcn_perm(0x64646464u, w[j], 0x04030402u));
+                }
+                const win_u4 u = {x[0], x[1], x[2], x[3]}, v = {x[4], x[5], x[6], x[7]};
+
+                s.k[key * CH + (ch ^ (key / RW % CH))] = u;
+                s.k[key * CH + ((ch + 1) ^ (key / RW % CH))] = v;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            const int e = tid + 256 * i, c = e / (DP / 4), ch = e % (DP / 4) * 4;
+
+            if (VU % 256 == 0 || e < VU) {
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const unsigned sel = 0x0c000c00u | (4u + k) << 16 | (unsigned)k;
+                    win_u4 x;
+
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        x[j] = win_codes(__builtin_amdgcn_perm(vr[i][2 * j + 1] ^ 0x80808080u,
+                                                               vr[i][2 * j] ^ 0x80808080u, sel) |
+                                         0x64006400u);
+                    s.v[(ch + k) * 8 + (c ^ ((ch + k) >> 1 & 7))] = x;
+                }
+            }
+        }
+        if (wave == 0) {
+            const unsigned long long keep = __ballot(kept);
+
+            s.ks[lane] = sr;
+            if (lane == 0)
+                s.keep = keep;
+        }
+        else if (wave == 1) {
+            /* Value scales times a power of two that brings the largest to
+             * 2^WIN_VEXP; a scale of NaN, and one far below the largest, is for
+             * the float32 path. */
+            const bool bad = sr != sr;
+            const unsigned top = wave_umax(bad ? 0u : q8_mag(sr)) >> 23;
+            const int e = min((int)top, 253 + WIN_VEXP);
+            const float up = __builtin_bit_cast(float, (unsigned)min(254 + WIN_VEXP - e, 253) << 23);
+            const float x = bad ? 0.0f : sr * up;
+
+            s.vs[lane] = x;
+            const int w = __any(bad || (x != 0.0f && x < WIN_VMIN) || !(x < 0x1p12f));
+
+            if (lane == 0) {
+                s.vf = 1.0f / up;
+                s.wild = w;
+            }
+        }
+    };
+
+    pages(t0);
+    fetch(t0);
+    if (t0 + 1 < t1)
+        pages(t0 + 1);
+    stash(lds[0]);
+    if (t0 + 1 < t1) {
+        fetch(t0 + 1);
+        if (t0 + 2 < t1)
+            pages(t0 + 2);
+    }
+    __syncthreads();
+    for (int t = t0; t < t1; t++) {
+        const tile_lds &s = lds[(t - t0) & 1];
+        const int k0 = span.tile(t) * WIN_KT;
+        /* Some row of the wave sees some key; all see all. */
+        const bool some = live && k0 <= hi1 && (k0 + WIN_KT > lo0 || k0 < a.sinks);
+        const bool all = s.keep == ~0ull && k0 + WIN_KT - 1 <= hi0 && (k0 >= lo1 || k0 + WIN_KT <= a.sinks);
+        win_u4 ph[4], pl[4];
+
+        wild = wild || s.wild;
+        if (some) {
+            win_f16x sc[2];
+            float x[2][16], mx = -INFINITY, sum = 0.0f;
+
+#pragma unroll
+            for (int e = 0; e < 16; e++)
+                sc[0][e] = sc[1][e] = 0.0f;
+#pragma unroll
+            for (int st = 0; st < 2 * ND; st++)
+#pragma unroll
+                for (int tt = 0; tt < 2; tt++) {
+                    const int key = 32 * tt + col;
+                    const win_h8 k = __builtin_bit_cast(win_h8, s.k[key * CH + ((2 * st + half) ^ (key / RW % CH))]);
+
+                    sc[tt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, __builtin_bit_cast(win_h8, ql[st]), sc[tt], 0, 0, 0);
+                    sc[tt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, __builtin_bit_cast(win_h8, qh[st]), sc[tt], 0, 0, 0);
+                }
+            /* Register e of tile tt is key 32 tt + 8 (e / 4) + 4 half + e % 4. */
+#pragma unroll
+            for (int tt = 0; tt < 2; tt++)
+#pragma unroll
+                for (int e = 0; e < 16; e += 4) {
+                    const float4 k = *(const float4 *)&s.ks[32 * tt + 2 * e + 4 * half];
+
+                    x[tt][e] = sc[tt][e] * k.x;
+                    x[tt][e + 1] = sc[tt][e + 1] * k.y;
+                    x[tt][e + 2] = sc[tt][e + 2] * k.z;
+                    x[tt][e + 3] = sc[tt][e + 3] * k.w;
+                }
+            if (!all) {
+#pragma unroll
+                for (int tt = 0; tt < 2; tt++) {
+                    const unsigned keep = (unsigned)(s.keep >> (32 * tt + 4 * half));
+
+#pragma unroll
+                    for (int e = 0; e < 16; e++) {
+                        const int off = 8 * (e >> 2) + (e & 3), k = k0 + 32 * tt + 4 * half + off;
+
+                        x[tt][e] = (keep >> off & 1) && k <= hi && (k >= lo || k < a.sinks) ? x[tt][e] : -INFINITY;
+                    }
+                }
+            }
+#pragma unroll
+            for (int tt = 0; tt < 2; tt++)
+#pragma unroll
+                for (int e = 0; e < 16; e++)
+                    mx = fmaxf(mx, x[tt][e]);
+            mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * qf;
+            const bool need = mx > m + WIN_TAU;
+
+            if (__any(need)) {
+                const float mn = need ? mx : m;
+                const float corr = need ? __builtin_amdgcn_exp2f(m - mn) : 1.0f;
+
+                m = mn;
+                l *= corr;
+#pragma unroll
+                for (int tt = 0; tt < ND; tt++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++)
+                        o[tt][e] *= corr;
+            }
+            const float ref = m == -INFINITY ? 0.0f : m;
+
+#pragma unroll
+            for (int tt = 0; tt < 2; tt++)
+#pragma unroll
+                for (int e = 0; e < 16; e += 4) {
+                    const float4 v = *(const float4 *)&s.vs[32 * tt + 2 * e + 4 * half];
+                    unsigned u0, u1, v0, v1;
+
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        x[tt][e + j] = __builtin_amdgcn_exp2f(fmaf(x[tt][e + j], qf, -ref));
+                        sum += x[tt][e + j];
+                    }
+                    win_split(x[tt][e] * v.x, x[tt][e + 1] * v.y, u0, v0);
+                    win_split(x[tt][e + 2] * v.z, x[tt][e + 3] * v.w, u1, v1);
+                    ph[2 * tt + e / 8][e / 2 % 4] = u0;
+                    ph[2 * tt + e / 8][e / 2 % 4 + 1] = u1;
+                    pl[2 * tt + e / 8][e / 2 % 4] = v0;
+                    pl[2 * tt + e / 8][e / 2 % 4 + 1] = v1;
+                }
+            l += sum + __shfl_xor(sum, 32, 64);
+        }
+        /* The next tile into the other buffer, which was last read a tile ago,
+         * before the barrier; then its successor's loads. */
+        if (t + 1 < t1) {
+            stash(lds[(t + 1 - t0) & 1]);
+            if (t + 2 < t1) {
+                fetch(t + 2);
+                if (t + 3 < t1)
+                    pages(t + 3);
+            }
+        }
+        if (some) {
+            const float vf = s.vf;
+
+#pragma unroll
+            for (int tt = 0; tt < ND; tt++) {
+                const int dd = 32 * tt + col;
+                win_f16x part;
+
+#pragma unroll
+                for (int e = 0; e < 16; e++)
+                    part[e] = 0.0f;
+#pragma unroll
+                for (int u = 0; u < 4; u++) {
+                    const win_h8 v = __builtin_bit_cast(win_h8, s.v[dd * 8 + ((2 * u + half) ^ (dd >> 1 & 7))]);
+
+                    part = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, __builtin_bit_cast(win_h8, pl[u]), part, 0, 0, 0);
+                    part = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, __builtin_bit_cast(win_h8, ph[u]), part, 0, 0, 0);
+                }
+#pragma unroll
+                for (int e = 0; e < 16; e++)
+                    o[tt][e] = fmaf(part[e], vf, o[tt][e]);
+            }
+        }
+        __syncthreads();
+    }
+    float z = l * 0.0f;
+
+#pragma unroll
+    for (int tt = 0; tt < ND; tt++)
+#pragma unroll
+        for (int e = 0; e < 16; e++)
+            z = fmaf(o[tt][e], 0.0f, z);
+    const bool again = wild || z != 0.0f;
+    unsigned long long redo = __ballot(again && mine);
+
+    redo = (redo | redo >> 32) & 0xffffffffull;
+    const bool good = mine && !(redo >> col & 1);
+    const bool direct = parts == 1;
+
+    if (good) {
+        const float inv = direct ? (l > 0.0f ? 1.0f / l : 0.0f) : 1.0f;
+        float *to = direct ? a.O + row * a.ldo + (long long)h * d : a.part + out * DP;
+
+#pragma unroll
+        for (int tt = 0; tt < ND; tt++)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+                const int c = 32 * tt + 2 * e + 4 * half;
+
+                if (c + 4 <= d)
+                    store4(to + c, o[tt][e] * inv, o[tt][e + 1] * inv, o[tt][e + 2] * inv, o[tt][e + 3] * inv);
+                else {
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        if (c + j < d)
+                            to[c + j] = o[tt][e + j] * inv;
+                }
+            }
+        if (half == 0 && a.splits > 1)
+            a.ml[out] = direct ? make_float2(0.0f, WIN_WRITTEN) : make_float2(m, l);
+    }
+    /* Rows with a sum that is not finite, and all of a block that met value
+     * scales it cannot hold: again in float32. */
+    for (; redo; redo &= redo - 1) {
+        const int rr = wr + __builtin_ctzll(redo), q1 = rr / g, h1 = jb.kvh * g + rr - q1 * g;
+        const win_row wrow = {jb.b, jb.p0 + q1, jb.nk};
+        float y[2], m1, l1;
+
+        win_row_f32<true>(a, wrow, jb.first + q1, h1, span, t0, t1, ps[wave], y, m1, l1);
+        win_put(a, jb.first + q1, h1, split, parts, y, m1, l1);
+    }
 }
 
 /* Parts of a row and head joined: a wave each, lane s with split s, s + 64, ..
@@ -276,9 +761,10 @@ __global__ void __launch_bounds__(256) win_merge_kernel(const win_args a)
         return;
     const float2 *ml = a.ml + u * a.splits;
 
-    if (ml[0].y == WIN_WRITTEN)
-        return;
     const int row = (int)(u / a.nh), h = (int)(u % a.nh);
+
+    if ((a.c.n && seq_of(a.c, row) < 0) || ml[0].y == WIN_WRITTEN)
+        return;
     float m = -INFINITY, l = 0.0f, o[2] = {0, 0};
 
     for (int s = lane; s < a.splits; s += 64)
@@ -332,31 +818,44 @@ extern "C" size_t ops_attention_cache_work_bytes(int rows, int nh, int d)
     return ops_attention_window_work_bytes(rows, nh, d);
 }
 
-/* Splits of keys of a call whose rows see at most `keys` each. */
-static int win_splits(const win_args &a, long long keys, int cus)
+/* Splits of keys, `blocks` blocks of threads without any, of a call whose rows
+ * see at most `keys` each. */
+static int win_splits(const win_args &a, long long blocks, long long keys, int want)
 {
-    const long long waves = (long long)a.rows * a.nh, want = 16LL * cus;
-    long long n = std::min((want + waves - 1) / waves, keys / 256);
+    long long n = std::min((want + blocks - 1) / blocks, keys / 256);
 
-    n = std::min(n, WIN_PART_ROWS / waves);
+    n = std::min(n, WIN_PART_ROWS / ((long long)a.rows * a.nh));
     return (int)std::max(1LL, std::min(n, (long long)WIN_MAX_SPLITS));
 }
 
 template <bool CACHE> static void win_launch(struct ops *o, win_args &a, long long keys, cl_mem work)
 {
+    const int cus = o->ocl->cu_count > 0 ? o->ocl->cu_count : 256;
     const long long heads = (long long)a.rows * a.nh;
+    const long long blocks = CACHE ? (heads / a.nhk / WIN_ROWS + a.c.n) * a.nhk : (heads + 3) / 4;
 
-    a.splits = win_splits(a, keys, o->ocl->cu_count > 0 ? o->ocl->cu_count : 256);
+    a.splits = win_splits(a, blocks, keys, 4 * cus);
     if (a.splits > 1) {
         a.part = fptr(work);
         a.ml = (float2 *)(a.part + heads * a.splits * win_width(a.d));
     }
-    const dim3 grid(grid_of((heads * a.splits + 3) / 4, 256, "attention rows"));
     const device_scope on(o->ocl);
     const hipStream_t s = stream_of(o->ocl);
 
     prof_scope ps(o->ocl, CACHE ? "attention_cache" : "attention_window");
-    hipLaunchKernelGGL(win_row_kernel<CACHE>, grid, dim3(256), 0, s, a);
+    if (CACHE) {
+        const dim3 grid(grid_of(blocks * a.splits, 256, "attention tiles")), block(256);
+
+        if (a.d <= 32)
+            hipLaunchKernelGGL(win_cache_kernel<1>, grid, block, 0, s, a);
+        else if (a.d <= 64)
+            hipLaunchKernelGGL(win_cache_kernel<2>, grid, block, 0, s, a);
+        else
+            hipLaunchKernelGGL(win_cache_kernel<4>, grid, block, 0, s, a);
+    }
+    else
+        hipLaunchKernelGGL(win_row_kernel<CACHE>, dim3(grid_of((heads * a.splits + 3) / 4, 256, "attention rows")),
+                           dim3(256), 0, s, a);
     launch_check("attention rows");
     if (a.splits > 1) {
         hipLaunchKernelGGL(win_merge_kernel, dim3((unsigned)((heads + 3) / 4)), dim3(256), 0, s, a);
