@@ -23,6 +23,7 @@
 #include "ops.h"
 #include "reduce.h"
 #include "seqs.h"
+#include "split.h"
 
 using namespace icoreg;
 
@@ -45,7 +46,7 @@ struct win_args {
     float2 *ml;
 };
 
-/* A row's sequence and position; keys of its sequence. */
+/* A row's sequence and position, and the keys of its sequence. */
 struct win_row {
     int b, p, nk;
 };
@@ -69,6 +70,18 @@ static __device__ __forceinline__ int win_lo(const win_args &a, int p)
     return a.left < 0 || p <= a.left ? 0 : p - a.left;
 }
 
+/* The lowest n of 32 bits (n < 0: none). */
+static __device__ __forceinline__ unsigned win_below(int n)
+{
+    return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1;
+}
+
+/* Bit i: a row of window lo .. hi sees key k0 + i, if it is kept. */
+static __device__ __forceinline__ unsigned win_sees(const win_args &a, int lo, int hi, int k0)
+{
+    return win_below(hi - k0 + 1) & (~win_below(lo - k0) | win_below(a.sinks - k0));
+}
+
 template <int KT>
 static __device__ __forceinline__ win_tiles win_span(const win_args &a, int p_lo, int p_hi, int nk)
 {
@@ -89,23 +102,11 @@ static __device__ __forceinline__ win_tiles win_span(const win_args &a, int p_lo
     return t;
 }
 
-template <bool CACHE>
-static __device__ __forceinline__ win_row win_row_of(const win_args &a, int row)
-{
-    if (!CACHE)
-        return {0, a.q0 + row, a.Nk};
-    const int b = seq_of(a.c, row);
-
-    if (b < 0)
-        return {-1, 0, 0};
-    return {b, (int)(max(a.c.len[b], 0) - (long long)(seq_start(a.c, b + 1) - row)), seq_len(a.c, b)};
-}
-
-/* One row and head over the tiles t0 .. t1 - 1 of 64 keys, in float32, by a
+/* One row and head over the tiles t0 .. t1 - 1 of KT <= 64 keys, in float32, by a
  * wave: lane k has key k's score, then every 64th channel. Seen keys alone are
  * read for the output, whatever the others hold. p: 64 floats of LDS of this
  * wave. Output unnormalised, o[j] channel lane + 64 j. */
-template <bool CACHE>
+template <bool CACHE, int KT>
 static __device__ __forceinline__ void win_row_f32(const win_args &a, const win_row &r, int row, int h,
                                                    const win_tiles &t, int t0, int t1, float *ps,
                                                    float (&o)[2], float &m, float &l)
@@ -117,8 +118,8 @@ static __device__ __forceinline__ void win_row_f32(const win_args &a, const win_
     m = -INFINITY;
     l = o[0] = o[1] = 0.0f;
     for (int i = t0; i < t1; i++) {
-        const int k0 = t.tile(i) * 64, k = k0 + lane;
-        bool see = k <= hi && (k >= lo || k < a.sinks);
+        const int k0 = t.tile(i) * KT, k = k0 + lane;
+        bool see = lane < KT && k <= hi && (k >= lo || k < a.sinks);
         long long at = 0;
 
         if (CACHE) {
@@ -228,40 +229,6 @@ static __device__ __forceinline__ int win_parts(int tiles, int splits)
     return min(splits, max(1, tiles / 4));
 }
 
-/* A wave a row, head and split. */
-template <bool CACHE> __global__ void __launch_bounds__(256) win_row_kernel(const win_args a)
-{
-    __shared__ float ps[4][64];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const long long u = (long long)blockIdx.x * 4 + wave;
-
-    if (u >= (long long)a.rows * a.nh * a.splits)
-        return;
-    const int split = (int)(u % a.splits), h = (int)(u / a.splits % a.nh);
-    const int row = (int)(u / a.splits / a.nh);
-    const win_row r = win_row_of<CACHE>(a, row);
-
-    if (r.b < 0) {
-        /* Nothing to write, and nothing to join. */
-        if (a.splits > 1 && lane == 0)
-            a.ml[u] = make_float2(0.0f, WIN_WRITTEN);
-        return;
-    }
-    const win_tiles t = win_span<64>(a, r.p, r.p, r.nk);
-    const int parts = win_parts(t.n, a.splits);
-
-    if (split >= parts) {
-        if (lane == 0)
-            a.ml[u] = make_float2(-INFINITY, 0.0f);
-        return;
-    }
-    float o[2], m, l;
-
-    win_row_f32<CACHE>(a, r, row, h, t, (int)((long long)t.n * split / parts),
-                       (int)((long long)t.n * (split + 1) / parts), ps[wave], o, m, l);
-    win_put(a, row, h, split, parts, o, m, l);
-}
-
 /* ---- a tile of rows over a cache ------------------------------------------------ */
 
 typedef _Float16 win_h2 __attribute__((ext_vector_type(2)));
@@ -339,6 +306,54 @@ static __device__ __forceinline__ win_job win_job_of(const win_args &a, int tile
     j.p0 = max(a.c.len[j.b], 0) - rows;
     j.nk = seq_len(a.c, j.b);
     return j;
+}
+
+/* A wave's 32 rows to their places, `down` times the accumulators; rows to do
+ * again (a sum that is not finite, values that the matrix instructions' parts
+ * cannot hold) in float32. */
+template <int ND, bool CACHE, int KT>
+static __device__ __forceinline__ void win_finish(const win_args &a, const win_job &jb, const win_tiles &span, int t0,
+                                                  int t1, int parts, int split, const win_f16x (&o)[ND], float down,
+                                                  float m, float l, bool again, float *ps, int d)
+{
+    const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31, g = a.nh / a.nhk;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), last = jb.r0 + jb.n - 1;
+    const int wr = jb.r0 + 32 * wave, r = min(wr + col, last), qi = r / g, h = jb.kvh * g + r - qi * g;
+    const bool mine = wr + col <= last, direct = parts == 1;
+    const long long row = jb.first + qi, out = (row * a.nh + h) * a.splits + split;
+    unsigned long long redo = __ballot(again && mine);
+
+    redo = (redo | redo >> 32) & 0xffffffffull;
+    if (mine && !(redo >> col & 1)) {
+        const float inv = direct ? (l > 0.0f ? down / l : 0.0f) : down;
+        float *to = direct ? a.O + row * a.ldo + (long long)h * d : a.part + out * (32 * ND);
+
+#pragma unroll
+        for (int tt = 0; tt < ND; tt++)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+                const int c = 32 * tt + 2 * e + 4 * half;
+
+                if (c + 4 <= d)
+                    store4(to + c, o[tt][e] * inv, o[tt][e + 1] * inv, o[tt][e + 2] * inv, o[tt][e + 3] * inv);
+                else {
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        if (c + j < d)
+                            to[c + j] = o[tt][e + j] * inv;
+                }
+            }
+        if (half == 0 && a.splits > 1)
+            a.ml[out] = direct ? make_float2(0.0f, WIN_WRITTEN) : make_float2(m, l);
+    }
+    for (; redo; redo &= redo - 1) {
+        const int rr = wr + __builtin_ctzll(redo), q1 = rr / g, h1 = jb.kvh * g + rr - q1 * g;
+        const win_row wrow = {jb.b, jb.p0 + q1, jb.nk};
+        float y[2], m1, l1;
+
+        win_row_f32<CACHE, KT>(a, wrow, jb.first + q1, h1, span, t0, t1, ps, y, m1, l1);
+        win_put(a, jb.first + q1, h1, split, parts, y, m1, l1);
+    }
 }
 
 /* A tile's place among a key head's: from both ends in turn, so that a stretch
@@ -612,14 +627,15 @@ __global__ void __launch_bounds__(256, ND == 4 ? 2 : 3) win_cache_kernel(const w
             if (!all) {
 #pragma unroll
                 for (int tt = 0; tt < 2; tt++) {
-                    const unsigned keep = (unsigned)(s.keep >> (32 * tt + 4 * half));
+                    unsigned see = (unsigned)(s.keep >> 32 * tt) & win_sees(a, lo, hi, k0 + 32 * tt);
 
+                    see >>= 4 * half;
+                    /* Tested here: as conditions kept they fill the scalar
+                     * registers. */
+                    asm volatile("" : "+v"(see));
 #pragma unroll
-                    for (int e = 0; e < 16; e++) {
-                        const int off = 8 * (e >> 2) + (e & 3), k = k0 + 32 * tt + 4 * half + off;
-
-                        x[tt][e] = (keep >> off & 1) && k <= hi && (k >= lo || k < a.sinks) ? x[tt][e] : -INFINITY;
-                    }
+                    for (int e = 0; e < 16; e++)
+                        x[tt][e] = see >> (8 * (e >> 2) + (e & 3)) & 1 ? x[tt][e] : -INFINITY;
                 }
             }
 #pragma unroll
@@ -707,93 +723,429 @@ __global__ void __launch_bounds__(256, ND == 4 ? 2 : 3) win_cache_kernel(const w
 #pragma unroll
         for (int e = 0; e < 16; e++)
             z = fmaf(o[tt][e], 0.0f, z);
-    const bool again = wild || z != 0.0f;
-    unsigned long long redo = __ballot(again && mine);
-
-    redo = (redo | redo >> 32) & 0xffffffffull;
-    const bool good = mine && !(redo >> col & 1);
-    const bool direct = parts == 1;
-
-    if (good) {
-        const float inv = direct ? (l > 0.0f ? 1.0f / l : 0.0f) : 1.0f;
-        float *to = direct ? a.O + row * a.ldo + (long long)h * d : a.part + out * DP;
-
-#pragma unroll
-        for (int tt = 0; tt < ND; tt++)
-#pragma unroll
-            for (int e = 0; e < 16; e += 4) {
-                const int c = 32 * tt + 2 * e + 4 * half;
-
-                if (c + 4 <= d)
-                    store4(to + c, o[tt][e] * inv, o[tt][e + 1] * inv, o[tt][e + 2] * inv, o[tt][e + 3] * inv);
-                else {
-#pragma unroll
-                    for (int j = 0; j < 4; j++)
-                        if (c + j < d)
-                            to[c + j] = o[tt][e + j] * inv;
-                }
-            }
-        if (half == 0 && a.splits > 1)
-            a.ml[out] = direct ? make_float2(0.0f, WIN_WRITTEN) : make_float2(m, l);
-    }
-    /* Rows with a sum that is not finite, and all of a block that met value
-     * scales it cannot hold: again in float32. */
-    for (; redo; redo &= redo - 1) {
-        const int rr = wr + __builtin_ctzll(redo), q1 = rr / g, h1 = jb.kvh * g + rr - q1 * g;
-        const win_row wrow = {jb.b, jb.p0 + q1, jb.nk};
-        float y[2], m1, l1;
-
-        win_row_f32<true>(a, wrow, jb.first + q1, h1, span, t0, t1, ps[wave], y, m1, l1);
-        win_put(a, jb.first + q1, h1, split, parts, y, m1, l1);
-    }
+    win_finish<ND, true, WIN_KT>(a, jb, span, t0, t1, parts, split, o, 1.0f, m, l, wild || z != 0.0f, ps[wave], d);
 }
 
-/* Parts of a row and head joined: a wave each, lane s with split s, s + 64, ..
- */
-__global__ void __launch_bounds__(256) win_merge_kernel(const win_args a)
+/* ---- a tile of rows over float32 keys and values --------------------------------- */
+
+#define WIN_FKT 32            /* keys of a tile */
+#define WIN_FTAU 8.0f         /* as WIN_TAU */
+#define WIN_QUP 0x1p32f       /* scale of the queries split into bf16 parts */
+
+template <int ND, bool FULL>
+__global__ void __launch_bounds__(256, ND == 4 ? 1 : 3) win_float_kernel(const win_args a)
 {
-    __shared__ float ws[4][WIN_MAX_SPLITS];
+    constexpr int DP = 32 * ND, CH = DP / 8;
+    constexpr int RW = 16 / CH < 1 ? 1 : 16 / CH; /* K rows in 256 bytes */
+    constexpr int PK = WIN_FKT * CH;              /* chunks of a part: K and V alike */
+    constexpr int NL = (PK + 255) / 256;
+    __shared__ split_u4 lds[2][6 * PK];
+    __shared__ float ps[4][64];
+    const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, col = lane & 31;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int g = a.nh / a.nhk, d = FULL ? DP : a.d;
+    const int tiles = (int)(((long long)a.rows * g + WIN_ROWS - 1) / WIN_ROWS);
+    const int unit = xcd_tile(blockIdx.x, gridDim.x), split = unit % a.splits;
+    const win_job jb = win_job_of<false>(a, win_order(unit / a.splits % tiles, tiles), unit / a.splits / tiles);
+    const int last = jb.r0 + jb.n - 1;
+    const win_tiles span = win_span<WIN_FKT>(a, jb.p0 + jb.r0 / g, jb.p0 + last / g, jb.nk);
+    const int parts = win_parts(span.n, a.splits);
+    /* This lane's row; lanes without one take the last. */
+    const int wr = jb.r0 + 32 * wave, r = min(wr + col, last), qi = r / g, h = jb.kvh * g + r - qi * g;
+    const bool mine = wr + col <= last;
+    const long long row = qi, out = (row * a.nh + h) * a.splits + split;
+
+    if (split >= parts) {
+        if (mine && half == 0)
+            a.ml[out] = make_float2(-INFINITY, 0.0f);
+        return;
+    }
+    const int t0 = (int)((long long)span.n * split / parts), t1 = (int)((long long)span.n * (split + 1) / parts);
+    const int p0 = jb.p0 + qi, hi = win_hi(a, p0, jb.nk), lo = win_lo(a, p0);
+    const bool live = wr <= last;
+    const int pa = jb.p0 + min(wr, last) / g, pb = jb.p0 + min(wr + 31, last) / g;
+    const int hi0 = win_hi(a, pa, jb.nk), hi1 = win_hi(a, pb, jb.nk), lo0 = win_lo(a, pa), lo1 = win_lo(a, pb);
+    const float *K = a.K + (long long)jb.kvh * d, *V = a.V + (long long)jb.kvh * d;
+    /* Threads past the chunks (32 channels a head): none in K, all in V. */
+    constexpr bool APART = PK < 256;
+    const bool has_k = !APART || tid < PK;
+    const int vt = APART ? tid - PK : tid;
+    float kr[NL][8], vr[NL][8];
+    split_u4 q[2 * ND][3];
+    /* The output's small products: of all keys (LOW), or of 16 at a time
+     * where 16 registers a 32 channels more would spill. */
+    constexpr bool LOW = ND != 2;
+    win_f16x o[ND], low[LOW ? ND : 1];
+    float m = -INFINITY, l = 0.0f;
+    unsigned seen = 0, next = ~0u;
+
+    {
+        const float *qp = a.Q + row * a.ldq + (long long)h * d;
+        const float up = a.scale * WIN_LOG2E * WIN_QUP;
+
+#pragma unroll
+        for (int st = 0; st < 2 * ND; st++) {
+            float u[4], v[4], x[8];
+
+            if (FULL) {
+                load4(qp + st * 16 + half * 8, u);
+                load4(qp + st * 16 + half * 8 + 4, v);
+            }
+            else {
+                load4_row(qp, st * 16 + half * 8, d, u);
+                load4_row(qp, st * 16 + half * 8 + 4, d, v);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                x[j] = u[j];
+                x[4 + j] = v[j];
+            }
+            split8(x, up, q[st][0], q[st][1], q[st][2]);
+        }
+    }
+#pragma unroll
+    for (int tt = 0; tt < ND; tt++)
+#pragma unroll
+        for (int e = 0; e < 16; e++)
+            o[tt][e] = low[LOW ? tt : 0][e] = 0.0f;
+
+    /* Tile t into registers: K chunk e is key e / CH, channels 8 (e % CH) ..; V
+     * chunk e channel e % DP, slots 8 (e / DP) .. + 7. Behind the last key it
+     * is read again; behind d K is zero (so that what lies there cannot be
+     * NaN) and V the last channel. next: the tile's kept keys. */
+    auto fetch = [&](int t) {
+        const int k0 = span.tile(t) * WIN_FKT, end = jb.nk - 1 - k0;
+
+        if (has_k) {
+#pragma unroll
+            for (int i = 0; i < NL; i++) {
+                const int e = tid + 256 * i, dd = e % CH * 8;
+                const float *p = K + (k0 + min(e / CH, end)) * a.ldk;
+                float u[4], v[4];
+
+                if (FULL) {
+                    load4(p + dd, u);
+                    load4(p + dd + 4, v);
+                }
+                else {
+                    load4_row(p, dd, d, u);
+                    load4_row(p, dd + 4, d, v);
+                }
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    kr[i][j] = u[j];
+                    kr[i][4 + j] = v[j];
+                }
+            }
+        }
+        if (!APART || !has_k) {
+#pragma unroll
+            for (int i = 0; i < NL; i++) {
+                const int e = vt + 256 * i, dd = FULL ? e % DP : min(e % DP, d - 1);
+                const int c = ND == 1 ? e / DP : __builtin_amdgcn_readfirstlane(e / DP);
+
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const int kk = (c >> 1) * 16 + (j >> 2) * 8 + (c & 1) * 4 + (j & 3);
+
+                    vr[i][j] = (V + (k0 + min(kk, end)) * a.ldv)[dd];
+                }
+            }
+        }
+        if (a.kmask)
+            next = col <= end && a.kmask[k0 + col];
+    };
+    /* keep: the kept keys of the registers' tile; values of others are zero,
+     * whatever they hold. */
+    auto stash = [&](split_u4 *ks, unsigned keep) {
+        split_u4 *vs = ks + 3 * PK, x, y, z;
+
+        if (has_k) {
+#pragma unroll
+            for (int i = 0; i < NL; i++) {
+                const int e = tid + 256 * i, key = e / CH;
+                const int at = key * CH + ((e % CH) ^ (key / RW % CH));
+
+                split8(kr[i], 1.0f, x, y, z);
+                ks[at] = x;
+                ks[PK + at] = y;
+                ks[2 * PK + at] = z;
+            }
+        }
+        if (!APART || !has_k) {
+#pragma unroll
+            for (int i = 0; i < NL; i++) {
+                const int e = vt + 256 * i, dd = e % DP, c = e / DP;
+                const int at = dd * 4 + (c ^ (dd >> 2 & 3));
+
+                if (keep != ~0u) {
+                    const unsigned k = keep >> ((c >> 1) * 16 + (c & 1) * 4);
+
+#pragma unroll
+                    for (int j = 0; j < 8; j++)
+                        vr[i][j] = k >> ((j >> 2) * 8 + (j & 3)) & 1 ? vr[i][j] : 0.0f;
+                }
+                split8(vr[i], SPLIT_UP, x, y, z);
+                vs[at] = x;
+                vs[PK + at] = y;
+                vs[2 * PK + at] = z;
+            }
+        }
+    };
+    constexpr int pa6[6] = {0, 2, 1, 0, 1, 0}, pb6[6] = {2, 0, 1, 1, 0, 0};
+    unsigned keep = ~0u;
+
+    if (t0 < t1) {
+        fetch(t0);
+        if (a.kmask)
+            keep = (unsigned)__ballot(next);
+        stash(lds[0], keep);
+        if (t0 + 1 < t1)
+            fetch(t0 + 1);
+    }
+    __syncthreads();
+    for (int t = t0; t < t1; t++) {
+        const split_u4 *ks = lds[(t - t0) & 1], *vs = ks + 3 * PK;
+        const int k0 = span.tile(t) * WIN_FKT;
+        /* Some row of the wave sees some key; all see all. */
+        const bool some = live && k0 <= hi1 && (k0 + WIN_FKT > lo0 || k0 < a.sinks);
+        const bool all = keep == ~0u && k0 + WIN_FKT - 1 <= hi0 && (k0 >= lo1 || k0 + WIN_FKT <= a.sinks);
+        const unsigned after = a.kmask && t + 1 < t1 ? (unsigned)__ballot(next) : ~0u;
+        float p[16];
+
+        if (some) {
+            win_f16x s;
+            float mx = -INFINITY, sum = 0.0f;
+            auto key = [&](int w, int st) {
+                return __builtin_bit_cast(split_b8, ks[w * PK + col * CH + ((2 * st + half) ^ (col / RW % CH))]);
+            };
+
+#pragma unroll
+            for (int e = 0; e < 16; e++)
+                s[e] = 0.0f;
+            /* The small products first, then the large ones. */
+#pragma unroll
+            for (int st = 0; st < 2 * ND; st++) {
+                const split_b8 kf[3] = {key(0, st), key(1, st), key(2, st)};
+
+#pragma unroll
+                for (int w = 0; w < 5; w++)
+                    s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+                        kf[pa6[w]], __builtin_bit_cast(split_b8, q[st][pb6[w]]), s, 0, 0, 0);
+            }
+#pragma unroll
+            for (int st = 0; st < 2 * ND; st++)
+                s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+                    key(0, st), __builtin_bit_cast(split_b8, q[st][0]), s, 0, 0, 0);
+            if (all) {
+                seen = 1;
+#pragma unroll
+                for (int e = 0; e < 16; e++)
+                    p[e] = s[e];
+            }
+            else {
+                unsigned see = keep & win_sees(a, lo, hi, k0);
+
+                seen |= see;
+                see >>= 4 * half;
+                /* Tested here: as conditions kept they fill the scalar
+                 * registers. */
+                asm volatile("" : "+v"(see));
+#pragma unroll
+                for (int e = 0; e < 16; e++)
+                    p[e] = see >> (8 * (e >> 2) + (e & 3)) & 1 ? s[e] : -INFINITY;
+            }
+#pragma unroll
+            for (int e = 0; e < 16; e++)
+                mx = fmaxf(mx, p[e]);
+            mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * (1.0f / WIN_QUP);
+            const bool need = mx > m + WIN_FTAU;
+
+            if (__any(need)) {
+                const float mn = need ? mx : m;
+                const float corr = need ? __builtin_amdgcn_exp2f(m - mn) : 1.0f;
+
+                m = mn;
+                l *= corr;
+#pragma unroll
+                for (int tt = 0; tt < ND; tt++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) {
+                        o[tt][e] *= corr;
+                        if (LOW)
+                            low[LOW ? tt : 0][e] *= corr;
+                    }
+            }
+            const float ref = m == -INFINITY ? 0.0f : m;
+
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+                p[e] = __builtin_amdgcn_exp2f(fmaf(p[e], 1.0f / WIN_QUP, -ref));
+                sum += p[e];
+            }
+            l += sum + __shfl_xor(sum, 32, 64);
+        }
+        /* The next tile into the other buffer, which was last read a tile ago,
+         * before the barrier; then its successor's loads. */
+        if (t + 1 < t1) {
+            stash(lds[(t + 1 - t0) & 1], after);
+            if (t + 2 < t1)
+                fetch(t + 2);
+        }
+        if (some) {
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                float x[8];
+                split_u4 pp[3];
+
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+                    x[j] = p[8 * u + j];
+                split8(x, SPLIT_UP, pp[0], pp[1], pp[2]);
+#pragma unroll
+                for (int tt = 0; tt < ND; tt++) {
+                    const int dd = tt * 32 + col;
+                    split_b8 vf[3];
+                    win_f16x &small = low[LOW ? tt : 0];
+
+                    if (!LOW)
+#pragma unroll
+                        for (int e = 0; e < 16; e++)
+                            small[e] = 0.0f;
+#pragma unroll
+                    for (int k = 0; k < 3; k++)
+                        vf[k] = __builtin_bit_cast(split_b8, vs[k * PK + dd * 4 + ((2 * u + half) ^ (dd >> 2 & 3))]);
+#pragma unroll
+                    for (int w = 0; w < 6; w++) {
+                        win_f16x &c = w == 5 ? o[tt] : small;
+
+                        c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+                            vf[pa6[w]], __builtin_bit_cast(split_b8, pp[pb6[w]]), c, 0, 0, 0);
+                    }
+                    if (!LOW)
+#pragma unroll
+                        for (int e = 0; e < 16; e++)
+                            o[tt][e] += small[e];
+                }
+            }
+        }
+        keep = after;
+        __syncthreads();
+    }
+    float z = l * 0.0f;
+
+#pragma unroll
+    for (int tt = 0; tt < ND; tt++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) {
+            if (LOW)
+                o[tt][e] += low[LOW ? tt : 0][e];
+            z = fmaf(o[tt][e], 0.0f, z);
+        }
+    /* No probability at all for keys that are seen: their scores lie below the
+     * range of the split. */
+    win_finish<ND, false, WIN_FKT>(a, jb, span, t0, t1, parts, split, o, SPLIT_DOWN, m, l,
+                                   z != 0.0f || (l == 0.0f && seen), ps[wave], d);
+}
+
+/* Parts of a row and head joined, by W waves: softmax over all of them from
+ * their maxima and sums, then DP / 4 lanes a part, 256 W / DP parts at a time. */
+template <int DP, int W> __global__ void __launch_bounds__(256) win_merge_kernel(const win_args a)
+{
+    constexpr int RB = 4 / W, LV = DP / 4, GV = 64 * W / LV; /* rows of a block; groups of lanes of a row */
+    __shared__ float ws[RB][WIN_MAX_SPLITS];
+    __shared__ float red[2][4];
+    __shared__ float4 sums[W > 1 ? 4 : 1][LV];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const long long u = (long long)blockIdx.x * 4 + wave;
-    const int dp = a.d <= 32 ? 32 : a.d <= 64 ? 64 : 128;
+    const int sub = wave % W, mine = wave / W, t = 64 * sub + lane, n = a.splits;
+    const long long u = (long long)blockIdx.x * RB + mine;
 
     if (u >= (long long)a.rows * a.nh)
         return;
-    const float2 *ml = a.ml + u * a.splits;
-
-    const int row = (int)(u / a.nh), h = (int)(u % a.nh);
+    const int row = (int)(u / a.nh), h = (int)(u % a.nh), c = 4 * (t % LV);
+    const float2 *ml = a.ml + u * n;
+    const float *part = a.part + u * n * DP + c;
 
     if ((a.c.n && seq_of(a.c, row) < 0) || ml[0].y == WIN_WRITTEN)
         return;
-    float m = -INFINITY, l = 0.0f, o[2] = {0, 0};
+    /* At most WIN_MAX_SPLITS = 256 parts: 4 a lane of a wave. */
+    constexpr int NS = WIN_MAX_SPLITS / 64 / W;
+    float2 x[NS];
+    float m = -INFINITY, l = 0.0f, o[4] = {0, 0, 0, 0};
 
-    for (int s = lane; s < a.splits; s += 64)
-        m = fmaxf(m, ml[s].x);
+#pragma unroll
+    for (int i = 0; i < NS; i++) {
+        x[i] = t + 64 * W * i < n ? ml[t + 64 * W * i] : make_float2(-INFINITY, 0.0f);
+        m = fmaxf(m, x[i].x);
+    }
     m = wave_max_full(m);
-    for (int s = lane; s < a.splits; s += 64) {
-        const float2 x = ml[s];
-        const float w = x.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x.x - m);
+    if constexpr (W > 1) {
+        if (lane == 0)
+            red[0][wave] = m;
+        __syncthreads();
+        m = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+    }
+#pragma unroll
+    for (int i = 0; i < NS; i++) {
+        const float w = x[i].x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x[i].x - m);
 
-        ws[wave][s] = w;
-        l += w * x.y;
+        if (t + 64 * W * i < n)
+            ws[mine][t + 64 * W * i] = w;
+        l += w * x[i].y;
     }
     l = wave_sum_full(l);
-    __builtin_amdgcn_wave_barrier();
-    for (int s = 0; s < a.splits; s++) {
-        const float w = ws[wave][s];
-
-        if (w != 0.0f)
-#pragma unroll
-            for (int e = 0; e < 2; e++)
-                if (lane + 64 * e < a.d)
-                    o[e] = fmaf(w, a.part[(u * a.splits + s) * dp + lane + 64 * e], o[e]);
+    if constexpr (W > 1) {
+        if (lane == 0)
+            red[1][wave] = l;
+        __syncthreads();
+        l = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
     }
-    float *out = a.O + row * a.ldo + (long long)h * a.d;
+    else
+        __builtin_amdgcn_wave_barrier();
+    /* Parts of no weight hold nothing, or what does not count. */
+    for (int s0 = t / LV; s0 < n; s0 += 4 * GV) {
+        float4 p[4];
+        float w[4];
 
 #pragma unroll
-    for (int e = 0; e < 2; e++)
-        if (lane + 64 * e < a.d)
-            out[lane + 64 * e] = l == 0.0f ? 0.0f : o[e] / l;
+        for (int i = 0; i < 4; i++) {
+            const int s = s0 + i * GV;
+
+            w[i] = s < n ? ws[mine][s] : 0.0f;
+            p[i] = w[i] != 0.0f ? *(const float4 *)(part + (long long)s * DP) : make_float4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            o[0] = fmaf(w[i], p[i].x, o[0]);
+            o[1] = fmaf(w[i], p[i].y, o[1]);
+            o[2] = fmaf(w[i], p[i].z, o[2]);
+            o[3] = fmaf(w[i], p[i].w, o[3]);
+        }
+    }
+#pragma unroll
+    for (int s = LV; s < 64; s *= 2)
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            o[j] += __shfl_xor(o[j], s, 64);
+    if constexpr (W > 1) {
+        if (lane < LV)
+            sums[wave][lane] = make_float4(o[0], o[1], o[2], o[3]);
+        __syncthreads();
+        if (t >= LV)
+            return;
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            o[j] = (((const float *)&sums[0][t])[j] + ((const float *)&sums[1][t])[j]) +
+                   (((const float *)&sums[2][t])[j] + ((const float *)&sums[3][t])[j]);
+    }
+    if (t < LV) {
+        float *out = a.O + row * a.ldo + (long long)h * a.d;
+
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            if (c + j < a.d)
+                out[c + j] = l == 0.0f ? 0.0f : o[j] / l;
+    }
 }
 
 /* ---- on the host -------------------------------------------------------------- */
@@ -832,7 +1184,8 @@ template <bool CACHE> static void win_launch(struct ops *o, win_args &a, long lo
 {
     const int cus = o->ocl->cu_count > 0 ? o->ocl->cu_count : 256;
     const long long heads = (long long)a.rows * a.nh;
-    const long long blocks = CACHE ? (heads / a.nhk / WIN_ROWS + a.c.n) * a.nhk : (heads + 3) / 4;
+    const long long rows = heads / a.nhk; /* of a key head */
+    const long long blocks = (CACHE ? rows / WIN_ROWS + a.c.n : (rows + WIN_ROWS - 1) / WIN_ROWS) * a.nhk;
 
     a.splits = win_splits(a, blocks, keys, 4 * cus);
     if (a.splits > 1) {
@@ -843,22 +1196,43 @@ template <bool CACHE> static void win_launch(struct ops *o, win_args &a, long lo
     const hipStream_t s = stream_of(o->ocl);
 
     prof_scope ps(o->ocl, CACHE ? "attention_cache" : "attention_window");
-    if (CACHE) {
-        const dim3 grid(grid_of(blocks * a.splits, 256, "attention tiles")), block(256);
+    const dim3 grid(grid_of(blocks * a.splits, 256, "attention tiles")), block(256);
 
-        if (a.d <= 32)
-            hipLaunchKernelGGL(win_cache_kernel<1>, grid, block, 0, s, a);
-        else if (a.d <= 64)
-            hipLaunchKernelGGL(win_cache_kernel<2>, grid, block, 0, s, a);
-        else
-            hipLaunchKernelGGL(win_cache_kernel<4>, grid, block, 0, s, a);
-    }
+#define WIN_LAUNCH(ND_)                                                               \
+    do {                                                                              \
+        if (CACHE)                                                                    \
+            hipLaunchKernelGGL(win_cache_kernel<ND_>, grid, block, 0, s, a);          \
+        else if (a.d == 32 * ND_)                                                     \
+            hipLaunchKernelGGL((win_float_kernel<ND_, true>), grid, block, 0, s, a);  \
+        else                                                                          \
+            hipLaunchKernelGGL((win_float_kernel<ND_, false>), grid, block, 0, s, a); \
+    } while (0)
+    if (a.d <= 32)
+        WIN_LAUNCH(1);
+    else if (a.d <= 64)
+        WIN_LAUNCH(2);
     else
-        hipLaunchKernelGGL(win_row_kernel<CACHE>, dim3(grid_of((heads * a.splits + 3) / 4, 256, "attention rows")),
-                           dim3(256), 0, s, a);
-    launch_check("attention rows");
+        WIN_LAUNCH(4);
+#undef WIN_LAUNCH
+    launch_check("attention tiles");
     if (a.splits > 1) {
-        hipLaunchKernelGGL(win_merge_kernel, dim3((unsigned)((heads + 3) / 4)), dim3(256), 0, s, a);
+        const bool wide = a.splits > 16;
+        const dim3 mgrid(grid_of(wide ? heads : (heads + 3) / 4, 256, "attention merge"));
+
+#define MERGE_LAUNCH(DP_)                                                                \
+    do {                                                                                 \
+        if (wide)                                                                        \
+            hipLaunchKernelGGL((win_merge_kernel<DP_, 4>), mgrid, block, 0, s, a);       \
+        else                                                                             \
+            hipLaunchKernelGGL((win_merge_kernel<DP_, 1>), mgrid, block, 0, s, a);       \
+    } while (0)
+        if (a.d <= 32)
+            MERGE_LAUNCH(32);
+        else if (a.d <= 64)
+            MERGE_LAUNCH(64);
+        else
+            MERGE_LAUNCH(128);
+#undef MERGE_LAUNCH
         launch_check("attention merge");
     }
 }
