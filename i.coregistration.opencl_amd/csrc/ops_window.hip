@@ -270,23 +270,23 @@ struct win_job {
     int b, kvh, r0, n, first, p0, nk;
 };
 
-template <bool CACHE>
+template <bool CACHE, int TR>
 static __device__ __forceinline__ win_job win_job_of(const win_args &a, int tile, int kvh)
 {
     const int g = a.nh / a.nhk;
     win_job j = {0, kvh, 0, 0, 0, 0, 0};
 
     if (!CACHE) {
-        j.r0 = tile * WIN_ROWS;
-        j.n = (int)min((long long)a.rows * g - j.r0, (long long)WIN_ROWS);
+        j.r0 = tile * TR;
+        j.n = (int)min((long long)a.rows * g - j.r0, (long long)TR);
         j.p0 = a.q0;
         j.nk = a.Nk;
         return j;
     }
-    /* Sequence b has the tiles from start[b] g / WIN_ROWS + b on, one more than
+    /* Sequence b has the tiles of TR rows from start[b] g / TR + b on, one more than
      * it can need; the last that starts at or before this one, 64 sequences
      * at a time. */
-    auto from = [&](int b) { return (long long)seq_start(a.c, b) * g / WIN_ROWS + b; };
+    auto from = [&](int b) { return (long long)seq_start(a.c, b) * g / TR + b; };
     const int lane = threadIdx.x & 63;
     int count = 0;
 
@@ -301,8 +301,8 @@ static __device__ __forceinline__ win_job win_job_of(const win_args &a, int tile
     j.first = seq_start(a.c, j.b);
     const int rows = max(seq_start(a.c, j.b + 1) - j.first, 0);
 
-    j.r0 = (int)max(tile - from(j.b), 0LL) * WIN_ROWS;
-    j.n = (int)min((long long)rows * g - j.r0, (long long)WIN_ROWS);
+    j.r0 = (int)max(tile - from(j.b), 0LL) * TR;
+    j.n = (int)min((long long)rows * g - j.r0, (long long)TR);
     j.p0 = max(a.c.len[j.b], 0) - rows;
     j.nk = seq_len(a.c, j.b);
     return j;
@@ -382,7 +382,7 @@ __global__ void __launch_bounds__(256, ND == 4 ? 2 : 3) win_cache_kernel(const w
     const int g = a.nh / a.nhk, d = a.d, pitch = a.c.pitch;
     const int tiles = (int)((long long)a.rows * g / WIN_ROWS) + a.c.n;
     const int unit = xcd_tile(blockIdx.x, gridDim.x), split = unit % a.splits;
-    const win_job jb = win_job_of<true>(a, win_order(unit / a.splits % tiles, tiles), unit / a.splits / tiles);
+    const win_job jb = win_job_of<true, WIN_ROWS>(a, win_order(unit / a.splits % tiles, tiles), unit / a.splits / tiles);
 
     if (jb.n <= 0)
         return;
@@ -726,13 +726,33 @@ __global__ void __launch_bounds__(256, ND == 4 ? 2 : 3) win_cache_kernel(const w
     win_finish<ND, true, WIN_KT>(a, jb, span, t0, t1, parts, split, o, 1.0f, m, l, wild || z != 0.0f, ps[wave], d);
 }
 
+/* Channels of a head: any number (a load a float), a multiple of 4, or all
+ * that the kernel has room for. */
+enum { WIN_ANY, WIN_FOUR, WIN_FULL };
+
+/* Floats c .. c + 3 of a row of d; behind the last channel some of them again,
+ * for products with zeros and sums that are not stored. */
+template <int CHANNELS>
+static __device__ __forceinline__ void win_load4(const float *p, int c, int d, float (&x)[4])
+{
+    if (CHANNELS == WIN_FULL)
+        load4(p + c, x);
+    else if (CHANNELS == WIN_FOUR)
+        load4(p + min(c, d - 4), x);
+    else {
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            x[j] = p[min(c + j, d - 1)];
+    }
+}
+
 /* ---- a tile of rows over float32 keys and values --------------------------------- */
 
 #define WIN_FKT 32            /* keys of a tile */
 #define WIN_FTAU 8.0f         /* as WIN_TAU */
 #define WIN_QUP 0x1p32f       /* scale of the queries split into bf16 parts */
 
-template <int ND, bool FULL>
+template <int ND, int CHANNELS>
 __global__ void __launch_bounds__(256, ND == 4 ? 1 : 3) win_float_kernel(const win_args a)
 {
     constexpr int DP = 32 * ND, CH = DP / 8;
@@ -743,10 +763,10 @@ __global__ void __launch_bounds__(256, ND == 4 ? 1 : 3) win_float_kernel(const w
     __shared__ float ps[4][64];
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, col = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int g = a.nh / a.nhk, d = FULL ? DP : a.d;
+    const int g = a.nh / a.nhk, d = CHANNELS == WIN_FULL ? DP : a.d;
     const int tiles = (int)(((long long)a.rows * g + WIN_ROWS - 1) / WIN_ROWS);
     const int unit = xcd_tile(blockIdx.x, gridDim.x), split = unit % a.splits;
-    const win_job jb = win_job_of<false>(a, win_order(unit / a.splits % tiles, tiles), unit / a.splits / tiles);
+    const win_job jb = win_job_of<false, WIN_ROWS>(a, win_order(unit / a.splits % tiles, tiles), unit / a.splits / tiles);
     const int last = jb.r0 + jb.n - 1;
     const win_tiles span = win_span<WIN_FKT>(a, jb.p0 + jb.r0 / g, jb.p0 + last / g, jb.nk);
     const int parts = win_parts(span.n, a.splits);
@@ -787,14 +807,8 @@ __global__ void __launch_bounds__(256, ND == 4 ? 1 : 3) win_float_kernel(const w
         for (int st = 0; st < 2 * ND; st++) {
             float u[4], v[4], x[8];
 
-            if (FULL) {
-                load4(qp + st * 16 + half * 8, u);
-                load4(qp + st * 16 + half * 8 + 4, v);
-            }
-            else {
-                load4_row(qp, st * 16 + half * 8, d, u);
-                load4_row(qp, st * 16 + half * 8 + 4, d, v);
-            }
+            load4_row(qp, st * 16 + half * 8, d, u);
+            load4_row(qp, st * 16 + half * 8 + 4, d, v);
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 x[j] = u[j];
@@ -811,8 +825,7 @@ __global__ void __launch_bounds__(256, ND == 4 ? 1 : 3) win_float_kernel(const w
 
     /* Tile t into registers: K chunk e is key e / CH, channels 8 (e % CH) ..; V
      * chunk e channel e % DP, slots 8 (e / DP) .. + 7. Behind the last key it
-     * is read again; behind d K is zero (so that what lies there cannot be
-     * NaN) and V the last channel. next: the tile's kept keys. */
+     * is read again. next: the tile's kept keys. */
     auto fetch = [&](int t) {
         const int k0 = span.tile(t) * WIN_FKT, end = jb.nk - 1 - k0;
 
@@ -823,14 +836,8 @@ __global__ void __launch_bounds__(256, ND == 4 ? 1 : 3) win_float_kernel(const w
                 const float *p = K + (k0 + min(e / CH, end)) * a.ldk;
                 float u[4], v[4];
 
-                if (FULL) {
-                    load4(p + dd, u);
-                    load4(p + dd + 4, v);
-                }
-                else {
-                    load4_row(p, dd, d, u);
-                    load4_row(p, dd + 4, d, v);
-                }
+                win_load4<CHANNELS>(p, dd, d, u);
+                win_load4<CHANNELS>(p, dd + 4, d, v);
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
                     kr[i][j] = u[j];
@@ -841,7 +848,7 @@ __global__ void __launch_bounds__(256, ND == 4 ? 1 : 3) win_float_kernel(const w
         if (!APART || !has_k) {
 #pragma unroll
             for (int i = 0; i < NL; i++) {
-                const int e = vt + 256 * i, dd = FULL ? e % DP : min(e % DP, d - 1);
+                const int e = vt + 256 * i, dd = CHANNELS == WIN_FULL ? e % DP : min(e % DP, d - 1);
                 const int c = ND == 1 ? e / DP : __builtin_amdgcn_readfirstlane(e / DP);
 
 #pragma unroll
@@ -1048,6 +1055,445 @@ __global__ void __launch_bounds__(256, ND == 4 ? 1 : 3) win_float_kernel(const w
                                    z != 0.0f || (l == 0.0f && seen), ps[wave], d);
 }
 
+/* ---- few rows ---------------------------------------------------------------------- */
+
+#define WIN_FEW 16  /* rows of a tile */
+#define WIN_STEP 32 /* keys of a step of a wave */
+
+typedef float win_f4 __attribute__((ext_vector_type(4)));
+
+/* At most 16 rows, as a decoding step has: nothing is shared by rows of other
+ * waves, so each wave goes through steps of keys of its own, from memory to
+ * registers to the matrix instructions without LDS or barriers; the block's
+ * four join their outputs at the end. v_mfma_f32_16x16x32_bf16: scores have
+ * the keys as rows (lane % 16 of either 16) and the queries as columns, and
+ * leave a lane with the keys 16 t + 4 (lane / 16) + r of its query lane % 16,
+ * which slot 4 t + r of the second product takes as they are. Queries and
+ * weights are three bf16 parts each (split.h), codes are bf16 values: exact. */
+template <int ND, bool CACHE, int CHANNELS>
+__global__ void __launch_bounds__(256, CACHE && ND == 4 ? 3 : 2) win_few_kernel(const win_args a)
+{
+    constexpr int DP = 32 * ND, NT = 2 * ND;  /* channels, tiles of 16 of them */
+    constexpr int VL = DP / 16;               /* channels of a lane */
+    constexpr int KW = CACHE ? (ND == 1 ? 2 : 4) : 8; /* words of a load of K: 8 or 16 bytes, 8 floats */
+    constexpr int KL = CACHE ? (ND == 4 ? 2 : 1) : ND; /* loads of a key */
+    constexpr int VW = CACHE ? (ND == 4 ? 2 : 1) : VL; /* words of a key's channels of V */
+    __shared__ float os[4][WIN_FEW][DP + 4];
+    __shared__ float ms[4][WIN_FEW], lsum[4][WIN_FEW], ps[4][64];
+    __shared__ int redo[WIN_FEW];
+    const int tid = threadIdx.x, lane = tid & 63, grp = lane >> 4, col = lane & 15;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int g = a.nh / a.nhk, d = CHANNELS == WIN_FULL ? DP : a.d, pitch = a.c.pitch;
+    const int tiles = CACHE ? (int)((long long)a.rows * g / WIN_FEW) + a.c.n
+                            : (int)(((long long)a.rows * g + WIN_FEW - 1) / WIN_FEW);
+    const int unit = xcd_tile(blockIdx.x, gridDim.x), split = unit % a.splits;
+    const win_job jb = win_job_of<CACHE, WIN_FEW>(a, unit / a.splits % tiles, unit / a.splits / tiles);
+
+    if (jb.n <= 0)
+        return;
+    const int last = jb.r0 + jb.n - 1;
+    const win_tiles span = win_span<WIN_STEP>(a, jb.p0 + jb.r0 / g, jb.p0 + last / g, jb.nk);
+    const int parts = win_parts(span.n, a.splits);
+    /* This lane's row; lanes without one take the last. */
+    const int r = min(jb.r0 + col, last), qi = r / g, h = jb.kvh * g + r - qi * g;
+    const bool mine = jb.r0 + col <= last;
+    const long long row = jb.first + qi;
+
+    if (split >= parts) {
+        if (mine && tid < WIN_FEW)
+            a.ml[(row * a.nh + h) * a.splits + split] = make_float2(-INFINITY, 0.0f);
+        return;
+    }
+    const int t0 = (int)((long long)span.n * split / parts), t1 = (int)((long long)span.n * (split + 1) / parts);
+    /* This wave's steps. */
+    const int s0 = t0 + (int)((long long)(t1 - t0) * wave / 4), s1 = t0 + (int)((long long)(t1 - t0) * (wave + 1) / 4);
+    const int p0 = jb.p0 + qi, hi = win_hi(a, p0, jb.nk), lo = win_lo(a, p0);
+    /* What every row sees. */
+    const int hi0 = win_hi(a, jb.p0 + jb.r0 / g, jb.nk), lo1 = win_lo(a, jb.p0 + last / g);
+    const float *K = CACHE ? nullptr : a.K + (long long)jb.kvh * d, *V = CACHE ? nullptr : a.V + (long long)jb.kvh * d;
+    split_u4 q[ND][3];
+    win_f4 o[NT];
+    float m = -INFINITY, l = 0.0f;
+    unsigned seen = 0;
+
+    if (tid < WIN_FEW)
+        redo[tid] = 0;
+    /* Slot j of a lane's 8 of step s of the first product: this channel. */
+    auto channel = [&](int s) {
+        return CACHE && ND > 1 ? 64 * (s / 2) + 16 * grp + 8 * (s % 2) : 32 * s + 8 * grp;
+    };
+    {
+        const float *qp = a.Q + row * a.ldq + (long long)h * d;
+
+#pragma unroll
+        for (int s = 0; s < ND; s++) {
+            float u[4], v[4], x[8];
+
+            load4_row(qp, channel(s), d, u);
+            load4_row(qp, channel(s) + 4, d, v);
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                x[j] = u[j];
+                x[4 + j] = v[j];
+            }
+            split8(x, a.scale * WIN_LOG2E * WIN_QUP, q[s][0], q[s][1], q[s][2]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < NT; i++)
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            o[i][e] = 0.0f;
+
+    unsigned kr[2][KL][KW], vr[8][VW], next = ~0u;
+    float kscale[2][4], vscale[2][4];
+    int pg = -1, pg0 = s0;
+
+    /* Pages of 32 steps from i on, two runs of 16 keys a step, one a lane. */
+    auto pages = [&](int i) {
+        const int key = 32 * span.tile(min(i + (lane >> 1), s1 - 1)) + 16 * (lane & 1);
+
+        pg0 = i;
+        pg = key < jb.nk ? seq_page(a.c, jb.b, key) : -1;
+    };
+    auto page_of = [&](int i, int t) { return __builtin_amdgcn_readlane(pg, 2 * (i - pg0) + t); };
+    auto fetch_k = [&](int i) {
+        const int k0 = 32 * span.tile(i);
+
+        if constexpr (CACHE) {
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                const int page = page_of(i, t);
+
+#pragma unroll
+                for (int c = 0; c < KL; c++)
+#pragma unroll
+                    for (int w = 0; w < KW; w++)
+                        kr[t][c][w] = 0;
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    kscale[t][e] = 0.0f;
+                if (page < 0)
+                    continue;
+                const signed char *k = a.c.kc + cache_row(a.c, page, jb.kvh, k0 + 16 * t + col) * pitch;
+
+                load4(a.c.ks + cache_row(a.c, page, jb.kvh, k0 + 16 * t + 4 * grp), kscale[t]);
+#pragma unroll
+                for (int c = 0; c < KL; c++) {
+                    const int at = 64 * c + 4 * KW * grp;
+
+                    if (at < pitch) {
+                        if constexpr (KW == 4) {
+                            const uint4 x = *(const uint4 *)(k + at);
+
+                            kr[t][c][0] = x.x, kr[t][c][1] = x.y, kr[t][c][2] = x.z, kr[t][c][3] = x.w;
+                        }
+                        else {
+                            const uint2 x = *(const uint2 *)(k + at);
+
+                            kr[t][c][0] = x.x, kr[t][c][1] = x.y;
+                        }
+                    }
+                }
+            }
+        }
+        else {
+            const int end = jb.nk - 1 - k0;
+
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                const float *k = K + (k0 + min(16 * t + col, end)) * a.ldk;
+
+#pragma unroll
+                for (int s = 0; s < ND; s++) {
+                    float u[4], v[4];
+
+                    win_load4<CHANNELS>(k, channel(s), d, u);
+                    win_load4<CHANNELS>(k, channel(s) + 4, d, v);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        kr[t][s][j] = __builtin_bit_cast(unsigned, u[j]);
+                        kr[t][s][4 + j] = __builtin_bit_cast(unsigned, v[j]);
+                    }
+                }
+            }
+            if (a.kmask)
+                next = lane <= end && lane < 32 && a.kmask[k0 + lane];
+        }
+    };
+    /* Slot j is key 16 (j / 4) + 4 grp + j % 4. */
+    auto fetch_v = [&](int i) {
+        const int k0 = 32 * span.tile(i);
+
+        if constexpr (CACHE) {
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                const int page = page_of(i, t);
+
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+#pragma unroll
+                    for (int w = 0; w < VW; w++)
+                        vr[4 * t + j][w] = 0;
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    vscale[t][e] = 0.0f;
+                if (page < 0)
+                    continue;
+                const long long at = cache_row(a.c, page, jb.kvh, k0 + 16 * t + 4 * grp);
+                const signed char *v = a.c.vc + at * pitch + VL * col;
+
+                load4(a.c.vs + at, vscale[t]);
+                if (VL * col < pitch) {
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        if constexpr (VL == 8) {
+                            const uint2 x = *(const uint2 *)(v + j * pitch);
+
+                            vr[4 * t + j][0] = x.x, vr[4 * t + j][1] = x.y;
+                        }
+                        else if constexpr (VL == 4)
+                            vr[4 * t + j][0] = *(const unsigned *)(v + j * pitch);
+                        else
+                            vr[4 * t + j][0] = *(const unsigned short *)(v + j * pitch);
+                    }
+                }
+            }
+        }
+        else {
+            const int end = jb.nk - 1 - k0;
+
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const float *v = V + (k0 + min(16 * (j >> 2) + 4 * grp + (j & 3), end)) * a.ldv;
+
+                /* Channels 64 c + 4 col .., or 2 col .. of 32. */
+                if constexpr (ND == 1) {
+                    vr[j][0] = __builtin_bit_cast(unsigned, v[min(2 * col, d - 1)]);
+                    vr[j][1] = __builtin_bit_cast(unsigned, v[min(2 * col + 1, d - 1)]);
+                }
+                else {
+#pragma unroll
+                    for (int c = 0; c < ND / 2; c++) {
+                        float u[4];
+
+                        win_load4<CHANNELS>(v, 64 * c + 4 * col, d, u);
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            vr[j][4 * c + e] = __builtin_bit_cast(unsigned, u[e]);
+                    }
+                }
+            }
+        }
+    };
+    auto code = [](unsigned w, int k) { return (float)((int)(w << (24 - 8 * k)) >> 24); };
+    constexpr int pa6[6] = {0, 2, 1, 0, 1, 0}, pb6[6] = {2, 0, 1, 1, 0, 0};
+
+    if (s0 < s1) {
+        if (CACHE)
+            pages(s0);
+        fetch_k(s0);
+    }
+    for (int i = s0; i < s1; i++) {
+        const int k0 = 32 * span.tile(i);
+        win_f4 s[2];
+        float x[8], mx = -INFINITY;
+        unsigned keep = ~0u;
+
+        fetch_v(i);
+        if constexpr (CACHE) {
+            if (page_of(i, 0) < 0)
+                keep &= 0xffff0000u;
+            if (page_of(i, 1) < 0)
+                keep &= 0x0000ffffu;
+        }
+        else if (a.kmask)
+            keep = (unsigned)__ballot(next);
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                s[t][e] = 0.0f;
+            if constexpr (CACHE) {
+#pragma unroll
+                for (int st = 0; st < ND; st++) {
+                    split_u4 k;
+
+#pragma unroll
+                    for (int w = 0; w < 4; w++) {
+                        const unsigned y = kr[t][ND == 1 ? 0 : st / 2][ND == 1 ? w / 2 : 2 * (st % 2) + w / 2];
+
+                        k[w] = split_pk(code(y, 2 * (w % 2)), code(y, 2 * (w % 2) + 1));
+                    }
+#pragma unroll
+                    for (int w = 2; w >= 0; w--)
+                        s[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                            __builtin_bit_cast(split_b8, k), __builtin_bit_cast(split_b8, q[st][w]), s[t], 0, 0, 0);
+                }
+            }
+            else {
+#pragma unroll
+                for (int st = 0; st < ND; st++) {
+                    split_u4 k[3];
+                    float y[8];
+
+#pragma unroll
+                    for (int j = 0; j < 8; j++)
+                        y[j] = __builtin_bit_cast(float, kr[t][st][j]);
+                    split8(y, 1.0f, k[0], k[1], k[2]);
+#pragma unroll
+                    for (int w = 0; w < 6; w++)
+                        s[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(split_b8, k[pa6[w]]),
+                                                                       __builtin_bit_cast(split_b8, q[st][pb6[w]]), s[t],
+                                                                       0, 0, 0);
+                }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+            x[j] = CACHE ? s[j / 4][j % 4] * kscale[j / 4][j % 4] : s[j / 4][j % 4];
+        unsigned see = ~0u;
+
+        if (keep != ~0u || k0 + 31 > hi0 || !(k0 >= lo1 || k0 + 32 <= a.sinks)) {
+            see = keep & win_sees(a, lo, hi, k0);
+            seen |= see;
+            see >>= 4 * grp;
+            asm volatile("" : "+v"(see));
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                x[j] = see >> (16 * (j / 4) + j % 4) & 1 ? x[j] : -INFINITY;
+        }
+        else
+            seen = 1;
+        if (i + 1 < s1) {
+            if (CACHE && i + 1 - pg0 >= 32)
+                pages(i + 1);
+            fetch_k(i + 1);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+            mx = fmaxf(mx, x[j]);
+        if (__any(mx * (1.0f / WIN_QUP) > m + WIN_FTAU)) {
+            mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+            mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * (1.0f / WIN_QUP);
+            const float mn = mx > m + WIN_FTAU ? mx : m;
+            const float corr = mx > m + WIN_FTAU ? __builtin_amdgcn_exp2f(m - mn) : 1.0f;
+
+            m = mn;
+            l *= corr;
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    o[t][e] *= corr;
+        }
+        const float ref = m == -INFINITY ? 0.0f : m;
+        split_u4 pp[3];
+
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            x[j] = __builtin_amdgcn_exp2f(fmaf(x[j], 1.0f / WIN_QUP, -ref));
+            l += x[j];
+            /* What is not seen counts nothing, whatever its value is. */
+            if (CACHE)
+                x[j] = see >> (16 * (j / 4) + j % 4) & 1 ? x[j] * vscale[j / 4][j % 4] : 0.0f;
+        }
+        split8(x, SPLIT_UP, pp[0], pp[1], pp[2]);
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+            if constexpr (CACHE) {
+                split_u4 v;
+
+#pragma unroll
+                for (int w = 0; w < 4; w++)
+                    v[w] = split_pk(code(vr[2 * w][t / 4], t % 4), code(vr[2 * w + 1][t / 4], t % 4));
+#pragma unroll
+                for (int w = 2; w >= 0; w--)
+                    o[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                        __builtin_bit_cast(split_b8, v), __builtin_bit_cast(split_b8, pp[w]), o[t], 0, 0, 0);
+            }
+            else {
+                split_u4 v[3];
+                float y[8];
+
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    y[j] = __builtin_bit_cast(float, vr[j][t]);
+                    if (keep != ~0u)
+                        y[j] = keep >> (16 * (j / 4) + 4 * grp + j % 4) & 1 ? y[j] : 0.0f;
+                }
+                split8(y, SPLIT_UP, v[0], v[1], v[2]);
+#pragma unroll
+                for (int w = 0; w < 6; w++)
+                    o[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(split_b8, v[pa6[w]]),
+                                                                   __builtin_bit_cast(split_b8, pp[pb6[w]]), o[t], 0, 0,
+                                                                   0);
+            }
+        }
+    }
+    /* A lane has channels of rows 4 grp + e of the tiles. */
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+    if (grp == 0) {
+        ms[wave][col] = m;
+        lsum[wave][col] = l;
+    }
+    float z = l * 0.0f;
+
+#pragma unroll
+    for (int t = 0; t < NT; t++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const int w = 4 * grp + e;
+            const int c = CACHE || ND == 1 ? VL * w + t : 64 * (t / 4) + 4 * w + t % 4;
+
+            os[wave][col][c] = o[t][e];
+            z = fmaf(o[t][e], 0.0f, z);
+        }
+    __syncthreads();
+    if (z != 0.0f || (l == 0.0f && seen))
+        redo[col] = 1;
+    __syncthreads();
+    const int qr = tid >> 4, c0 = VL * (tid & 15), rr = jb.r0 + qr;
+
+    if (rr <= last && !redo[qr]) {
+        const int q1 = rr / g, h1 = jb.kvh * g + rr - q1 * g;
+        const long long row1 = jb.first + q1, out = (row1 * a.nh + h1) * a.splits + split;
+        const float top = fmaxf(fmaxf(ms[0][qr], ms[1][qr]), fmaxf(ms[2][qr], ms[3][qr]));
+        float y[VL] = {}, sum = 0.0f;
+
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+            const float f = ms[w][qr] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ms[w][qr] - top);
+
+            sum = fmaf(f, lsum[w][qr], sum);
+#pragma unroll
+            for (int e = 0; e < VL; e++)
+                y[e] = fmaf(f, os[w][qr][c0 + e], y[e]);
+        }
+        /* Codes are not scaled, float32 values are. */
+        const float down = CACHE ? 1.0f / SPLIT_UP : SPLIT_DOWN;
+        const float inv = parts > 1 ? down : sum > 0.0f ? down / sum : 0.0f;
+        float *to = parts > 1 ? a.part + out * DP : a.O + row1 * a.ldo + (long long)h1 * d;
+
+#pragma unroll
+        for (int e = 0; e < VL; e++)
+            if (c0 + e < d)
+                to[c0 + e] = y[e] * inv;
+        if ((tid & 15) == 0 && a.splits > 1)
+            a.ml[out] = parts > 1 ? make_float2(top, sum) : make_float2(0.0f, WIN_WRITTEN);
+    }
+    for (int e = wave; e < jb.n; e += 4)
+        if (redo[e]) {
+            const int r1 = jb.r0 + e, q1 = r1 / g, h1 = jb.kvh * g + r1 - q1 * g;
+            const win_row wrow = {jb.b, jb.p0 + q1, jb.nk};
+            float y[2], m1, l1;
+
+            win_row_f32<CACHE, WIN_STEP>(a, wrow, jb.first + q1, h1, span, t0, t1, ps[wave], y, m1, l1);
+            win_put(a, jb.first + q1, h1, split, parts, y, m1, l1);
+        }
+}
+
 /* Parts of a row and head joined, by W waves: softmax over all of them from
  * their maxima and sums, then DP / 4 lanes a part, 256 W / DP parts at a time. */
 template <int DP, int W> __global__ void __launch_bounds__(256) win_merge_kernel(const win_args a)
@@ -1174,20 +1620,29 @@ extern "C" size_t ops_attention_cache_work_bytes(int rows, int nh, int d)
  * see at most `keys` each. */
 static int win_splits(const win_args &a, long long blocks, long long keys, int want)
 {
-    long long n = std::min((want + blocks - 1) / blocks, keys / 256);
+    long long n = std::min((want + blocks - 1) / blocks, keys / 128);
 
     n = std::min(n, WIN_PART_ROWS / ((long long)a.rows * a.nh));
     return (int)std::max(1LL, std::min(n, (long long)WIN_MAX_SPLITS));
 }
 
+/* Whether a call goes by tiles of few rows. */
+static bool win_few(const win_args &a, bool cache)
+{
+    const long long rows = (long long)a.rows * (a.nh / a.nhk);
+
+    return rows <= (long long)WIN_FEW * (cache ? a.c.n : 1);
+}
+
 template <bool CACHE> static void win_launch(struct ops *o, win_args &a, long long keys, cl_mem work)
 {
     const int cus = o->ocl->cu_count > 0 ? o->ocl->cu_count : 256;
-    const long long heads = (long long)a.rows * a.nh;
-    const long long rows = heads / a.nhk; /* of a key head */
-    const long long blocks = (CACHE ? rows / WIN_ROWS + a.c.n : (rows + WIN_ROWS - 1) / WIN_ROWS) * a.nhk;
+    const bool few = win_few(a, CACHE);
+    const int tr = few ? WIN_FEW : WIN_ROWS;
+    const long long heads = (long long)a.rows * a.nh, rows = heads / a.nhk; /* of a key head */
+    const long long blocks = (CACHE ? rows / tr + a.c.n : (rows + tr - 1) / tr) * a.nhk;
 
-    a.splits = win_splits(a, blocks, keys, 4 * cus);
+    a.splits = win_splits(a, blocks, keys, few ? 3 * cus : 4 * cus);
     if (a.splits > 1) {
         a.part = fptr(work);
         a.ml = (float2 *)(a.part + heads * a.splits * win_width(a.d));
@@ -1198,14 +1653,25 @@ template <bool CACHE> static void win_launch(struct ops *o, win_args &a, long lo
     prof_scope ps(o->ocl, CACHE ? "attention_cache" : "attention_window");
     const dim3 grid(grid_of(blocks * a.splits, 256, "attention tiles")), block(256);
 
-#define WIN_LAUNCH(ND_)                                                               \
-    do {                                                                              \
-        if (CACHE)                                                                    \
-            hipLaunchKernelGGL(win_cache_kernel<ND_>, grid, block, 0, s, a);          \
-        else if (a.d == 32 * ND_)                                                     \
-            hipLaunchKernelGGL((win_float_kernel<ND_, true>), grid, block, 0, s, a);  \
-        else                                                                          \
-            hipLaunchKernelGGL((win_float_kernel<ND_, false>), grid, block, 0, s, a); \
+#define WIN_FLOAT(ND_, CH_)                                                                    \
+    do {                                                                                       \
+        if (few)                                                                               \
+            hipLaunchKernelGGL((win_few_kernel<ND_, false, CH_>), grid, block, 0, s, a);       \
+        else                                                                                   \
+            hipLaunchKernelGGL((win_float_kernel<ND_, CH_>), grid, block, 0, s, a);            \
+    } while (0)
+#define WIN_LAUNCH(ND_)                                                                     \
+    do {                                                                                    \
+        if (CACHE && few)                                                                       \
+            hipLaunchKernelGGL((win_few_kernel<ND_, true, WIN_ANY>), grid, block, 0, s, a);     \
+        else if (CACHE)                                                                         \
+            hipLaunchKernelGGL(win_cache_kernel<ND_>, grid, block, 0, s, a);                    \
+        else if (a.d == 32 * ND_)                                                               \
+            WIN_FLOAT(ND_, WIN_FULL);                                                           \
+        else if (a.d % 4 == 0)                                                                  \
+            WIN_FLOAT(ND_, WIN_FOUR);                                                           \
+        else                                                                                    \
+            WIN_FLOAT(ND_, WIN_ANY);                                                            \
     } while (0)
     if (a.d <= 32)
         WIN_LAUNCH(1);
@@ -1214,6 +1680,7 @@ template <bool CACHE> static void win_launch(struct ops *o, win_args &a, long lo
     else
         WIN_LAUNCH(4);
 #undef WIN_LAUNCH
+#undef WIN_FLOAT
     launch_check("attention tiles");
     if (a.splits > 1) {
         const bool wide = a.splits > 16;
