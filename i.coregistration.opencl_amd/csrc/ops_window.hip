@@ -361,7 +361,7 @@ static __device__ __forceinline__ void win_finish(const win_args &a, const win_j
 static __device__ __forceinline__ int win_order(int i, int n) { return i & 1 ? i >> 1 : n - 1 - (i >> 1); }
 
 template <int ND>
-__global__ void __launch_bounds__(256, ND == 4 ? 2 : 3) win_cache_kernel(const win_args a)
+__global__ void __launch_bounds__(256, ND == 1 ? 3 : 2) win_cache_kernel(const win_args a)
 {
     constexpr int DP = 32 * ND, CH = DP / 8;
     constexpr int RW = 16 / CH < 1 ? 1 : 16 / CH;  /* K rows in 256 bytes */
@@ -456,57 +456,55 @@ __global__ void __launch_bounds__(256, ND == 4 ? 2 : 3) win_cache_kernel(const w
      * / 4), slot 8 c + j being the key that register 8 (c / 2 % 2) + j of the
      * scores' tile c / 4 holds in lane half c % 2: 16 c / 2 + 8 (j / 4) + 4 (c %
      * 2) + j % 4. Pages hold at least 16 keys, so a unit lies in one. */
-    int kp[NK], vp[NV], sp;
     bool kept = false;
     uint4 kr[NK];
     unsigned vr[NV][8];
     float sr;
+    int pg = -1, pg0 = t0;
 
+    /* Pages of 16 tiles from t on, a run of 16 keys a lane. */
     auto pages = [&](int t) {
-        const int k0 = span.tile(t) * WIN_KT;
+        const int key = span.tile(min(t + (lane >> 2), t1 - 1)) * WIN_KT + 16 * (lane & 3);
 
-#pragma unroll
-        for (int i = 0; i < NK; i++) {
-            const int key = k0 + (tid + 256 * i) / (DP / 16);
-
-            kp[i] = key < jb.nk && tid + 256 * i < KU ? seq_page(a.c, jb.b, key) : -1;
-        }
-#pragma unroll
-        for (int i = 0; i < NV; i++) {
-            const int key = k0 + (tid + 256 * i) / (DP / 4) / 2 * 16;
-
-            vp[i] = key < jb.nk && tid + 256 * i < VU ? seq_page(a.c, jb.b, key) : -1;
-        }
-        sp = -1;
-        if (wave < 2 && k0 + lane < jb.nk)
-            sp = seq_page(a.c, jb.b, k0 + lane);
+        pg0 = t;
+        pg = key < jb.nk ? seq_page(a.c, jb.b, key) : -1;
     };
-    /* Tile t into registers, its pages looked up before. Places of a page
+    /* Tile t into registers. Places of a page
      * behind the last key hold old codes, which are bytes like others. */
     auto fetch = [&](int t) {
         const int k0 = span.tile(t) * WIN_KT;
+        /* The page of the keys' run of 16. */
+        auto page_of = [&](int run) { return __shfl(pg, 4 * (t - pg0) + run, 64); };
 
 #pragma unroll
         for (int i = 0; i < NK; i++) {
-            const int e = tid + 256 * i, key = k0 + e / (DP / 16), at = e % (DP / 16) * 16;
+            const int e = tid + 256 * i, key = e / (DP / 16), at = e % (DP / 16) * 16;
+            const int page = page_of(key >> 4 & 3);
 
             kr[i] = make_uint4(0, 0, 0, 0);
-            if (kp[i] >= 0 && at < pitch)
-                kr[i] = *(const uint4 *)(a.c.kc + cache_row(a.c, kp[i], jb.kvh, key) * pitch + at);
+            if (page >= 0 && at < pitch && (KU % 256 == 0 || e < KU))
+                kr[i] = *(const uint4 *)(a.c.kc + cache_row(a.c, page, jb.kvh, k0 + key) * pitch + at);
         }
 #pragma unroll
         for (int i = 0; i < NV; i++) {
             const int e = tid + 256 * i, c = e / (DP / 4), at = e % (DP / 4) * 4;
-            const signed char *v = a.c.vc + cache_row(a.c, max(vp[i], 0), jb.kvh, k0 + (c >> 1) * 16 + (c & 1) * 4) * pitch + at;
+            const int page = page_of(c >> 1 & 3);
+            const bool in = page >= 0 && at < pitch && (VU % 256 == 0 || e < VU);
+            const signed char *v =
+                a.c.vc + cache_row(a.c, max(page, 0), jb.kvh, k0 + (c >> 1) * 16 + (c & 1) * 4) * pitch + at;
 
 #pragma unroll
             for (int j = 0; j < 8; j++)
-                vr[i][j] = vp[i] >= 0 && at < pitch ? *(const unsigned *)(v + ((j >> 2) * 8 + (j & 3)) * pitch) : 0u;
+                vr[i][j] = in ? *(const unsigned *)(v + ((j >> 2) * 8 + (j & 3)) * pitch) : 0u;
         }
         sr = 0.0f;
-        kept = sp >= 0;
-        if (kept)
-            sr = (wave ? a.c.vs : a.c.ks)[cache_row(a.c, sp, jb.kvh, k0 + lane)];
+        if (wave < 2) {
+            const int page = page_of(lane >> 4);
+
+            kept = page >= 0 && k0 + lane < jb.nk;
+            if (kept)
+                sr = (wave ? a.c.vs : a.c.ks)[cache_row(a.c, page, jb.kvh, k0 + lane)];
+        }
     };
     auto stash = [&](tile_lds &s) {
 #pragma unroll
@@ -575,15 +573,12 @@ __global__ void __launch_bounds__(256, ND == 4 ? 2 : 3) win_cache_kernel(const w
         }
     };
 
-    pages(t0);
-    fetch(t0);
-    if (t0 + 1 < t1)
-        pages(t0 + 1);
-    stash(lds[0]);
-    if (t0 + 1 < t1) {
-        fetch(t0 + 1);
-        if (t0 + 2 < t1)
-            pages(t0 + 2);
+    if (t0 < t1) {
+        pages(t0);
+        fetch(t0);
+        stash(lds[0]);
+        if (t0 + 1 < t1)
+            fetch(t0 + 1);
     }
     __syncthreads();
     for (int t = t0; t < t1; t++) {
@@ -686,9 +681,9 @@ __global__ void __launch_bounds__(256, ND == 4 ? 2 : 3) win_cache_kernel(const w
         if (t + 1 < t1) {
             stash(lds[(t + 1 - t0) & 1]);
             if (t + 2 < t1) {
+                if (t + 2 - pg0 >= 16)
+                    pages(t + 2);
                 fetch(t + 2);
-                if (t + 3 < t1)
-                    pages(t + 3);
             }
         }
         if (some) {
@@ -753,7 +748,7 @@ static __device__ __forceinline__ void win_load4(const float *p, int c, int d, f
 #define WIN_QUP 0x1p32f       /* scale of the queries split into bf16 parts */
 
 template <int ND, int CHANNELS>
-__global__ void __launch_bounds__(256, ND == 4 ? 1 : 3) win_float_kernel(const win_args a)
+__global__ void __launch_bounds__(256, ND == 4 ? 1 : ND == 2 ? 2 : 3) win_float_kernel(const win_args a)
 {
     constexpr int DP = 32 * ND, CH = DP / 8;
     constexpr int RW = 16 / CH < 1 ? 1 : 16 / CH; /* K rows in 256 bytes */
