@@ -240,8 +240,8 @@ typedef unsigned win_u4 __attribute__((ext_vector_type(4)));
 #define WIN_ROWS 128    /* rows (queries times the heads of a key head) of a tile */
 #define WIN_KT 64       /* keys of a tile */
 #define WIN_TAU 4.0f    /* the running maximum is raised when a score passes it by this (base 2) */
-#define WIN_VEXP 10     /* exponent of a tile's largest value scale: weights up to 2^TAU stay below 2^16 */
-#define WIN_VMIN 0.25f  /* smaller ones than this lose bits */
+#define WIN_VEXP 10     /* exponent of the largest value scale: weights up to 2^TAU stay below 2^16 */
+#define WIN_VMIN 0.125f /* smaller ones lose bits: 2^13 below the largest */
 
 /* Codes of 8 bits in f16, exactly: a byte u = code + 128 behind 0x64 is the
  * f16 value 1024 + u. */
@@ -251,6 +251,9 @@ static __device__ __forceinline__ unsigned win_codes(unsigned bytes)
 
     return __builtin_bit_cast(unsigned, x + off);
 }
+
+/* The power of two of biased exponent e, 1 .. 254. */
+static __device__ __forceinline__ float win_power(int e) { return __builtin_bit_cast(float, (unsigned)e << 23); }
 
 /* Two floats as the sum of two f16 values each, 11 bits and 11 more. */
 static __device__ __forceinline__ void win_split(float a, float b, unsigned &hi, unsigned &lo)
@@ -372,8 +375,7 @@ __global__ void __launch_bounds__(256, ND == 1 ? 3 : 2) win_cache_kernel(const w
         win_u4 k[KSZ], v[VSZ];
         float ks[WIN_KT], vs[WIN_KT];
         unsigned long long keep;
-        float vf;
-        int wild;
+        int vexp, wild;
     };
     __shared__ tile_lds lds[2];
     __shared__ float ps[4][64];
@@ -431,9 +433,9 @@ __global__ void __launch_bounds__(256, ND == 1 ? 3 : 2) win_cache_kernel(const w
         }
         mag = max(mag, (unsigned)__shfl_xor((int)mag, 32, 64));
         const int e = min(max((int)(mag >> 23), 15), 254);
-        const float up = __builtin_bit_cast(float, (unsigned)(268 - e) << 23);
+        const float up = win_power(268 - e);
 
-        qf = __builtin_bit_cast(float, (unsigned)(e - 14) << 23);
+        qf = win_power(e - 14);
 #pragma unroll
         for (int st = 0; st < 2 * ND; st++)
 #pragma unroll
@@ -460,7 +462,7 @@ __global__ void __launch_bounds__(256, ND == 1 ? 3 : 2) win_cache_kernel(const w
     uint4 kr[NK];
     unsigned vr[NV][8];
     float sr;
-    int pg = -1, pg0 = t0;
+    int pg = -1, pg0 = t0, vexp = 12;
 
     /* Pages of 16 tiles from t on, a run of 16 keys a lane. */
     auto pages = [&](int t) {
@@ -469,41 +471,42 @@ __global__ void __launch_bounds__(256, ND == 1 ? 3 : 2) win_cache_kernel(const w
         pg0 = t;
         pg = key < jb.nk ? seq_page(a.c, jb.b, key) : -1;
     };
-    /* Tile t into registers. Places of a page
-     * behind the last key hold old codes, which are bytes like others. */
+    /* The page of run `run` of tile t; `same`: of all lanes alike. */
+    auto page_of = [&](int t, int run, bool same) {
+        const int at = 4 * (t - pg0) + run;
+
+        return same ? __builtin_amdgcn_readlane(pg, __builtin_amdgcn_readfirstlane(at)) : __shfl(pg, at, 64);
+    };
+    /* Tile t into registers. Where there is no page, and behind a row's codes,
+     * something else is read that counts nothing: no lane has a branch. */
     auto fetch = [&](int t) {
         const int k0 = span.tile(t) * WIN_KT;
-        /* The page of the keys' run of 16. */
-        auto page_of = [&](int run) { return __shfl(pg, 4 * (t - pg0) + run, 64); };
 
 #pragma unroll
         for (int i = 0; i < NK; i++) {
-            const int e = tid + 256 * i, key = e / (DP / 16), at = e % (DP / 16) * 16;
-            const int page = page_of(key >> 4 & 3);
+            const int e = min(tid + 256 * i, KU - 1), key = e / (DP / 16), at = e % (DP / 16) * 16;
+            const int page = max(page_of(t, key >> 4, ND > 1), 0);
 
-            kr[i] = make_uint4(0, 0, 0, 0);
-            if (page >= 0 && at < pitch && (KU % 256 == 0 || e < KU))
-                kr[i] = *(const uint4 *)(a.c.kc + cache_row(a.c, page, jb.kvh, k0 + key) * pitch + at);
+            kr[i] = *(const uint4 *)(a.c.kc + cache_row(a.c, page, jb.kvh, k0 + key) * pitch + min(at, pitch - 16));
         }
 #pragma unroll
         for (int i = 0; i < NV; i++) {
-            const int e = tid + 256 * i, c = e / (DP / 4), at = e % (DP / 4) * 4;
-            const int page = page_of(c >> 1 & 3);
-            const bool in = page >= 0 && at < pitch && (VU % 256 == 0 || e < VU);
-            const signed char *v =
-                a.c.vc + cache_row(a.c, max(page, 0), jb.kvh, k0 + (c >> 1) * 16 + (c & 1) * 4) * pitch + at;
+            const int e = min(tid + 256 * i, VU - 1), c = e / (DP / 4), at = e % (DP / 4) * 4;
+            const int page = max(page_of(t, c >> 1, ND == 4), 0);
+            const signed char *v = a.c.vc +
+                                   cache_row(a.c, page, jb.kvh, k0 + (c >> 1) * 16 + (c & 1) * 4) * pitch +
+                                   min(at, pitch - 4);
 
 #pragma unroll
             for (int j = 0; j < 8; j++)
-                vr[i][j] = in ? *(const unsigned *)(v + ((j >> 2) * 8 + (j & 3)) * pitch) : 0u;
+                vr[i][j] = *(const unsigned *)(v + ((j >> 2) * 8 + (j & 3)) * pitch);
         }
-        sr = 0.0f;
         if (wave < 2) {
-            const int page = page_of(lane >> 4);
+            const int page = page_of(t, lane >> 4, false);
 
             kept = page >= 0 && k0 + lane < jb.nk;
-            if (kept)
-                sr = (wave ? a.c.vs : a.c.ks)[cache_row(a.c, page, jb.kvh, k0 + lane)];
+            sr = (wave ? a.c.vs : a.c.ks)[cache_row(a.c, max(page, 0), jb.kvh, k0 + lane)];
+            sr = kept ? sr : 0.0f;
         }
     };
     auto stash = [&](tile_lds &s) {
@@ -554,20 +557,19 @@ __global__ void __launch_bounds__(256, ND == 1 ? 3 : 2) win_cache_kernel(const w
                 s.keep = keep;
         }
         else if (wave == 1) {
-            /* Value scales times a power of two that brings the largest to
-             * 2^WIN_VEXP; a scale of NaN, and one far below the largest, is for
-             * the float32 path. */
+            /* Value scales times a power of two that brings the largest so
+             * far to 2^WIN_VEXP; a scale of NaN, and one far below the largest,
+             * is for the float32 path. */
             const bool bad = sr != sr;
-            const unsigned top = wave_umax(bad ? 0u : q8_mag(sr)) >> 23;
-            const int e = min((int)top, 253 + WIN_VEXP);
-            const float up = __builtin_bit_cast(float, (unsigned)min(254 + WIN_VEXP - e, 253) << 23);
-            const float x = bad ? 0.0f : sr * up;
+
+            vexp = max(vexp, min((int)(wave_umax(bad ? 0u : q8_mag(sr)) >> 23), 253));
+            const float x = bad ? 0.0f : sr * win_power(254 + WIN_VEXP - vexp);
 
             s.vs[lane] = x;
             const int w = __any(bad || (x != 0.0f && x < WIN_VMIN) || !(x < 0x1p12f));
 
             if (lane == 0) {
-                s.vf = 1.0f / up;
+                s.vexp = vexp;
                 s.wild = w;
             }
         }
@@ -581,48 +583,58 @@ __global__ void __launch_bounds__(256, ND == 1 ? 3 : 2) win_cache_kernel(const w
             fetch(t0 + 1);
     }
     __syncthreads();
+    int oexp = lds[0].vexp; /* o counts in 2^(oexp - 127 - WIN_VEXP) */
+
     for (int t = t0; t < t1; t++) {
         const tile_lds &s = lds[(t - t0) & 1];
-        const int k0 = span.tile(t) * WIN_KT;
-        /* Some row of the wave sees some key; all see all. */
-        const bool some = live && k0 <= hi1 && (k0 + WIN_KT > lo0 || k0 < a.sinks);
-        const bool all = s.keep == ~0ull && k0 + WIN_KT - 1 <= hi0 && (k0 >= lo1 || k0 + WIN_KT <= a.sinks);
-        win_u4 ph[4], pl[4];
+        const int base = span.tile(t) * WIN_KT;
 
         wild = wild || s.wild;
-        if (some) {
-            win_f16x sc[2];
-            float x[2][16], mx = -INFINITY, sum = 0.0f;
+        if (s.vexp != oexp) {
+            const float down = win_power(max(127 + oexp - s.vexp, 1));
+
+            oexp = s.vexp;
+#pragma unroll
+            for (int tt = 0; tt < ND; tt++)
+#pragma unroll
+                for (int e = 0; e < 16; e++)
+                    o[tt][e] *= down;
+        }
+#pragma unroll
+        for (int part = 0; part < 2; part++) {
+            const int k0 = base + 32 * part;
+            /* Some row of the wave sees some key; all see all. */
+            const bool some = live && k0 <= hi1 && (k0 + 32 > lo0 || k0 < a.sinks);
+            const unsigned keep = (unsigned)(s.keep >> 32 * part);
+
+            if (some) {
+                win_f16x sc;
+                win_u4 ph[2], pl[2];
+                float x[16], mx = -INFINITY, sum = 0.0f;
 
 #pragma unroll
-            for (int e = 0; e < 16; e++)
-                sc[0][e] = sc[1][e] = 0.0f;
+                for (int e = 0; e < 16; e++)
+                    sc[e] = 0.0f;
 #pragma unroll
-            for (int st = 0; st < 2 * ND; st++)
-#pragma unroll
-                for (int tt = 0; tt < 2; tt++) {
-                    const int key = 32 * tt + col;
+                for (int st = 0; st < 2 * ND; st++) {
+                    const int key = 32 * part + col;
                     const win_h8 k = __builtin_bit_cast(win_h8, s.k[key * CH + ((2 * st + half) ^ (key / RW % CH))]);
 
-                    sc[tt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, __builtin_bit_cast(win_h8, ql[st]), sc[tt], 0, 0, 0);
-                    sc[tt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, __builtin_bit_cast(win_h8, qh[st]), sc[tt], 0, 0, 0);
+                    sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, __builtin_bit_cast(win_h8, ql[st]), sc, 0, 0, 0);
+                    sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, __builtin_bit_cast(win_h8, qh[st]), sc, 0, 0, 0);
                 }
-            /* Register e of tile tt is key 32 tt + 8 (e / 4) + 4 half + e % 4. */
-#pragma unroll
-            for (int tt = 0; tt < 2; tt++)
+                /* Register e is key 8 (e / 4) + 4 half + e % 4. */
 #pragma unroll
                 for (int e = 0; e < 16; e += 4) {
-                    const float4 k = *(const float4 *)&s.ks[32 * tt + 2 * e + 4 * half];
+                    const float4 k = *(const float4 *)&s.ks[32 * part + 2 * e + 4 * half];
 
-                    x[tt][e] = sc[tt][e] * k.x;
-                    x[tt][e + 1] = sc[tt][e + 1] * k.y;
-                    x[tt][e + 2] = sc[tt][e + 2] * k.z;
-                    x[tt][e + 3] = sc[tt][e + 3] * k.w;
+                    x[e] = sc[e] * k.x;
+                    x[e + 1] = sc[e + 1] * k.y;
+                    x[e + 2] = sc[e + 2] * k.z;
+                    x[e + 3] = sc[e + 3] * k.w;
                 }
-            if (!all) {
-#pragma unroll
-                for (int tt = 0; tt < 2; tt++) {
-                    unsigned see = (unsigned)(s.keep >> 32 * tt) & win_sees(a, lo, hi, k0 + 32 * tt);
+                if (keep != ~0u || k0 + 31 > hi0 || !(k0 >= lo1 || k0 + 32 <= a.sinks)) {
+                    unsigned see = keep & win_sees(a, lo, hi, k0);
 
                     see >>= 4 * half;
                     /* Tested here: as conditions kept they fill the scalar
@@ -630,87 +642,72 @@ __global__ void __launch_bounds__(256, ND == 1 ? 3 : 2) win_cache_kernel(const w
                     asm volatile("" : "+v"(see));
 #pragma unroll
                     for (int e = 0; e < 16; e++)
-                        x[tt][e] = see >> (8 * (e >> 2) + (e & 3)) & 1 ? x[tt][e] : -INFINITY;
+                        x[e] = see >> (8 * (e >> 2) + (e & 3)) & 1 ? x[e] : -INFINITY;
                 }
-            }
-#pragma unroll
-            for (int tt = 0; tt < 2; tt++)
 #pragma unroll
                 for (int e = 0; e < 16; e++)
-                    mx = fmaxf(mx, x[tt][e]);
-            mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * qf;
-            const bool need = mx > m + WIN_TAU;
+                    mx = fmaxf(mx, x[e]);
+                mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * qf;
+                const bool need = mx > m + WIN_TAU;
 
-            if (__any(need)) {
-                const float mn = need ? mx : m;
-                const float corr = need ? __builtin_amdgcn_exp2f(m - mn) : 1.0f;
+                if (__any(need)) {
+                    const float mn = need ? mx : m;
+                    const float corr = need ? __builtin_amdgcn_exp2f(m - mn) : 1.0f;
 
-                m = mn;
-                l *= corr;
+                    m = mn;
+                    l *= corr;
 #pragma unroll
-                for (int tt = 0; tt < ND; tt++)
+                    for (int tt = 0; tt < ND; tt++)
 #pragma unroll
-                    for (int e = 0; e < 16; e++)
-                        o[tt][e] *= corr;
-            }
-            const float ref = m == -INFINITY ? 0.0f : m;
+                        for (int e = 0; e < 16; e++)
+                            o[tt][e] *= corr;
+                }
+                const float ref = m == -INFINITY ? 0.0f : m;
 
-#pragma unroll
-            for (int tt = 0; tt < 2; tt++)
 #pragma unroll
                 for (int e = 0; e < 16; e += 4) {
-                    const float4 v = *(const float4 *)&s.vs[32 * tt + 2 * e + 4 * half];
+                    const float4 v = *(const float4 *)&s.vs[32 * part + 2 * e + 4 * half];
                     unsigned u0, u1, v0, v1;
 
 #pragma unroll
                     for (int j = 0; j < 4; j++) {
-                        x[tt][e + j] = __builtin_amdgcn_exp2f(fmaf(x[tt][e + j], qf, -ref));
-                        sum += x[tt][e + j];
+                        x[e + j] = __builtin_amdgcn_exp2f(fmaf(x[e + j], qf, -ref));
+                        sum += x[e + j];
                     }
-                    win_split(x[tt][e] * v.x, x[tt][e + 1] * v.y, u0, v0);
-                    win_split(x[tt][e + 2] * v.z, x[tt][e + 3] * v.w, u1, v1);
-                    ph[2 * tt + e / 8][e / 2 % 4] = u0;
-                    ph[2 * tt + e / 8][e / 2 % 4 + 1] = u1;
-                    pl[2 * tt + e / 8][e / 2 % 4] = v0;
-                    pl[2 * tt + e / 8][e / 2 % 4 + 1] = v1;
+                    win_split(x[e] * v.x, x[e + 1] * v.y, u0, v0);
+                    win_split(x[e + 2] * v.z, x[e + 3] * v.w, u1, v1);
+                    ph[e / 8][e / 2 % 4] = u0;
+                    ph[e / 8][e / 2 % 4 + 1] = u1;
+                    pl[e / 8][e / 2 % 4] = v0;
+                    pl[e / 8][e / 2 % 4 + 1] = v1;
                 }
-            l += sum + __shfl_xor(sum, 32, 64);
-        }
-        /* The next tile into the other buffer, which was last read a tile ago,
-         * before the barrier; then its successor's loads. */
-        if (t + 1 < t1) {
-            stash(lds[(t + 1 - t0) & 1]);
-            if (t + 2 < t1) {
-                if (t + 2 - pg0 >= 16)
-                    pages(t + 2);
-                fetch(t + 2);
+                l += sum;
+#pragma unroll
+                for (int u = 0; u < 2; u++)
+#pragma unroll
+                    for (int tt = 0; tt < ND; tt++) {
+                        const int dd = 32 * tt + col;
+                        const win_h8 v = __builtin_bit_cast(
+                            win_h8, s.v[dd * 8 + ((4 * part + 2 * u + half) ^ (dd >> 1 & 7))]);
+
+                        o[tt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, __builtin_bit_cast(win_h8, pl[u]), o[tt], 0, 0, 0);
+                        o[tt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, __builtin_bit_cast(win_h8, ph[u]), o[tt], 0, 0, 0);
+                    }
             }
-        }
-        if (some) {
-            const float vf = s.vf;
-
-#pragma unroll
-            for (int tt = 0; tt < ND; tt++) {
-                const int dd = 32 * tt + col;
-                win_f16x part;
-
-#pragma unroll
-                for (int e = 0; e < 16; e++)
-                    part[e] = 0.0f;
-#pragma unroll
-                for (int u = 0; u < 4; u++) {
-                    const win_h8 v = __builtin_bit_cast(win_h8, s.v[dd * 8 + ((2 * u + half) ^ (dd >> 1 & 7))]);
-
-                    part = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, __builtin_bit_cast(win_h8, pl[u]), part, 0, 0, 0);
-                    part = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, __builtin_bit_cast(win_h8, ph[u]), part, 0, 0, 0);
+            /* The next tile into the other buffer, which was last read a tile
+             * ago, before the barrier; then its successor's loads. */
+            if (part == 0 && t + 1 < t1) {
+                stash(lds[(t + 1 - t0) & 1]);
+                if (t + 2 < t1) {
+                    if (t + 2 - pg0 >= 16)
+                        pages(t + 2);
+                    fetch(t + 2);
                 }
-#pragma unroll
-                for (int e = 0; e < 16; e++)
-                    o[tt][e] = fmaf(part[e], vf, o[tt][e]);
             }
         }
         __syncthreads();
     }
+    l += __shfl_xor(l, 32, 64);
     float z = l * 0.0f;
 
 #pragma unroll
@@ -718,7 +715,8 @@ __global__ void __launch_bounds__(256, ND == 1 ? 3 : 2) win_cache_kernel(const w
 #pragma unroll
         for (int e = 0; e < 16; e++)
             z = fmaf(o[tt][e], 0.0f, z);
-    win_finish<ND, true, WIN_KT>(a, jb, span, t0, t1, parts, split, o, 1.0f, m, l, wild || z != 0.0f, ps[wave], d);
+    win_finish<ND, true, WIN_KT>(a, jb, span, t0, t1, parts, split, o, win_power(max(oexp - WIN_VEXP, 1)), m, l, wild || z != 0.0f,
+                                 ps[wave], d);
 }
 
 /* Channels of a head: any number (a load a float), a multiple of 4, or all
@@ -1785,6 +1783,8 @@ extern "C" void ops_attention_cache(struct ops *o, const struct ops_cache *c, co
     win_args a = {};
 
     a.c = cache_check(c, s, rows, op);
+    if (a.c.pages == 0)
+        a.c.ldt = 0; /* no keys */
     if (nh < 1 || nh % c->nhk || sinks < 0)
         icoreg_fatal("%s: invalid sizes nh=%d nhk=%d sinks=%d", op, nh, c->nhk, sinks);
     if (rows == 0 || s->n == 0)
