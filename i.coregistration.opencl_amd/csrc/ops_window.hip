@@ -18,7 +18,6 @@
 #include <algorithm>
 
 #include "common.h"
-#include "gemm_dev.h"
 #include "load4.h"
 #include "ops.h"
 #include "reduce.h"
@@ -359,9 +358,19 @@ static __device__ __forceinline__ void win_finish(const win_args &a, const win_j
     }
 }
 
-/* A tile's place among a key head's: from both ends in turn, so that a stretch
- * of them has short rows and long ones alike where later rows see more. */
-static __device__ __forceinline__ int win_order(int i, int n) { return i & 1 ? i >> 1 : n - 1 - (i >> 1); }
+/* A block's split, key head and tile of `tiles`: tiles from the last one down,
+ * which where later rows see more are the longest, so that the short ones fill
+ * the CUs' gaps at the end; key heads within, so that an XCD (blocks are dealt
+ * to the 8 in turn) has few of them in its L2 where their number has a factor
+ * in common with 8. */
+static __device__ __forceinline__ int win_unit(const win_args &a, int tiles, int &split, int &kvh)
+{
+    const int per = a.nhk * a.splits, u = blockIdx.x % per;
+
+    split = u / a.nhk;
+    kvh = u % a.nhk;
+    return tiles - 1 - blockIdx.x / per;
+}
 
 template <int ND>
 __global__ void __launch_bounds__(256, ND == 1 ? 3 : 2) win_cache_kernel(const win_args a)
@@ -383,8 +392,9 @@ __global__ void __launch_bounds__(256, ND == 1 ? 3 : 2) win_cache_kernel(const w
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = a.nh / a.nhk, d = a.d, pitch = a.c.pitch;
     const int tiles = (int)((long long)a.rows * g / WIN_ROWS) + a.c.n;
-    const int unit = xcd_tile(blockIdx.x, gridDim.x), split = unit % a.splits;
-    const win_job jb = win_job_of<true, WIN_ROWS>(a, win_order(unit / a.splits % tiles, tiles), unit / a.splits / tiles);
+    int split, kvh;
+    const int tile = win_unit(a, tiles, split, kvh);
+    const win_job jb = win_job_of<true, WIN_ROWS>(a, tile, kvh);
 
     if (jb.n <= 0)
         return;
@@ -758,8 +768,9 @@ __global__ void __launch_bounds__(256, ND == 4 ? 1 : ND == 2 ? 2 : 3) win_float_
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = a.nh / a.nhk, d = CHANNELS == WIN_FULL ? DP : a.d;
     const int tiles = (int)(((long long)a.rows * g + WIN_ROWS - 1) / WIN_ROWS);
-    const int unit = xcd_tile(blockIdx.x, gridDim.x), split = unit % a.splits;
-    const win_job jb = win_job_of<false, WIN_ROWS>(a, win_order(unit / a.splits % tiles, tiles), unit / a.splits / tiles);
+    int split, kvh;
+    const int tile = win_unit(a, tiles, split, kvh);
+    const win_job jb = win_job_of<false, WIN_ROWS>(a, tile, kvh);
     const int last = jb.r0 + jb.n - 1;
     const win_tiles span = win_span<WIN_FKT>(a, jb.p0 + jb.r0 / g, jb.p0 + last / g, jb.nk);
     const int parts = win_parts(span.n, a.splits);
@@ -1079,8 +1090,9 @@ __global__ void __launch_bounds__(256, CACHE && ND == 4 ? 3 : 2) win_few_kernel(
     const int g = a.nh / a.nhk, d = CHANNELS == WIN_FULL ? DP : a.d, pitch = a.c.pitch;
     const int tiles = CACHE ? (int)((long long)a.rows * g / WIN_FEW) + a.c.n
                             : (int)(((long long)a.rows * g + WIN_FEW - 1) / WIN_FEW);
-    const int unit = xcd_tile(blockIdx.x, gridDim.x), split = unit % a.splits;
-    const win_job jb = win_job_of<CACHE, WIN_FEW>(a, unit / a.splits % tiles, unit / a.splits / tiles);
+    int split, kvh;
+    const int tile = win_unit(a, tiles, split, kvh);
+    const win_job jb = win_job_of<CACHE, WIN_FEW>(a, tile, kvh);
 
     if (jb.n <= 0)
         return;
