@@ -16,6 +16,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "common.h"
 #include "load4.h"
@@ -238,6 +239,7 @@ typedef unsigned win_u4 __attribute__((ext_vector_type(4)));
 
 #define WIN_ROWS 128    /* rows (queries times the heads of a key head) of a tile */
 #define WIN_KT 64       /* keys of a tile */
+#define WIN_AHEAD 2     /* operands on their way from LDS */
 #define WIN_TAU 4.0f    /* the running maximum is raised when a score passes it by this (base 2) */
 #define WIN_VEXP 10     /* exponent of the largest value scale: weights up to 2^TAU stay below 2^16 */
 #define WIN_VMIN 0.125f /* smaller ones lose bits: 2^13 below the largest */
@@ -372,13 +374,15 @@ static __device__ __forceinline__ int win_unit(const win_args &a, int tiles, int
     return tiles - 1 - blockIdx.x / per;
 }
 
+#define WIN_CROWS 256 /* rows of a tile over a cache, 8 waves of 32 */
+
 template <int ND>
-__global__ void __launch_bounds__(256, ND == 1 ? 3 : 2) win_cache_kernel(const win_args a)
+__global__ void __launch_bounds__(512, 2) win_cache_kernel(const win_args a)
 {
     constexpr int DP = 32 * ND, CH = DP / 8;
     constexpr int RW = 16 / CH < 1 ? 1 : 16 / CH;  /* K rows in 256 bytes */
     constexpr int KU = 4 * DP, NK = (KU + 255) / 256; /* 16-byte units of codes of a tile of K */
-    constexpr int VU = 2 * DP, NV = (VU + 255) / 256; /* units of 8 keys x 4 channels of V */
+    constexpr int VU = 2 * DP;                        /* units of 8 keys x 4 channels of V */
     constexpr int KSZ = WIN_KT * CH, VSZ = DP * 8;    /* 16-byte chunks in LDS */
     struct tile_lds {
         win_u4 k[KSZ], v[VSZ];
@@ -387,14 +391,14 @@ __global__ void __launch_bounds__(256, ND == 1 ? 3 : 2) win_cache_kernel(const w
         int vexp, wild;
     };
     __shared__ tile_lds lds[2];
-    __shared__ float ps[4][64];
+    __shared__ float ps[8][64];
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, col = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = a.nh / a.nhk, d = a.d, pitch = a.c.pitch;
-    const int tiles = (int)((long long)a.rows * g / WIN_ROWS) + a.c.n;
+    const int tiles = (int)((long long)a.rows * g / WIN_CROWS) + a.c.n;
     int split, kvh;
     const int tile = win_unit(a, tiles, split, kvh);
-    const win_job jb = win_job_of<true, WIN_ROWS>(a, tile, kvh);
+    const win_job jb = win_job_of<true, WIN_CROWS>(a, tile, kvh);
 
     if (jb.n <= 0)
         return;
@@ -463,14 +467,16 @@ __global__ void __launch_bounds__(256, ND == 1 ? 3 : 2) win_cache_kernel(const w
         for (int e = 0; e < 16; e++)
             o[tt][e] = 0.0f;
 
-    /* Units of this thread: K unit e is key e / (DP / 16), bytes 16 (e % (DP /
-     * 16)) ..; V unit e channels 4 (e % (DP / 4)) .., slots 8 c .. 8 c + 7, c = e / (DP
-     * / 4), slot 8 c + j being the key that register 8 (c / 2 % 2) + j of the
-     * scores' tile c / 4 holds in lane half c % 2: 16 c / 2 + 8 (j / 4) + 4 (c %
-     * 2) + j % 4. Pages hold at least 16 keys, so a unit lies in one. */
+    /* Waves 0 .. 3 stage values, 4 .. 7 keys: unit e of K is key e / (DP / 16),
+     * bytes 16 (e % (DP / 16)) ..; of V channels 4 (e % (DP / 4)) .., slots 8 c ..
+     * 8 c + 7, c = e / (DP / 4), slot 8 c + j being the key that register 8 (c /
+     * 2 % 2) + j of the scores of keys 32 (c / 4) .. holds in lane half c % 2: 16
+     * (c / 2) + 8 (j / 4) + 4 (c % 2) + j % 4. Pages hold at least 16 keys, so
+     * a unit lies in one. */
+    const bool values = wave < 4;
+    const int ht = tid & 255;
     bool kept = false;
-    uint4 kr[NK];
-    unsigned vr[NV][8];
+    uint4 kr[2]; /* NK of them, or 8 words of V */
     float sr;
     int pg = -1, pg0 = t0, vexp = 12;
 
@@ -481,48 +487,74 @@ __global__ void __launch_bounds__(256, ND == 1 ? 3 : 2) win_cache_kernel(const w
         pg0 = t;
         pg = key < jb.nk ? seq_page(a.c, jb.b, key) : -1;
     };
-    /* The page of run `run` of tile t; `same`: of all lanes alike. */
-    auto page_of = [&](int t, int run, bool same) {
-        const int at = 4 * (t - pg0) + run;
-
-        return same ? __builtin_amdgcn_readlane(pg, __builtin_amdgcn_readfirstlane(at)) : __shfl(pg, at, 64);
-    };
+    /* The page of run `run` of tile t. */
+    auto page_of = [&](int t, int run) { return __shfl(pg, 4 * (t - pg0) + run, 64); };
     /* Tile t into registers. Where there is no page, and behind a row's codes,
-     * something else is read that counts nothing: no lane has a branch. */
+     * something else is read that counts nothing: no lane has a branch. The
+     * run of 16 keys is the same for a wave's lanes where SAME says so: the
+     * address is a scalar one and an offset that never changes. */
+    auto row_of = [&](auto same, int t, int run, int k0) {
+        if constexpr (same) {
+            const int r = __builtin_amdgcn_readfirstlane(run);
+            const int page = max(__builtin_amdgcn_readlane(pg, 4 * (t - pg0) + r), 0);
+
+            return cache_row(a.c, page, jb.kvh, k0 + 16 * r) * pitch;
+        }
+        else
+            return cache_row(a.c, max(page_of(t, run), 0), jb.kvh, k0 + 16 * run) * pitch;
+    };
     auto fetch = [&](int t) {
         const int k0 = span.tile(t) * WIN_KT;
 
-#pragma unroll
-        for (int i = 0; i < NK; i++) {
-            const int e = min(tid + 256 * i, KU - 1), key = e / (DP / 16), at = e % (DP / 16) * 16;
-            const int page = max(page_of(t, key >> 4, ND > 1), 0);
-
-            kr[i] = *(const uint4 *)(a.c.kc + cache_row(a.c, page, jb.kvh, k0 + key) * pitch + min(at, pitch - 16));
-        }
-#pragma unroll
-        for (int i = 0; i < NV; i++) {
-            const int e = min(tid + 256 * i, VU - 1), c = e / (DP / 4), at = e % (DP / 4) * 4;
-            const int page = max(page_of(t, c >> 1, ND == 4), 0);
-            const signed char *v = a.c.vc +
-                                   cache_row(a.c, page, jb.kvh, k0 + (c >> 1) * 16 + (c & 1) * 4) * pitch +
-                                   min(at, pitch - 4);
+        if (values) {
+            const int e = min(ht, VU - 1), c = e / (DP / 4), at = e % (DP / 4) * 4;
+            const signed char *v = a.c.vc + row_of(std::bool_constant<ND == 4>{}, t, c >> 1, k0);
+            const unsigned off = (c & 1) * 4 * pitch + min(at, pitch - 4);
+            unsigned *to = (unsigned *)kr;
 
 #pragma unroll
             for (int j = 0; j < 8; j++)
-                vr[i][j] = *(const unsigned *)(v + ((j >> 2) * 8 + (j & 3)) * pitch);
+                to[j] = *(const unsigned *)(v + ((j >> 2) * 8 + (j & 3)) * pitch + off);
         }
-        if (wave < 2) {
-            const int page = page_of(t, lane >> 4, false);
+        else {
+#pragma unroll
+            for (int i = 0; i < NK; i++) {
+                const int e = min(ht + 256 * i, KU - 1), key = e / (DP / 16), at = e % (DP / 16) * 16;
+                const signed char *k = a.c.kc + row_of(std::bool_constant<(ND > 1)>{}, t, key >> 4, k0);
 
-            kept = page >= 0 && k0 + lane < jb.nk;
-            sr = (wave ? a.c.vs : a.c.ks)[cache_row(a.c, max(page, 0), jb.kvh, k0 + lane)];
-            sr = kept ? sr : 0.0f;
+                kr[i] = *(const uint4 *)(k + (unsigned)((key & 15) * pitch + min(at, pitch - 16)));
+            }
+            if (wave < 6) {
+                const int page = page_of(t, lane >> 4);
+
+                kept = page >= 0 && k0 + lane < jb.nk;
+                sr = (wave == 4 ? a.c.ks : a.c.vs)[cache_row(a.c, max(page, 0), jb.kvh, k0 + lane)];
+                sr = kept ? sr : 0.0f;
+            }
         }
     };
     auto stash = [&](tile_lds &s) {
+        if (values) {
+            const int c = ht / (DP / 4), ch = ht % (DP / 4) * 4;
+            const unsigned *w = (const unsigned *)kr;
+
+            if (VU < 256 && ht >= VU)
+                return;
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const unsigned sel = 0x0c000c00u | (4u + k) << 16 | (unsigned)k;
+                win_u4 x;
+
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    x[j] = win_codes(__builtin_amdgcn_perm(w[2 * j + 1], w[2 * j], sel) ^ 0x64806480u);
+                s.v[(ch + k) * 8 + (c ^ ((ch + k) >> 1 & 7))] = x;
+            }
+            return;
+        }
 #pragma unroll
         for (int i = 0; i < NK; i++) {
-            const int e = tid + 256 * i, key = e / (DP / 16), ch = e % (DP / 16) * 2;
+            const int e = ht + 256 * i, key = e / (DP / 16), ch = e % (DP / 16) * 2;
 
             if (KU % 256 == 0 || e < KU) {
                 const unsigned w[4] = {kr[i].x ^ 0x80808080u, kr[i].y ^ 0x80808080u, kr[i].z ^ 0x80808080u,
@@ -540,33 +572,14 @@ __global__ void __launch_bounds__(256, ND == 1 ? 3 : 2) win_cache_kernel(const w
                 s.k[key * CH + ((ch + 1) ^ (key / RW % CH))] = v;
             }
         }
-#pragma unroll
-        for (int i = 0; i < NV; i++) {
-            const int e = tid + 256 * i, c = e / (DP / 4), ch = e % (DP / 4) * 4;
-
-            if (VU % 256 == 0 || e < VU) {
-#pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    const unsigned sel = 0x0c000c00u | (4u + k) << 16 | (unsigned)k;
-                    win_u4 x;
-
-#pragma unroll
-                    for (int j = 0; j < 4; j++)
-                        x[j] = win_codes(__builtin_amdgcn_perm(vr[i][2 * j + 1] ^ 0x80808080u,
-                                                               vr[i][2 * j] ^ 0x80808080u, sel) |
-                                         0x64006400u);
-                    s.v[(ch + k) * 8 + (c ^ ((ch + k) >> 1 & 7))] = x;
-                }
-            }
-        }
-        if (wave == 0) {
+        if (wave == 4) {
             const unsigned long long keep = __ballot(kept);
 
             s.ks[lane] = sr;
             if (lane == 0)
                 s.keep = keep;
         }
-        else if (wave == 1) {
+        else if (wave == 5) {
             /* Value scales times a power of two that brings the largest so
              * far to 2^WIN_VEXP; a scale of NaN, and one far below the largest,
              * is for the float32 path. */
@@ -625,13 +638,26 @@ __global__ void __launch_bounds__(256, ND == 1 ? 3 : 2) win_cache_kernel(const w
 #pragma unroll
                 for (int e = 0; e < 16; e++)
                     sc[e] = 0.0f;
+                /* Operands are read WIN_AHEAD steps before their products. */
+                win_h8 kf[WIN_AHEAD];
+                auto key = [&](int st) {
+                    const int k = 32 * part + col;
+
+                    return __builtin_bit_cast(win_h8, s.k[k * CH + ((2 * st + half) ^ (k / RW % CH))]);
+                };
+
+#pragma unroll
+                for (int st = 0; st < WIN_AHEAD && st < 2 * ND; st++)
+                    kf[st] = key(st);
 #pragma unroll
                 for (int st = 0; st < 2 * ND; st++) {
-                    const int key = 32 * part + col;
-                    const win_h8 k = __builtin_bit_cast(win_h8, s.k[key * CH + ((2 * st + half) ^ (key / RW % CH))]);
+                    win_h8 &k = kf[st % WIN_AHEAD];
 
                     sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, __builtin_bit_cast(win_h8, ql[st]), sc, 0, 0, 0);
                     sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, __builtin_bit_cast(win_h8, qh[st]), sc, 0, 0, 0);
+                    if (st + WIN_AHEAD < 2 * ND)
+                        k = key(st + WIN_AHEAD);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
                 /* Register e is key 8 (e / 4) + 4 half + e % 4. */
 #pragma unroll
@@ -673,7 +699,17 @@ __global__ void __launch_bounds__(256, ND == 1 ? 3 : 2) win_cache_kernel(const w
                             o[tt][e] *= corr;
                 }
                 const float ref = m == -INFINITY ? 0.0f : m;
+                win_h8 vf[WIN_AHEAD];
+                auto value = [&](int i) {
+                    const int dd = 32 * (i % ND) + col;
 
+                    return __builtin_bit_cast(win_h8,
+                                              s.v[dd * 8 + ((4 * part + 2 * (i / ND) + half) ^ (dd >> 1 & 7))]);
+                };
+
+#pragma unroll
+                for (int i = 0; i < WIN_AHEAD && i < 2 * ND; i++)
+                    vf[i] = value(i);
 #pragma unroll
                 for (int e = 0; e < 16; e += 4) {
                     const float4 v = *(const float4 *)&s.vs[32 * part + 2 * e + 4 * half];
@@ -692,21 +728,24 @@ __global__ void __launch_bounds__(256, ND == 1 ? 3 : 2) win_cache_kernel(const w
                     pl[e / 8][e / 2 % 4 + 1] = v1;
                 }
                 l += sum;
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int u = 0; u < 2; u++)
-#pragma unroll
-                    for (int tt = 0; tt < ND; tt++) {
-                        const int dd = 32 * tt + col;
-                        const win_h8 v = __builtin_bit_cast(
-                            win_h8, s.v[dd * 8 + ((4 * part + 2 * u + half) ^ (dd >> 1 & 7))]);
+                for (int i = 0; i < 2 * ND; i++) {
+                    const int u = i / ND, tt = i % ND;
+                    win_h8 &v = vf[i % WIN_AHEAD];
 
-                        o[tt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, __builtin_bit_cast(win_h8, pl[u]), o[tt], 0, 0, 0);
-                        o[tt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, __builtin_bit_cast(win_h8, ph[u]), o[tt], 0, 0, 0);
-                    }
+                    o[tt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, __builtin_bit_cast(win_h8, pl[u]), o[tt], 0, 0, 0);
+                    o[tt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, __builtin_bit_cast(win_h8, ph[u]), o[tt], 0, 0, 0);
+                    if (i + WIN_AHEAD < 2 * ND)
+                        v = value(i + WIN_AHEAD);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
             }
             /* The next tile into the other buffer, which was last read a tile
-             * ago, before the barrier; then its successor's loads. */
-            if (part == 0 && t + 1 < t1) {
+             * ago, before the barrier; then its successor's loads. Half of a
+             * SIMD's waves do it here and half there, so that one's products
+             * run beside the other's vector instructions. */
+            if (part == (values ? 0 : 1) && t + 1 < t1) {
                 stash(lds[(t + 1 - t0) & 1]);
                 if (t + 2 < t1) {
                     if (t + 2 - pg0 >= 16)
@@ -1643,7 +1682,7 @@ template <bool CACHE> static void win_launch(struct ops *o, win_args &a, long lo
 {
     const int cus = o->ocl->cu_count > 0 ? o->ocl->cu_count : 256;
     const bool few = win_few(a, CACHE);
-    const int tr = few ? WIN_FEW : WIN_ROWS;
+    const int tr = few ? WIN_FEW : CACHE ? WIN_CROWS : WIN_ROWS;
     const long long heads = (long long)a.rows * a.nh, rows = heads / a.nhk; /* of a key head */
     const long long blocks = (CACHE ? rows / tr + a.c.n : (rows + tr - 1) / tr) * a.nhk;
 
@@ -1656,7 +1695,7 @@ template <bool CACHE> static void win_launch(struct ops *o, win_args &a, long lo
     const hipStream_t s = stream_of(o->ocl);
 
     prof_scope ps(o->ocl, CACHE ? "attention_cache" : "attention_window");
-    const dim3 grid(grid_of(blocks * a.splits, 256, "attention tiles")), block(256);
+    const dim3 grid(grid_of(blocks * a.splits, tr == WIN_CROWS ? 512 : 256, "attention tiles")), block(256);
 
 #define WIN_FLOAT(ND_, CH_)                                                                    \
     do {                                                                                       \
@@ -1670,7 +1709,7 @@ template <bool CACHE> static void win_launch(struct ops *o, win_args &a, long lo
         if (CACHE && few)                                                                       \
             hipLaunchKernelGGL((win_few_kernel<ND_, true, WIN_ANY>), grid, block, 0, s, a);     \
         else if (CACHE)                                                                         \
-            hipLaunchKernelGGL(win_cache_kernel<ND_>, grid, block, 0, s, a);                    \
+            hipLaunchKernelGGL(win_cache_kernel<ND_>, grid, dim3(512), 0, s, a);                \
         else if (a.d == 32 * ND_)                                                               \
             WIN_FLOAT(ND_, WIN_FULL);                                                           \
         else if (a.d % 4 == 0)                                                                  \
