@@ -606,12 +606,28 @@ __global__ void __launch_bounds__(512, 2) win_cache_kernel(const win_args a)
             fetch(t0 + 1);
     }
     __syncthreads();
+    /* The tile behind t into the other buffer, which was last read a tile ago,
+     * before the barrier; then its successor's loads. Half of a SIMD's waves
+     * do it at the start of a tile and half at its end, so that one's products
+     * run beside the other's vector instructions. */
+    auto next = [&](int t) {
+        if (t + 1 < t1) {
+            stash(lds[(t + 1 - t0) & 1]);
+            if (t + 2 < t1) {
+                if (t + 2 - pg0 >= 16)
+                    pages(t + 2);
+                fetch(t + 2);
+            }
+        }
+    };
     int oexp = lds[0].vexp; /* o counts in 2^(oexp - 127 - WIN_VEXP) */
 
     for (int t = t0; t < t1; t++) {
         const tile_lds &s = lds[(t - t0) & 1];
         const int base = span.tile(t) * WIN_KT;
 
+        if (!values)
+            next(t);
         wild = wild || s.wild;
         if (s.vexp != oexp) {
             const float down = win_power(max(127 + oexp - s.vexp, 1));
@@ -741,19 +757,9 @@ __global__ void __launch_bounds__(512, 2) win_cache_kernel(const win_args a)
                     __builtin_amdgcn_sched_barrier(0);
                 }
             }
-            /* The next tile into the other buffer, which was last read a tile
-             * ago, before the barrier; then its successor's loads. Half of a
-             * SIMD's waves do it here and half there, so that one's products
-             * run beside the other's vector instructions. */
-            if (part == (values ? 0 : 1) && t + 1 < t1) {
-                stash(lds[(t + 1 - t0) & 1]);
-                if (t + 2 < t1) {
-                    if (t + 2 - pg0 >= 16)
-                        pages(t + 2);
-                    fetch(t + 2);
-                }
-            }
         }
+        if (values)
+            next(t);
         __syncthreads();
     }
     l += __shfl_xor(l, 32, 64);
