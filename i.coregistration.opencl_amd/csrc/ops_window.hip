@@ -237,8 +237,7 @@ typedef float win_f2 __attribute__((ext_vector_type(2)));
 typedef float win_f16x __attribute__((ext_vector_type(16)));
 typedef unsigned win_u4 __attribute__((ext_vector_type(4)));
 
-#define WIN_ROWS 128    /* rows (queries times the heads of a key head) of a tile */
-#define WIN_KT 64       /* keys of a tile */
+#define WIN_KT 64       /* keys of a tile of a cache */
 #define WIN_AHEAD 2     /* operands on their way from LDS */
 #define WIN_TAU 4.0f    /* the running maximum is raised when a score passes it by this (base 2) */
 #define WIN_VEXP 10     /* exponent of the largest value scale: weights up to 2^TAU stay below 2^16 */
@@ -374,45 +373,89 @@ static __device__ __forceinline__ int win_unit(const win_args &a, int tiles, int
     return tiles - 1 - blockIdx.x / per;
 }
 
-#define WIN_CROWS 256 /* rows of a tile over a cache, 8 waves of 32 */
+/* Channels of a head: any number (a load a float), a multiple of 4, or all
+ * that the kernel has room for. */
+enum { WIN_ANY, WIN_FOUR, WIN_FULL };
 
-template <int ND>
-__global__ void __launch_bounds__(512, 2) win_cache_kernel(const win_args a)
+/* Floats c .. c + 3 of a row of d; behind the last channel some of them again,
+ * for products with zeros and sums that are not stored. */
+template <int CHANNELS>
+static __device__ __forceinline__ void win_load4(const float *p, int c, int d, float (&x)[4])
 {
-    constexpr int DP = 32 * ND, CH = DP / 8;
-    constexpr int RW = 16 / CH < 1 ? 1 : 16 / CH;  /* K rows in 256 bytes */
-    constexpr int KU = 4 * DP, NK = (KU + 255) / 256; /* 16-byte units of codes of a tile of K */
-    constexpr int VU = 2 * DP;                        /* units of 8 keys x 4 channels of V */
-    constexpr int KSZ = WIN_KT * CH, VSZ = DP * 8;    /* 16-byte chunks in LDS */
+    if (CHANNELS == WIN_FULL)
+        load4(p + c, x);
+    else if (CHANNELS == WIN_FOUR)
+        load4(p + min(c, d - 4), x);
+    else {
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            x[j] = p[min(c + j, d - 1)];
+    }
+}
+
+#define WIN_LAG 12   /* a row's scale is at most 2^12 below the largest so far, its values smaller instead */
+#define WIN_DEEP 14  /* float32 values keep 22 bits 2^14 below that */
+#define WIN_CODES 24 /* codes keep all 2^24 below */
+
+typedef short win_s4 __attribute__((ext_vector_type(4)));
+typedef _Float16 win_h4 __attribute__((ext_vector_type(4)));
+
+/* Largest of the L lanes of a row, L = 4, 8 or 16. */
+template <int L> static __device__ __forceinline__ unsigned win_row_max(unsigned v)
+{
+    v = max(v, (unsigned)dpp_i((int)v, 0xB1));
+    v = max(v, (unsigned)dpp_i((int)v, 0x4E));
+    if (L > 4)
+        v = max(v, (unsigned)dpp_i((int)v, 0x141));
+    if (L > 8)
+        v = max(v, (unsigned)dpp_i((int)v, 0x140));
+    return v;
+}
+
+/* NW waves of 32 rows, KT keys at a time. */
+template <int ND, bool CACHE, int CHANNELS, int NW, int KT>
+__global__ void __launch_bounds__(64 * NW, ND == 1 ? 4 : 2) win_tile_kernel(const win_args a)
+{
+    constexpr int DP = 32 * ND, CH = DP / 8, P = CACHE ? 1 : 2; /* channels, 16-byte chunks of a key, f16 parts */
+    /* Chunks between keys in LDS: 16 neighbouring keys' chunks of one place, as
+     * the scores' operands are read, and 4 neighbouring keys' 64 bytes, as the
+     * outputs' are, lie in banks of their own. */
+    constexpr int KS = CH + 1, VS = ND == 1 ? 4 : CH + 4;
+    constexpr int HT = 32 * NW;                  /* threads that stage keys, and values */
+    constexpr int UC = CACHE ? CH / 2 : CH;      /* units of a key: 16 codes, or 8 floats */
+    constexpr int U = KT * UC, NU = (U + HT - 1) / HT, RW = CACHE ? 4 : 8;
+    constexpr bool SAME = 64 / UC <= 16;         /* a wave's units lie in one run of 16 keys */
     struct tile_lds {
-        win_u4 k[KSZ], v[VSZ];
-        float ks[WIN_KT], vs[WIN_KT];
+        win_u4 k[P * KT * KS], v[P * KT * VS];
+        float ks[KT], vs[KT];
         unsigned long long keep;
-        int vexp, wild;
+        int top[NW / 2], low[NW / 2]; /* largest and smallest scale of a wave's values, exponents */
+        int wild;
     };
+    static_assert(KT == 64 || !CACHE, "a lane a key");
     __shared__ tile_lds lds[2];
-    __shared__ float ps[8][64];
+    __shared__ float ps[NW][64];
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, col = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int g = a.nh / a.nhk, d = a.d, pitch = a.c.pitch;
-    const int tiles = (int)((long long)a.rows * g / WIN_CROWS) + a.c.n;
+    const int g = a.nh / a.nhk, d = CHANNELS == WIN_FULL ? DP : a.d, pitch = a.c.pitch;
+    const long long rows = (long long)a.rows * g;
+    const int tiles = (int)(CACHE ? rows / (32 * NW) + a.c.n : (rows + 32 * NW - 1) / (32 * NW));
     int split, kvh;
     const int tile = win_unit(a, tiles, split, kvh);
-    const win_job jb = win_job_of<true, WIN_CROWS>(a, tile, kvh);
+    const win_job jb = win_job_of<CACHE, 32 * NW>(a, tile, kvh);
 
     if (jb.n <= 0)
         return;
     const int last = jb.r0 + jb.n - 1;
-    const win_tiles span = win_span<WIN_KT>(a, jb.p0 + jb.r0 / g, jb.p0 + last / g, jb.nk);
+    const win_tiles span = win_span<KT>(a, jb.p0 + jb.r0 / g, jb.p0 + last / g, jb.nk);
     const int parts = win_parts(span.n, a.splits);
     /* This lane's row; lanes without one take the last. */
     const int wr = jb.r0 + 32 * wave, r = min(wr + col, last), qi = r / g, h = jb.kvh * g + r - qi * g;
-    const bool mine = wr + col <= last;
-    const long long row = jb.first + qi, out = (row * a.nh + h) * a.splits + split;
+    const long long row = jb.first + qi;
 
     if (split >= parts) {
-        if (mine && half == 0)
-            a.ml[out] = make_float2(-INFINITY, 0.0f);
+        if (wr + col <= last && half == 0)
+            a.ml[(row * a.nh + h) * a.splits + split] = make_float2(-INFINITY, 0.0f);
         return;
     }
     const int t0 = (int)((long long)span.n * split / parts), t1 = (int)((long long)span.n * (split + 1) / parts);
@@ -467,18 +510,16 @@ __global__ void __launch_bounds__(512, 2) win_cache_kernel(const win_args a)
         for (int e = 0; e < 16; e++)
             o[tt][e] = 0.0f;
 
-    /* Waves 0 .. 3 stage values, 4 .. 7 keys: unit e of K is key e / (DP / 16),
-     * bytes 16 (e % (DP / 16)) ..; of V channels 4 (e % (DP / 4)) .., slots 8 c ..
-     * 8 c + 7, c = e / (DP / 4), slot 8 c + j being the key that register 8 (c /
-     * 2 % 2) + j of the scores of keys 32 (c / 4) .. holds in lane half c % 2: 16
-     * (c / 2) + 8 (j / 4) + 4 (c % 2) + j % 4. Pages hold at least 16 keys, so
-     * a unit lies in one. */
-    const bool values = wave < 4;
-    const int ht = tid & 255;
-    bool kept = false;
-    uint4 kr[2]; /* NK of them, or 8 words of V */
-    float sr;
-    int pg = -1, pg0 = t0, vexp = 12;
+    /* The first half of the waves stages values, the other keys: unit e is key
+     * e / UC, 16 codes or 8 floats from channel 16 (e % UC) or 8 (e % UC) on. */
+    const bool values = wave < NW / 2;
+    const int ht = tid % HT, hw = wave % (NW / 2);
+    unsigned reg[NU][RW];
+    float sc1[NU];              /* a cache's value scales, of the units */
+    bool kept[NU], kept1 = false; /* of the units; of key `lane` */
+    float sr = 0.0f;            /* a cache's scale of key `lane` */
+    int pg = -1, pg0 = t0;
+    int vexp = 12; /* exponent of the largest value scale so far; o counts in 2^(vexp - 127 - WIN_VEXP) */
 
     /* Pages of 16 tiles from t on, a run of 16 keys a lane. */
     auto pages = [&](int t) {
@@ -487,160 +528,270 @@ __global__ void __launch_bounds__(512, 2) win_cache_kernel(const win_args a)
         pg0 = t;
         pg = key < jb.nk ? seq_page(a.c, jb.b, key) : -1;
     };
-    /* The page of run `run` of tile t. */
     auto page_of = [&](int t, int run) { return __shfl(pg, 4 * (t - pg0) + run, 64); };
-    /* Tile t into registers. Where there is no page, and behind a row's codes,
-     * something else is read that counts nothing: no lane has a branch. The
-     * run of 16 keys is the same for a wave's lanes where SAME says so: the
-     * address is a scalar one and an offset that never changes. */
-    auto row_of = [&](auto same, int t, int run, int k0) {
-        if constexpr (same) {
-            const int r = __builtin_amdgcn_readfirstlane(run);
-            const int page = max(__builtin_amdgcn_readlane(pg, 4 * (t - pg0) + r), 0);
-
-            return cache_row(a.c, page, jb.kvh, k0 + 16 * r) * pitch;
-        }
-        else
-            return cache_row(a.c, max(page_of(t, run), 0), jb.kvh, k0 + 16 * run) * pitch;
-    };
+    /* Tile t into registers. Where there is no key or page, and behind a row's
+     * channels, something else is read that counts nothing: no lane has a
+     * branch. */
     auto fetch = [&](int t) {
-        const int k0 = span.tile(t) * WIN_KT;
+        const int k0 = span.tile(t) * KT;
 
-        if (values) {
-            const int e = min(ht, VU - 1), c = e / (DP / 4), at = e % (DP / 4) * 4;
-            const signed char *v = a.c.vc + row_of(std::bool_constant<ND == 4>{}, t, c >> 1, k0);
-            const unsigned off = (c & 1) * 4 * pitch + min(at, pitch - 4);
-            unsigned *to = (unsigned *)kr;
+        if constexpr (CACHE) {
+            const signed char *codes = values ? a.c.vc : a.c.kc;
 
 #pragma unroll
-            for (int j = 0; j < 8; j++)
-                to[j] = *(const unsigned *)(v + ((j >> 2) * 8 + (j & 3)) * pitch + off);
-        }
-        else {
-#pragma unroll
-            for (int i = 0; i < NK; i++) {
-                const int e = min(ht + 256 * i, KU - 1), key = e / (DP / 16), at = e % (DP / 16) * 16;
-                const signed char *k = a.c.kc + row_of(std::bool_constant<(ND > 1)>{}, t, key >> 4, k0);
+            for (int i = 0; i < NU; i++) {
+                const int e = min(ht + HT * i, U - 1), key = e / UC, at = e % UC * 16;
+                uint4 x;
 
-                kr[i] = *(const uint4 *)(k + (unsigned)((key & 15) * pitch + min(at, pitch - 16)));
+                /* The address is a scalar one and an offset that never changes
+                 * where a wave's lanes lie in one run. */
+                if constexpr (SAME) {
+                    const int run = __builtin_amdgcn_readfirstlane(key >> 4);
+                    const int page = __builtin_amdgcn_readlane(pg, 4 * (t - pg0) + run);
+                    const long long first = cache_row(a.c, max(page, 0), jb.kvh, k0 + 16 * run);
+
+                    x = *(const uint4 *)(codes + first * pitch + (unsigned)((key & 15) * pitch + min(at, pitch - 16)));
+                    if (values) {
+                        kept[i] = page >= 0 && k0 + key < jb.nk;
+                        sc1[i] = (a.c.vs + first)[key & 15];
+                    }
+                }
+                else {
+                    const int page = page_of(t, key >> 4);
+                    const long long cell = cache_row(a.c, max(page, 0), jb.kvh, k0 + key);
+
+                    x = *(const uint4 *)(codes + cell * pitch + min(at, pitch - 16));
+                    if (values) {
+                        kept[i] = page >= 0 && k0 + key < jb.nk;
+                        sc1[i] = a.c.vs[cell];
+                    }
+                }
+                reg[i][0] = x.x, reg[i][1] = x.y, reg[i][2] = x.z, reg[i][3] = x.w;
             }
-            if (wave < 6) {
+            if (hw == 0) {
                 const int page = page_of(t, lane >> 4);
 
-                kept = page >= 0 && k0 + lane < jb.nk;
-                sr = (wave == 4 ? a.c.ks : a.c.vs)[cache_row(a.c, max(page, 0), jb.kvh, k0 + lane)];
-                sr = kept ? sr : 0.0f;
+                kept1 = page >= 0 && k0 + lane < jb.nk;
+                sr = (values ? a.c.vs : a.c.ks)[cache_row(a.c, max(page, 0), jb.kvh, k0 + lane)];
+            }
+        }
+        else {
+            const int end = jb.nk - 1 - k0;
+            const float *from = (values ? a.V : a.K) + (long long)jb.kvh * d;
+            const long long ld = values ? a.ldv : a.ldk;
+
+#pragma unroll
+            for (int i = 0; i < NU; i++) {
+                const int e = min(ht + HT * i, U - 1), key = e / UC, at = e % UC * 8;
+                const float *x = from + (k0 + min(key, end)) * ld;
+                float u[4], v[4];
+
+                win_load4<CHANNELS>(x, at, d, u);
+                win_load4<CHANNELS>(x, at + 4, d, v);
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    reg[i][j] = __builtin_bit_cast(unsigned, u[j]);
+                    reg[i][4 + j] = __builtin_bit_cast(unsigned, v[j]);
+                }
+                kept[i] = key <= end;
+                if (a.kmask && values)
+                    kept[i] = kept[i] && a.kmask[k0 + min(key, end)];
+            }
+            if (hw == 0 && !values) {
+                kept1 = lane <= end && lane < KT;
+                if (a.kmask)
+                    kept1 = kept1 && a.kmask[k0 + min(lane, end)];
             }
         }
     };
     auto stash = [&](tile_lds &s) {
-        if (values) {
-            const int c = ht / (DP / 4), ch = ht % (DP / 4) * 4;
-            const unsigned *w = (const unsigned *)kr;
+        win_u4 *to = values ? s.v : s.k;
+        const int stride = values ? VS : KS;
 
-            if (VU < 256 && ht >= VU)
-                return;
+        if constexpr (CACHE) {
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
-                const unsigned sel = 0x0c000c00u | (4u + k) << 16 | (unsigned)k;
-                win_u4 x;
+            for (int i = 0; i < NU; i++) {
+                const int e = ht + HT * i, key = e / UC;
+                win_u4 x[2];
+
+                if (U % HT && e >= U)
+                    continue;
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const unsigned w = reg[i][j] ^ 0x80808080u;
+
+                    x[j / 2][2 * j % 4] = win_codes(__builtin_amdgcn_perm(0x64646464u, w, 0x04010400u));
+                    x[j / 2][2 * j % 4 + 1] = win_codes(__builtin_amdgcn_perm(0x64646464u, w, 0x04030402u));
+                }
+                if (values) {
+                    /* Codes of a scale far below the largest: smaller, exactly. */
+                    const int k = vexp - WIN_LAG - (int)(q8_mag(sc1[i]) >> 23);
+
+                    if (__any(k > 0 && kept[i])) {
+                        const int n = min(max(k, 0), WIN_CODES);
+                        const unsigned short f = n <= 14 ? (unsigned short)((15 - n) << 10) : (unsigned short)(1 << (WIN_CODES - n));
+                        const _Float16 down = __builtin_bit_cast(_Float16, f);
+                        const win_h2 two = {down, down};
 
 #pragma unroll
-                for (int j = 0; j < 4; j++)
-                    x[j] = win_codes(__builtin_amdgcn_perm(w[2 * j + 1], w[2 * j], sel) ^ 0x64806480u);
-                s.v[(ch + k) * 8 + (c ^ ((ch + k) >> 1 & 7))] = x;
+                        for (int j = 0; j < 8; j++)
+                            x[j / 4][j % 4] = __builtin_bit_cast(unsigned, __builtin_bit_cast(win_h2, (unsigned)x[j / 4][j % 4]) * two);
+                    }
+                }
+                to[key * stride + e % UC * 2] = x[0];
+                to[key * stride + e % UC * 2 + 1] = x[1];
             }
-            return;
-        }
-#pragma unroll
-        for (int i = 0; i < NK; i++) {
-            const int e = ht + 256 * i, key = e / (DP / 16), ch = e % (DP / 16) * 2;
+            if (hw == 0 && !values) {
+                const unsigned long long keep = __ballot(kept1);
 
-            if (KU % 256 == 0 || e < KU) {
-                const unsigned w[4] = {kr[i].x ^ 0x80808080u, kr[i].y ^ 0x80808080u, kr[i].z ^ 0x80808080u,
-                                       kr[i].w ^ 0x80808080u};
-                unsigned x[8];
+                s.ks[lane] = sr;
+                if (lane == 0)
+                    s.keep = keep;
+            }
+            else if (hw == 0) {
+                /* Value scales times a power of two that brings the largest so
+                 * far to 2^WIN_VEXP; a scale of NaN, and one too far below the
+                 * largest, is for the float32 path. */
+                const float x = kept1 ? sr : 0.0f;
+                const bool bad = !(q8_mag(x) < 0x7f800000u);
+                const int e = bad ? 0 : (int)(q8_mag(x) >> 23), n = max(vexp - WIN_LAG - e, 0);
+                const int top = max(vexp, min((int)wave_umax(e), 253));
+                /* Twice, as one power may pass the range. */
+                const float y = bad || n > WIN_CODES ? 0.0f : x * win_power(127 + n) * win_power(254 + WIN_VEXP - top);
+                const bool w = __any(bad || (x != 0.0f && y < WIN_VMIN));
+
+                s.vs[lane] = y;
+                if (lane == 0) {
+                    s.top[0] = top;
+                    s.wild = w;
+                }
+            }
+        }
+        else {
+            unsigned top = 0, least = 0; /* exponents; least: 255 less the smallest */
+            bool bad = false;
+
+#pragma unroll
+            for (int i = 0; i < NU; i++) {
+                const int e = ht + HT * i, key = e / UC;
+                unsigned mag = 0;
+                win_u4 x, y;
+
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+                    mag = max(mag, reg[i][j] & 0x7fffffffu);
+                mag = win_row_max<UC>(mag);
+                const bool none = values && (!kept[i] || mag >= 0x7f800000u);
+                int ex = min(max((int)(mag >> 23), 15), 254);
+
+                if (values) {
+                    bad = bad || (kept[i] && (mag >= 0x7f800000u || (mag && ex - 14 < vexp - WIN_LAG - WIN_DEEP)));
+                    ex = max(ex, vexp - WIN_LAG + 14);
+                    if (kept[i] && mag && mag < 0x7f800000u) {
+                        top = max(top, (unsigned)ex - 14);
+                        least = max(least, 269u - ex);
+                    }
+                }
+                const float up = win_power(268 - ex);
 
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
-                    x[2 * j] = win_codes(__builtin_amdgcn_perm(0x64646464u, w[j], 0x04010400u));
-                    x[2 * j + 1] = win_codes(__builtin_amdgcn_perm(0x64646464u, w[j], 0x04030402u));
-                }
-                const win_u4 u = {x[0], x[1], x[2], x[3]}, v = {x[4], x[5], x[6], x[7]};
+                    const float u = none ? 0.0f : __builtin_bit_cast(float, reg[i][2 * j]) * up;
+                    const float v = none ? 0.0f : __builtin_bit_cast(float, reg[i][2 * j + 1]) * up;
+                    unsigned b, c;
 
-                s.k[key * CH + (ch ^ (key / RW % CH))] = u;
-                s.k[key * CH + ((ch + 1) ^ (key / RW % CH))] = v;
+                    win_split(u, v, b, c);
+                    x[j] = b;
+                    y[j] = c;
+                }
+                if (U % HT && e >= U)
+                    continue;
+                to[key * stride + e % UC] = x;
+                to[(KT + key) * stride + e % UC] = y;
+                if (e % UC == 0)
+                    (values ? s.vs : s.ks)[key] = none ? 0.0f : mag >= 0x7f800000u ? __builtin_nanf("") : win_power(ex - 14);
+            }
+            if (values) {
+                top = wave_umax(top);
+                least = wave_umax(least);
+                bad = __any(bad);
+                if (lane == 0) {
+                    s.top[hw] = (int)top | (bad ? 0x10000 : 0);
+                    s.low[hw] = 255 - (int)least;
+                }
+            }
+            else if (hw == 0) {
+                const unsigned long long keep = __ballot(kept1);
+
+                if (lane == 0)
+                    s.keep = keep;
             }
         }
-        if (wave == 4) {
-            const unsigned long long keep = __ballot(kept);
-
-            s.ks[lane] = sr;
-            if (lane == 0)
-                s.keep = keep;
-        }
-        else if (wave == 5) {
-            /* Value scales times a power of two that brings the largest so
-             * far to 2^WIN_VEXP; a scale of NaN, and one far below the largest,
-             * is for the float32 path. */
-            const bool bad = sr != sr;
-
-            vexp = max(vexp, min((int)(wave_umax(bad ? 0u : q8_mag(sr)) >> 23), 253));
-            const float x = bad ? 0.0f : sr * win_power(254 + WIN_VEXP - vexp);
-
-            s.vs[lane] = x;
-            const int w = __any(bad || (x != 0.0f && x < WIN_VMIN) || !(x < 0x1p12f));
-
-            if (lane == 0) {
-                s.vexp = vexp;
-                s.wild = w;
+    };
+    /* The tile behind t into the other buffer, which was last read a tile ago,
+     * before the barrier; then its successor's loads. Half of a SIMD's waves do
+     * it at the start of a tile and half at its end, so that one's products run
+     * beside the other's vector instructions. */
+    auto next = [&](int t) {
+        if (t + 1 < t1) {
+            stash(lds[(t + 1 - t0) & 1]);
+            if (t + 2 < t1) {
+                if (CACHE && t + 2 - pg0 >= 16)
+                    pages(t + 2);
+                fetch(t + 2);
             }
         }
     };
 
     if (t0 < t1) {
-        pages(t0);
+        if (CACHE)
+            pages(t0);
         fetch(t0);
         stash(lds[0]);
         if (t0 + 1 < t1)
             fetch(t0 + 1);
     }
     __syncthreads();
-    /* The tile behind t into the other buffer, which was last read a tile ago,
-     * before the barrier; then its successor's loads. Half of a SIMD's waves
-     * do it at the start of a tile and half at its end, so that one's products
-     * run beside the other's vector instructions. */
-    auto next = [&](int t) {
-        if (t + 1 < t1) {
-            stash(lds[(t + 1 - t0) & 1]);
-            if (t + 2 < t1) {
-                if (t + 2 - pg0 >= 16)
-                    pages(t + 2);
-                fetch(t + 2);
-            }
-        }
-    };
-    int oexp = lds[0].vexp; /* o counts in 2^(oexp - 127 - WIN_VEXP) */
-
     for (int t = t0; t < t1; t++) {
         const tile_lds &s = lds[(t - t0) & 1];
-        const int base = span.tile(t) * WIN_KT;
+        const int base = span.tile(t) * KT;
+        /* This lane's places: a key's chunks; of the values, which come
+         * transposed by 4 x 16, 4 channels of a key. */
+        const win_u4 *kp = s.k + col * KS + half;
+        const char *vp = (const char *)(s.v + (4 * half + (lane & 15) / 4) * VS + 2 * (lane >> 4 & 1)) + 8 * (lane & 3);
+        int top = s.top[0];
 
         if (!values)
             next(t);
-        wild = wild || s.wild;
-        if (s.vexp != oexp) {
-            const float down = win_power(max(127 + oexp - s.vexp, 1));
+        if constexpr (!CACHE) {
+            int bits = 0, low = s.low[0];
 
-            oexp = s.vexp;
+#pragma unroll
+            for (int w = 0; w < NW / 2; w++) {
+                bits |= s.top[w];
+                low = min(low, s.low[w]);
+                top = max(top & 0xffff, s.top[w] & 0xffff);
+            }
+            top = max(top, vexp);
+            wild = wild || bits >> 16 || low < top - WIN_VEXP - 3;
+        }
+        else
+            wild = wild || s.wild;
+        top = __builtin_amdgcn_readfirstlane(top);
+        if (top != vexp) {
+            const float down = win_power(max(127 + vexp - top, 1));
+
+            vexp = top;
 #pragma unroll
             for (int tt = 0; tt < ND; tt++)
 #pragma unroll
                 for (int e = 0; e < 16; e++)
                     o[tt][e] *= down;
         }
+        const float vup = win_power(254 + WIN_VEXP - vexp);
+
 #pragma unroll
-        for (int part = 0; part < 2; part++) {
+        for (int part = 0; part < KT / 32; part++) {
             const int k0 = base + 32 * part;
             /* Some row of the wave sees some key; all see all. */
             const bool some = live && k0 <= hi1 && (k0 + 32 > lo0 || k0 < a.sinks);
@@ -650,29 +801,32 @@ __global__ void __launch_bounds__(512, 2) win_cache_kernel(const win_args a)
                 win_f16x sc;
                 win_u4 ph[2], pl[2];
                 float x[16], mx = -INFINITY, sum = 0.0f;
+                /* Operands are read WIN_AHEAD steps before their products. */
+                win_h8 kf[WIN_AHEAD][P];
+                auto key = [&](int st, int part2) {
+                    return __builtin_bit_cast(win_h8, kp[(32 * part + KT * part2) * KS + 2 * st]);
+                };
 
 #pragma unroll
                 for (int e = 0; e < 16; e++)
                     sc[e] = 0.0f;
-                /* Operands are read WIN_AHEAD steps before their products. */
-                win_h8 kf[WIN_AHEAD];
-                auto key = [&](int st) {
-                    const int k = 32 * part + col;
-
-                    return __builtin_bit_cast(win_h8, s.k[k * CH + ((2 * st + half) ^ (k / RW % CH))]);
-                };
-
 #pragma unroll
                 for (int st = 0; st < WIN_AHEAD && st < 2 * ND; st++)
-                    kf[st] = key(st);
+#pragma unroll
+                    for (int i = 0; i < P; i++)
+                        kf[st][i] = key(st, i);
 #pragma unroll
                 for (int st = 0; st < 2 * ND; st++) {
-                    win_h8 &k = kf[st % WIN_AHEAD];
+                    win_h8(&k)[P] = kf[st % WIN_AHEAD];
 
-                    sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, __builtin_bit_cast(win_h8, ql[st]), sc, 0, 0, 0);
-                    sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, __builtin_bit_cast(win_h8, qh[st]), sc, 0, 0, 0);
+                    sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[0], __builtin_bit_cast(win_h8, ql[st]), sc, 0, 0, 0);
+                    if constexpr (P > 1)
+                        sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[1], __builtin_bit_cast(win_h8, qh[st]), sc, 0, 0, 0);
+                    sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[0], __builtin_bit_cast(win_h8, qh[st]), sc, 0, 0, 0);
                     if (st + WIN_AHEAD < 2 * ND)
-                        k = key(st + WIN_AHEAD);
+#pragma unroll
+                        for (int i = 0; i < P; i++)
+                            k[i] = key(st + WIN_AHEAD, i);
                     __builtin_amdgcn_sched_barrier(0);
                 }
                 /* Register e is key 8 (e / 4) + 4 half + e % 4. */
@@ -715,22 +869,35 @@ __global__ void __launch_bounds__(512, 2) win_cache_kernel(const win_args a)
                             o[tt][e] *= corr;
                 }
                 const float ref = m == -INFINITY ? 0.0f : m;
-                win_h8 vf[WIN_AHEAD];
-                auto value = [&](int i) {
-                    const int dd = 32 * (i % ND) + col;
+                win_h8 vf[WIN_AHEAD][P];
+                /* Step i: keys 16 (i / ND) .., channels 32 (i % ND) ..; slot j of a
+                 * lane half is the key that register 8 (i / ND) + j of the
+                 * scores is. */
+                auto value = [&](int i, int part2) {
+                    win_h4 y[2];
 
-                    return __builtin_bit_cast(win_h8,
-                                              s.v[dd * 8 + ((4 * part + 2 * (i / ND) + half) ^ (dd >> 1 & 7))]);
+#pragma unroll
+                    for (int r8 = 0; r8 < 2; r8++) {
+                        const char *at = vp + 16 * ((KT * part2 + 32 * part + 16 * (i / ND) + 8 * r8) * VS + 4 * (i % ND));
+
+                        y[r8] = __builtin_bit_cast(win_h4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                                               (__attribute__((address_space(3))) win_s4 *)at));
+                    }
+                    return __builtin_shufflevector(y[0], y[1], 0, 1, 2, 3, 4, 5, 6, 7);
                 };
 
 #pragma unroll
                 for (int i = 0; i < WIN_AHEAD && i < 2 * ND; i++)
-                    vf[i] = value(i);
+#pragma unroll
+                    for (int k = 0; k < P; k++)
+                        vf[i][k] = value(i, k);
 #pragma unroll
                 for (int e = 0; e < 16; e += 4) {
-                    const float4 v = *(const float4 *)&s.vs[32 * part + 2 * e + 4 * half];
+                    float4 v = *(const float4 *)&s.vs[32 * part + 2 * e + 4 * half];
                     unsigned u0, u1, v0, v1;
 
+                    if constexpr (!CACHE)
+                        v = make_float4(v.x * vup, v.y * vup, v.z * vup, v.w * vup);
 #pragma unroll
                     for (int j = 0; j < 4; j++) {
                         x[e + j] = __builtin_amdgcn_exp2f(fmaf(x[e + j], qf, -ref));
@@ -748,12 +915,16 @@ __global__ void __launch_bounds__(512, 2) win_cache_kernel(const win_args a)
 #pragma unroll
                 for (int i = 0; i < 2 * ND; i++) {
                     const int u = i / ND, tt = i % ND;
-                    win_h8 &v = vf[i % WIN_AHEAD];
+                    win_h8(&v)[P] = vf[i % WIN_AHEAD];
 
-                    o[tt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, __builtin_bit_cast(win_h8, pl[u]), o[tt], 0, 0, 0);
-                    o[tt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, __builtin_bit_cast(win_h8, ph[u]), o[tt], 0, 0, 0);
+                    o[tt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[0], __builtin_bit_cast(win_h8, pl[u]), o[tt], 0, 0, 0);
+                    if constexpr (P > 1)
+                        o[tt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[1], __builtin_bit_cast(win_h8, ph[u]), o[tt], 0, 0, 0);
+                    o[tt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[0], __builtin_bit_cast(win_h8, ph[u]), o[tt], 0, 0, 0);
                     if (i + WIN_AHEAD < 2 * ND)
-                        v = value(i + WIN_AHEAD);
+#pragma unroll
+                        for (int k = 0; k < P; k++)
+                            v[k] = value(i + WIN_AHEAD, k);
                     __builtin_amdgcn_sched_barrier(0);
                 }
             }
@@ -770,339 +941,12 @@ __global__ void __launch_bounds__(512, 2) win_cache_kernel(const win_args a)
 #pragma unroll
         for (int e = 0; e < 16; e++)
             z = fmaf(o[tt][e], 0.0f, z);
-    win_finish<ND, true, WIN_KT>(a, jb, span, t0, t1, parts, split, o, win_power(max(oexp - WIN_VEXP, 1)), m, l, wild || z != 0.0f,
-                                 ps[wave], d);
+    win_finish<ND, CACHE, KT>(a, jb, span, t0, t1, parts, split, o, win_power(max(vexp - WIN_VEXP, 1)), m, l,
+                              wild || z != 0.0f, ps[wave], d);
 }
 
-/* Channels of a head: any number (a load a float), a multiple of 4, or all
- * that the kernel has room for. */
-enum { WIN_ANY, WIN_FOUR, WIN_FULL };
-
-/* Floats c .. c + 3 of a row of d; behind the last channel some of them again,
- * for products with zeros and sums that are not stored. */
-template <int CHANNELS>
-static __device__ __forceinline__ void win_load4(const float *p, int c, int d, float (&x)[4])
-{
-    if (CHANNELS == WIN_FULL)
-        load4(p + c, x);
-    else if (CHANNELS == WIN_FOUR)
-        load4(p + min(c, d - 4), x);
-    else {
-#pragma unroll
-        for (int j = 0; j < 4; j++)
-            x[j] = p[min(c + j, d - 1)];
-    }
-}
-
-/* ---- a tile of rows over float32 keys and values --------------------------------- */
-
-#define WIN_FKT 32            /* keys of a tile */
 #define WIN_FTAU 8.0f         /* as WIN_TAU */
 #define WIN_QUP 0x1p32f       /* scale of the queries split into bf16 parts */
-
-template <int ND, int CHANNELS>
-__global__ void __launch_bounds__(256, ND == 4 ? 1 : ND == 2 ? 2 : 3) win_float_kernel(const win_args a)
-{
-    constexpr int DP = 32 * ND, CH = DP / 8;
-    constexpr int RW = 16 / CH < 1 ? 1 : 16 / CH; /* K rows in 256 bytes */
-    constexpr int PK = WIN_FKT * CH;              /* chunks of a part: K and V alike */
-    constexpr int NL = (PK + 255) / 256;
-    __shared__ split_u4 lds[2][6 * PK];
-    __shared__ float ps[4][64];
-    const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, col = lane & 31;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int g = a.nh / a.nhk, d = CHANNELS == WIN_FULL ? DP : a.d;
-    const int tiles = (int)(((long long)a.rows * g + WIN_ROWS - 1) / WIN_ROWS);
-    int split, kvh;
-    const int tile = win_unit(a, tiles, split, kvh);
-    const win_job jb = win_job_of<false, WIN_ROWS>(a, tile, kvh);
-    const int last = jb.r0 + jb.n - 1;
-    const win_tiles span = win_span<WIN_FKT>(a, jb.p0 + jb.r0 / g, jb.p0 + last / g, jb.nk);
-    const int parts = win_parts(span.n, a.splits);
-    /* This lane's row; lanes without one take the last. */
-    const int wr = jb.r0 + 32 * wave, r = min(wr + col, last), qi = r / g, h = jb.kvh * g + r - qi * g;
-    const bool mine = wr + col <= last;
-    const long long row = qi, out = (row * a.nh + h) * a.splits + split;
-
-    if (split >= parts) {
-        if (mine && half == 0)
-            a.ml[out] = make_float2(-INFINITY, 0.0f);
-        return;
-    }
-    const int t0 = (int)((long long)span.n * split / parts), t1 = (int)((long long)span.n * (split + 1) / parts);
-    const int p0 = jb.p0 + qi, hi = win_hi(a, p0, jb.nk), lo = win_lo(a, p0);
-    const bool live = wr <= last;
-    const int pa = jb.p0 + min(wr, last) / g, pb = jb.p0 + min(wr + 31, last) / g;
-    const int hi0 = win_hi(a, pa, jb.nk), hi1 = win_hi(a, pb, jb.nk), lo0 = win_lo(a, pa), lo1 = win_lo(a, pb);
-    const float *K = a.K + (long long)jb.kvh * d, *V = a.V + (long long)jb.kvh * d;
-    /* Threads past the chunks (32 channels a head): none in K, all in V. */
-    constexpr bool APART = PK < 256;
-    const bool has_k = !APART || tid < PK;
-    const int vt = APART ? tid - PK : tid;
-    float kr[NL][8], vr[NL][8];
-    split_u4 q[2 * ND][3];
-    /* The output's small products: of all keys (LOW), or of 16 at a time
-     * where 16 registers a 32 channels more would spill. */
-    constexpr bool LOW = ND != 2;
-    win_f16x o[ND], low[LOW ? ND : 1];
-    float m = -INFINITY, l = 0.0f;
-    unsigned seen = 0, next = ~0u;
-
-    {
-        const float *qp = a.Q + row * a.ldq + (long long)h * d;
-        const float up = a.scale * WIN_LOG2E * WIN_QUP;
-
-#pragma unroll
-        for (int st = 0; st < 2 * ND; st++) {
-            float u[4], v[4], x[8];
-
-            load4_row(qp, st * 16 + half * 8, d, u);
-            load4_row(qp, st * 16 + half * 8 + 4, d, v);
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                x[j] = u[j];
-                x[4 + j] = v[j];
-            }
-            split8(x, up, q[st][0], q[st][1], q[st][2]);
-        }
-    }
-#pragma unroll
-    for (int tt = 0; tt < ND; tt++)
-#pragma unroll
-        for (int e = 0; e < 16; e++)
-            o[tt][e] = low[LOW ? tt : 0][e] = 0.0f;
-
-    /* Tile t into registers: K chunk e is key e / CH, channels 8 (e % CH) ..; V
-     * chunk e channel e % DP, slots 8 (e / DP) .. + 7. Behind the last key it
-     * is read again. next: the tile's kept keys. */
-    auto fetch = [&](int t) {
-        const int k0 = span.tile(t) * WIN_FKT, end = jb.nk - 1 - k0;
-
-        if (has_k) {
-#pragma unroll
-            for (int i = 0; i < NL; i++) {
-                const int e = tid + 256 * i, dd = e % CH * 8;
-                const float *p = K + (k0 + min(e / CH, end)) * a.ldk;
-                float u[4], v[4];
-
-                win_load4<CHANNELS>(p, dd, d, u);
-                win_load4<CHANNELS>(p, dd + 4, d, v);
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    kr[i][j] = u[j];
-                    kr[i][4 + j] = v[j];
-                }
-            }
-        }
-        if (!APART || !has_k) {
-#pragma unroll
-            for (int i = 0; i < NL; i++) {
-                const int e = vt + 256 * i, dd = CHANNELS == WIN_FULL ? e % DP : min(e % DP, d - 1);
-                const int c = ND == 1 ? e / DP : __builtin_amdgcn_readfirstlane(e / DP);
-
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    const int kk = (c >> 1) * 16 + (j >> 2) * 8 + (c & 1) * 4 + (j & 3);
-
-                    vr[i][j] = (V + (k0 + min(kk, end)) * a.ldv)[dd];
-                }
-            }
-        }
-        if (a.kmask)
-            next = col <= end && a.kmask[k0 + col];
-    };
-    /* keep: the kept keys of the registers' tile; values of others are zero,
-     * whatever they hold. */
-    auto stash = [&](split_u4 *ks, unsigned keep) {
-        split_u4 *vs = ks + 3 * PK, x, y, z;
-
-        if (has_k) {
-#pragma unroll
-            for (int i = 0; i < NL; i++) {
-                const int e = tid + 256 * i, key = e / CH;
-                const int at = key * CH + ((e % CH) ^ (key / RW % CH));
-
-                split8(kr[i], 1.0f, x, y, z);
-                ks[at] = x;
-                ks[PK + at] = y;
-                ks[2 * PK + at] = z;
-            }
-        }
-        if (!APART || !has_k) {
-#pragma unroll
-            for (int i = 0; i < NL; i++) {
-                const int e = vt + 256 * i, dd = e % DP, c = e / DP;
-                const int at = dd * 4 + (c ^ (dd >> 2 & 3));
-
-                if (keep != ~0u) {
-                    const unsigned k = keep >> ((c >> 1) * 16 + (c & 1) * 4);
-
-#pragma unroll
-                    for (int j = 0; j < 8; j++)
-                        vr[i][j] = k >> ((j >> 2) * 8 + (j & 3)) & 1 ? vr[i][j] : 0.0f;
-                }
-                split8(vr[i], SPLIT_UP, x, y, z);
-                vs[at] = x;
-                vs[PK + at] = y;
-                vs[2 * PK + at] = z;
-            }
-        }
-    };
-    constexpr int pa6[6] = {0, 2, 1, 0, 1, 0}, pb6[6] = {2, 0, 1, 1, 0, 0};
-    unsigned keep = ~0u;
-
-    if (t0 < t1) {
-        fetch(t0);
-        if (a.kmask)
-            keep = (unsigned)__ballot(next);
-        stash(lds[0], keep);
-        if (t0 + 1 < t1)
-            fetch(t0 + 1);
-    }
-    __syncthreads();
-    for (int t = t0; t < t1; t++) {
-        const split_u4 *ks = lds[(t - t0) & 1], *vs = ks + 3 * PK;
-        const int k0 = span.tile(t) * WIN_FKT;
-        /* Some row of the wave sees some key; all see all. */
-        const bool some = live && k0 <= hi1 && (k0 + WIN_FKT > lo0 || k0 < a.sinks);
-        const bool all = keep == ~0u && k0 + WIN_FKT - 1 <= hi0 && (k0 >= lo1 || k0 + WIN_FKT <= a.sinks);
-        const unsigned after = a.kmask && t + 1 < t1 ? (unsigned)__ballot(next) : ~0u;
-        float p[16];
-
-        if (some) {
-            win_f16x s;
-            float mx = -INFINITY, sum = 0.0f;
-            auto key = [&](int w, int st) {
-                return __builtin_bit_cast(split_b8, ks[w * PK + col * CH + ((2 * st + half) ^ (col / RW % CH))]);
-            };
-
-#pragma unroll
-            for (int e = 0; e < 16; e++)
-                s[e] = 0.0f;
-            /* The small products first, then the large ones. */
-#pragma unroll
-            for (int st = 0; st < 2 * ND; st++) {
-                const split_b8 kf[3] = {key(0, st), key(1, st), key(2, st)};
-
-#pragma unroll
-                for (int w = 0; w < 5; w++)
-                    s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-                        kf[pa6[w]], __builtin_bit_cast(split_b8, q[st][pb6[w]]), s, 0, 0, 0);
-            }
-#pragma unroll
-            for (int st = 0; st < 2 * ND; st++)
-                s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-                    key(0, st), __builtin_bit_cast(split_b8, q[st][0]), s, 0, 0, 0);
-            if (all) {
-                seen = 1;
-#pragma unroll
-                for (int e = 0; e < 16; e++)
-                    p[e] = s[e];
-            }
-            else {
-                unsigned see = keep & win_sees(a, lo, hi, k0);
-
-                seen |= see;
-                see >>= 4 * half;
-                /* Tested here: as conditions kept they fill the scalar
-                 * registers. */
-                asm volatile("" : "+v"(see));
-#pragma unroll
-                for (int e = 0; e < 16; e++)
-                    p[e] = see >> (8 * (e >> 2) + (e & 3)) & 1 ? s[e] : -INFINITY;
-            }
-#pragma unroll
-            for (int e = 0; e < 16; e++)
-                mx = fmaxf(mx, p[e]);
-            mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * (1.0f / WIN_QUP);
-            const bool need = mx > m + WIN_FTAU;
-
-            if (__any(need)) {
-                const float mn = need ? mx : m;
-                const float corr = need ? __builtin_amdgcn_exp2f(m - mn) : 1.0f;
-
-                m = mn;
-                l *= corr;
-#pragma unroll
-                for (int tt = 0; tt < ND; tt++)
-#pragma unroll
-                    for (int e = 0; e < 16; e++) {
-                        o[tt][e] *= corr;
-                        if (LOW)
-                            low[LOW ? tt : 0][e] *= corr;
-                    }
-            }
-            const float ref = m == -INFINITY ? 0.0f : m;
-
-#pragma unroll
-            for (int e = 0; e < 16; e++) {
-                p[e] = __builtin_amdgcn_exp2f(fmaf(p[e], 1.0f / WIN_QUP, -ref));
-                sum += p[e];
-            }
-            l += sum + __shfl_xor(sum, 32, 64);
-        }
-        /* The next tile into the other buffer, which was last read a tile ago,
-         * before the barrier; then its successor's loads. */
-        if (t + 1 < t1) {
-            stash(lds[(t + 1 - t0) & 1], after);
-            if (t + 2 < t1)
-                fetch(t + 2);
-        }
-        if (some) {
-#pragma unroll
-            for (int u = 0; u < 2; u++) {
-                float x[8];
-                split_u4 pp[3];
-
-#pragma unroll
-                for (int j = 0; j < 8; j++)
-                    x[j] = p[8 * u + j];
-                split8(x, SPLIT_UP, pp[0], pp[1], pp[2]);
-#pragma unroll
-                for (int tt = 0; tt < ND; tt++) {
-                    const int dd = tt * 32 + col;
-                    split_b8 vf[3];
-                    win_f16x &small = low[LOW ? tt : 0];
-
-                    if (!LOW)
-#pragma unroll
-                        for (int e = 0; e < 16; e++)
-                            small[e] = 0.0f;
-#pragma unroll
-                    for (int k = 0; k < 3; k++)
-                        vf[k] = __builtin_bit_cast(split_b8, vs[k * PK + dd * 4 + ((2 * u + half) ^ (dd >> 2 & 3))]);
-#pragma unroll
-                    for (int w = 0; w < 6; w++) {
-                        win_f16x &c = w == 5 ? o[tt] : small;
-
-                        c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-                            vf[pa6[w]], __builtin_bit_cast(split_b8, pp[pb6[w]]), c, 0, 0, 0);
-                    }
-                    if (!LOW)
-#pragma unroll
-                        for (int e = 0; e < 16; e++)
-                            o[tt][e] += small[e];
-                }
-            }
-        }
-        keep = after;
-        __syncthreads();
-    }
-    float z = l * 0.0f;
-
-#pragma unroll
-    for (int tt = 0; tt < ND; tt++)
-#pragma unroll
-        for (int e = 0; e < 16; e++) {
-            if (LOW)
-                o[tt][e] += low[LOW ? tt : 0][e];
-            z = fmaf(o[tt][e], 0.0f, z);
-        }
-    /* No probability at all for keys that are seen: their scores lie below the
-     * range of the split. */
-    win_finish<ND, false, WIN_FKT>(a, jb, span, t0, t1, parts, split, o, SPLIT_DOWN, m, l,
-                                   z != 0.0f || (l == 0.0f && seen), ps[wave], d);
-}
 
 /* ---- few rows ---------------------------------------------------------------------- */
 
@@ -1688,11 +1532,11 @@ template <bool CACHE> static void win_launch(struct ops *o, win_args &a, long lo
 {
     const int cus = o->ocl->cu_count > 0 ? o->ocl->cu_count : 256;
     const bool few = win_few(a, CACHE);
-    const int tr = few ? WIN_FEW : CACHE ? WIN_CROWS : WIN_ROWS;
+    const int tr = few ? WIN_FEW : 256;
     const long long heads = (long long)a.rows * a.nh, rows = heads / a.nhk; /* of a key head */
     const long long blocks = (CACHE ? rows / tr + a.c.n : (rows + tr - 1) / tr) * a.nhk;
 
-    a.splits = win_splits(a, blocks, keys, few ? 3 * cus : 4 * cus);
+    a.splits = win_splits(a, blocks, keys, few ? 3 * cus : cus);
     if (a.splits > 1) {
         a.part = fptr(work);
         a.ml = (float2 *)(a.part + heads * a.splits * win_width(a.d));
@@ -1701,27 +1545,25 @@ template <bool CACHE> static void win_launch(struct ops *o, win_args &a, long lo
     const hipStream_t s = stream_of(o->ocl);
 
     prof_scope ps(o->ocl, CACHE ? "attention_cache" : "attention_window");
-    const dim3 grid(grid_of(blocks * a.splits, tr == WIN_CROWS ? 512 : 256, "attention tiles")), block(256);
+    const dim3 grid(grid_of(blocks * a.splits, few ? 256 : 512, "attention tiles")), block(256), eight(512);
 
-#define WIN_FLOAT(ND_, CH_)                                                                    \
+#define WIN_FLOAT(ND_, CH_, KT_)                                                               \
     do {                                                                                       \
         if (few)                                                                               \
-            hipLaunchKernelGGL((win_few_kernel<ND_, false, CH_>), grid, block, 0, s, a);       \
+            hipLaunchKernelGGL((win_few_kernel<ND_, CACHE, CH_>), grid, block, 0, s, a);       \
         else                                                                                   \
-            hipLaunchKernelGGL((win_float_kernel<ND_, CH_>), grid, block, 0, s, a);            \
+            hipLaunchKernelGGL((win_tile_kernel<ND_, CACHE, CH_, 8, KT_>), grid, eight, 0, s, a); \
     } while (0)
-#define WIN_LAUNCH(ND_)                                                                     \
-    do {                                                                                    \
-        if (CACHE && few)                                                                       \
-            hipLaunchKernelGGL((win_few_kernel<ND_, true, WIN_ANY>), grid, block, 0, s, a);     \
-        else if (CACHE)                                                                         \
-            hipLaunchKernelGGL(win_cache_kernel<ND_>, grid, dim3(512), 0, s, a);                \
-        else if (a.d == 32 * ND_)                                                               \
-            WIN_FLOAT(ND_, WIN_FULL);                                                           \
-        else if (a.d % 4 == 0)                                                                  \
-            WIN_FLOAT(ND_, WIN_FOUR);                                                           \
-        else                                                                                    \
-            WIN_FLOAT(ND_, WIN_ANY);                                                            \
+#define WIN_LAUNCH(ND_)                                 \
+    do {                                                \
+        if constexpr (CACHE)                            \
+            WIN_FLOAT(ND_, WIN_ANY, 64);                \
+        else if (a.d == 32 * ND_)                       \
+            WIN_FLOAT(ND_, WIN_FULL, ND_ == 4 ? 32 : 64); \
+        else if (a.d % 4 == 0)                          \
+            WIN_FLOAT(ND_, WIN_FOUR, ND_ == 4 ? 32 : 64); \
+        else                                            \
+            WIN_FLOAT(ND_, WIN_ANY, ND_ == 4 ? 32 : 64);  \
     } while (0)
     if (a.d <= 32)
         WIN_LAUNCH(1);
