@@ -222,11 +222,11 @@ static __device__ __forceinline__ void win_put(const win_args &a, long long row,
         a.ml[u] = parts == 1 ? make_float2(0.0f, WIN_WRITTEN) : make_float2(m, l);
 }
 
-/* Parts that t tiles of keys are split into, of at most `splits`: at least 4
- * tiles each. */
-static __device__ __forceinline__ int win_parts(int tiles, int splits)
+/* Parts that t tiles of keys are split into, of at most `splits`: at least
+ * `least` tiles each. */
+static __device__ __forceinline__ int win_parts(int tiles, int splits, int least)
 {
-    return min(splits, max(1, tiles / 4));
+    return min(splits, max(1, tiles / least));
 }
 
 /* ---- a tile of rows over a cache ------------------------------------------------ */
@@ -412,8 +412,9 @@ template <int L> static __device__ __forceinline__ unsigned win_row_max(unsigned
     return v;
 }
 
-/* NW waves of 32 rows, KT keys at a time. */
-template <int ND, bool CACHE, int CHANNELS, int NW, int KT>
+/* NW / KG waves of 32 rows, KT keys at a time. KG = 2: half of the waves takes
+ * the first 32 of them and half the others, joined at the end. */
+template <int ND, bool CACHE, int CHANNELS, int NW, int KG, int KT>
 __global__ void __launch_bounds__(64 * NW, ND == 1 ? 4 : 2) win_tile_kernel(const win_args a)
 {
     constexpr int DP = 32 * ND, CH = DP / 8, P = CACHE ? 1 : 2; /* channels, 16-byte chunks of a key, f16 parts */
@@ -432,29 +433,31 @@ __global__ void __launch_bounds__(64 * NW, ND == 1 ? 4 : 2) win_tile_kernel(cons
         int top[NW / 2], low[NW / 2]; /* largest and smallest scale of a wave's values, exponents */
         int wild;
     };
-    static_assert(KT == 64 || !CACHE, "a lane a key");
+    constexpr int RG = NW / KG, TR = 32 * RG;    /* waves of rows, rows */
+    static_assert((KT == 64 || !CACHE) && KT >= 32 * KG, "a lane a key, 32 keys a wave");
     __shared__ tile_lds lds[2];
     __shared__ float ps[NW][64];
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, col = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = a.nh / a.nhk, d = CHANNELS == WIN_FULL ? DP : a.d, pitch = a.c.pitch;
     const long long rows = (long long)a.rows * g;
-    const int tiles = (int)(CACHE ? rows / (32 * NW) + a.c.n : (rows + 32 * NW - 1) / (32 * NW));
+    const int tiles = (int)(CACHE ? rows / TR + a.c.n : (rows + TR - 1) / TR);
     int split, kvh;
     const int tile = win_unit(a, tiles, split, kvh);
-    const win_job jb = win_job_of<CACHE, 32 * NW>(a, tile, kvh);
+    const win_job jb = win_job_of<CACHE, TR>(a, tile, kvh);
 
     if (jb.n <= 0)
         return;
     const int last = jb.r0 + jb.n - 1;
     const win_tiles span = win_span<KT>(a, jb.p0 + jb.r0 / g, jb.p0 + last / g, jb.nk);
-    const int parts = win_parts(span.n, a.splits);
+    const int parts = win_parts(span.n, a.splits, 4);
     /* This lane's row; lanes without one take the last. */
-    const int wr = jb.r0 + 32 * wave, r = min(wr + col, last), qi = r / g, h = jb.kvh * g + r - qi * g;
+    const int rg = wave % RG, kg = wave / RG;
+    const int wr = jb.r0 + 32 * rg, r = min(wr + col, last), qi = r / g, h = jb.kvh * g + r - qi * g;
     const long long row = jb.first + qi;
 
     if (split >= parts) {
-        if (wr + col <= last && half == 0)
+        if (wr + col <= last && half == 0 && kg == 0)
             a.ml[(row * a.nh + h) * a.splits + split] = make_float2(-INFINITY, 0.0f);
         return;
     }
@@ -791,7 +794,8 @@ __global__ void __launch_bounds__(64 * NW, ND == 1 ? 4 : 2) win_tile_kernel(cons
         const float vup = win_power(254 + WIN_VEXP - vexp);
 
 #pragma unroll
-        for (int part = 0; part < KT / 32; part++) {
+        for (int half_tile = 0; half_tile < KT / 32 / KG; half_tile++) {
+            const int part = KG > 1 ? kg : half_tile;
             const int k0 = base + 32 * part;
             /* Some row of the wave sees some key; all see all. */
             const bool some = live && k0 <= hi1 && (k0 + 32 > lo0 || k0 < a.sinks);
@@ -934,6 +938,34 @@ __global__ void __launch_bounds__(64 * NW, ND == 1 ? 4 : 2) win_tile_kernel(cons
         __syncthreads();
     }
     l += __shfl_xor(l, 32, 64);
+    if constexpr (KG > 1) {
+        /* The other keys' sums, through LDS: a lane's registers as they are. */
+        static_assert(sizeof(lds) >= RG * 64 * (16 * ND + 2) * 4, "room for the sums");
+        float *to = (float *)lds + rg * 64 + lane;
+
+        if (kg) {
+            to[0] = m;
+            to[RG * 64] = wild ? __builtin_nanf("") : l;
+#pragma unroll
+            for (int tt = 0; tt < ND; tt++)
+#pragma unroll
+                for (int e = 0; e < 16; e++)
+                    to[(2 + 16 * tt + e) * RG * 64] = o[tt][e];
+        }
+        __syncthreads();
+        if (kg)
+            return;
+        const float m2 = to[0], top = fmaxf(m, m2), ref = top == -INFINITY ? 0.0f : top;
+        const float c1 = __builtin_amdgcn_exp2f(m - ref), c2 = __builtin_amdgcn_exp2f(m2 - ref);
+
+        m = top;
+        l = l * c1 + to[RG * 64] * c2;
+#pragma unroll
+        for (int tt = 0; tt < ND; tt++)
+#pragma unroll
+            for (int e = 0; e < 16; e++)
+                o[tt][e] = o[tt][e] * c1 + to[(2 + 16 * tt + e) * RG * 64] * c2;
+    }
     float z = l * 0.0f;
 
 #pragma unroll
@@ -987,7 +1019,7 @@ __global__ void __launch_bounds__(256, CACHE && ND == 4 ? 3 : 2) win_few_kernel(
         return;
     const int last = jb.r0 + jb.n - 1;
     const win_tiles span = win_span<WIN_STEP>(a, jb.p0 + jb.r0 / g, jb.p0 + last / g, jb.nk);
-    const int parts = win_parts(span.n, a.splits);
+    const int parts = win_parts(span.n, a.splits, 2);
     /* This lane's row; lanes without one take the last. */
     const int r = min(jb.r0 + col, last), qi = r / g, h = jb.kvh * g + r - qi * g;
     const bool mine = jb.r0 + col <= last;
@@ -1510,33 +1542,62 @@ extern "C" size_t ops_attention_cache_work_bytes(int rows, int nh, int d)
     return ops_attention_window_work_bytes(rows, nh, d);
 }
 
-/* Splits of keys, `blocks` blocks of threads without any, of a call whose rows
- * see at most `keys` each. */
-static int win_splits(const win_args &a, long long blocks, long long keys, int want)
+/* The kernel of a call and its blocks of threads. */
+struct win_plan {
+    bool few;
+    int groups;            /* of a tile's keys, as KG of win_tile_kernel */
+    int tile, splits;      /* rows, parts of the keys */
+    long long blocks;      /* without the splits */
+};
+
+/* Rows see at most `keys` each. One block of tiles is held by a CU (32 channels:
+ * two); more of them than that, splits included, take a second round.
+ *
+ * Rows of a tile, us: 1601 rows of 16 heads of 64, window 321: 256 rows 40
+ * (112 blocks), 128 with the keys shared by two groups of waves 27; 6400 of 8
+ * heads of 32, window 641: 38, 36; 4096 of 16 on 4 key heads of 128 (256 blocks, 512), window
+ * 1025: 117, 145. Splits: 2000 rows of 4 heads on one of 128, window 2048, 32
+ * blocks: none 188, 2 107, 4 65, 8 54, 12 69 (a second round); 1601 rows as above
+ * in two parts 50. Few rows: 4 heads of 128 on 131005 keys, 64 parts 40, 96 40, 128 35,
+ * 192 37, 256 39; on 4096 float32 ones, 16 19, 32 16, 48 and more 13; 64
+ * sequences of unlike lengths, window 4096, 2 68, 4 62, 6 59, 8 64, 12 69: parts of
+ * unlike length want more of them, if they keep some 600 keys. */
+static win_plan win_plan_of(const win_args &a, bool cache, long long keys, int cus)
 {
-    long long n = std::min((want + blocks - 1) / blocks, keys / 128);
+    const long long heads = (long long)a.rows * a.nh, rows = heads / a.nhk; /* of a key head */
+    win_plan p;
 
-    n = std::min(n, WIN_PART_ROWS / ((long long)a.rows * a.nh));
-    return (int)std::max(1LL, std::min(n, (long long)WIN_MAX_SPLITS));
-}
+    p.few = rows <= (long long)WIN_FEW * (cache ? a.c.n : 1);
+    p.groups = 1;
+    p.tile = p.few ? WIN_FEW : 256;
+    auto blocks = [&](int tile) { return (cache ? rows / tile + a.c.n : (rows + tile - 1) / tile) * a.nhk; };
+    /* Half of the sequences have the tile more that they may need. */
+    auto filled = [&](int tile) {
+        return cache ? std::max((rows / tile + (a.c.n + 1) / 2) * a.nhk, (long long)a.nhk) : blocks(tile);
+    };
+    const long long held = (p.few || a.d <= 32 ? 2LL : 1LL) * cus;
 
-/* Whether a call goes by tiles of few rows. */
-static bool win_few(const win_args &a, bool cache)
-{
-    const long long rows = (long long)a.rows * (a.nh / a.nhk);
+    if (!p.few && (cache || a.d <= 64) && filled(128) <= held) {
+        p.groups = 2;
+        p.tile = 128;
+    }
+    p.blocks = blocks(p.tile);
+    long long n = held / filled(p.tile);
 
-    return rows <= (long long)WIN_FEW * (cache ? a.c.n : 1);
+    if (p.few && cache && a.c.n > 1)
+        n = std::max(n, std::min(6LL * cus / filled(p.tile), keys / 640));
+    n = std::min(n, std::min(keys / (p.few ? 64 : 128), WIN_PART_ROWS / heads));
+    p.splits = (int)std::max(1LL, std::min(n, (long long)WIN_MAX_SPLITS));
+    return p;
 }
 
 template <bool CACHE> static void win_launch(struct ops *o, win_args &a, long long keys, cl_mem work)
 {
     const int cus = o->ocl->cu_count > 0 ? o->ocl->cu_count : 256;
-    const bool few = win_few(a, CACHE);
-    const int tr = few ? WIN_FEW : 256;
-    const long long heads = (long long)a.rows * a.nh, rows = heads / a.nhk; /* of a key head */
-    const long long blocks = (CACHE ? rows / tr + a.c.n : (rows + tr - 1) / tr) * a.nhk;
+    const win_plan p = win_plan_of(a, CACHE, keys, cus);
+    const long long heads = (long long)a.rows * a.nh;
 
-    a.splits = win_splits(a, blocks, keys, few ? 3 * cus : cus);
+    a.splits = p.splits;
     if (a.splits > 1) {
         a.part = fptr(work);
         a.ml = (float2 *)(a.part + heads * a.splits * win_width(a.d));
@@ -1545,25 +1606,31 @@ template <bool CACHE> static void win_launch(struct ops *o, win_args &a, long lo
     const hipStream_t s = stream_of(o->ocl);
 
     prof_scope ps(o->ocl, CACHE ? "attention_cache" : "attention_window");
-    const dim3 grid(grid_of(blocks * a.splits, few ? 256 : 512, "attention tiles")), block(256), eight(512);
+    const dim3 grid(grid_of(p.blocks * a.splits, p.few ? 256 : 512, "attention tiles")), block(256), eight(512);
 
-#define WIN_FLOAT(ND_, CH_, KT_)                                                               \
-    do {                                                                                       \
-        if (few)                                                                               \
-            hipLaunchKernelGGL((win_few_kernel<ND_, CACHE, CH_>), grid, block, 0, s, a);       \
-        else                                                                                   \
-            hipLaunchKernelGGL((win_tile_kernel<ND_, CACHE, CH_, 8, KT_>), grid, eight, 0, s, a); \
+#define WIN_KERNEL(ND_, CH_, KG_, KT_) \
+    hipLaunchKernelGGL((win_tile_kernel<ND_, CACHE, CH_, 8, KG_, KT_>), grid, eight, 0, s, a)
+#define WIN_CHANNELS(ND_, CH_)                                                           \
+    do {                                                                                 \
+        if (p.few)                                                                       \
+            hipLaunchKernelGGL((win_few_kernel<ND_, CACHE, CH_>), grid, block, 0, s, a); \
+        else if constexpr (!CACHE && ND_ == 4)                                           \
+            WIN_KERNEL(ND_, CH_, 1, 32);                                                 \
+        else if (p.groups == 2)                                                          \
+            WIN_KERNEL(ND_, CH_, 2, 64);                                                 \
+        else                                                                             \
+            WIN_KERNEL(ND_, CH_, 1, 64);                                                 \
     } while (0)
-#define WIN_LAUNCH(ND_)                                 \
-    do {                                                \
-        if constexpr (CACHE)                            \
-            WIN_FLOAT(ND_, WIN_ANY, 64);                \
-        else if (a.d == 32 * ND_)                       \
-            WIN_FLOAT(ND_, WIN_FULL, ND_ == 4 ? 32 : 64); \
-        else if (a.d % 4 == 0)                          \
-            WIN_FLOAT(ND_, WIN_FOUR, ND_ == 4 ? 32 : 64); \
-        else                                            \
-            WIN_FLOAT(ND_, WIN_ANY, ND_ == 4 ? 32 : 64);  \
+#define WIN_LAUNCH(ND_)                   \
+    do {                                  \
+        if constexpr (CACHE)              \
+            WIN_CHANNELS(ND_, WIN_ANY);   \
+        else if (a.d == 32 * ND_)         \
+            WIN_CHANNELS(ND_, WIN_FULL);  \
+        else if (a.d % 4 == 0)            \
+            WIN_CHANNELS(ND_, WIN_FOUR);  \
+        else                              \
+            WIN_CHANNELS(ND_, WIN_ANY);   \
     } while (0)
     if (a.d <= 32)
         WIN_LAUNCH(1);
@@ -1572,7 +1639,8 @@ template <bool CACHE> static void win_launch(struct ops *o, win_args &a, long lo
     else
         WIN_LAUNCH(4);
 #undef WIN_LAUNCH
-#undef WIN_FLOAT
+#undef WIN_CHANNELS
+#undef WIN_KERNEL
     launch_check("attention tiles");
     if (a.splits > 1) {
         const bool wide = a.splits > 16;
