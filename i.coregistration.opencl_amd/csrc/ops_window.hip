@@ -76,6 +76,15 @@ static __device__ __forceinline__ unsigned win_below(int n)
     return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1;
 }
 
+/* x where bit `bit` of see is set, else minus infinity: a field and a bitwise
+ * choice, where 16 conditions would fill the scalar registers. */
+static __device__ __forceinline__ float win_if(unsigned see, int bit, float x)
+{
+    const unsigned on = (unsigned)__builtin_amdgcn_sbfe((int)see, bit, 1);
+
+    return __builtin_bit_cast(float, (on & __builtin_bit_cast(unsigned, x)) | (~on & 0xff800000u));
+}
+
 /* Bit i: a row of window lo .. hi sees key k0 + i, if it is kept. */
 static __device__ __forceinline__ unsigned win_sees(const win_args &a, int lo, int hi, int k0)
 {
@@ -393,12 +402,43 @@ static __device__ __forceinline__ void win_load4(const float *p, int c, int d, f
     }
 }
 
+#define WIN_NONE 0   /* exponent of the value scales before the first */
 #define WIN_LAG 12   /* a row's scale is at most 2^12 below the largest so far, its values smaller instead */
 #define WIN_DEEP 14  /* float32 values keep 22 bits 2^14 below that */
 #define WIN_CODES 24 /* codes keep all 2^24 below */
 
 typedef short win_s4 __attribute__((ext_vector_type(4)));
 typedef _Float16 win_h4 __attribute__((ext_vector_type(4)));
+
+typedef unsigned short win_us2 __attribute__((ext_vector_type(2)));
+
+/* Largest of a wave's upper and of its lower 16 bits, each. */
+static __device__ __forceinline__ unsigned win_wave_max2(unsigned v)
+{
+    auto larger = [](unsigned x, unsigned y) {
+        return __builtin_bit_cast(unsigned, __builtin_elementwise_max(__builtin_bit_cast(win_us2, x),
+                                                                      __builtin_bit_cast(win_us2, y)));
+    };
+
+    v = larger(v, (unsigned)dpp_i((int)v, 0xB1));
+    v = larger(v, (unsigned)dpp_i((int)v, 0x4E));
+    v = larger(v, (unsigned)dpp_i((int)v, 0x141));
+    v = larger(v, (unsigned)dpp_i((int)v, 0x140));
+    return larger(larger((unsigned)__builtin_amdgcn_readlane((int)v, 0), (unsigned)__builtin_amdgcn_readlane((int)v, 16)),
+                  larger((unsigned)__builtin_amdgcn_readlane((int)v, 32), (unsigned)__builtin_amdgcn_readlane((int)v, 48)));
+}
+
+/* The larger of lane l's and lane l ^ 32's: the halves swapped between two
+ * copies, which leaves both values in every lane. */
+static __device__ __forceinline__ float win_halves(float v)
+{
+    const unsigned b = __builtin_bit_cast(unsigned, v);
+    const auto s = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+    /* Copies: a bit cast of a vector's element takes the first one. */
+    const unsigned x = s[0], y = s[1];
+
+    return fmaxf(__builtin_bit_cast(float, x), __builtin_bit_cast(float, y));
+}
 
 /* Largest of the L lanes of a row, L = 4, 8 or 16. */
 template <int L> static __device__ __forceinline__ unsigned win_row_max(unsigned v)
@@ -430,8 +470,7 @@ __global__ void __launch_bounds__(64 * NW, ND == 1 ? 4 : 2) win_tile_kernel(cons
         win_u4 k[P * KT * KS], v[P * KT * VS];
         float ks[KT], vs[KT];
         unsigned long long keep;
-        int top[NW / 2], low[NW / 2]; /* largest and smallest scale of a wave's values, exponents */
-        int wild;
+        int top[NW / 2], low[NW / 2], wild; /* largest and smallest scale of a wave's values, exponents */
     };
     constexpr int RG = NW / KG, TR = 32 * RG;    /* waves of rows, rows */
     static_assert((KT == 64 || !CACHE) && KT >= 32 * KG, "a lane a key, 32 keys a wave");
@@ -521,8 +560,9 @@ __global__ void __launch_bounds__(64 * NW, ND == 1 ? 4 : 2) win_tile_kernel(cons
     float sc1[NU];              /* a cache's value scales, of the units */
     bool kept[NU], kept1 = false; /* of the units; of key `lane` */
     float sr = 0.0f;            /* a cache's scale of key `lane` */
+    unsigned byte[NU];          /* of the mask, as kept; looked at when they have come */
     int pg = -1, pg0 = t0;
-    int vexp = 12; /* exponent of the largest value scale so far; o counts in 2^(vexp - 127 - WIN_VEXP) */
+    int vexp = WIN_NONE; /* exponent of the largest value scale so far; o counts in 2^(vexp - 127 - WIN_VEXP) */
 
     /* Pages of 16 tiles from t on, a run of 16 keys a lane. */
     auto pages = [&](int t) {
@@ -598,12 +638,12 @@ __global__ void __launch_bounds__(64 * NW, ND == 1 ? 4 : 2) win_tile_kernel(cons
                 }
                 kept[i] = key <= end;
                 if (a.kmask && values)
-                    kept[i] = kept[i] && a.kmask[k0 + min(key, end)];
+                    byte[i] = a.kmask[k0 + min(key, end)];
             }
             if (hw == 0 && !values) {
                 kept1 = lane <= end && lane < KT;
                 if (a.kmask)
-                    kept1 = kept1 && a.kmask[k0 + min(lane, end)];
+                    byte[0] = a.kmask[k0 + min(lane, end)];
             }
         }
     };
@@ -658,7 +698,7 @@ __global__ void __launch_bounds__(64 * NW, ND == 1 ? 4 : 2) win_tile_kernel(cons
                 const float x = kept1 ? sr : 0.0f;
                 const bool bad = !(q8_mag(x) < 0x7f800000u);
                 const int e = bad ? 0 : (int)(q8_mag(x) >> 23), n = max(vexp - WIN_LAG - e, 0);
-                const int top = max(vexp, min((int)wave_umax(e), 253));
+                const int top = max(max(vexp, WIN_VEXP), min((int)wave_umax(e), 253));
                 /* Twice, as one power may pass the range. */
                 const float y = bad || n > WIN_CODES ? 0.0f : x * win_power(127 + n) * win_power(254 + WIN_VEXP - top);
                 const bool w = __any(bad || (x != 0.0f && y < WIN_VMIN));
@@ -671,39 +711,53 @@ __global__ void __launch_bounds__(64 * NW, ND == 1 ? 4 : 2) win_tile_kernel(cons
             }
         }
         else {
-            unsigned top = 0, least = 0; /* exponents; least: 255 less the smallest */
-            bool bad = false;
+            int top = 0, low = 255; /* exponents */
+            /* What a value's scale counts in now; other tiles' largest one may
+             * change that. */
+            const float vup = vexp == WIN_NONE ? 1.0f : win_power(254 + WIN_VEXP - vexp);
 
 #pragma unroll
             for (int i = 0; i < NU; i++) {
                 const int e = ht + HT * i, key = e / UC;
-                unsigned mag = 0;
+                float f[8];
                 win_u4 x, y;
 
 #pragma unroll
                 for (int j = 0; j < 8; j++)
-                    mag = max(mag, reg[i][j] & 0x7fffffffu);
-                mag = win_row_max<UC>(mag);
-                const bool none = values && (!kept[i] || mag >= 0x7f800000u);
+                    f[j] = __builtin_bit_cast(float, reg[i][j]);
+                /* Values of keys that are left out are zeros, whatever they
+                 * hold. */
+                const bool in = kept[i] && (!a.kmask || byte[i]);
+
+                if (values && __any(!in)) {
+#pragma unroll
+                    for (int j = 0; j < 8; j++)
+                        f[j] = in ? f[j] : 0.0f;
+                }
+                const float most = fmaxf(fmaxf(fmaxf(fabsf(f[0]), fabsf(f[1])), fmaxf(fabsf(f[2]), fabsf(f[3]))),
+                                         fmaxf(fmaxf(fabsf(f[4]), fabsf(f[5])), fmaxf(fabsf(f[6]), fabsf(f[7]))));
+                /* Infinities and NaN make the parts NaN, and the rows that meet
+                 * them are done again. */
+                const unsigned mag = win_row_max<UC>(__builtin_bit_cast(unsigned, most));
                 int ex = min(max((int)(mag >> 23), 15), 254);
 
                 if (values) {
-                    bad = bad || (kept[i] && (mag >= 0x7f800000u || (mag && ex - 14 < vexp - WIN_LAG - WIN_DEEP)));
+                    /* Too far below the largest: for the float32 path. */
+                    if (mag && ex - 14 < vexp - WIN_LAG - WIN_DEEP)
+                        low = 0;
                     ex = max(ex, vexp - WIN_LAG + 14);
-                    if (kept[i] && mag && mag < 0x7f800000u) {
-                        top = max(top, (unsigned)ex - 14);
-                        least = max(least, 269u - ex);
+                    if (mag) {
+                        top = max(top, ex - 14);
+                        low = min(low, ex - 14);
                     }
                 }
                 const float up = win_power(268 - ex);
 
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
-                    const float u = none ? 0.0f : __builtin_bit_cast(float, reg[i][2 * j]) * up;
-                    const float v = none ? 0.0f : __builtin_bit_cast(float, reg[i][2 * j + 1]) * up;
                     unsigned b, c;
 
-                    win_split(u, v, b, c);
+                    win_split(f[2 * j] * up, f[2 * j + 1] * up, b, c);
                     x[j] = b;
                     y[j] = c;
                 }
@@ -712,19 +766,18 @@ __global__ void __launch_bounds__(64 * NW, ND == 1 ? 4 : 2) win_tile_kernel(cons
                 to[key * stride + e % UC] = x;
                 to[(KT + key) * stride + e % UC] = y;
                 if (e % UC == 0)
-                    (values ? s.vs : s.ks)[key] = none ? 0.0f : mag >= 0x7f800000u ? __builtin_nanf("") : win_power(ex - 14);
+                    (values ? s.vs : s.ks)[key] = win_power(ex - 14) * (values ? vup : 1.0f);
             }
             if (values) {
-                top = wave_umax(top);
-                least = wave_umax(least);
-                bad = __any(bad);
+                const unsigned both = win_wave_max2((unsigned)top << 16 | (255u - low));
+
                 if (lane == 0) {
-                    s.top[hw] = (int)top | (bad ? 0x10000 : 0);
-                    s.low[hw] = 255 - (int)least;
+                    s.top[hw] = (int)(both >> 16);
+                    s.low[hw] = 255 - (int)(both & 0xffffu);
                 }
             }
             else if (hw == 0) {
-                const unsigned long long keep = __ballot(kept1);
+                const unsigned long long keep = __ballot(kept1 && (!a.kmask || byte[0]));
 
                 if (lane == 0)
                     s.keep = keep;
@@ -767,23 +820,36 @@ __global__ void __launch_bounds__(64 * NW, ND == 1 ? 4 : 2) win_tile_kernel(cons
         if (!values)
             next(t);
         if constexpr (!CACHE) {
-            int bits = 0, low = s.low[0];
+            int low = s.low[0];
 
 #pragma unroll
-            for (int w = 0; w < NW / 2; w++) {
-                bits |= s.top[w];
+            for (int w = 1; w < NW / 2; w++) {
                 low = min(low, s.low[w]);
-                top = max(top & 0xffff, s.top[w] & 0xffff);
+                top = max(top, s.top[w]);
             }
-            top = max(top, vexp);
-            wild = wild || bits >> 16 || low < top - WIN_VEXP - 3;
+            /* From where its power of two has one that undoes it. */
+            top = max(top > WIN_NONE ? max(top, WIN_VEXP + 2) : WIN_NONE, vexp);
+            /* Values from 2^127 on may be infinite. */
+            wild = wild || low < top - WIN_VEXP - 3 || top >= 240;
         }
         else
             wild = wild || s.wild;
         top = __builtin_amdgcn_readfirstlane(top);
+        /* A tile's float32 scales count in the exponent before it: its weights
+         * are 2^vshift of what they are in the sums. The first ones count in
+         * none. */
+        const bool first = !CACHE && vexp == WIN_NONE && top > WIN_NONE;
+        int vshift = 0;
+
         if (top != vexp) {
             const float down = win_power(max(127 + vexp - top, 1));
 
+            if (vexp > WIN_NONE) {
+                if (!CACHE)
+                    vshift = max(vexp - top, -64);
+                /* Sums that would pass the range below. */
+                wild = wild || top - vexp > 64;
+            }
             vexp = top;
 #pragma unroll
             for (int tt = 0; tt < ND; tt++)
@@ -791,7 +857,7 @@ __global__ void __launch_bounds__(64 * NW, ND == 1 ? 4 : 2) win_tile_kernel(cons
                 for (int e = 0; e < 16; e++)
                     o[tt][e] *= down;
         }
-        const float vup = win_power(254 + WIN_VEXP - vexp);
+        const float unshift = win_power(127 - vshift);
 
 #pragma unroll
         for (int half_tile = 0; half_tile < KT / 32 / KG; half_tile++) {
@@ -844,20 +910,16 @@ __global__ void __launch_bounds__(64 * NW, ND == 1 ? 4 : 2) win_tile_kernel(cons
                     x[e + 3] = sc[e + 3] * k.w;
                 }
                 if (keep != ~0u || k0 + 31 > hi0 || !(k0 >= lo1 || k0 + 32 <= a.sinks)) {
-                    unsigned see = keep & win_sees(a, lo, hi, k0);
+                    const unsigned see = (keep & win_sees(a, lo, hi, k0)) >> 4 * half;
 
-                    see >>= 4 * half;
-                    /* Tested here: as conditions kept they fill the scalar
-                     * registers. */
-                    asm volatile("" : "+v"(see));
 #pragma unroll
                     for (int e = 0; e < 16; e++)
-                        x[e] = see >> (8 * (e >> 2) + (e & 3)) & 1 ? x[e] : -INFINITY;
+                        x[e] = win_if(see, 8 * (e >> 2) + (e & 3), x[e]);
                 }
 #pragma unroll
                 for (int e = 0; e < 16; e++)
                     mx = fmaxf(mx, x[e]);
-                mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * qf;
+                mx = win_halves(mx) * qf;
                 const bool need = mx > m + WIN_TAU;
 
                 if (__any(need)) {
@@ -872,7 +934,7 @@ __global__ void __launch_bounds__(64 * NW, ND == 1 ? 4 : 2) win_tile_kernel(cons
                         for (int e = 0; e < 16; e++)
                             o[tt][e] *= corr;
                 }
-                const float ref = m == -INFINITY ? 0.0f : m;
+                const float ref = (m == -INFINITY ? 0.0f : m) - (float)vshift;
                 win_h8 vf[WIN_AHEAD][P];
                 /* Step i: keys 16 (i / ND) .., channels 32 (i % ND) ..; slot j of a
                  * lane half is the key that register 8 (i / ND) + j of the
@@ -900,8 +962,12 @@ __global__ void __launch_bounds__(64 * NW, ND == 1 ? 4 : 2) win_tile_kernel(cons
                     float4 v = *(const float4 *)&s.vs[32 * part + 2 * e + 4 * half];
                     unsigned u0, u1, v0, v1;
 
-                    if constexpr (!CACHE)
-                        v = make_float4(v.x * vup, v.y * vup, v.z * vup, v.w * vup);
+                    if (first) {
+                        const float up = win_power(254 + WIN_VEXP - vexp);
+
+                        v = make_float4(v.x * up, v.y * up, v.z * up, v.w * up);
+                        asm volatile(""); /* a branch, no products with 1 */
+                    }
 #pragma unroll
                     for (int j = 0; j < 4; j++) {
                         x[e + j] = __builtin_amdgcn_exp2f(fmaf(x[e + j], qf, -ref));
@@ -914,7 +980,7 @@ __global__ void __launch_bounds__(64 * NW, ND == 1 ? 4 : 2) win_tile_kernel(cons
                     pl[e / 8][e / 2 % 4] = v0;
                     pl[e / 8][e / 2 % 4 + 1] = v1;
                 }
-                l += sum;
+                l = fmaf(sum, unshift, l);
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int i = 0; i < 2 * ND; i++) {
