@@ -136,94 +136,139 @@ struct cache_args {
     long long ldk, ldv;
 };
 
-/* A row and key head: L lanes of four channels, 256 / L of them a block of
- * threads; blockIdx.y 0 is keys, 1 values. */
+/* A row's R key heads from h on: L lanes of four channels, 256 / L groups of
+ * them a block of threads; blockIdx.y 0 is keys, 1 values. */
 struct cache_item {
-    int row, h, ch, b, p, page;
+    int row, h, ch, p, page;
+    bool in; /* of a sequence */
 };
 
-template <int L> __device__ __forceinline__ bool cache_item_of(const cache_view &c, cache_item &it)
+/* The item of this group of lanes, `in` clear behind the last. */
+template <int L, int R> __device__ __forceinline__ cache_item cache_first(const cache_view &c)
 {
+    const int per = (c.nhk + R - 1) / R;
     const long long i = (long long)blockIdx.x * (256 / L) + threadIdx.x / L;
 
-    it.ch = 4 * (threadIdx.x % L);
-    it.row = (int)min(i / c.nhk, (long long)c.rows - 1);
-    it.h = (int)(i % c.nhk);
-    it.b = i < (long long)c.rows * c.nhk ? seq_of(c, it.row) : -1;
-    it.p = it.page = -1;
-    if (it.b < 0)
-        return false;
-    const long long p = (long long)max(c.len[it.b], 0) - (seq_start(c, it.b + 1) - it.row);
-
-    if (p >= 0 && p < (long long)c.ldt << c.page_log) {
-        it.p = (int)p;
-        it.page = seq_page(c, it.b, it.p);
-    }
-    return true;
+    return {(int)min(i / per, (long long)c.rows - 1), (int)(i % per) * R, 4 * (int)(threadIdx.x % L), 0, -1,
+            i < (long long)c.rows * per};
 }
 
-template <int L> __global__ void __launch_bounds__(256) cache_write_kernel(const cache_args a)
+/* Its place. The row's sequence is the last of those that start at or before
+ * it, looked for by L lanes at a time. */
+template <int L, int R> __device__ __forceinline__ void cache_look_up(const cache_view &c, cache_item &it)
+{
+    const int sub = threadIdx.x % L, at = threadIdx.x & 63 & ~(L - 1);
+    int count = 0;
+
+    for (int b = 0; b < c.n; b += L) {
+        const bool before = b + sub < c.n && seq_start(c, min(b + sub, c.n - 1)) <= it.row;
+        const int n = __popcll(__ballot(before) >> at & ((1ull << L) - 1));
+
+        count += n;
+        if (n < L)
+            break;
+    }
+    const int b = max(count - 1, 0), end = seq_start(c, b + 1);
+    const long long p = (long long)max(c.len[b], 0) - (end - it.row);
+
+    it.in = it.in && count > 0 && it.row < end;
+    if (it.in && p >= 0 && p < (long long)c.ldt << c.page_log) {
+        it.p = (int)p;
+        it.page = seq_page(c, b, it.p);
+    }
+}
+
+/* Both kernels are bound by memory, and ask for R heads' lines before they
+ * use the first: some 21000 tokens of 8 heads of 64, 86 MB of float32 and 23 of codes
+ * and scales, 24 us written and 20 read; one head at a time 32 and 33. */
+template <int L, int R> __global__ void __launch_bounds__(256) cache_write_kernel(const cache_args a)
 {
     const bool values = blockIdx.y;
     const cache_view &c = a.c;
-    cache_item it;
-    const bool in = cache_item_of<L>(c, it) && it.page >= 0;
-    const float *x = (values ? a.V + it.row * a.ldv : a.K + it.row * a.ldk) + (long long)it.h * c.d;
-    float v[4];
-    unsigned mag = 0;
+    cache_item it = cache_first<L, R>(c);
+    const float *x = values ? a.V + it.row * a.ldv : a.K + it.row * a.ldk;
+    float v[R][4];
 
-    load4_row(x, it.ch, c.d, v);
+    /* On their way while the place is looked up. */
 #pragma unroll
-    for (int j = 0; j < 4; j++)
-        mag = max(mag, q8_mag(v[j]));
-    mag = max(mag, (unsigned)dpp_i((int)mag, 0xB1));
-    mag = max(mag, (unsigned)dpp_i((int)mag, 0x4E));
-    mag = max(mag, (unsigned)dpp_i((int)mag, 0x141));
-    if (L > 8)
-        mag = max(mag, (unsigned)dpp_i((int)mag, 0x140));
-    if (L > 16)
-        mag = max(mag, (unsigned)__shfl_xor((int)mag, 16, 64));
-    const q8_scale q = q8_scale_of(mag);
+    for (int i = 0; i < R; i++)
+        load4_row(x + (long long)min(it.h + i, c.nhk - 1) * c.d, it.ch, c.d, v[i]);
+    cache_look_up<L, R>(c, it);
 
-    if (!in)
-        return;
-    const long long at = cache_row(c, it.page, it.h, it.p);
+#pragma unroll
+    for (int i = 0; i < R; i++) {
+        unsigned mag = 0;
 
-    if (it.ch < c.pitch)
-        *(unsigned *)((values ? c.vc : c.kc) + at * c.pitch + it.ch) =
-            q8_code4(v[0], v[1], v[2], v[3], q.r);
-    if (it.ch == 0)
-        (values ? c.vs : c.ks)[at] = q.s;
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            mag = max(mag, q8_mag(v[i][j]));
+        mag = max(mag, (unsigned)dpp_i((int)mag, 0xB1));
+        mag = max(mag, (unsigned)dpp_i((int)mag, 0x4E));
+        mag = max(mag, (unsigned)dpp_i((int)mag, 0x141));
+        if (L > 8)
+            mag = max(mag, (unsigned)dpp_i((int)mag, 0x140));
+        if (L > 16)
+            mag = max(mag, (unsigned)__shfl_xor((int)mag, 16, 64));
+        const q8_scale q = q8_scale_of(mag);
+
+        if (it.page < 0 || it.h + i >= c.nhk)
+            continue;
+        const long long at = cache_row(c, it.page, it.h + i, it.p);
+
+        if (it.ch < c.pitch)
+            *(unsigned *)((values ? c.vc : c.kc) + at * c.pitch + it.ch) =
+                q8_code4(v[i][0], v[i][1], v[i][2], v[i][3], q.r);
+        if (it.ch == 0)
+            (values ? c.vs : c.ks)[at] = q.s;
+    }
 }
 
-template <int L> __global__ void __launch_bounds__(256) cache_read_kernel(const cache_args a)
+template <int L, int R> __global__ void __launch_bounds__(256) cache_read_kernel(const cache_args a)
 {
     const bool values = blockIdx.y;
     const cache_view &c = a.c;
     float *to = values ? a.V : a.K;
-    cache_item it;
+    cache_item it = cache_first<L, R>(c);
+    int w[R];
+    float s[R];
 
-    if (!to || !cache_item_of<L>(c, it))
+    if (!to)
         return;
-    float *y = to + it.row * (values ? a.ldv : a.ldk) + (long long)it.h * c.d;
-    float v[4] = {0, 0, 0, 0};
-
-    if (it.page >= 0 && it.ch < c.pitch) {
-        const long long at = cache_row(c, it.page, it.h, it.p);
-        const int w = *(const int *)((values ? c.vc : c.kc) + at * c.pitch + it.ch);
-        const float s = (values ? c.vs : c.ks)[at];
-
+    cache_look_up<L, R>(c, it);
+    if (!it.in)
+        return;
 #pragma unroll
-        for (int j = 0; j < 4; j++)
-            v[j] = (float)(w << (24 - 8 * j) >> 24) * s;
+    for (int i = 0; i < R; i++) {
+        w[i] = 0;
+        s[i] = 0.0f;
+        if (it.page >= 0 && it.ch < c.pitch) {
+            const long long at = cache_row(c, it.page, min(it.h + i, c.nhk - 1), it.p);
+
+            w[i] = *(const int *)((values ? c.vc : c.kc) + at * c.pitch + it.ch);
+            s[i] = (values ? c.vs : c.ks)[at];
+        }
     }
-    if (it.ch + 4 <= c.d)
-        store4(y + it.ch, v[0], v[1], v[2], v[3]);
-    else {
+    float *y = to + it.row * (values ? a.ldv : a.ldk) + it.ch;
+
+#pragma unroll
+    for (int i = 0; i < R; i++) {
+        float v[4];
+
+        if (it.h + i >= c.nhk)
+            continue;
 #pragma unroll
         for (int j = 0; j < 4; j++)
-            if (it.ch + j < c.d)
-                y[it.ch + j] = v[j];
+            v[j] = (float)(w[i] << (24 - 8 * j) >> 24) * s[i];
+        float *z = y + (long long)(it.h + i) * c.d;
+
+        if (it.ch + 4 <= c.d)
+            store4(z, v[0], v[1], v[2], v[3]);
+        else {
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (it.ch + j < c.d)
+                    z[j] = v[j];
+        }
     }
 }
 
@@ -268,18 +313,29 @@ static void cache_move(struct ops *o, const struct ops_cache *c, const struct op
     if (!write && K.buf && V.buf)
         need_rows_apart(a.K, a.ldk, w, rows, a.V, a.ldv, w, rows, op, "K and V");
     const int L = c->d <= 32 ? 8 : c->d <= 64 ? 16 : 32;
-    const long long items = (long long)rows * c->nhk;
+    /* Heads a group of lanes, where one a group fills the CUs twice. 1 and 4, us,
+     * written and read: 4 heads of 128, 128 rows 5.0, 6.3; some 300 5.8, 7.0; 1200
+     * 8.4, 8.1; 3000 13.8, 11.7; 8 heads of 32, 3000 9.4, 8.6. */
+    const int R = c->nhk >= 4 && (long long)rows * c->nhk * L >= 512LL * o->ocl->cu_count ? 4 : 1;
+    const long long items = (long long)rows * ((c->nhk + R - 1) / R);
     const unsigned n = grid_of((items * L + 255) / 256, 2 * 256, op);
     const device_scope on(o->ocl);
     const hipStream_t st = stream_of(o->ocl);
 
     prof_scope ps(o->ocl, write ? "cache_write" : "cache_read");
-#define CACHE_LAUNCH(L_)                                                                  \
-    do {                                                                                  \
-        if (write)                                                                        \
-            hipLaunchKernelGGL(cache_write_kernel<L_>, dim3(n, 2), dim3(256), 0, st, a);  \
-        else                                                                              \
-            hipLaunchKernelGGL(cache_read_kernel<L_>, dim3(n, 2), dim3(256), 0, st, a);   \
+#define CACHE_KERNEL(L_, R_)                                                                  \
+    do {                                                                                      \
+        if (write)                                                                            \
+            hipLaunchKernelGGL((cache_write_kernel<L_, R_>), dim3(n, 2), dim3(256), 0, st, a); \
+        else                                                                                  \
+            hipLaunchKernelGGL((cache_read_kernel<L_, R_>), dim3(n, 2), dim3(256), 0, st, a);  \
+    } while (0)
+#define CACHE_LAUNCH(L_)         \
+    do {                         \
+        if (R == 4)              \
+            CACHE_KERNEL(L_, 4); \
+        else                     \
+            CACHE_KERNEL(L_, 1); \
     } while (0)
     if (L == 8)
         CACHE_LAUNCH(8);
@@ -288,6 +344,7 @@ static void cache_move(struct ops *o, const struct ops_cache *c, const struct op
     else
         CACHE_LAUNCH(32);
 #undef CACHE_LAUNCH
+#undef CACHE_KERNEL
     launch_check(op);
 }
 

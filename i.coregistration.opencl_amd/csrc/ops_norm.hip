@@ -75,7 +75,10 @@ __device__ __forceinline__ void store4_row(float *row, int c, int n, const float
 /* W waves a row, four channels a lane and step. Rows of up to 256 NV W channels
  * stay in registers between the sum, the maximum and the codes; longer ones
  * (NV = 0) are read again: h, where it is kept, from there, as it may lie over
- * x or r. */
+ * x or r. Bound by memory, which each value passes once: 12805 x 4096 with the
+ * residual, to h and codes (682 MB), 129 us, 5.3 TB/s (a large copy 4.8); 3202 x
+ * 1024 to h and y (52 MB, some of it still in the last cache) 9 us. The 64-bit
+ * products and sums run beside the loads. */
 template <int NV, int W>
 __global__ void __launch_bounds__(W > 4 ? 64 * W : 256) rms_norm_kernel(const norm_args a)
 {
@@ -312,13 +315,20 @@ extern "C" void ops_rms_norm(struct ops *o, long rows, int C, struct opnd X, str
                 b.S += r;
             }
             b.rows = n;
+            /* Few rows, several waves each, us: of 1024 channels 1 row 4.2 -> 2.9,
+             * 512 rows 5.0 -> 3.5, 2048 6.3 -> 6.0, 3202 9.2 -> 9.4; of 4096, 16 waves
+             * for 4, 1 row 4.6 -> 3.8, 256 rows 5.6 -> 4.8, 512 6.3 -> 6.5. */
 #define NORM_LAUNCH(NV_, W_)                                                          \
     hipLaunchKernelGGL((rms_norm_kernel<NV_, W_>), dim3((unsigned)(W_ > 1 ? n : (n + 3) / 4)), \
                        dim3(W_ > 4 ? 64 * W_ : 256), 0, s, b)
             if (C <= 256)
                 NORM_LAUNCH(1, 1);
+            else if (C <= 1024 && n < 2560)
+                NORM_LAUNCH(1, 4);
             else if (C <= 1024)
                 NORM_LAUNCH(4, 1);
+            else if (C <= 4096 && n < 384)
+                NORM_LAUNCH(1, 16);
             else if (C <= 4096)
                 NORM_LAUNCH(4, 4);
             else if (C <= 16384)
