@@ -470,7 +470,9 @@ __global__ void __launch_bounds__(64 * NW, ND == 1 ? 4 : 2) win_tile_kernel(cons
         win_u4 k[P * KT * KS], v[P * KT * VS];
         float ks[KT], vs[KT];
         unsigned long long keep;
-        int top[NW / 2], low[NW / 2], wild; /* largest and smallest scale of a wave's values, exponents */
+        /* Largest and smallest scale of a wave's values, exponents; zero: some
+         * are zeros alone. */
+        int top[NW / 2], low[NW / 2], zero[NW / 2], wild, lag;
     };
     constexpr int RG = NW / KG, TR = 32 * RG;    /* waves of rows, rows */
     static_assert((KT == 64 || !CACHE) && KT >= 32 * KG, "a lane a key, 32 keys a wave");
@@ -509,7 +511,7 @@ __global__ void __launch_bounds__(64 * NW, ND == 1 ? 4 : 2) win_tile_kernel(cons
     win_u4 qh[2 * ND], ql[2 * ND];
     win_f16x o[ND];
     float m = -INFINITY, l = 0.0f, qf;
-    bool wild = false;
+    bool wild = false, lag = false;
 
     /* The query times scale and log2 e, times a power of two that brings its
      * largest magnitude to 2^14 .. 2^15; qf takes it back. */
@@ -702,16 +704,19 @@ __global__ void __launch_bounds__(64 * NW, ND == 1 ? 4 : 2) win_tile_kernel(cons
                 /* Twice, as one power may pass the range. */
                 const float y = bad || n > WIN_CODES ? 0.0f : x * win_power(127 + n) * win_power(254 + WIN_VEXP - top);
                 const bool w = __any(bad || (x != 0.0f && y < WIN_VMIN));
+                const bool lags = __any(kept1 && e < top - WIN_LAG);
 
                 s.vs[lane] = y;
                 if (lane == 0) {
                     s.top[0] = top;
                     s.wild = w;
+                    s.lag = lags;
                 }
             }
         }
         else {
             int top = 0, low = 255; /* exponents */
+            bool zero = false;
             /* What a value's scale counts in now; other tiles' largest one may
              * change that. */
             const float vup = vexp == WIN_NONE ? 1.0f : win_power(254 + WIN_VEXP - vexp);
@@ -742,14 +747,12 @@ __global__ void __launch_bounds__(64 * NW, ND == 1 ? 4 : 2) win_tile_kernel(cons
                 int ex = min(max((int)(mag >> 23), 15), 254);
 
                 if (values) {
-                    /* Too far below the largest: for the float32 path. */
-                    if (mag && ex - 14 < vexp - WIN_LAG - WIN_DEEP)
-                        low = 0;
-                    ex = max(ex, vexp - WIN_LAG + 14);
                     if (mag) {
                         top = max(top, ex - 14);
                         low = min(low, ex - 14);
                     }
+                    zero = zero || (in && !mag);
+                    ex = max(ex, vexp - WIN_LAG + 14);
                 }
                 const float up = win_power(268 - ex);
 
@@ -770,10 +773,12 @@ __global__ void __launch_bounds__(64 * NW, ND == 1 ? 4 : 2) win_tile_kernel(cons
             }
             if (values) {
                 const unsigned both = win_wave_max2((unsigned)top << 16 | (255u - low));
+                const bool zeros = __any(zero);
 
                 if (lane == 0) {
                     s.top[hw] = (int)(both >> 16);
                     s.low[hw] = 255 - (int)(both & 0xffffu);
+                    s.zero[hw] = zeros;
                 }
             }
             else if (hw == 0) {
@@ -820,20 +825,25 @@ __global__ void __launch_bounds__(64 * NW, ND == 1 ? 4 : 2) win_tile_kernel(cons
         if (!values)
             next(t);
         if constexpr (!CACHE) {
-            int low = s.low[0];
+            int low = s.low[0], zero = s.zero[0];
 
 #pragma unroll
             for (int w = 1; w < NW / 2; w++) {
                 low = min(low, s.low[w]);
                 top = max(top, s.top[w]);
+                zero |= s.zero[w];
             }
             /* From where its power of two has one that undoes it. */
             top = max(top > WIN_NONE ? max(top, WIN_VEXP + 2) : WIN_NONE, vexp);
-            /* Values from 2^127 on may be infinite. */
-            wild = wild || low < top - WIN_VEXP - 3 || top >= 240;
+            /* Too far below the largest before this tile or, as they were
+             * staged without it, in it; values from 2^127 on may be infinite. */
+            wild = wild || low < vexp - WIN_LAG - WIN_DEEP || max(low, vexp - WIN_LAG) < top - WIN_VEXP - 3 || top >= 240;
+            lag = lag || zero || low < top - WIN_LAG;
         }
-        else
+        else {
             wild = wild || s.wild;
+            lag = lag || s.lag;
+        }
         top = __builtin_amdgcn_readfirstlane(top);
         /* A tile's float32 scales count in the exponent before it: its weights
          * are 2^vshift of what they are in the sums. The first ones count in
@@ -1032,13 +1042,20 @@ __global__ void __launch_bounds__(64 * NW, ND == 1 ? 4 : 2) win_tile_kernel(cons
             for (int e = 0; e < 16; e++)
                 o[tt][e] = o[tt][e] * c1 + to[(2 + 16 * tt + e) * RG * 64] * c2;
     }
-    float z = l * 0.0f;
+    float z = l * 0.0f, most = 0.0f;
 
 #pragma unroll
     for (int tt = 0; tt < ND; tt++)
 #pragma unroll
-        for (int e = 0; e < 16; e++)
+        for (int e = 0; e < 16; e++) {
             z = fmaf(o[tt][e], 0.0f, z);
+            most = fmaxf(most, fabsf(o[tt][e]));
+        }
+    /* A weight times scale is off by up to 2^-25, which times the largest value
+     * is 2^-35 of that: where values are far smaller, or zeros, and the output
+     * is so too, that may be many units of the output. */
+    if (lag && win_halves(most) < l * (CACHE ? 0x1p3f : 0x1p11f))
+        wild = true;
     win_finish<ND, CACHE, KT>(a, jb, span, t0, t1, parts, split, o, win_power(max(vexp - WIN_VEXP, 1)), m, l,
                               wild || z != 0.0f, ps[wave], d);
 }

@@ -356,8 +356,14 @@ void ops_cache_read(struct ops *o, const struct ops_cache *c,
  * for ops_attention_blocks. No key left: zeros. A NaN among the seen scores
  * makes the row NaN; what unseen keys and values hold does not matter; a key's
  * weight under 2^-126 of the row's largest may count as zero, and sums of
- * values from 2^115 on may pass float32's range before they are divided. O may
- * be Q (same offset and ld), any other overlap of O is an error. */
+ * values from 2^115 on may pass float32's range before they are divided.
+ * Sums, maxima and outputs are float32's. What enters the products may be
+ * rounded: queries, keys and values to 22 bits or to 2^-39 of their row and
+ * head's largest; a weighted value to 2^-23 of itself or to 2^-35 of the
+ * largest value among the keys up to the row's last, but not to more than 2^-20
+ * of the row and head's largest output. O may be Q (same offset and ld), any
+ * other overlap of O is an error. work: what a call needs while it runs; calls
+ * that may run at once, recorded ones too, have one each. */
 size_t ops_attention_window_work_bytes(int Nq, int nh, int d);
 void ops_attention_window(struct ops *o, struct opnd Q, struct opnd K,
                           struct opnd V, struct opnd O, int Nq, int Nk, int nh,
