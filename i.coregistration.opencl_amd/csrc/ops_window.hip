@@ -297,26 +297,36 @@ static __device__ __forceinline__ win_job win_job_of(const win_args &a, int tile
     }
     /* Sequence b has the tiles of TR rows from start[b] g / TR + b on, one more than
      * it can need; the last that starts at or before this one, 64 sequences
-     * at a time. */
-    auto from = [&](int b) { return (long long)seq_start(a.c, b) * g / TR + b; };
+     * at a time, each lane with all that is known of one. None: the tile is of
+     * rows before the first sequence. */
     const int lane = threadIdx.x & 63;
-    int count = 0;
+    int end = 0, len = 0;
+    long long from = 0;
+    bool any = false;
 
     for (int b0 = 0; b0 < a.c.n; b0 += 64) {
-        const int n = __popcll(__ballot(b0 + lane < a.c.n && from(min(b0 + lane, a.c.n - 1)) <= tile));
+        const int b = min(b0 + lane, a.c.n - 1), s0 = seq_start(a.c, b), s1 = seq_start(a.c, b + 1), l = a.c.len[b];
+        const int n = __popcll(__ballot(b0 + lane < a.c.n && (long long)s0 * g / TR + b <= tile));
 
-        count += n;
+        if (n) {
+            any = true;
+            j.b = b0 + n - 1;
+            j.first = __builtin_amdgcn_readlane(s0, n - 1);
+            end = __builtin_amdgcn_readlane(s1, n - 1);
+            len = max(__builtin_amdgcn_readlane(l, n - 1), 0);
+            from = (long long)j.first * g / TR + j.b;
+        }
         if (n < 64)
             break;
     }
-    j.b = max(count - 1, 0);
-    j.first = seq_start(a.c, j.b);
-    const int rows = max(seq_start(a.c, j.b + 1) - j.first, 0);
+    if (!any)
+        return j;
+    const int rows = max(end - j.first, 0);
 
-    j.r0 = (int)max(tile - from(j.b), 0LL) * TR;
+    j.r0 = (int)(tile - from) * TR;
     j.n = (int)min((long long)rows * g - j.r0, (long long)TR);
-    j.p0 = max(a.c.len[j.b], 0) - rows;
-    j.nk = seq_len(a.c, j.b);
+    j.p0 = len - rows;
+    j.nk = (int)min((long long)len, (long long)a.c.ldt << a.c.page_log);
     return j;
 }
 

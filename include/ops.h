@@ -327,7 +327,7 @@ struct ops_cache {
  * position len[b] - (start[b + 1] - start[b]) + i. Position i is place i % page
  * of page table[b ldt + i / page] (int32). A position that is negative or
  * behind the table, or whose entry is no page (-1: given back), is not kept.
- * Rows behind start[n] belong to no sequence. */
+ * Rows before start[0] and behind start[n] belong to no sequence. */
 struct ops_seqs {
     cl_mem start, len, table;
     cl_int n, ldt;

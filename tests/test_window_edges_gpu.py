@@ -268,3 +268,21 @@ def test_single_tokens_from_a_graph(dev, ic):
             dev.finish()
     finally:
         ic.lib().ocl_graph_free(graph)
+
+
+@pytest.mark.parametrize("before,new", [(600, 1), (600, 200), (1, 40)])
+def test_rows_before_the_first_sequence(before, new, dev, ic):
+    """Rows before start[0] are left as they are, and the first sequence's are
+    computed once, over their queries too."""
+    kv, h, d, page, n = 2, 8, 32, 16, 300
+    rng = np.random.default_rng(before + new)
+    held = Held(dev, ic, 40, page, kv, d)
+    table = rng.permutation(40)[:38].reshape(2, 19).astype(np.int32)
+    start, lengths, rows = [before, before + new, before + new + 3], [n, 77], before + new + 5
+    q, scale = 1.5 * rng.standard_normal((rows, h, d)).astype(np.float32), np.float32(d ** -0.5)
+    Q, s = dev.upload(q), held.seqs(start, lengths, table)
+    work = dev.alloc(dev.api.ops_attention_cache_work_bytes(rows, h, d))
+    call(dev, ic, held, s, rows, Q, Q, h, -1, 0, scale, work)
+    got = dev.read(Q).reshape(q.shape)
+    assert np.array_equal(got[:before], q[:before]) and np.array_equal(got[start[2]:], q[start[2]:])
+    look(got, q, held, start, lengths, table, -1, 0, scale, rng)
