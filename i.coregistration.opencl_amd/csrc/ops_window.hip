@@ -1514,33 +1514,48 @@ __global__ void __launch_bounds__(256, CACHE && ND == 4 ? 3 : 2) win_few_kernel(
 }
 
 /* Parts of a row and head joined, by W waves: softmax over all of them from
- * their maxima and sums, then DP / 4 lanes a part, 256 W / DP parts at a time. */
+ * their maxima and sums, then LV lanes of four channels a part, GV parts at a
+ * time, the first of them on their way before the maxima have come. W = 4: 32
+ * channels a block. */
 template <int DP, int W> __global__ void __launch_bounds__(256) win_merge_kernel(const win_args a)
 {
-    constexpr int RB = 4 / W, LV = DP / 4, GV = 64 * W / LV; /* rows of a block; groups of lanes of a row */
+    constexpr int RB = 4 / W, CB = W > 1 ? DP / 32 : 1; /* rows of a block, blocks of a row */
+    constexpr int LV = DP / CB / 4, GV = 64 * W / LV;
     __shared__ float ws[RB][WIN_MAX_SPLITS];
     __shared__ float red[2][4];
     __shared__ float4 sums[W > 1 ? 4 : 1][LV];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int sub = wave % W, mine = wave / W, t = 64 * sub + lane, n = a.splits;
-    const long long u = (long long)blockIdx.x * RB + mine;
+    const long long u = (long long)(blockIdx.x / CB) * RB + mine;
 
     if (u >= (long long)a.rows * a.nh)
         return;
-    const int row = (int)(u / a.nh), h = (int)(u % a.nh), c = 4 * (t % LV);
+    const int row = (int)(u / a.nh), h = (int)(u % a.nh), c = DP / CB * (blockIdx.x % CB) + 4 * (t % LV);
     const float2 *ml = a.ml + u * n;
     const float *part = a.part + u * n * DP + c;
-
-    if ((a.c.n && seq_of(a.c, row) < 0) || ml[0].y == WIN_WRITTEN)
-        return;
     /* At most WIN_MAX_SPLITS = 256 parts: 4 a lane of a wave. */
     constexpr int NS = WIN_MAX_SPLITS / 64 / W;
     float2 x[NS];
+    float4 p[4];
     float m = -INFINITY, l = 0.0f, o[4] = {0, 0, 0, 0};
+    auto fetch = [&](int s0) {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            p[i] = *(const float4 *)(part + (long long)min(s0 + i * GV, n - 1) * DP);
+    };
 
 #pragma unroll
+    for (int i = 0; i < NS; i++)
+        x[i] = ml[min(t + 64 * W * i, n - 1)];
+    const float written = ml[0].y;
+
+    fetch(t / LV);
+    if (written == WIN_WRITTEN || (a.c.n && (row < seq_start(a.c, 0) || row >= seq_start(a.c, a.c.n))))
+        return;
+#pragma unroll
     for (int i = 0; i < NS; i++) {
-        x[i] = t + 64 * W * i < n ? ml[t + 64 * W * i] : make_float2(-INFINITY, 0.0f);
+        if (t + 64 * W * i >= n)
+            x[i] = make_float2(-INFINITY, 0.0f);
         m = fmaxf(m, x[i].x);
     }
     m = wave_max_full(m);
@@ -1569,23 +1584,18 @@ template <int DP, int W> __global__ void __launch_bounds__(256) win_merge_kernel
         __builtin_amdgcn_wave_barrier();
     /* Parts of no weight hold nothing, or what does not count. */
     for (int s0 = t / LV; s0 < n; s0 += 4 * GV) {
-        float4 p[4];
-        float w[4];
-
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const int s = s0 + i * GV;
+            const float w = s < n ? ws[mine][s] : 0.0f;
 
-            w[i] = s < n ? ws[mine][s] : 0.0f;
-            p[i] = w[i] != 0.0f ? *(const float4 *)(part + (long long)s * DP) : make_float4(0, 0, 0, 0);
+            o[0] = w != 0.0f ? fmaf(w, p[i].x, o[0]) : o[0];
+            o[1] = w != 0.0f ? fmaf(w, p[i].y, o[1]) : o[1];
+            o[2] = w != 0.0f ? fmaf(w, p[i].z, o[2]) : o[2];
+            o[3] = w != 0.0f ? fmaf(w, p[i].w, o[3]) : o[3];
         }
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            o[0] = fmaf(w[i], p[i].x, o[0]);
-            o[1] = fmaf(w[i], p[i].y, o[1]);
-            o[2] = fmaf(w[i], p[i].z, o[2]);
-            o[3] = fmaf(w[i], p[i].w, o[3]);
-        }
+        if (s0 + 4 * GV < n)
+            fetch(s0 + 4 * GV);
     }
 #pragma unroll
     for (int s = LV; s < 64; s *= 2)
@@ -1737,7 +1747,7 @@ template <bool CACHE> static void win_launch(struct ops *o, win_args &a, long lo
     launch_check("attention tiles");
     if (a.splits > 1) {
         const bool wide = a.splits > 16;
-        const dim3 mgrid(grid_of(wide ? heads : (heads + 3) / 4, 256, "attention merge"));
+        const dim3 mgrid(grid_of(wide ? heads * (win_width(a.d) / 32) : (heads + 3) / 4, 256, "attention merge"));
 
 #define MERGE_LAUNCH(DP_)                                                                \
     do {                                                                                 \

@@ -28,12 +28,6 @@ static __device__ __forceinline__ int seq_start(const cache_view &c, int b)
     return min(max(c.start[b], 0), c.rows);
 }
 
-/* Kept tokens of sequence b that the table has room for. */
-static __device__ __forceinline__ int seq_len(const cache_view &c, int b)
-{
-    return (int)min((long long)max(c.len[b], 0), (long long)c.ldt << c.page_log);
-}
-
 /* The page of position p (0 <= p < ldt page) of sequence b, -1 for none. */
 static __device__ __forceinline__ int seq_page(const cache_view &c, int b, int p)
 {
@@ -46,25 +40,6 @@ static __device__ __forceinline__ int seq_page(const cache_view &c, int b, int p
 static __device__ __forceinline__ long long cache_row(const cache_view &c, int page, int h, int p)
 {
     return (((long long)page * c.nhk + h) << c.page_log) + (p & ((1 << c.page_log) - 1));
-}
-
-/* The sequence of a row: the last of those that start at or before it, -1
- * where none does or the last has ended. */
-static __device__ __forceinline__ int seq_of(const cache_view &c, int row)
-{
-    int lo = 0, hi = c.n; /* start[lo] <= row < start[hi], if any */
-
-    if (row < seq_start(c, 0) || row >= seq_start(c, c.n))
-        return -1;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-
-        if (seq_start(c, mid) <= row)
-            lo = mid;
-        else
-            hi = mid;
-    }
-    return lo;
 }
 
 namespace icoreg {
