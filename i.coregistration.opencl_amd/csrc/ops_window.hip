@@ -6,10 +6,23 @@
  * cache (seqs.h, q8.h), there with right = 0 and the queries of several
  * sequences in one call.
  *
+ * One pass over the keys: with the running maximum m of a row's scores s
+ * (scale and log2 e in the query), the sum l of 2^(s - m) and the output o of
+ * 2^(s - m) v, a larger maximum m' multiplies l and o by 2^(m - m') and the
+ * result is o / l. Any m serves that keeps the powers in range, so it is
+ * raised only when a score passes it by WIN_TAU.
+ *
+ * A cache's value is scale times code: the scale goes with the weight, and the
+ * products take codes, which are exact in 16 bits. float32 operands are sums of
+ * parts of 16 bits, as the matrix instructions of float32 have a 16th of the
+ * rate: three bf16 parts for few rows (all 24 bits, split.h; memory bounds
+ * them), two f16 parts for tiles of many (22 bits, a row and head brought to
+ * 2^14 .. 2^15 by a power of two; three products instead of six).
+ *
  * The keys that any row of a tile of rows sees are one or two runs of tiles of
- * keys (win_span). Where there are few rows, the tiles of keys are split over
- * blocks of threads, maximum, sum and unnormalised output of each to the work
- * buffer, and a second kernel joins them. */
+ * keys (win_span); no others are read. Where rows do not fill the CUs, the
+ * tiles of keys are split over blocks of threads, maximum, sum and unnormalised
+ * output of each to the work buffer, and a second kernel joins them. */
 
 #include <hip/hip_runtime.h>
 
@@ -238,7 +251,7 @@ static __device__ __forceinline__ int win_parts(int tiles, int splits, int least
     return min(splits, max(1, tiles / least));
 }
 
-/* ---- a tile of rows over a cache ------------------------------------------------ */
+/* ---- a tile of rows ---------------------------------------------------------------- */
 
 typedef _Float16 win_h2 __attribute__((ext_vector_type(2)));
 typedef _Float16 win_h8 __attribute__((ext_vector_type(8)));
@@ -246,8 +259,8 @@ typedef float win_f2 __attribute__((ext_vector_type(2)));
 typedef float win_f16x __attribute__((ext_vector_type(16)));
 typedef unsigned win_u4 __attribute__((ext_vector_type(4)));
 
-#define WIN_KT 64       /* keys of a tile of a cache */
-#define WIN_AHEAD 2     /* operands on their way from LDS */
+#define WIN_KT 64       /* keys of a tile; 32 of float32 ones of 128 channels, whose parts fill LDS */
+#define WIN_AHEAD 2     /* operands on their way from LDS; 3 and 4 measured the same */
 #define WIN_TAU 4.0f    /* the running maximum is raised when a score passes it by this (base 2) */
 #define WIN_VEXP 10     /* exponent of the largest value scale: weights up to 2^TAU stay below 2^16 */
 #define WIN_VMIN 0.125f /* smaller ones lose bits: 2^13 below the largest */
@@ -463,7 +476,30 @@ template <int L> static __device__ __forceinline__ unsigned win_row_max(unsigned
 }
 
 /* NW / KG waves of 32 rows, KT keys at a time. KG = 2: half of the waves takes
- * the first 32 of them and half the others, joined at the end. */
+ * the first 32 of them and half the others, joined at the end.
+ *
+ * v_mfma_f32_32x32x16_f16 with the keys as rows and the queries as columns: a
+ * lane has 16 scores of one query, its maximum and sum need one exchange with
+ * lane ^ 32, and the weights are the second product's operand as they lie;
+ * values come to it transposed by the LDS read. Keys and values are made f16
+ * once for all rows of the block, as they go from registers to one of two LDS
+ * tiles, while the next tile's loads are on their way: one barrier a tile.
+ * Rows are query-major, the heads of a key head within, so that these share
+ * its keys.
+ *
+ * Weights are two f16 parts, p times the value scale relative to the largest
+ * one so far (exponent vexp, to 2^WIN_VEXP): 22 bits of those over 2^-13 of it,
+ * 2^-35 of it else. Sums, maxima and outputs are float32. Rows for which that
+ * is not enough (win_finish's `again`) are computed by win_row_f32.
+ *
+ * Bound by the instructions that two waves a SIMD issue: 3 sequences of up to 4096
+ * new tokens of 8192, 16 heads on 4 of 128 channels: 795 us, 1010
+ * TFLOP/s of f16 products, matrix instructions 44 % and vector ones 42 % of
+ * the cycles; a large matrix product of f16 has 1309 TFLOP/s. 16380 float32
+ * tokens, window 2048: 860 us, 900 TFLOP/s. 1601 tokens of 16 heads of 64,
+ * window 321: 27 us, of which prologue, join and stores 6. A tile's phases held
+ * apart between the halves of the waves by barriers: 837 us for the first.
+ */
 template <int ND, bool CACHE, int CHANNELS, int NW, int KG, int KT>
 __global__ void __launch_bounds__(64 * NW, ND == 1 ? 4 : 2) win_tile_kernel(const win_args a)
 {
@@ -1070,7 +1106,7 @@ __global__ void __launch_bounds__(64 * NW, ND == 1 ? 4 : 2) win_tile_kernel(cons
                               wild || z != 0.0f, ps[wave], d);
 }
 
-#define WIN_FTAU 8.0f         /* as WIN_TAU */
+#define WIN_FTAU 8.0f         /* as WIN_TAU: bf16 parts have float32's range */
 #define WIN_QUP 0x1p32f       /* scale of the queries split into bf16 parts */
 
 /* ---- few rows ---------------------------------------------------------------------- */
@@ -1087,7 +1123,10 @@ typedef float win_f4 __attribute__((ext_vector_type(4)));
  * the keys as rows (lane % 16 of either 16) and the queries as columns, and
  * leave a lane with the keys 16 t + 4 (lane / 16) + r of its query lane % 16,
  * which slot 4 t + r of the second product takes as they are. Queries and
- * weights are three bf16 parts each (split.h), codes are bf16 values: exact. */
+ * weights are three bf16 parts each (split.h), codes are bf16 values: exact.
+ * Bound by the cache's bytes: one query of 16 heads on 131005 keys of 4 heads
+ * of 128, 139 MB in 31 us; 64 sequences of up to 16384 keys, 278 MB in 60. A
+ * step's keys are asked for a step before, its values at its start. */
 template <int ND, bool CACHE, int CHANNELS>
 __global__ void __launch_bounds__(256, CACHE && ND == 4 ? 3 : 2) win_few_kernel(const win_args a)
 {
@@ -1516,7 +1555,8 @@ __global__ void __launch_bounds__(256, CACHE && ND == 4 ? 3 : 2) win_few_kernel(
 /* Parts of a row and head joined, by W waves: softmax over all of them from
  * their maxima and sums, then LV lanes of four channels a part, GV parts at a
  * time, the first of them on their way before the maxima have come. W = 4: 32
- * channels a block. */
+ * channels a block. Bound by the latency of two dependent loads: 16 rows of 128
+ * parts 4 us, 5.9 with all channels in one block and the parts asked for last. */
 template <int DP, int W> __global__ void __launch_bounds__(256) win_merge_kernel(const win_args a)
 {
     constexpr int RB = 4 / W, CB = W > 1 ? DP / 32 : 1; /* rows of a block, blocks of a row */
