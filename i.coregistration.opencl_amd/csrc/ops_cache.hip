@@ -37,7 +37,7 @@ cache_view cache_check(const struct ops_cache *c, const struct ops_seqs *s, int 
         icoreg_fatal("%s: head dimension %d is not 1 .. %d", op, c->d, OPS_MAX_HEAD_DIM);
     if (c->pages < 0 || c->nhk < 1 || (__int128)c->pages * c->nhk * c->page > 1LL << 53)
         icoreg_fatal("%s: invalid cache of %d pages of %d heads", op, c->pages, c->nhk);
-    if (rows < 0 || s->n < 0 || s->n == 0x7fffffff || s->ldt < 0 ||
+    if (rows < 0 || s->n < 0 || s->n > SEQ_MAX_POS || s->ldt < 0 ||
         (long long)s->ldt * c->page > SEQ_MAX_POS)
         icoreg_fatal("%s: invalid sizes rows=%d, %d sequences of %d pages", op, rows, s->n, s->ldt);
     v.n = s->n;
@@ -154,24 +154,29 @@ template <int L, int R> __device__ __forceinline__ cache_item cache_first(const 
 }
 
 /* Its place. The row's sequence is the last of those that start at or before
- * it, looked for by L lanes at a time. */
+ * it, looked for by L lanes at L places of what is left of the sequences. */
 template <int L, int R> __device__ __forceinline__ void cache_look_up(const cache_view &c, cache_item &it)
 {
     const int sub = threadIdx.x % L, at = threadIdx.x & 63 & ~(L - 1);
-    int count = 0;
+    int b = 0;
 
-    for (int b = 0; b < c.n; b += L) {
-        const bool before = b + sub < c.n && seq_start(c, min(b + sub, c.n - 1)) <= it.row;
+    for (int left = c.n; left > 0;) {
+        const int step = (left + L - 1) / L, to = sub * step;
+        const bool before = to < left && seq_start(c, b + (to < left ? to : 0)) <= it.row;
         const int n = __popcll(__ballot(before) >> at & ((1ull << L) - 1));
 
-        count += n;
-        if (n < L)
+        /* Before the first sequence. */
+        if (n == 0) {
+            it.in = false;
             break;
+        }
+        b += (n - 1) * step;
+        left = step > 1 ? min(step, left - (n - 1) * step) : 0;
     }
-    const int b = max(count - 1, 0), end = seq_start(c, b + 1);
+    const int end = seq_start(c, b + 1);
     const long long p = (long long)max(c.len[b], 0) - (end - it.row);
 
-    it.in = it.in && count > 0 && it.row < end;
+    it.in = it.in && it.row < end;
     if (it.in && p >= 0 && p < (long long)c.ldt << c.page_log) {
         it.p = (int)p;
         it.page = seq_page(c, b, it.p);

@@ -309,31 +309,32 @@ static __device__ __forceinline__ win_job win_job_of(const win_args &a, int tile
         return j;
     }
     /* Sequence b has the tiles of TR rows from start[b] g / TR + b on, one more than
-     * it can need; the last that starts at or before this one, 64 sequences
-     * at a time, each lane with all that is known of one. None: the tile is of
-     * rows before the first sequence. */
+     * it can need; the last that starts at or before this one: of 64 places of
+     * what is left of the sequences, until that is 64 of them, each lane with
+     * all that is known of one. None: the tile is of rows before the first
+     * sequence. */
     const int lane = threadIdx.x & 63;
-    int end = 0, len = 0;
-    long long from = 0;
-    bool any = false;
+    int b0 = 0, left = a.c.n;
 
-    for (int b0 = 0; b0 < a.c.n; b0 += 64) {
-        const int b = min(b0 + lane, a.c.n - 1), s0 = seq_start(a.c, b), s1 = seq_start(a.c, b + 1), l = a.c.len[b];
-        const int n = __popcll(__ballot(b0 + lane < a.c.n && (long long)s0 * g / TR + b <= tile));
+    while (left > 64) {
+        const int step = (left + 63) / 64, b = b0 + lane * step;
+        const bool in = lane * step < left;
+        const int n = __popcll(__ballot(in && (long long)seq_start(a.c, in ? b : b0) * g / TR + b <= tile));
 
-        if (n) {
-            any = true;
-            j.b = b0 + n - 1;
-            j.first = __builtin_amdgcn_readlane(s0, n - 1);
-            end = __builtin_amdgcn_readlane(s1, n - 1);
-            len = max(__builtin_amdgcn_readlane(l, n - 1), 0);
-            from = (long long)j.first * g / TR + j.b;
-        }
-        if (n < 64)
-            break;
+        if (n == 0)
+            return j;
+        b0 += (n - 1) * step;
+        left = min(step, left - (n - 1) * step);
     }
-    if (!any)
+    const int b = b0 + min(lane, left - 1), s0 = seq_start(a.c, b), s1 = seq_start(a.c, b + 1), l = a.c.len[b];
+    const int n = __popcll(__ballot(lane < left && (long long)s0 * g / TR + b <= tile));
+
+    if (n == 0)
         return j;
+    j.b = b0 + n - 1;
+    j.first = __builtin_amdgcn_readlane(s0, n - 1);
+    const int end = __builtin_amdgcn_readlane(s1, n - 1), len = max(__builtin_amdgcn_readlane(l, n - 1), 0);
+    const long long from = (long long)j.first * g / TR + j.b;
     const int rows = max(end - j.first, 0);
 
     j.r0 = (int)(tile - from) * TR;
@@ -1099,8 +1100,9 @@ __global__ void __launch_bounds__(64 * NW, ND == 1 ? 4 : 2) win_tile_kernel(cons
         }
     /* A weight times scale is off by up to 2^-25, which times the largest value
      * is 2^-35 of that: where values are far smaller, or zeros, and the output
-     * is so too, that may be many units of the output. */
-    if (lag && win_halves(most) < l * (CACHE ? 0x1p3f : 0x1p11f))
+     * is so too (2^-14), that may be many units of the output. Zeros alone are
+     * exact. */
+    if (lag && vexp > WIN_NONE && win_halves(most) < l * (CACHE ? 0x1p3f : 0x1p11f))
         wild = true;
     win_finish<ND, CACHE, KT>(a, jb, span, t0, t1, parts, split, o, win_power(max(vexp - WIN_VEXP, 1)), m, l,
                               wild || z != 0.0f, ps[wave], d);

@@ -286,3 +286,62 @@ def test_rows_before_the_first_sequence(before, new, dev, ic):
     got = dev.read(Q).reshape(q.shape)
     assert np.array_equal(got[:before], q[:before]) and np.array_equal(got[start[2]:], q[start[2]:])
     look(got, q, held, start, lengths, table, -1, 0, scale, rng)
+
+
+@pytest.mark.parametrize("n", [64, 65, 700, 4097, 5000])
+@pytest.mark.parametrize("d", [16, 40, 128])
+def test_many_sequences(n, d, dev, ic):
+    """More sequences than are looked at together, some without rows: written,
+    read back, attended to."""
+    kv, h, page = 1, 2, 16
+    rng = np.random.default_rng(n + d)
+    new = rng.choice([0, 1, 1, 1, 3], n)
+    new[[0, n - 1]] = rng.integers(0, 2, 2)
+    lengths = (new + rng.integers(0, 20, n)).astype(np.int32)
+    table = np.arange(3 * n, dtype=np.int32).reshape(n, 3)
+    start, rows = np.concatenate([[0], np.cumsum(new)]) + 2, int(new.sum()) + 5
+    held = Held(dev, ic, 3 * n, page, kv, d)
+    s = held.seqs(start, lengths, table)
+    k, v, q = (rng.standard_normal((rows, x, d)).astype(np.float32) for x in (kv, kv, h))
+    K, V, Q = dev.upload(k), dev.upload(v), dev.upload(q)
+    dev.api.ops_cache_write(dev.po, held.p, ic.C.byref(s), rows, ic.mat(K, 0, d), ic.mat(V, 0, d))
+    held.ref.write(k, v, start, lengths, table)
+    held.matches()
+    want = [np.full((rows, kv, d), 5, np.float32) for _ in "kv"]
+    out = [dev.upload(x) for x in want]
+    held.ref.read(start, lengths, table, *want)
+    dev.api.ops_cache_read(dev.po, held.p, ic.C.byref(s), rows, *(ic.mat(o, 0, d) for o in out))
+    for o, x in zip(out, want):
+        assert np.array_equal(dev.read(o).reshape(x.shape), x)
+    work, scale = dev.alloc(dev.api.ops_attention_cache_work_bytes(rows, h, d)), np.float32(d ** -0.5)
+    call(dev, ic, held, s, rows, Q, Q, h, -1, 0, scale, work)
+    got = dev.read(Q).reshape(q.shape)
+    assert np.array_equal(got[:2], q[:2]) and np.array_equal(got[start[-1]:], q[start[-1]:])
+    for b in {0, 1, n - 2, n - 1, *(i for i in (63, 64, 65, 127, 128, 4095, 4096) if i < n), *rng.integers(0, n, 30).tolist()}:
+        at = slice(start[b], start[b + 1])
+        if new[b]:
+            k8, v8, kept = held.ref.keys(b, lengths, table)
+            check(got[at], q[at], k8, v8, sees(np.arange(lengths[b] - new[b], lengths[b]), len(k8), -1, 0, 0) & kept, scale)
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.3])
+@pytest.mark.parametrize("nq", [2, 90])
+def test_other_scales(nq, scale, dev, ic):
+    q, k, v = data(nq, 200, 2, 1, 48)
+    see = sees(np.arange(nq) + 200 - nq, 200, 70, 0, 1)
+    check(run(dev, ic, q, k, v, 200 - nq, 70, 0, 1, scale), q, k, v, see, np.float32(scale))
+
+
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("nq", [1, 90])
+def test_values_of_zero(nq, d, dev, ic):
+    """Zeros come out as zeros, beside a tile of others too."""
+    q, k, v = data(nq, 300, 2, 1, d)
+    v[:] = 0
+    for some in (False, True):
+        if some:
+            v[:20] = 1
+        got = run(dev, ic, q, k, v, 300 - nq, 40, 0, 0, 0.1)
+        assert not got.any()
+        see = sees(np.arange(nq) + 300 - nq, 300, -1, 0, 0)
+        check(run(dev, ic, q, k, v, 300 - nq, -1, 0, 0, 0.1), q, k, v, see, np.float32(0.1))
