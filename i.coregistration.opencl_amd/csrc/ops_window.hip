@@ -485,7 +485,12 @@ template <int L> static __device__ __forceinline__ unsigned win_row_max(unsigned
  * values come to it transposed by the LDS read. Keys and values are made f16
  * once for all rows of the block, as they go from registers to one of two LDS
  * tiles, while the next tile's loads are on their way: one barrier a tile.
- * Rows are query-major, the heads of a key head within, so that these share
+ * PW > 0: by waves that do nothing else, beside the others' products; us
+ * without and with them, of 64 channels: 1601 tokens of 16 heads, window 321: 27.1
+ * and 24.3; 16000 of 4, 201 and 2001: 39 and 35, 142 and 124; 2 sequences of 4096 new
+ * tokens of 8192 in a cache: 309 and 270. With 32 channels they take the place
+ * of a second block on a CU (6400 tokens of 8 heads 39 and 61), with 128 the
+ * registers (168 of a wave) do not suffice. Rows are query-major, the heads of a key head within, so that these share
  * its keys.
  *
  * Weights are two f16 parts, p times the value scale relative to the largest
@@ -498,11 +503,11 @@ template <int L> static __device__ __forceinline__ unsigned win_row_max(unsigned
  * TFLOP/s of f16 products, matrix instructions 44 % and vector ones 42 % of
  * the cycles; a large matrix product of f16 has 1309 TFLOP/s. 16380 float32
  * tokens, window 2048: 860 us, 900 TFLOP/s. 1601 tokens of 16 heads of 64,
- * window 321: 27 us, of which prologue, join and stores 6. A tile's phases held
+ * window 321: 24 us, of which prologue, join and stores 6. A tile's phases held
  * apart between the halves of the waves by barriers: 837 us for the first.
  */
-template <int ND, bool CACHE, int CHANNELS, int NW, int KG, int KT>
-__global__ void __launch_bounds__(64 * NW, ND == 1 ? 4 : 2) win_tile_kernel(const win_args a)
+template <int ND, bool CACHE, int CHANNELS, int NW, int KG, int KT, int PW>
+__global__ void __launch_bounds__(64 * (NW + PW), PW ? 3 : ND == 1 ? 4 : 2) win_tile_kernel(const win_args a)
 {
     constexpr int DP = 32 * ND, CH = DP / 8, P = CACHE ? 1 : 2; /* channels, 16-byte chunks of a key, f16 parts */
     /* Chunks between keys in LDS: 16 neighbouring keys' chunks of one place, as
@@ -510,6 +515,7 @@ __global__ void __launch_bounds__(64 * NW, ND == 1 ? 4 : 2) win_tile_kernel(cons
      * outputs' are, lie in banks of their own. */
     constexpr int KS = CH + 1, VS = ND == 1 ? 4 : CH + 4;
     constexpr int HT = 32 * NW;                  /* threads that stage keys, and values */
+    static_assert(PW == 0 || 64 * PW == HT, "a unit's thread");
     constexpr int UC = CACHE ? CH / 2 : CH;      /* units of a key: 16 codes, or 8 floats */
     constexpr int U = KT * UC, NU = (U + HT - 1) / HT, RW = CACHE ? 4 : 8;
     constexpr bool SAME = 64 / UC <= 16;         /* a wave's units lie in one run of 16 keys */
@@ -527,6 +533,7 @@ __global__ void __launch_bounds__(64 * NW, ND == 1 ? 4 : 2) win_tile_kernel(cons
     __shared__ float ps[NW][64];
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, col = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const bool mover = wave >= NW; /* one of PW */
     const int g = a.nh / a.nhk, d = CHANNELS == WIN_FULL ? DP : a.d, pitch = a.c.pitch;
     const long long rows = (long long)a.rows * g;
     const int tiles = (int)(CACHE ? rows / TR + a.c.n : (rows + TR - 1) / TR);
@@ -552,64 +559,23 @@ __global__ void __launch_bounds__(64 * NW, ND == 1 ? 4 : 2) win_tile_kernel(cons
     const int t0 = (int)((long long)span.n * split / parts), t1 = (int)((long long)span.n * (split + 1) / parts);
     const int p = jb.p0 + qi, hi = win_hi(a, p, jb.nk), lo = win_lo(a, p);
     /* Those of the wave's first and last row, and whether it has any. */
-    const bool live = wr <= last;
+    const bool live = wr <= last && !mover;
     const int pa = jb.p0 + min(wr, last) / g, pb = jb.p0 + min(wr + 31, last) / g;
     const int hi0 = win_hi(a, pa, jb.nk), hi1 = win_hi(a, pb, jb.nk), lo0 = win_lo(a, pa), lo1 = win_lo(a, pb);
-    win_u4 qh[2 * ND], ql[2 * ND];
-    win_f16x o[ND];
-    float m = -INFINITY, l = 0.0f, qf;
     bool wild = false, lag = false;
 
-    /* The query times scale and log2 e, times a power of two that brings its
-     * largest magnitude to 2^14 .. 2^15; qf takes it back. */
-    {
-        const float *q = a.Q + row * a.ldq + (long long)h * d;
-        float x[2 * ND][8];
-        unsigned mag = 0;
-
-#pragma unroll
-        for (int st = 0; st < 2 * ND; st++) {
-            float u[4], v[4];
-
-            load4_row(q, st * 16 + half * 8, d, u);
-            load4_row(q, st * 16 + half * 8 + 4, d, v);
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                x[st][j] = (j < 4 ? u[j & 3] : v[j & 3]) * (a.scale * WIN_LOG2E);
-                mag = max(mag, q8_mag(x[st][j]));
-            }
-        }
-        mag = max(mag, (unsigned)__shfl_xor((int)mag, 32, 64));
-        const int e = min(max((int)(mag >> 23), 15), 254);
-        const float up = win_power(268 - e);
-
-        qf = win_power(e - 14);
-#pragma unroll
-        for (int st = 0; st < 2 * ND; st++)
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                unsigned u, v;
-
-                win_split(x[st][2 * j] * up, x[st][2 * j + 1] * up, u, v);
-                qh[st][j] = u;
-                ql[st][j] = v;
-            }
-    }
-#pragma unroll
-    for (int tt = 0; tt < ND; tt++)
-#pragma unroll
-        for (int e = 0; e < 16; e++)
-            o[tt][e] = 0.0f;
-
-    /* The first half of the waves stages values, the other keys: unit e is key
-     * e / UC, 16 codes or 8 floats from channel 16 (e % UC) or 8 (e % UC) on. */
+    /* PW waves stage keys and values, or the first half of the waves values and
+     * the other keys: unit e is key e / UC, 16 codes or 8 floats from channel 16
+     * (e % UC) or 8 (e % UC) on. */
     const bool values = wave < NW / 2;
     const int ht = tid % HT, hw = wave % (NW / 2);
-    unsigned reg[NU][RW];
-    float sc1[NU];              /* a cache's value scales, of the units */
-    bool kept[NU], kept1 = false; /* of the units; of key `lane` */
-    float sr = 0.0f;            /* a cache's scale of key `lane` */
-    unsigned byte[NU];          /* of the mask, as kept; looked at when they have come */
+    struct staged {
+        unsigned reg[NU][RW];
+        float sc1[NU];    /* a cache's value scales, of the units */
+        bool kept[NU], kept1; /* of the units; of key `lane` */
+        float sr;         /* a cache's scale of key `lane` */
+        unsigned byte[NU]; /* of the mask, as kept; looked at when they have come */
+    } mine, other;
     int pg = -1, pg0 = t0;
     int vexp = WIN_NONE; /* exponent of the largest value scale so far; o counts in 2^(vexp - 127 - WIN_VEXP) */
 
@@ -624,7 +590,7 @@ __global__ void __launch_bounds__(64 * NW, ND == 1 ? 4 : 2) win_tile_kernel(cons
     /* Tile t into registers. Where there is no key or page, and behind a row's
      * channels, something else is read that counts nothing: no lane has a
      * branch. */
-    auto fetch = [&](int t) {
+    auto fetch = [&](int t, const auto values, staged &r) {
         const int k0 = span.tile(t) * KT;
 
         if constexpr (CACHE) {
@@ -644,8 +610,8 @@ __global__ void __launch_bounds__(64 * NW, ND == 1 ? 4 : 2) win_tile_kernel(cons
 
                     x = *(const uint4 *)(codes + first * pitch + (unsigned)((key & 15) * pitch + min(at, pitch - 16)));
                     if (values) {
-                        kept[i] = page >= 0 && k0 + key < jb.nk;
-                        sc1[i] = (a.c.vs + first)[key & 15];
+                        r.kept[i] = page >= 0 && k0 + key < jb.nk;
+                        r.sc1[i] = (a.c.vs + first)[key & 15];
                     }
                 }
                 else {
@@ -654,17 +620,17 @@ __global__ void __launch_bounds__(64 * NW, ND == 1 ? 4 : 2) win_tile_kernel(cons
 
                     x = *(const uint4 *)(codes + cell * pitch + min(at, pitch - 16));
                     if (values) {
-                        kept[i] = page >= 0 && k0 + key < jb.nk;
-                        sc1[i] = a.c.vs[cell];
+                        r.kept[i] = page >= 0 && k0 + key < jb.nk;
+                        r.sc1[i] = a.c.vs[cell];
                     }
                 }
-                reg[i][0] = x.x, reg[i][1] = x.y, reg[i][2] = x.z, reg[i][3] = x.w;
+                r.reg[i][0] = x.x, r.reg[i][1] = x.y, r.reg[i][2] = x.z, r.reg[i][3] = x.w;
             }
             if (hw == 0) {
                 const int page = page_of(t, lane >> 4);
 
-                kept1 = page >= 0 && k0 + lane < jb.nk;
-                sr = (values ? a.c.vs : a.c.ks)[cache_row(a.c, max(page, 0), jb.kvh, k0 + lane)];
+                r.kept1 = page >= 0 && k0 + lane < jb.nk;
+                r.sr = (values ? a.c.vs : a.c.ks)[cache_row(a.c, max(page, 0), jb.kvh, k0 + lane)];
             }
         }
         else {
@@ -682,21 +648,21 @@ __global__ void __launch_bounds__(64 * NW, ND == 1 ? 4 : 2) win_tile_kernel(cons
                 win_load4<CHANNELS>(x, at + 4, d, v);
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
-                    reg[i][j] = __builtin_bit_cast(unsigned, u[j]);
-                    reg[i][4 + j] = __builtin_bit_cast(unsigned, v[j]);
+                    r.reg[i][j] = __builtin_bit_cast(unsigned, u[j]);
+                    r.reg[i][4 + j] = __builtin_bit_cast(unsigned, v[j]);
                 }
-                kept[i] = key <= end;
+                r.kept[i] = key <= end;
                 if (a.kmask && values)
-                    byte[i] = a.kmask[k0 + min(key, end)];
+                    r.byte[i] = a.kmask[k0 + min(key, end)];
             }
             if (hw == 0 && !values) {
-                kept1 = lane <= end && lane < KT;
+                r.kept1 = lane <= end && lane < KT;
                 if (a.kmask)
-                    byte[0] = a.kmask[k0 + min(lane, end)];
+                    r.byte[0] = a.kmask[k0 + min(lane, end)];
             }
         }
     };
-    auto stash = [&](tile_lds &s) {
+    auto stash = [&](tile_lds &s, const auto values, const staged &r) {
         win_u4 *to = values ? s.v : s.k;
         const int stride = values ? VS : KS;
 
@@ -710,16 +676,16 @@ __global__ void __launch_bounds__(64 * NW, ND == 1 ? 4 : 2) win_tile_kernel(cons
                     continue;
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
-                    const unsigned w = reg[i][j] ^ 0x80808080u;
+                    const unsigned w = r.reg[i][j] ^ 0x80808080u;
 
                     x[j / 2][2 * j % 4] = win_codes(__builtin_amdgcn_perm(0x64646464u, w, 0x04010400u));
                     x[j / 2][2 * j % 4 + 1] = win_codes(__builtin_amdgcn_perm(0x64646464u, w, 0x04030402u));
                 }
                 if (values) {
                     /* Codes of a scale far below the largest: smaller, exactly. */
-                    const int k = vexp - WIN_LAG - (int)(q8_mag(sc1[i]) >> 23);
+                    const int k = vexp - WIN_LAG - (int)(q8_mag(r.sc1[i]) >> 23);
 
-                    if (__any(k > 0 && kept[i])) {
+                    if (__any(k > 0 && r.kept[i])) {
                         const int n = min(max(k, 0), WIN_CODES);
                         const unsigned short f = n <= 14 ? (unsigned short)((15 - n) << 10) : (unsigned short)(1 << (WIN_CODES - n));
                         const _Float16 down = __builtin_bit_cast(_Float16, f);
@@ -734,9 +700,9 @@ __global__ void __launch_bounds__(64 * NW, ND == 1 ? 4 : 2) win_tile_kernel(cons
                 to[key * stride + e % UC * 2 + 1] = x[1];
             }
             if (hw == 0 && !values) {
-                const unsigned long long keep = __ballot(kept1);
+                const unsigned long long keep = __ballot(r.kept1);
 
-                s.ks[lane] = sr;
+                s.ks[lane] = r.sr;
                 if (lane == 0)
                     s.keep = keep;
             }
@@ -744,14 +710,14 @@ __global__ void __launch_bounds__(64 * NW, ND == 1 ? 4 : 2) win_tile_kernel(cons
                 /* Value scales times a power of two that brings the largest so
                  * far to 2^WIN_VEXP; a scale of NaN, and one too far below the
                  * largest, is for the float32 path. */
-                const float x = kept1 ? sr : 0.0f;
+                const float x = r.kept1 ? r.sr : 0.0f;
                 const bool bad = !(q8_mag(x) < 0x7f800000u);
                 const int e = bad ? 0 : (int)(q8_mag(x) >> 23), n = max(vexp - WIN_LAG - e, 0);
                 const int top = max(max(vexp, WIN_VEXP), min((int)wave_umax(e), 253));
                 /* Twice, as one power may pass the range. */
                 const float y = bad || n > WIN_CODES ? 0.0f : x * win_power(127 + n) * win_power(254 + WIN_VEXP - top);
                 const bool w = __any(bad || (x != 0.0f && y < WIN_VMIN));
-                const bool lags = __any(kept1 && e < top - WIN_LAG);
+                const bool lags = __any(r.kept1 && e < top - WIN_LAG);
 
                 s.vs[lane] = y;
                 if (lane == 0) {
@@ -776,10 +742,10 @@ __global__ void __launch_bounds__(64 * NW, ND == 1 ? 4 : 2) win_tile_kernel(cons
 
 #pragma unroll
                 for (int j = 0; j < 8; j++)
-                    f[j] = __builtin_bit_cast(float, reg[i][j]);
+                    f[j] = __builtin_bit_cast(float, r.reg[i][j]);
                 /* Values of keys that are left out are zeros, whatever they
                  * hold. */
-                const bool in = kept[i] && (!a.kmask || byte[i]);
+                const bool in = r.kept[i] && (!a.kmask || r.byte[i]);
 
                 if (values && __any(!in)) {
 #pragma unroll
@@ -829,48 +795,56 @@ __global__ void __launch_bounds__(64 * NW, ND == 1 ? 4 : 2) win_tile_kernel(cons
                 }
             }
             else if (hw == 0) {
-                const unsigned long long keep = __ballot(kept1 && (!a.kmask || byte[0]));
+                const unsigned long long keep = __ballot(r.kept1 && (!a.kmask || r.byte[0]));
 
                 if (lane == 0)
                     s.keep = keep;
             }
         }
     };
+    auto take = [&](int t) {
+        if constexpr (PW > 0) {
+            fetch(t, std::false_type(), mine);
+            fetch(t, std::true_type(), other);
+        }
+        else
+            fetch(t, values, mine);
+    };
+    auto put = [&](tile_lds &s) {
+        if constexpr (PW > 0) {
+            stash(s, std::false_type(), mine);
+            stash(s, std::true_type(), other);
+        }
+        else
+            stash(s, values, mine);
+    };
+    auto begin = [&]() {
+        if (t0 < t1) {
+            if (CACHE)
+                pages(t0);
+            take(t0);
+            put(lds[0]);
+            if (t0 + 1 < t1)
+                take(t0 + 1);
+        }
+    };
     /* The tile behind t into the other buffer, which was last read a tile ago,
-     * before the barrier; then its successor's loads. Half of a SIMD's waves do
-     * it at the start of a tile and half at its end, so that one's products run
-     * beside the other's vector instructions. */
+     * before the barrier; then its successor's loads. */
     auto next = [&](int t) {
         if (t + 1 < t1) {
-            stash(lds[(t + 1 - t0) & 1]);
+            put(lds[(t + 1 - t0) & 1]);
             if (t + 2 < t1) {
                 if (CACHE && t + 2 - pg0 >= 16)
                     pages(t + 2);
-                fetch(t + 2);
+                take(t + 2);
             }
         }
     };
 
-    if (t0 < t1) {
-        if (CACHE)
-            pages(t0);
-        fetch(t0);
-        stash(lds[0]);
-        if (t0 + 1 < t1)
-            fetch(t0 + 1);
-    }
-    __syncthreads();
-    for (int t = t0; t < t1; t++) {
-        const tile_lds &s = lds[(t - t0) & 1];
-        const int base = span.tile(t) * KT;
-        /* This lane's places: a key's chunks; of the values, which come
-         * transposed by 4 x 16, 4 channels of a key. */
-        const win_u4 *kp = s.k + col * KS + half;
-        const char *vp = (const char *)(s.v + (4 * half + (lane & 15) / 4) * VS + 2 * (lane >> 4 & 1)) + 8 * (lane & 3);
+    /* The largest value scale with tile t's, and what else its values say. */
+    auto scales = [&](const tile_lds &s) {
         int top = s.top[0];
 
-        if (!values)
-            next(t);
         if constexpr (!CACHE) {
             int low = s.low[0], zero = s.zero[0];
 
@@ -891,7 +865,88 @@ __global__ void __launch_bounds__(64 * NW, ND == 1 ? 4 : 2) win_tile_kernel(cons
             wild = wild || s.wild;
             lag = lag || s.lag;
         }
-        top = __builtin_amdgcn_readfirstlane(top);
+        return __builtin_amdgcn_readfirstlane(top);
+    };
+
+    if constexpr (PW > 0) {
+        if (mover) {
+            /* Where the others have half of a tile's keys each, they wait for
+             * the next one: 1000 rows of 16 heads on 8000 keys 153 us without,
+             * 147 with; 16000 rows in tiles of 256 123 and 129. */
+            if (KG > 1)
+                __builtin_amdgcn_s_setprio(2);
+            begin();
+            __syncthreads();
+            for (int t = t0; t < t1; t++) {
+                vexp = scales(lds[(t - t0) & 1]);
+                next(t);
+                __syncthreads();
+            }
+            return;
+        }
+    }
+
+    win_u4 qh[2 * ND], ql[2 * ND];
+    win_f16x o[ND];
+    float m = -INFINITY, l = 0.0f, qf;
+
+    /* The query times scale and log2 e, times a power of two that brings its
+     * largest magnitude to 2^14 .. 2^15; qf takes it back. */
+    {
+        const float *q = a.Q + row * a.ldq + (long long)h * d;
+        float x[2 * ND][8];
+        unsigned mag = 0;
+
+#pragma unroll
+        for (int st = 0; st < 2 * ND; st++) {
+            float u[4], v[4];
+
+            load4_row(q, st * 16 + half * 8, d, u);
+            load4_row(q, st * 16 + half * 8 + 4, d, v);
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                x[st][j] = (j < 4 ? u[j & 3] : v[j & 3]) * (a.scale * WIN_LOG2E);
+                mag = max(mag, q8_mag(x[st][j]));
+            }
+        }
+        mag = max(mag, (unsigned)__shfl_xor((int)mag, 32, 64));
+        const int e = min(max((int)(mag >> 23), 15), 254);
+        const float up = win_power(268 - e);
+
+        qf = win_power(e - 14);
+#pragma unroll
+        for (int st = 0; st < 2 * ND; st++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                unsigned u, v;
+
+                win_split(x[st][2 * j] * up, x[st][2 * j + 1] * up, u, v);
+                qh[st][j] = u;
+                ql[st][j] = v;
+            }
+    }
+#pragma unroll
+    for (int tt = 0; tt < ND; tt++)
+#pragma unroll
+        for (int e = 0; e < 16; e++)
+            o[tt][e] = 0.0f;
+
+    if (PW == 0)
+        begin();
+    __syncthreads();
+    for (int t = t0; t < t1; t++) {
+        const tile_lds &s = lds[(t - t0) & 1];
+        const int base = span.tile(t) * KT;
+        /* This lane's places: a key's chunks; of the values, which come
+         * transposed by 4 x 16, 4 channels of a key. */
+        const win_u4 *kp = s.k + col * KS + half;
+        const char *vp = (const char *)(s.v + (4 * half + (lane & 15) / 4) * VS + 2 * (lane >> 4 & 1)) + 8 * (lane & 3);
+        /* Half of a SIMD's waves at the start of a tile and half at its end, so
+         * that one's products run beside the other's vector instructions. */
+        if (PW == 0 && !values)
+            next(t);
+        const int top = scales(s);
+
         /* A tile's float32 scales count in the exponent before it: its weights
          * are 2^vshift of what they are in the sums. The first ones count in
          * none. */
@@ -1056,7 +1111,7 @@ __global__ void __launch_bounds__(64 * NW, ND == 1 ? 4 : 2) win_tile_kernel(cons
                 }
             }
         }
-        if (values)
+        if (PW == 0 && values)
             next(t);
         __syncthreads();
     }
@@ -1699,7 +1754,7 @@ struct win_plan {
  * two); more of them than that, splits included, take a second round.
  *
  * Rows of a tile, us: 1601 rows of 16 heads of 64, window 321: 256 rows 40
- * (112 blocks), 128 with the keys shared by two groups of waves 27; 6400 of 8
+ * (112 blocks), 128 with the keys shared by two groups of waves 24; 6400 of 8
  * heads of 32, window 641: 38, 36; 4096 of 16 on 4 key heads of 128 (256 blocks, 512), window
  * 1025: 117, 145. Splits: 2000 rows of 4 heads on one of 128, window 2048, 32
  * blocks: none 188, 2 107, 4 65, 8 54, 12 69 (a second round); 1601 rows as above
@@ -1751,10 +1806,11 @@ template <bool CACHE> static void win_launch(struct ops *o, win_args &a, long lo
     const hipStream_t s = stream_of(o->ocl);
 
     prof_scope ps(o->ocl, CACHE ? "attention_cache" : "attention_window");
-    const dim3 grid(grid_of(p.blocks * a.splits, p.few ? 256 : 512, "attention tiles")), block(256), eight(512);
+    const dim3 grid(grid_of(p.blocks * a.splits, p.few ? 256 : 768, "attention tiles")), block(256);
 
-#define WIN_KERNEL(ND_, CH_, KG_, KT_) \
-    hipLaunchKernelGGL((win_tile_kernel<ND_, CACHE, CH_, 8, KG_, KT_>), grid, eight, 0, s, a)
+#define WIN_KERNEL(ND_, CH_, KG_, KT_)                                                               \
+    hipLaunchKernelGGL((win_tile_kernel<ND_, CACHE, CH_, 8, KG_, KT_, ND_ == 2 ? 4 : 0>), grid,      \
+                       dim3(ND_ == 2 ? 768 : 512), 0, s, a)
 #define WIN_CHANNELS(ND_, CH_)                                                           \
     do {                                                                                 \
         if (p.few)                                                                       \
