@@ -154,38 +154,40 @@ template <int L, int R> __device__ __forceinline__ cache_item cache_first(const 
 }
 
 /* Its place. The row's sequence is the last of those that start at or before
- * it, looked for by L lanes at L places of what is left of the sequences. */
+ * it, looked for by L lanes at L places of what is left of the sequences, at
+ * last each lane with all that is known of one. */
 template <int L, int R> __device__ __forceinline__ void cache_look_up(const cache_view &c, cache_item &it)
 {
     const int sub = threadIdx.x % L, at = threadIdx.x & 63 & ~(L - 1);
-    int b = 0;
+    int b0 = 0, left = c.n;
+    auto before = [&](bool yes) { return __popcll(__ballot(yes) >> at & ((1ull << L) - 1)); };
 
-    for (int left = c.n; left > 0;) {
+    while (left > L) {
         const int step = (left + L - 1) / L, to = sub * step;
-        const bool before = to < left && seq_start(c, b + (to < left ? to : 0)) <= it.row;
-        const int n = __popcll(__ballot(before) >> at & ((1ull << L) - 1));
+        const int n = before(to < left && seq_start(c, b0 + (to < left ? to : 0)) <= it.row);
 
-        /* Before the first sequence. */
         if (n == 0) {
             it.in = false;
-            break;
+            return;
         }
-        b += (n - 1) * step;
-        left = step > 1 ? min(step, left - (n - 1) * step) : 0;
+        b0 += (n - 1) * step;
+        left = min(step, left - (n - 1) * step);
     }
-    const int end = seq_start(c, b + 1);
-    const long long p = (long long)max(c.len[b], 0) - (end - it.row);
+    const int b = b0 + min(sub, left - 1), s0 = seq_start(c, b), s1 = seq_start(c, b + 1), l = c.len[b];
+    const int n = before(sub < left && s0 <= it.row), mine = at + max(n - 1, 0);
+    const int end = __shfl(s1, mine, 64), len = max(__shfl(l, mine, 64), 0);
+    const long long p = (long long)len - (end - it.row);
 
-    it.in = it.in && it.row < end;
+    it.in = it.in && n > 0 && it.row < end;
     if (it.in && p >= 0 && p < (long long)c.ldt << c.page_log) {
         it.p = (int)p;
-        it.page = seq_page(c, b, it.p);
+        it.page = seq_page(c, b0 + n - 1, it.p);
     }
 }
 
 /* Both kernels are bound by memory, and ask for R heads' lines before they
  * use the first: some 21000 tokens of 8 heads of 64, 86 MB of float32 and 23 of codes
- * and scales, 24 us written and 20 read; one head at a time 32 and 33. */
+ * and scales, 22 us written and 20 read; one head at a time 32 and 33. */
 template <int L, int R> __global__ void __launch_bounds__(256) cache_write_kernel(const cache_args a)
 {
     const bool values = blockIdx.y;

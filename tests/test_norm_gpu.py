@@ -143,3 +143,10 @@ def test_graph(dev, ic):
             dev.finish()
     finally:
         ic.lib().ocl_graph_free(graph)
+
+
+def test_rows_of_two_launches(dev, ic):
+    """More rows than one launch takes."""
+    n = (1 << 22) + 5
+    x, g = np.random.default_rng(4).standard_normal((n, 4), dtype=np.float32), np.array([1, 0.5, 2, -3], np.float32)
+    check(run(dev, ic, x, None, g, h=False), x, None, g)
