@@ -244,11 +244,11 @@ static __device__ __forceinline__ void win_put(const win_args &a, long long row,
         a.ml[u] = parts == 1 ? make_float2(0.0f, WIN_WRITTEN) : make_float2(m, l);
 }
 
-/* Parts that t tiles of keys are split into, of at most `splits`: at least
- * `least` tiles each. */
-static __device__ __forceinline__ int win_parts(int tiles, int splits, int least)
+/* Parts that the tiles of keys are split into, of at most `splits`: at least
+ * two tiles each. */
+static __device__ __forceinline__ int win_parts(int tiles, int splits)
 {
-    return min(splits, max(1, tiles / least));
+    return min(splits, max(1, tiles / 2));
 }
 
 /* ---- a tile of rows ---------------------------------------------------------------- */
@@ -545,7 +545,7 @@ __global__ void __launch_bounds__(64 * (NW + PW), PW ? 3 : ND == 1 ? 4 : 2) win_
         return;
     const int last = jb.r0 + jb.n - 1;
     const win_tiles span = win_span<KT>(a, jb.p0 + jb.r0 / g, jb.p0 + last / g, jb.nk);
-    const int parts = win_parts(span.n, a.splits, 4);
+    const int parts = win_parts(span.n, a.splits);
     /* This lane's row; lanes without one take the last. */
     const int rg = wave % RG, kg = wave / RG;
     const int wr = jb.r0 + 32 * rg, r = min(wr + col, last), qi = r / g, h = jb.kvh * g + r - qi * g;
@@ -1208,7 +1208,7 @@ __global__ void __launch_bounds__(256, CACHE && ND == 4 ? 3 : 2) win_few_kernel(
         return;
     const int last = jb.r0 + jb.n - 1;
     const win_tiles span = win_span<WIN_STEP>(a, jb.p0 + jb.r0 / g, jb.p0 + last / g, jb.nk);
-    const int parts = win_parts(span.n, a.splits, 2);
+    const int parts = win_parts(span.n, a.splits);
     /* This lane's row; lanes without one take the last. */
     const int r = min(jb.r0 + col, last), qi = r / g, h = jb.kvh * g + r - qi * g;
     const bool mine = jb.r0 + col <= last;
@@ -1750,7 +1750,7 @@ struct win_plan {
     long long blocks;      /* without the splits */
 };
 
-/* Rows see at most `keys` each. One block of tiles is held by a CU (32 channels:
+/* Rows see at most `keys` each of `most`. One block of tiles is held by a CU (32 channels:
  * two); more of them than that, splits included, take a second round.
  *
  * Rows of a tile, us: 1601 rows of 16 heads of 64, window 321: 256 rows 40
@@ -1761,8 +1761,13 @@ struct win_plan {
  * in two parts 50. Few rows: 4 heads of 128 on 131005 keys, 64 parts 40, 96 40, 128 35,
  * 192 37, 256 39; on 4096 float32 ones, 16 19, 32 16, 48 and more 13; 64
  * sequences of unlike lengths, window 4096, 2 68, 4 62, 6 59, 8 64, 12 69: parts of
- * unlike length want more of them, if they keep some 600 keys. */
-static win_plan win_plan_of(const win_args &a, bool cache, long long keys, int cus)
+ * unlike length want more of them, if they keep some 600 keys. Parts of two
+ * tiles or more, and one where the second launch costs more than it saves, us
+ * in one part and in more: one row of 4 heads of 64 on 256 keys 7.4, 8.0, 512
+ * 10.8, 8.0 (128 channels 256 11.9, 9.8); 100 rows on 256 14.2, 13.8, of 32
+ * channels 11.2, 11.6, 3 sequences of 200 in a cache 13.3, 15.9; 100 rows on 400
+ * 19.2, 15.4, on 2048 17.7 in parts of four tiles, 14.7 of two, 14.7 of one. */
+static win_plan win_plan_of(const win_args &a, bool cache, long long keys, long long most, int cus)
 {
     const long long heads = (long long)a.rows * a.nh, rows = heads / a.nhk; /* of a key head */
     win_plan p;
@@ -1786,15 +1791,21 @@ static win_plan win_plan_of(const win_args &a, bool cache, long long keys, int c
 
     if (p.few && cache && a.c.n > 1)
         n = std::max(n, std::min(6LL * cus / filled(p.tile), keys / 640));
-    n = std::min(n, std::min(keys / (p.few ? 64 : 128), WIN_PART_ROWS / heads));
+    const long long seen = p.few ? keys : std::min(most, keys + p.tile / (a.nh / a.nhk));
+    const bool wide = !cache && a.d > 64;
+
+    const long long whole = !wide ? 256 : p.few ? 128 : 64; /* keys that stay in one part */
+
+    n = seen <= whole ? 1 : std::min(n, seen / (p.few || wide ? 64 : 128));
+    n = std::min(n, WIN_PART_ROWS / heads);
     p.splits = (int)std::max(1LL, std::min(n, (long long)WIN_MAX_SPLITS));
     return p;
 }
 
-template <bool CACHE> static void win_launch(struct ops *o, win_args &a, long long keys, cl_mem work)
+template <bool CACHE> static void win_launch(struct ops *o, win_args &a, long long keys, long long most, cl_mem work)
 {
     const int cus = o->ocl->cu_count > 0 ? o->ocl->cu_count : 256;
-    const win_plan p = win_plan_of(a, CACHE, keys, cus);
+    const win_plan p = win_plan_of(a, CACHE, keys, most, cus);
     const long long heads = (long long)a.rows * a.nh;
 
     a.splits = p.splits;
@@ -1938,7 +1949,7 @@ extern "C" void ops_attention_window(struct ops *o, struct opnd Q, struct opnd K
     }
     const long long span = left < 0 || right < 0 ? Nk : (long long)left + right + 1 + sinks;
 
-    win_launch<false>(o, a, std::min<long long>(Nk, span), work);
+    win_launch<false>(o, a, std::min<long long>(Nk, span), Nk, work);
     ICOREG_API_END
 }
 
@@ -1972,6 +1983,6 @@ extern "C" void ops_attention_cache(struct ops *o, const struct ops_cache *c, co
     cache_apart(c, s, work->ptr, win_work_bytes(rows, nh, a.d), true, false, op, "work");
     const long long most = (long long)s->ldt * c->page;
 
-    win_launch<true>(o, a, left < 0 ? most : std::min(most, (long long)left + 1 + sinks), work);
+    win_launch<true>(o, a, left < 0 ? most : std::min(most, (long long)left + 1 + sinks), most, work);
     ICOREG_API_END
 }
