@@ -8,6 +8,7 @@
 
 #include <hip/hip_runtime.h>
 
+#include <limits.h>
 #include <stdarg.h>
 #include <stdio.h>
 #include <stdlib.h>
@@ -48,15 +49,21 @@ void need_bytes(cl_mem b, long long off, long long n, const char *op,
     if (!b || !b->ptr)
         icoreg_fatal("%s: %s is NULL but %lld bytes are accessed", op, operand,
                      n);
-    if (off < 0 || (unsigned long long)(off + n) > b->bytes)
+    if (off < 0 || (unsigned long long)off + (unsigned long long)n > b->bytes)
         icoreg_fatal("%s: %s accessed at bytes [%lld, %lld) of a %zu-byte "
                      "buffer",
-                     op, operand, off, off + n, b->bytes);
+                     op, operand, off, off > LLONG_MAX - n ? LLONG_MAX : off + n, b->bytes);
 }
 
 void need_floats(cl_mem b, long long off, long long n, const char *op,
                  const char *operand)
 {
+    if (n <= 0)
+        return;
+    /* Offsets, and rows times row lengths, of more floats than have a byte count. */
+    if (n > LLONG_MAX / 4 || off > LLONG_MAX / 4 || off < LLONG_MIN / 4)
+        icoreg_fatal("%s: %s accessed at %lld floats from float %lld of a %zu-byte buffer", op, operand,
+                     n, off, b ? b->bytes : (size_t)0);
     need_bytes(b, off * 4, n * 4, op, operand);
 }
 
