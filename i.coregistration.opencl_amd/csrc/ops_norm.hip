@@ -21,7 +21,7 @@
 using namespace icoreg;
 
 #define NORM_MAX_C (1 << 30)   /* channels are counted in int, past the last too */
-#define NORM_ROWS (1L << 22)   /* rows of a launch: 2^32 threads are too many */
+#define NORM_ROWS (1L << 21)   /* rows of a launch: 2^32 threads are too many */
 
 struct norm_args {
     const float *X, *R, *g;
@@ -318,9 +318,13 @@ extern "C" void ops_rms_norm(struct ops *o, long rows, int C, struct opnd X, str
             /* Few rows, several waves each, us: of 1024 channels 1 row 4.2 -> 2.9,
              * 512 rows 5.0 -> 3.5, 2048 6.3 -> 6.0, 3202 9.2 -> 9.4; of 4096, 16 waves
              * for 4, 1 row 4.6 -> 3.8, 256 rows 5.6 -> 4.8, 512 6.3 -> 6.5. */
-#define NORM_LAUNCH(NV_, W_)                                                          \
-    hipLaunchKernelGGL((rms_norm_kernel<NV_, W_>), dim3((unsigned)(W_ > 1 ? n : (n + 3) / 4)), \
-                       dim3(W_ > 4 ? 64 * W_ : 256), 0, s, b)
+#define NORM_LAUNCH(NV_, W_)                                                                          \
+    do {                                                                                              \
+        constexpr int threads = W_ > 4 ? 64 * W_ : 256;                                               \
+        static_assert(W_ * 64LL * NORM_ROWS < 1LL << 32, "threads of a launch");                      \
+        hipLaunchKernelGGL((rms_norm_kernel<NV_, W_>), dim3(grid_of(W_ > 1 ? n : (n + 3) / 4, threads, op)), \
+                           dim3(threads), 0, s, b);                                                   \
+    } while (0)
             if (C <= 256)
                 NORM_LAUNCH(1, 1);
             else if (C <= 1024 && n < 2560)
