@@ -264,6 +264,13 @@ typedef unsigned win_u4 __attribute__((ext_vector_type(4)));
 #define WIN_TAU 4.0f    /* the running maximum is raised when a score passes it by this (base 2) */
 #define WIN_VEXP 10     /* exponent of the largest value scale: weights up to 2^TAU stay below 2^16 */
 #define WIN_VMIN 0.125f /* smaller ones lose bits: 2^13 below the largest */
+/* Biased exponents of the largest key whose products with a query of 2^14 ..
+ * 2^15 stay finite when the key's power of two is put back, the query's own
+ * not yet: 128 products of 2^31 (2^22 of codes) times 2^(WIN_KEXP - 141), or a
+ * cache's scale of 2^(WIN_SEXP - 126). Above that a sum might be infinite
+ * below, a weight of 0, where the score is not. */
+#define WIN_KEXP 229
+#define WIN_SEXP 223
 
 /* Codes of 8 bits in f16, exactly: a byte u = code + 128 behind 0x64 is the
  * f16 value 1024 + u. */
@@ -702,7 +709,8 @@ __global__ void __launch_bounds__(64 * (NW + PW), PW ? 3 : ND == 1 ? 4 : 2) win_
             if (hw == 0 && !values) {
                 const unsigned long long keep = __ballot(r.kept1);
 
-                s.ks[lane] = r.sr;
+                /* NaN: rows that see the key are done again. */
+                s.ks[lane] = q8_mag(r.sr) >> 23 > WIN_SEXP ? __builtin_nanf("") : r.sr;
                 if (lane == 0)
                     s.keep = keep;
             }
@@ -754,10 +762,11 @@ __global__ void __launch_bounds__(64 * (NW + PW), PW ? 3 : ND == 1 ? 4 : 2) win_
                 }
                 const float most = fmaxf(fmaxf(fmaxf(fabsf(f[0]), fabsf(f[1])), fmaxf(fabsf(f[2]), fabsf(f[3]))),
                                          fmaxf(fmaxf(fabsf(f[4]), fabsf(f[5])), fmaxf(fabsf(f[6]), fabsf(f[7]))));
-                /* Infinities and NaN make the parts NaN, and the rows that meet
+                /* Infinities and NaN make the parts NaN, as larger keys than
+                 * WIN_KEXP do that pass f16's range, and the rows that meet
                  * them are done again. */
                 const unsigned mag = win_row_max<UC>(__builtin_bit_cast(unsigned, most));
-                int ex = min(max((int)(mag >> 23), 15), 254);
+                int ex = min(max((int)(mag >> 23), 15), values ? 254 : WIN_KEXP);
 
                 if (values) {
                     if (mag) {
