@@ -271,6 +271,15 @@ typedef unsigned win_u4 __attribute__((ext_vector_type(4)));
  * below, a weight of 0, where the score is not. */
 #define WIN_KEXP 229
 #define WIN_SEXP 223
+/* A query's or key's parts are off by 2^-22 of each channel's value or, of those
+ * far below the largest (2^14 .. 2^15 as they are scaled), by 2^-25: of d
+ * channels, with f and s the powers of two of query and key, a score by no more
+ * than d f s 2^15 2^-25 for each of the two, or, of codes, which are exact and
+ * below 2^7 s, d f s 2^7 2^-25 for the query's. Rows for which that passes
+ * WIN_LOST with the largest key of the tiles they look at are done again: 128
+ * normally distributed channels have 2^-29, and 2^-20 where the largest query
+ * times the largest key is 2^9 times as much beside the others. */
+#define WIN_LOST 0x1p-20f
 
 /* Codes of 8 bits in f16, exactly: a byte u = code + 128 behind 0x64 is the
  * f16 value 1024 + u. */
@@ -538,6 +547,7 @@ __global__ void __launch_bounds__(64 * (NW + PW), PW ? 3 : ND == 1 ? 4 : 2) win_
     static_assert((KT == 64 || !CACHE) && KT >= 32 * KG, "a lane a key, 32 keys a wave");
     __shared__ tile_lds lds[2];
     __shared__ float ps[NW][64];
+    __shared__ unsigned most_k[NW][64]; /* largest key scale of the tiles that a wave looked at, as bits */
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, col = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const bool mover = wave >= NW; /* one of PW */
@@ -923,6 +933,7 @@ __global__ void __launch_bounds__(64 * (NW + PW), PW ? 3 : ND == 1 ? 4 : 2) win_
         const float up = win_power(268 - e);
 
         qf = win_power(e - 14);
+        most_k[wave][lane] = 0;
 #pragma unroll
         for (int st = 0; st < 2 * ND; st++)
 #pragma unroll
@@ -956,6 +967,13 @@ __global__ void __launch_bounds__(64 * (NW + PW), PW ? 3 : ND == 1 ? 4 : 2) win_
             next(t);
         const int top = scales(s);
 
+        /* Every NW-th tile's keys, a lane each. */
+        if (((t - t0) & (NW - 1)) == wave) {
+            const int keep = ((const int *)&s.keep)[lane >> 5];
+
+            most_k[wave][lane] = max(most_k[wave][lane], __builtin_bit_cast(unsigned, s.ks[lane % KT]) &
+                                                             (unsigned)__builtin_amdgcn_sbfe(keep, col, 1));
+        }
         /* A tile's float32 scales count in the exponent before it: its weights
          * are 2^vshift of what they are in the sums. The first ones count in
          * none. */
@@ -1125,6 +1143,17 @@ __global__ void __launch_bounds__(64 * (NW + PW), PW ? 3 : ND == 1 ? 4 : 2) win_
         __syncthreads();
     }
     l += __shfl_xor(l, 32, 64);
+    /* Channels far below a query's or key's largest may have lost bits that
+     * count: see WIN_LOST. */
+    {
+        unsigned k = most_k[0][lane];
+
+#pragma unroll
+        for (int w = 1; w < NW; w++)
+            k = max(k, most_k[w][lane]);
+        if (!(__builtin_bit_cast(float, wave_umax(k)) * qf * (d * (CACHE ? 0x1p-18f : 0x1p-9f)) <= WIN_LOST))
+            l = __builtin_nanf("");
+    }
     if constexpr (KG > 1) {
         /* The other keys' sums, through LDS: a lane's registers as they are. */
         static_assert(sizeof(lds) >= RG * 64 * (16 * ND + 2) * 4, "room for the sums");

@@ -359,7 +359,8 @@ void ops_cache_read(struct ops *o, const struct ops_cache *c,
  * values from 2^115 on may pass float32's range before they are divided.
  * Sums, maxima and outputs are float32's. What enters the products may be
  * rounded: queries, keys and values to 22 bits or to 2^-39 of their row and
- * head's largest; a weighted value to 2^-23 of itself or to 2^-35 of the
+ * head's largest, but not to what moves a score log2 e by more than 2^-20
+ * beyond the 22 bits; a weighted value to 2^-23 of itself or to 2^-35 of the
  * largest value among the keys up to the row's last, but not to more than 2^-20
  * of the row and head's largest output. O may be Q (same offset and ld), any
  * other overlap of O is an error. work: what a call needs while it runs; calls
