@@ -84,7 +84,14 @@ __global__ void __launch_bounds__(W > 4 ? 64 * W : 256) rms_norm_kernel(const no
 {
 #pragma clang fp contract(off)
     constexpr int RB = W > 4 ? 1 : 4 / W; /* rows of a block */
-    __shared__ double sums[W > 1 ? W : 1];
+    /* Two kernels share the rows of 257 to 1024 channels, and of up to 4096, by how
+     * many there are, and a row is the same from both: each 256 channels, a step
+     * of a wave, have sums of their own, added in their order, by lanes and then
+     * over the lanes (up to 1024: the other way takes norms of 3202 rows 2 %
+     * longer), or over the lanes first. */
+    constexpr int NB = NV && NV * W <= 16 ? NV : 1;
+    constexpr bool LANES = NV * W == 4;
+    __shared__ double sums[W > 1 ? NB * W : 1][LANES && W > 1 ? 64 : 1];
     __shared__ unsigned tops[W > 1 ? W : 1];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int sub = wave % W, C = a.C;
@@ -92,7 +99,7 @@ __global__ void __launch_bounds__(W > 4 ? 64 * W : 256) rms_norm_kernel(const no
     const int steps = NV ? NV : (C + 256 * W - 1) / (256 * W);
     const long long words = q8_pitch(C) / 4;
     float v[NV ? NV : 1][4];
-    double sum = 0;
+    double part[NB] = {}, sum = 0;
 
     if (row >= a.rows)
         return;
@@ -118,20 +125,33 @@ __global__ void __launch_bounds__(W > 4 ? 64 * W : 256) rms_norm_kernel(const no
         load(k, x);
 #pragma unroll
         for (int j = 0; j < 4; j++)
-            sum += (double)x[j] * x[j];
+            part[NB > 1 ? k : 0] += (double)x[j] * x[j];
         if (H)
             store4_row(H, at(k), C, x);
     }
-    sum = wave_dsum(sum);
-    if constexpr (W > 1) {
-        if (lane == 0)
-            sums[sub] = sum;
-        __syncthreads();
-        sum = sums[0];
+    if constexpr (!LANES) {
 #pragma unroll
-        for (int e = 1; e < W; e++)
-            sum += sums[e];
+        for (int k = 0; k < NB; k++)
+            part[k] = wave_dsum(part[k]);
     }
+    if constexpr (W > 1) {
+        if (LANES || lane == 0) {
+#pragma unroll
+            for (int k = 0; k < NB; k++)
+                sums[W * k + sub][LANES ? lane : 0] = part[k];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < NB * W; e++)
+            sum += sums[e][LANES ? lane : 0];
+    }
+    else {
+#pragma unroll
+        for (int k = 0; k < NB; k++)
+            sum += part[k];
+    }
+    if constexpr (LANES)
+        sum = wave_dsum(sum);
     const float inv = (float)(1.0 / sqrt(sum / C + a.eps));
     unsigned mag = 0;
 
