@@ -155,7 +155,8 @@ __global__ void __launch_bounds__(W > 4 ? 64 * W : 256) rms_norm_kernel(const no
     const float inv = (float)(1.0 / sqrt(sum / C + a.eps));
     unsigned mag = 0;
 
-    /* Channels behind the last have y = 0. */
+    /* Channels behind the last have y = 0, or NaN where the row has one, whose
+     * codes are all 0: inv is never infinite, as eps is above 0. */
     auto scale = [&](int k, float (&x)[4]) {
         if (!NV) {
             if (H)
@@ -185,7 +186,7 @@ __global__ void __launch_bounds__(W > 4 ? 64 * W : 256) rms_norm_kernel(const no
             scale(k, x);
 #pragma unroll
             for (int j = 0; j < 4; j++)
-                mag = max(mag, at(k) + j < C ? q8_mag(x[j]) : 0u);
+                mag = max(mag, q8_mag(x[j]));
         }
     }
     q8_scale q = {};
@@ -213,15 +214,8 @@ __global__ void __launch_bounds__(W > 4 ? 64 * W : 256) rms_norm_kernel(const no
             scale(k, x);
         if (Y)
             store4_row(Y, at(k), C, x);
-        if (Q && w < words) {
-            /* Behind the last channel 0, where an infinite inv made NaN. */
-            if (at(k) + 4 > C) {
-#pragma unroll
-                for (int j = 0; j < 4; j++)
-                    x[j] = at(k) + j < C ? x[j] : 0.0f;
-            }
+        if (Q && w < words)
             Q[w] = q8_code4(x[0], x[1], x[2], x[3], q.r);
-        }
     }
 }
 
