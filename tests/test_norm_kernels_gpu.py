@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 
 import kept_ref
-from test_norm_gpu import run
+from test_norm_gpu import check, data, run
 
 pytestmark = pytest.mark.gpu
 
@@ -90,3 +90,34 @@ def test_same_from_every_kernel(c, many, dev, ic):
     among = run(dev, ic, np.concatenate([x, np.ones((many - len(x), c), np.float32)]))
     for k in ("y", "q", "s"):
         assert np.array_equal(alone[k], among[k][:len(x)]), k
+
+
+# Both sides of where kernels change hands, by rows and by channels, with parts
+# of a step of 4, 256 and 1024 channels left over.
+@pytest.mark.parametrize("n,c", [(2559, 1024), (2560, 1024), (2561, 257), (2600, 513), (3202, 1023), (2559, 300), (383, 4096),
+                                 (384, 4096), (400, 1025), (500, 4093), (600, 2049), (383, 3000), (300, 4097), (200, 16384)])
+def test_many_rows_of_every_width(n, c, dev, ic):
+    print(f"[norm] {n} x {c}", flush=True)
+    x, r, g = data(n, c)
+    check(run(dev, ic, x, r, g), x, r, g)
+    check(run(dev, ic, x, r, g, pads=(3, 1, 64, 2)), x, r, g)
+    check(run(dev, ic, x, None, None, h=False), x, None, None)
+    check(run(dev, ic, x, r, g, y=False), x, r, g)
+    check(run(dev, ic, x, r, g, q=False), x, r, g)
+    for alias in ([("h", "x")], [("h", "r"), ("y", "x")], [("y", "r")]):
+        check(run(dev, ic, x, r, g, alias=alias), x, r, g)
+
+
+@pytest.mark.parametrize("n,c", [(2560, 700), (390, 4000), (400, 4096)])
+def test_values_among_many_rows(n, c, dev, ic):
+    """Zeros, magnitudes whose squares pass float32's range, subnormal ones and
+    values that are not finite, each in rows of its own."""
+    x, _, g = data(n, c)
+    x[0] = 0
+    x[1] = 1e30 * np.sign(x[1])
+    x[2] *= np.float32(1e-30)
+    x[3] = np.float32(1e-42)
+    x[4, c // 2], x[n - 1, c - 1], x[5, 0] = np.inf, -np.inf, np.nan
+    x[6, 1:] = 0
+    for eps in (1e-6, 1e-45):
+        check(run(dev, ic, x, None, g, eps), x, None, g, eps)
