@@ -501,13 +501,18 @@ template <int L> static __device__ __forceinline__ unsigned win_row_max(unsigned
  * values come to it transposed by the LDS read. Keys and values are made f16
  * once for all rows of the block, as they go from registers to one of two LDS
  * tiles, while the next tile's loads are on their way: one barrier a tile.
- * PW > 0: by waves that do nothing else, beside the others' products; us
- * without and with them, of 64 channels: 1601 tokens of 16 heads, window 321: 27.1
- * and 24.3; 16000 of 4, 201 and 2001: 39 and 35, 142 and 124; 2 sequences of 4096 new
- * tokens of 8192 in a cache: 309 and 270. With 32 channels they take the place
- * of a second block on a CU (6400 tokens of 8 heads 39 and 61), with 128 the
- * registers (168 of a wave) do not suffice. Rows are query-major, the heads of a key head within, so that these share
- * its keys.
+ * PW > 0: by waves that do nothing else, beside the others' products. Us:
+ *
+ *   channels, call                                  without   with
+ *   64, 1601 tokens of 16 heads, window 321            27.1   24.3
+ *   64, 16000 tokens of 4 heads, window 201              39     35
+ *   64, 16000 tokens of 4 heads, window 2001            142    124
+ *   64, cache, 2 x 4096 new tokens of 8192              309    270
+ *   32, 6400 tokens of 8 heads, window 641               39     61
+ *
+ * With 32 channels they take the place of a second block on a CU; with 128 the
+ * registers (168 of a wave) do not suffice. Rows are query-major, the heads of a
+ * key head within, so that these share its keys.
  *
  * Weights are two f16 parts, p times the value scale relative to the largest
  * one so far (exponent vexp, to 2^WIN_VEXP): 22 bits of those over 2^-13 of it,
@@ -1789,22 +1794,40 @@ struct win_plan {
 };
 
 /* Rows see at most `keys` each of `most`. One block of tiles is held by a CU (32 channels:
- * two); more of them than that, splits included, take a second round.
+ * two); more of them than that, splits included, take a second round. A block
+ * has 256 rows, or 128 with the keys shared by two groups of waves where that
+ * leaves all blocks in one round. Us:
  *
- * Rows of a tile, us: 1601 rows of 16 heads of 64, window 321: 256 rows 40
- * (112 blocks), 128 with the keys shared by two groups of waves 24; 6400 of 8
- * heads of 32, window 641: 38, 36; 4096 of 16 on 4 key heads of 128 (256 blocks, 512), window
- * 1025: 117, 145. Splits: 2000 rows of 4 heads on one of 128, window 2048, 32
- * blocks: none 188, 2 107, 4 65, 8 54, 12 69 (a second round); 1601 rows as above
- * in two parts 50. Few rows: 4 heads of 128 on 131005 keys, 64 parts 40, 96 40, 128 35,
- * 192 37, 256 39; on 4096 float32 ones, 16 19, 32 16, 48 and more 13; 64
- * sequences of unlike lengths, window 4096, 2 68, 4 62, 6 59, 8 64, 12 69: parts of
- * unlike length want more of them, if they keep some 600 keys. Parts of two
- * tiles or more, and one where the second launch costs more than it saves, us
- * in one part and in more: one row of 4 heads of 64 on 256 keys 7.4, 8.0, 512
- * 10.8, 8.0 (128 channels 256 11.9, 9.8); 100 rows on 256 14.2, 13.8, of 32
- * channels 11.2, 11.6, 3 sequences of 200 in a cache 13.3, 15.9; 100 rows on 400
- * 19.2, 15.4, on 2048 17.7 in parts of four tiles, 14.7 of two, 14.7 of one. */
+ *   rows, heads (key heads), channels, window       256 rows      128 rows
+ *   1601, 16, 64, 321                                     40            24  (112 blocks of 256)
+ *   6400, 8, 32, 641                                      38            36
+ *   4096, 16 (4), 128, 1025, cache                       117           145  (256 blocks, 512)
+ *
+ * Keys are split until the blocks fill that round. Us by the number of parts:
+ *
+ *   2000 rows, 4 heads (1) of 128, window 2048, 32 blocks   1: 188   2: 107   4: 65   8: 54   12: 69
+ *   1 row, 4 heads of 128, 131005 keys of a cache           64: 40   96: 40   128: 35   192: 37   256: 39
+ *   1 row, 4 heads of 128, 4096 float32 keys                16: 19   32: 16   48 and more: 13
+ *   1 row each of 64 sequences of a cache, window 4096      2: 68   4: 62   6: 59   8: 64   12: 69
+ *
+ * Sequences of unlike lengths, the last line, make parts of unlike length and
+ * want more of them than fill one round; the limits there, 6 blocks a CU and
+ * 640 keys a part, were measured on that call alone.
+ *
+ * Parts have two tiles or more, and there is one part where the second launch
+ * costs more than it saves. Us in one part and in several:
+ *
+ *   1 row, 4 heads of 64, 256 keys            7.4    8.0
+ *   1 row, 4 heads of 64, 512 keys           10.8    8.0
+ *   1 row, 4 heads of 128, 256 keys          11.9    9.8
+ *   100 rows of 64 channels, 256 keys        14.2   13.8
+ *   100 rows of 32 channels, 256 keys        11.2   11.6
+ *   3 sequences of 200 in a cache            13.3   15.9
+ *   100 rows of 64 channels, 400 keys        19.2   15.4
+ *   100 rows of 64 channels, 2048 keys: parts of four tiles 17.7, of two 14.7, of one 14.7
+ *
+ * One kernel and one number of parts serve all sequences of a call: a single
+ * token beside a prompt of many rows is computed like a row of the prompt. */
 static win_plan win_plan_of(const win_args &a, bool cache, long long keys, long long most, int cus)
 {
     const long long heads = (long long)a.rows * a.nh, rows = heads / a.nhk; /* of a key head */
