@@ -76,7 +76,7 @@ __device__ __forceinline__ void store4_row(float *row, int c, int n, const float
  * stay in registers between the sum, the maximum and the codes; longer ones
  * (NV = 0) are read again: h, where it is kept, from there, as it may lie over
  * x or r. Bound by memory, which each value passes once: 12805 x 4096 with the
- * residual, to h and codes (682 MB), 129 us, 5.3 TB/s (a large copy 4.8); 3202 x
+ * residual, to h and codes (682 MB), 128 us, 5.3 TB/s (a large copy 4.8); 3202 x
  * 1024 to h and y (52 MB, some of it still in the last cache) 9 us. The 64-bit
  * products and sums run beside the loads. */
 template <int NV, int W>

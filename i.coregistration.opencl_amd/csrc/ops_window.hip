@@ -520,12 +520,13 @@ template <int L> static __device__ __forceinline__ unsigned win_row_max(unsigned
  * is not enough (win_finish's `again`) are computed by win_row_f32.
  *
  * Bound by the instructions that two waves a SIMD issue: 3 sequences of up to 4096
- * new tokens of 8192, 16 heads on 4 of 128 channels: 795 us, 1010
+ * new tokens of 8192, 16 heads on 4 of 128 channels: 785 us, 1020
  * TFLOP/s of f16 products, matrix instructions 44 % and vector ones 42 % of
  * the cycles; a large matrix product of f16 has 1309 TFLOP/s. 16380 float32
- * tokens, window 2048: 860 us, 900 TFLOP/s. 1601 tokens of 16 heads of 64,
+ * tokens, window 2048: 870 us, 890 TFLOP/s. 1601 tokens of 16 heads of 64,
  * window 321: 24 us, of which prologue, join and stores 6. A tile's phases held
- * apart between the halves of the waves by barriers: 837 us for the first.
+ * apart between the halves of the waves by barriers: 837 us for the first, 775 then
+ * without.
  */
 template <int ND, bool CACHE, int CHANNELS, int NW, int KG, int KT, int PW>
 __global__ void __launch_bounds__(64 * (NW + PW), PW ? 3 : ND == 1 ? 4 : 2) win_tile_kernel(const win_args a)
