@@ -1598,6 +1598,9 @@ __global__ void __launch_bounds__(256, CACHE && ND == 4 ? 3 : 2) win_few_kernel(
         lsum[wave][col] = l;
     }
     float z = l * 0.0f;
+    /* Codes are not scaled, float32 values are; taken back before the waves'
+     * sums are added, which might pass the range with it. */
+    const float down = CACHE ? 1.0f / SPLIT_UP : SPLIT_DOWN;
 
 #pragma unroll
     for (int t = 0; t < NT; t++)
@@ -1606,7 +1609,7 @@ __global__ void __launch_bounds__(256, CACHE && ND == 4 ? 3 : 2) win_few_kernel(
             const int w = 4 * grp + e;
             const int c = CACHE || ND == 1 ? VL * w + t : 64 * (t / 4) + 4 * w + t % 4;
 
-            os[wave][col][c] = o[t][e];
+            os[wave][col][c] = o[t][e] * down;
             z = fmaf(o[t][e], 0.0f, z);
         }
     __syncthreads();
@@ -1630,9 +1633,7 @@ __global__ void __launch_bounds__(256, CACHE && ND == 4 ? 3 : 2) win_few_kernel(
             for (int e = 0; e < VL; e++)
                 y[e] = fmaf(f, os[w][qr][c0 + e], y[e]);
         }
-        /* Codes are not scaled, float32 values are. */
-        const float down = CACHE ? 1.0f / SPLIT_UP : SPLIT_DOWN;
-        const float inv = parts > 1 ? down : sum > 0.0f ? down / sum : 0.0f;
+        const float inv = parts > 1 ? 1.0f : sum > 0.0f ? 1.0f / sum : 0.0f;
         float *to = parts > 1 ? a.part + out * DP : a.O + row1 * a.ldo + (long long)h1 * d;
 
 #pragma unroll

@@ -129,3 +129,28 @@ def test_one_large_key(h, d, n, masked, dev, ic):
         see &= mask != 0
         k[mask == 0] = v[mask == 0] = 0
     check_lost(got[rows], q[rows], k, v, see, scale)
+
+
+@pytest.mark.parametrize("power", [74, 76, 77, 78, 79, 80, 82, 100, 101, 102, 103, 104, 106, 108, 112])
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("nq", [1, 2, 200])
+def test_large_values(nq, d, power, dev, ic):
+    """Sums of values below 2^115 do not pass float32's range on the way to an
+    output."""
+    nk, h, kv, page = 320, 2, 1, 64
+    rng = np.random.default_rng(nq + d + power)
+    scale, q0 = np.float32(d ** -0.5), nk - nq
+    q, k = (rng.standard_normal((n, x, d)).astype(np.float32) for n, x in ((nq, h), (nk, kv)))
+    v = (rng.uniform(1, 2, (nk, kv, d)) * np.where(np.arange(d) % 3 == 0, -1, 1) * 2.0 ** power).astype(np.float32)
+    see = sees(np.arange(nq) + q0, nk, -1, 0, 0)
+    check(run(dev, ic, q, k, v, q0, -1, 0, 0, scale), q, k, v, see, scale)
+    held = Held(dev, ic, nk // page, page, kv, d)
+    table = np.arange(nk // page, dtype=np.int32)[None]
+    s, K, V = held.seqs([0, nk], [nk], table), dev.upload(k), dev.upload(v)
+    dev.api.ops_cache_write(dev.po, held.p, ic.C.byref(s), nk, ic.mat(K, 0, kv * d), ic.mat(V, 0, kv * d))
+    held.ref.write(k, v, [0, nk], [nk], table)
+    k8, v8, _ = held.ref.keys(0, [nk], table)
+    t, Q, O = held.seqs([0, nq], [nk], table), dev.upload(q), dev.zeros(q.size)
+    work = dev.alloc(dev.api.ops_attention_cache_work_bytes(nq, h, d))
+    call(dev, ic, held, t, nq, Q, O, h, -1, 0, scale, work)
+    check(dev.read(O).reshape(q.shape), q, k8, v8, see, scale)
