@@ -362,7 +362,10 @@ void ops_cache_read(struct ops *o, const struct ops_cache *c,
  * head's largest, but not to what moves a score log2 e by more than 2^-20
  * beyond the 22 bits; a weighted value to 2^-23 of itself or to 2^-35 of the
  * largest value among the keys up to the row's last, but not to more than 2^-20
- * of the row and head's largest output. O may be Q (same offset and ld), any
+ * of the row and head's largest output. So a channel of the values that is far
+ * below (2^-15) the others of its row and head keeps fewer bits than those; in
+ * calls of few rows (16 a key head and sequence) nothing is rounded to less
+ * than float32. O may be Q (same offset and ld), any
  * other overlap of O is an error. work: what a call needs while it runs; calls
  * that may run at once, recorded ones too, have one each. */
 size_t ops_attention_window_work_bytes(int Nq, int nh, int d);

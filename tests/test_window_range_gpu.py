@@ -154,3 +154,31 @@ def test_large_values(nq, d, power, dev, ic):
     work = dev.alloc(dev.api.ops_attention_cache_work_bytes(nq, h, d))
     call(dev, ic, held, t, nq, Q, O, h, -1, 0, scale, work)
     check(dev.read(O).reshape(q.shape), q, k8, v8, see, scale)
+
+
+@pytest.mark.parametrize("power", [8, 14, 18, 22, 26, 40, 72])
+@pytest.mark.parametrize("d", [12, 32, 50, 64, 128])
+@pytest.mark.parametrize("nq", [2, 200])
+def test_values_of_one_large_channel(nq, d, power, dev, ic):
+    """A channel of all values, of some keys' or of one key's, far above the
+    others. Few rows: each channel to the bound on its own terms. Many: to what
+    two f16 parts add to it, a value 2^-39 of its row's largest (with its weight's
+    parts 2^-38), a weight check_apart's share of the largest value."""
+    nk, h, kv = 320, 2, 1
+    rng = np.random.default_rng(nq + d + power)
+    scale, q0 = np.float32(d ** -0.5), nk - nq
+    q, k, v = (rng.standard_normal((n, x, d)).astype(np.float32) for n, x in ((nq, h), (nk, kv), (nk, kv)))
+    for keys in (slice(None), slice(None, None, 7), slice(nk - 40, nk - 39)):
+        w = v.copy()
+        w[keys, :, d // 2] *= np.float32(2.0 ** power)
+        for left in (-1, 70):
+            see = sees(np.arange(nq) + q0, nk, left, 0, 0)
+            want, bound = kept_ref.attend(q, k, w, see, scale)
+            err = np.abs(run(dev, ic, q, k, w, q0, left, 0, 0, scale) - want)
+            if nq > 16:
+                rows = np.abs(w).max(-1).astype(np.float64)
+                bound += 2.0 ** -38 * kept_ref.attend(q, k, np.repeat(rows[..., None], d, 2), see, scale)[0]
+                own = np.minimum(rows.max(0), 2.0 ** 15 * np.abs(want).max(-1))
+                bound += see.sum(1)[:, None, None] * 2.0 ** -35 * own[..., None]
+            print(f"  worst {np.max(err / (bound + 1e-37)):.3f} of the bound", flush=True)
+            assert np.all(err <= bound + 1e-37)
